@@ -297,6 +297,7 @@ int32_t tqf_hip_grouped_gemm_device(tqf_hip_ctx *ctx, const tqf_hip_layer *layer
 #define TQF_HIP_FORMAT_Q4_0 0
 #define TQF_HIP_FORMAT_Q4_K 1
 #define TQF_HIP_FORMAT_Q6_K 2
+#define TQF_HIP_FORMAT_F8 3
 /* Device bytes of a Q4_K upload of this shape; 0 unless cols is a positive
  * multiple of 256. */
 uint64_t tqf_hip_q4k_weights_bytes_for(uint32_t rows, uint32_t cols);
@@ -446,6 +447,109 @@ int32_t tqf_hip_lm_head_logits_device(tqf_hip_ctx *ctx, const tqf_hip_weights *w
                                       const float *d_x, uint32_t m, float *d_logits,
                                       uint32_t *d_tokens4, float *d_logits4);
 
+/* ---- 8-bit floating point with a scale for each block of 128 -----------------
+ * No counterpart in the reference, whose weights are GGML's; the format of
+ * checkpoints stored in 8 bits.  A matrix [rows x cols] is OCP e4m3 values q
+ * and f32 scales s [ceil(rows / 128) x ceil(cols / 128)], both row-major:
+ * W[r][k] = q[r][k] * s[r / 128][k / 128].  Any rows (<= 2^24) and cols
+ * (<= 65536); the last blocks may be short.
+ * Activation rows are quantised by the products themselves, each row in blocks
+ * of 128: with a the block's largest magnitude, scale = a / 448 and
+ * q = e4m3(x * (448 / a)), both quotients and the product rounded to f32, the
+ * conversion to nearest with ties to even; a block with a < 2^-100 is zero.  A
+ * row with a NaN or an infinity gives NaN; other rows do not see it.
+ * Element types of rows (`*_type`): */
+#define TQF_HIP_TYPE_F32 0
+#define TQF_HIP_TYPE_BF16 1
+/* Device bytes of an F8 upload of this shape; 0 on a shape the backend cannot
+ * hold. */
+uint64_t tqf_hip_f8_weights_bytes_for(uint32_t rows, uint32_t cols);
+/* len = rows * cols bytes, n_scales = ceil(rows / 128) * ceil(cols / 128).
+ * Lossless; handles are format TQF_HIP_FORMAT_F8 (only the f8 entry points
+ * accept them), freed with tqf_hip_weights_free. */
+int32_t tqf_hip_f8_weights_upload(tqf_hip_ctx *ctx, const uint8_t *q, size_t len, const float *scales,
+                                  size_t n_scales, uint32_t rows, uint32_t cols, tqf_hip_weights **out);
+int32_t tqf_hip_f8_weights_upload_device(tqf_hip_ctx *ctx, const void *d_q, size_t len, const float *d_scales,
+                                         size_t n_scales, uint32_t rows, uint32_t cols, tqf_hip_weights **out);
+/* The inverse: the bytes and scales that were uploaded. */
+int32_t tqf_hip_f8_weights_download(tqf_hip_ctx *ctx, const tqf_hip_weights *w, uint8_t *q, size_t len,
+                                    float *scales, size_t n_scales);
+/* y [t x rows] = Q(x [t x cols]) W^T, 1 <= t <= TQF_HIP_F8_MAX_TOKENS and
+ * t * cols (rounded up to 128) < 2^32.  Blocks are summed in f32 in the order
+ * of K.  With an f32 y (and, up to 16 rows, a bf16 y too) the products within a
+ * block are exact and only their f32 sums round; a larger bf16 y uses the fp8
+ * matrix cores, whose sum of a block is about 1.3e-5 of it off, 1/150 of the
+ * rounding to bf16.  x and y must not overlap. */
+#define TQF_HIP_F8_MAX_TOKENS 65536
+int32_t tqf_hip_f8_matmul_device(tqf_hip_ctx *ctx, const tqf_hip_weights *w, const void *d_x, int32_t x_type,
+                                 uint32_t t, void *d_y, int32_t y_type);
+/* The routed experts of a layer: gate[e], up[e] [width x hidden] and down[e]
+ * [hidden x width], all F8, n_experts of each (1..TQF_HIP_ROUTE_MAX_EXPERTS).
+ * The handle keeps their addresses: free it before them.  A shared expert can
+ * be one of them, given to every row by its route. */
+typedef struct tqf_hip_f8_experts tqf_hip_f8_experts;
+int32_t tqf_hip_f8_experts_prepare(tqf_hip_ctx *ctx, const tqf_hip_weights *const *gate,
+                                   const tqf_hip_weights *const *up, const tqf_hip_weights *const *down,
+                                   uint32_t n_experts, tqf_hip_f8_experts **out);
+int32_t tqf_hip_f8_experts_free(tqf_hip_ctx *ctx, tqf_hip_f8_experts *experts);
+/* x [t x hidden], ids [t x top_k], w [t x top_k] f32 ->
+ * y[t] = sum_k w[t,k] down(silu(gate x_t) * up x_t) of expert ids[t,k], summed
+ * in route order in f32; silu(gate) * up is quantised again for down.  An id of
+ * TQF_HIP_NO_EXPERT is an empty slot (its weight is not read); a row of them
+ * gives zeros.  The same expert may stand in several slots.  Any other id
+ * >= n_experts: *d_status (may be NULL, zeroed by the caller) is set to
+ * TQF_HIP_ERR_INVALID and y is not written.  1 <= t <=
+ * TQF_HIP_GROUPED_MAX_TOKENS, 1 <= top_k <= TQF_HIP_ROUTE_MAX_TOP_K.  A row's
+ * result does not depend on the other rows, but for the choice of path by t and
+ * top_k (up to 64 slots, and above that by the mean slots of an expert).  x
+ * and y must not overlap.  The counterpart for this format of
+ * tqf_hip_grouped_gemm_device. */
+#define TQF_HIP_NO_EXPERT 0xFFFFu
+#define TQF_HIP_ROUTE_MAX_EXPERTS 1024
+#define TQF_HIP_ROUTE_MAX_TOP_K 16
+int32_t tqf_hip_f8_experts_device(tqf_hip_ctx *ctx, const tqf_hip_f8_experts *experts, const void *d_x,
+                                  int32_t x_type, uint32_t t, const uint16_t *d_ids, const float *d_w,
+                                  uint32_t top_k, void *d_y, int32_t y_type, int32_t *d_status);
+
+/* ---- the router over the rows of a batch --------------------------------------
+ * For callers with more rows than a layer call takes, and for routers other
+ * than RouterResult::from_logits (experts/mod.rs:134-197: softmax, top-8,
+ * renormalised; TQF_HIP_TOP_K of n_experts with every other option off gives
+ * its ids).  router is an f32 tensor [n_experts x hidden], x [t x hidden];
+ * logits [t x n_experts] f32.  1 <= n_experts <= TQF_HIP_ROUTE_MAX_EXPERTS, 1 <=
+ * hidden <= 65536.  Up to 8 rows the products are summed in 64 bits; above that
+ * every product of a bf16 x is exact (of an f32 x to 2^-24 of it), sums are f32,
+ * and an f32 magnitude above 3.39e38 (the largest bf16) counts as infinite. */
+int32_t tqf_hip_router_logits_device(tqf_hip_ctx *ctx, const tqf_hip_tensor *router, const void *d_x,
+                                     int32_t x_type, uint32_t t, uint32_t n_experts, uint32_t hidden,
+                                     float *d_logits);
+#define TQF_HIP_SCORE_SOFTMAX 0
+#define TQF_HIP_SCORE_SIGMOID 1
+typedef struct tqf_hip_route_options {
+    int32_t score;        /* s = softmax(row) or sigmoid(logit)                          */
+    uint32_t top_k;       /* 1..TQF_HIP_ROUTE_MAX_TOP_K, at most the experts of the groups kept */
+    uint32_t n_groups;    /* 1..64, dividing n_experts: group g holds n_experts / n_groups
+                             consecutive experts                                         */
+    uint32_t top_groups;  /* 1..n_groups are kept                                        */
+    uint32_t group_best;  /* a group counts for the sum of its 1 or 2 best c             */
+    int32_t renormalise;  /* weights divided by their sum                                */
+    float scale;          /* and multiplied by this                                      */
+} tqf_hip_route_options;
+/* logits [t x n_experts], bias [n_experts] f32 (may be NULL) -> ids [t x top_k]
+ * by descending c = s + bias (ties: the lowest id; of groups, the lowest
+ * group), w [t x top_k] = s of those (without bias), renormalised and scaled.
+ * Scores, sums and comparisons are f64, w is rounded once.  A logit of -inf (or
+ * a c of -inf) takes its expert out; where fewer than top_k are left the
+ * last slots hold TQF_HIP_NO_EXPERT and weight 0.  A row with a NaN or +inf
+ * logit (or c of an expert that is in) has only such slots, and *d_status (may
+ * be NULL, zeroed by the caller) is set to TQF_HIP_ERR_ROUTER.  Weights whose
+ * sum is 0 stay 0.  ids and w feed tqf_hip_f8_experts_device; without empty
+ * slots and with top_k 8 also tqf_hip_grouped_gemm_device. */
+int32_t tqf_hip_route_tokens_device(tqf_hip_ctx *ctx, const void *d_logits, int32_t logits_type, uint32_t t,
+                                    uint32_t n_experts, const float *d_bias,
+                                    const tqf_hip_route_options *options, uint16_t *d_ids, float *d_w,
+                                    int32_t *d_status);
+
 /* ---- the decode loop's row kernels ------------------------------------------
  * Embedding rows (Qwen36Runtime::decode_step's embedding.row,
  * model/qwen36/runtime.rs:403; the row decoded per its dtype as
@@ -534,7 +638,10 @@ int32_t tqf_hip_recovery_counts(tqf_hip_ctx *ctx, uint64_t *stack_reruns, uint64
 #define TQF_HIP_KERNEL_Q4K_MATVEC 10     /* Q4_K matvec, Q8_K semantics       */
 #define TQF_HIP_KERNEL_Q6K_MATVEC 11     /* Q6_K matvec / LM head (+ top-4)   */
 #define TQF_HIP_KERNEL_SAMPLE 12         /* Sampler::select, reference-exact  */
-#define TQF_HIP_KERNEL_KINDS 13
+#define TQF_HIP_KERNEL_F8_MATMUL 13      /* e4m3 matrix product, with its quantisation */
+#define TQF_HIP_KERNEL_F8_EXPERTS 14     /* e4m3 routed experts, all launches of a call */
+#define TQF_HIP_KERNEL_ROUTER 15         /* batched router: logits, routes            */
+#define TQF_HIP_KERNEL_KINDS 16
 /* While enabled, eager (non-graph) launches of each kind are bracketed by HIP
  * events on the context stream.  Enabling clears the totals. */
 int32_t tqf_hip_profile_enable(tqf_hip_ctx *ctx, int32_t enable);

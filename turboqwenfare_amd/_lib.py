@@ -32,7 +32,10 @@ KERNEL_Q4K_GEMV = 9
 KERNEL_Q4K_MATVEC = 10
 KERNEL_Q6K_MATVEC = 11
 KERNEL_SAMPLE = 12
-KERNEL_KINDS = 13
+KERNEL_F8_MATMUL = 13
+KERNEL_F8_EXPERTS = 14
+KERNEL_ROUTER = 15
+KERNEL_KINDS = 16
 VARIANT_PERSISTENT = 0
 VARIANT_Q4K_FOLD = 1
 VARIANT_GRAPHS = 2
@@ -41,7 +44,16 @@ VARIANT_AUTO = 2  # a value, of VARIANT_PERSISTENT only
 FORMAT_Q4_0 = 0
 FORMAT_Q4_K = 1
 FORMAT_Q6_K = 2
+FORMAT_F8 = 3
 GROUPED_MAX_TOKENS = 4096
+TYPE_F32 = 0
+TYPE_BF16 = 1
+F8_MAX_TOKENS = 65536
+NO_EXPERT = 0xFFFF
+ROUTE_MAX_EXPERTS = 1024
+ROUTE_MAX_TOP_K = 16
+SCORE_SOFTMAX = 0
+SCORE_SIGMOID = 1
 
 _vp = C.c_void_p
 _i32 = C.c_int32
@@ -67,6 +79,20 @@ class MoeWeights(C.Structure):
         ("n_experts", _u32),
         ("hidden", _u32),
         ("width", _u32),
+    ]
+
+
+class RouteOptions(C.Structure):
+    """``tqf_hip_route_options``."""
+
+    _fields_ = [
+        ("score", _i32),
+        ("top_k", _u32),
+        ("n_groups", _u32),
+        ("top_groups", _u32),
+        ("group_best", _u32),
+        ("renormalise", _i32),
+        ("scale", _f32),
     ]
 
 
@@ -130,6 +156,17 @@ SIGNATURES = {
     "tqf_hip_top_logit_candidates": (_i32, [_vp, _vp, _u32, _u32, _vp, _vp]),
     "tqf_hip_grouped_gemm": (_i32, [_vp, _vp, _vp, _u32, _vp, _vp, _vp]),
     "tqf_hip_grouped_gemm_device": (_i32, [_vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
+    "tqf_hip_f8_weights_bytes_for": (_u64, [_u32, _u32]),
+    "tqf_hip_f8_weights_upload": (_i32, [_vp, _vp, _sz, _vp, _sz, _u32, _u32, _pp]),
+    "tqf_hip_f8_weights_upload_device": (_i32, [_vp, _vp, _sz, _vp, _sz, _u32, _u32, _pp]),
+    "tqf_hip_f8_weights_download": (_i32, [_vp, _vp, _vp, _sz, _vp, _sz]),
+    "tqf_hip_f8_matmul_device": (_i32, [_vp, _vp, _vp, _i32, _u32, _vp, _i32]),
+    "tqf_hip_f8_experts_prepare": (_i32, [_vp, _vp, _vp, _vp, _u32, _pp]),
+    "tqf_hip_f8_experts_free": (_i32, [_vp, _vp]),
+    "tqf_hip_f8_experts_device": (_i32, [_vp, _vp, _vp, _i32, _u32, _vp, _vp, _u32, _vp, _i32, _vp]),
+    "tqf_hip_router_logits_device": (_i32, [_vp, _vp, _vp, _i32, _u32, _u32, _u32, _vp]),
+    "tqf_hip_route_tokens_device": (
+        _i32, [_vp, _vp, _i32, _u32, _u32, _vp, C.POINTER(RouteOptions), _vp, _vp, _vp]),
     "tqf_hip_embed_rows_device": (_i32, [_vp, _vp, _vp, _u32, _vp, _vp, _vp]),
     "tqf_hip_rmsnorm_rows_device": (_i32, [_vp, _vp, _u32, _u32, _vp, _vp]),
     "tqf_hip_verify_step_device": (

@@ -33,6 +33,23 @@ def _ptr(a: np.ndarray) -> int:
     return a.ctypes.data
 
 
+_TYPES = {"f32": _lib.TYPE_F32, "bf16": _lib.TYPE_BF16}
+_TYPE_BYTES = {_lib.TYPE_F32: 4, _lib.TYPE_BF16: 2}
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _row_type(name: str) -> int:
+    if name not in _TYPES:
+        raise ValueError('element types are "f32" and "bf16"')
+    return _TYPES[name]
+
+
+def _hold(what: str, *needs) -> None:
+    for buf, nbytes in needs:
+        if buf.nbytes < nbytes:
+            raise ValueError(f"{what}: a buffer of {buf.nbytes} bytes, {nbytes} needed")
+
+
 @dataclass
 class Q4Weights:
     handle: int
@@ -54,6 +71,25 @@ class Q6KWeights:
     handle: int
     rows: int
     cols: int
+
+
+@dataclass
+class F8Weights:
+    """An e4m3 matrix on the device, with a scale for each block of 128 x 128."""
+    handle: int
+    rows: int
+    cols: int
+
+
+class F8Experts:
+    """The prepared F8 experts of a layer, plus the matrices they use."""
+
+    def __init__(self, handle: int, n_experts: int, hidden: int, width: int, owned: list):
+        self.handle = handle
+        self.n_experts = n_experts
+        self.hidden = hidden
+        self.width = width
+        self.owned = owned
 
 
 @dataclass
@@ -458,6 +494,157 @@ class HipBackend:
         self._check(self.lib.tqf_hip_grouped_gemm_device(
             self.ctx, layer.handle, d_x.ptr, t, d_ids.ptr, d_w.ptr, d_y.ptr,
             d_status.ptr if d_status else None))
+
+    # ---- e4m3 with a scale for each block of 128 -----------------------------------
+    @staticmethod
+    def f8_weights_bytes_for(rows: int, cols: int) -> int:
+        return int(_lib.load().tqf_hip_f8_weights_bytes_for(rows, cols))
+
+    def upload_f8(self, q: np.ndarray, scales: np.ndarray) -> F8Weights:
+        """q [rows, cols] u8 (e4m3 bytes), scales [ceil(rows / 128), ceil(cols / 128)] f32."""
+        q = np.ascontiguousarray(q, dtype=np.uint8)
+        s = np.ascontiguousarray(scales, dtype=np.float32)
+        if q.ndim != 2 or s.shape != (-(-q.shape[0] // 128), -(-q.shape[1] // 128)):
+            raise ValueError("upload_f8: q [rows, cols] and one scale for each block of 128 x 128")
+        h = C.c_void_p()
+        self._check(self.lib.tqf_hip_f8_weights_upload(self.ctx, _ptr(q), q.nbytes, _ptr(s), s.size, q.shape[0],
+                                                       q.shape[1], C.byref(h)))
+        return F8Weights(h.value, q.shape[0], q.shape[1])
+
+    def upload_f8_device(self, d_q: DeviceBuffer, d_scales: DeviceBuffer, rows: int, cols: int) -> F8Weights:
+        n = -(-rows // 128) * -(-cols // 128)
+        if d_q.nbytes < rows * cols or d_scales.nbytes < 4 * n:
+            raise ValueError("upload_f8_device: buffers smaller than the matrix")
+        h = C.c_void_p()
+        self._check(self.lib.tqf_hip_f8_weights_upload_device(self.ctx, d_q.ptr, rows * cols, d_scales.ptr, n, rows,
+                                                              cols, C.byref(h)))
+        return F8Weights(h.value, rows, cols)
+
+    def download_f8(self, w: F8Weights) -> tuple[np.ndarray, np.ndarray]:
+        q = np.empty((w.rows, w.cols), dtype=np.uint8)
+        s = np.empty((-(-w.rows // 128), -(-w.cols // 128)), dtype=np.float32)
+        self._check(self.lib.tqf_hip_f8_weights_download(self.ctx, w.handle, _ptr(q), q.nbytes, _ptr(s), s.size))
+        return q, s
+
+    def f8_matmul_device(self, w: F8Weights, d_x: DeviceBuffer, t: int, d_y: DeviceBuffer, x_type: str = "f32",
+                         y_type: str = "f32") -> None:
+        """d_y [t x rows] = Q(d_x [t x cols]) W^T; types "f32" or "bf16"."""
+        xt, yt = _row_type(x_type), _row_type(y_type)
+        _hold("f8_matmul_device", (d_x, t * w.cols * _TYPE_BYTES[xt]), (d_y, t * w.rows * _TYPE_BYTES[yt]))
+        self._check(self.lib.tqf_hip_f8_matmul_device(self.ctx, w.handle, d_x.ptr, xt, t, d_y.ptr, yt))
+
+    def f8_matmul(self, w: F8Weights, x: np.ndarray) -> np.ndarray:
+        """Host form: x [cols] or [t, cols] f32 -> [rows] or [t, rows] f32."""
+        x = np.ascontiguousarray(x, dtype=np.float32)
+        x2 = x.reshape(1, -1) if x.ndim == 1 else x
+        if x2.shape[1] != w.cols:
+            raise ValueError(f"x has {x2.shape[1]} columns, matrix has {w.cols}")
+        with self._buffers(x2, 4 * x2.shape[0] * w.rows) as (d_x, d_y):
+            self.f8_matmul_device(w, d_x, x2.shape[0], d_y)
+            y = self.read(d_y, np.float32, (x2.shape[0], w.rows))
+        return y[0] if x.ndim == 1 else y
+
+    def prepare_f8_experts(self, gate: Sequence[F8Weights], up: Sequence[F8Weights],
+                           down: Sequence[F8Weights]) -> F8Experts:
+        """gate, up [width x hidden] and down [hidden x width] of each expert."""
+        E = len(gate)
+        if E == 0 or len(up) != E or len(down) != E:
+            raise ValueError("prepare_f8_experts: one gate, up and down matrix for each expert")
+        arr = [(C.c_void_p * E)(*[w.handle for w in ws]) for ws in (gate, up, down)]
+        h = C.c_void_p()
+        self._check(self.lib.tqf_hip_f8_experts_prepare(self.ctx, *arr, E, C.byref(h)))
+        return F8Experts(h.value, E, gate[0].cols, gate[0].rows, [*gate, *up, *down])
+
+    def free_f8_experts(self, ex: F8Experts) -> None:
+        self._check(self.lib.tqf_hip_f8_experts_free(self.ctx, ex.handle))
+
+    def f8_experts_device(self, ex: F8Experts, d_x: DeviceBuffer, t: int, d_ids: DeviceBuffer, d_w: DeviceBuffer,
+                          top_k: int, d_y: DeviceBuffer, x_type: str = "f32", y_type: str = "f32",
+                          d_status: DeviceBuffer | None = None) -> None:
+        """d_y [t x hidden] = the route-weighted sum of the routed experts (d_ids u16, d_w f32 [t x top_k])."""
+        xt, yt = _row_type(x_type), _row_type(y_type)
+        _hold("f8_experts_device", (d_x, t * ex.hidden * _TYPE_BYTES[xt]), (d_y, t * ex.hidden * _TYPE_BYTES[yt]),
+              (d_ids, 2 * t * top_k), (d_w, 4 * t * top_k))
+        self._check(self.lib.tqf_hip_f8_experts_device(self.ctx, ex.handle, d_x.ptr, xt, t, d_ids.ptr, d_w.ptr, top_k,
+                                                       d_y.ptr, yt, d_status.ptr if d_status else None))
+
+    def f8_experts(self, ex: F8Experts, x: np.ndarray, ids: np.ndarray, w: np.ndarray) -> np.ndarray:
+        """Host form: x [t, hidden] f32, ids [t, k] u16, w [t, k] f32 -> [t, hidden] f32."""
+        x = np.ascontiguousarray(x, dtype=np.float32)
+        ids = np.ascontiguousarray(ids, dtype=np.uint16)
+        w = np.ascontiguousarray(w, dtype=np.float32)
+        if x.ndim != 2 or x.shape[1] != ex.hidden or ids.ndim != 2 or ids.shape[0] != x.shape[0] or w.shape != ids.shape:
+            raise ValueError("f8_experts: x [t, hidden], ids and w [t, top_k]")
+        with self._buffers(x, ids, w, x.nbytes, np.zeros(1, np.int32)) as (d_x, d_i, d_w, d_y, d_s):
+            self.f8_experts_device(ex, d_x, x.shape[0], d_i, d_w, ids.shape[1], d_y, d_status=d_s)
+            y, st = self.read(d_y, np.float32, x.shape), int(self.read(d_s, np.int32, (1,))[0])
+        if st:
+            raise HipError(st, "f8_experts: an expert id is out of range")
+        return y
+
+    # ---- the router over the rows of a batch ---------------------------------------
+    def router_logits_device(self, router: F32Tensor, d_x: DeviceBuffer, t: int, n_experts: int, hidden: int,
+                             d_logits: DeviceBuffer, x_type: str = "f32") -> None:
+        """d_logits [t x n_experts] f32 = d_x [t x hidden] times router [n_experts x hidden]."""
+        xt = _row_type(x_type)
+        _hold("router_logits_device", (d_x, t * hidden * _TYPE_BYTES[xt]), (d_logits, 4 * t * n_experts))
+        self._check(self.lib.tqf_hip_router_logits_device(self.ctx, router.handle, d_x.ptr, xt, t, n_experts, hidden,
+                                                          d_logits.ptr))
+
+    def router_logits(self, router: F32Tensor, x: np.ndarray) -> np.ndarray:
+        """Host form: x [t, hidden] f32 -> [t, n_experts] f32."""
+        x = np.ascontiguousarray(x, dtype=np.float32)
+        if x.ndim != 2 or x.shape[1] == 0 or router.count % x.shape[1]:
+            raise ValueError("router_logits: x [t, hidden] and a router of n_experts * hidden values")
+        n = router.count // x.shape[1]
+        with self._buffers(x, 4 * x.shape[0] * n) as (d_x, d_l):
+            self.router_logits_device(router, d_x, x.shape[0], n, x.shape[1], d_l)
+            return self.read(d_l, np.float32, (x.shape[0], n))
+
+    def route_tokens_device(self, d_logits: DeviceBuffer, t: int, n_experts: int, top_k: int, d_ids: DeviceBuffer,
+                            d_w: DeviceBuffer, logits_type: str = "f32", score: str = "softmax",
+                            d_bias: DeviceBuffer | None = None, n_groups: int = 1, top_groups: int = 1,
+                            group_best: int = 1, renormalise: bool = True, scale: float = 1.0,
+                            d_status: DeviceBuffer | None = None) -> None:
+        """d_ids u16 and d_w f32 [t x top_k] from d_logits [t x n_experts] (tqf_hip_route_tokens_device)."""
+        if score not in _SCORES:
+            raise ValueError('score is "softmax" or "sigmoid"')
+        lt = _row_type(logits_type)
+        _hold("route_tokens_device", (d_logits, t * n_experts * _TYPE_BYTES[lt]), (d_ids, 2 * t * top_k),
+              (d_w, 4 * t * top_k), *([(d_bias, 4 * n_experts)] if d_bias else []))
+        o = _lib.RouteOptions(_SCORES[score], top_k, n_groups, top_groups, group_best, 1 if renormalise else 0,
+                              float(scale))
+        self._check(self.lib.tqf_hip_route_tokens_device(
+            self.ctx, d_logits.ptr, lt, t, n_experts, d_bias.ptr if d_bias else None, C.byref(o), d_ids.ptr, d_w.ptr,
+            d_status.ptr if d_status else None))
+
+    def route_tokens(self, logits: np.ndarray, top_k: int, bias: np.ndarray | None = None, **options):
+        """Host form: logits [t, n_experts] f32 -> (ids [t, top_k] u16, w [t, top_k] f32); options as
+        route_tokens_device.  Raises HipError(ERR_ROUTER) where a row's routing fails."""
+        lg = np.ascontiguousarray(logits, dtype=np.float32)
+        if lg.ndim != 2 or (bias is not None and np.shape(bias) != (lg.shape[1],)):
+            raise ValueError("route_tokens: logits [t, n_experts] and bias [n_experts]")
+        t, n = lg.shape
+        b = np.zeros(0, np.float32) if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+        with self._buffers(lg, b, 2 * t * top_k, 4 * t * top_k, np.zeros(1, np.int32)) as (d_l, d_b, d_i, d_w, d_s):
+            self.route_tokens_device(d_l, t, n, top_k, d_i, d_w, d_bias=None if bias is None else d_b, d_status=d_s, **options)
+            ids, w = self.read(d_i, np.uint16, (t, top_k)), self.read(d_w, np.float32, (t, top_k))
+            st = int(self.read(d_s, np.int32, (1,))[0])
+        if st:
+            raise HipError(st, "route_tokens: a row's routing fails (NaN or +inf)")
+        return ids, w
+
+    @contextlib.contextmanager
+    def _buffers(self, *specs):
+        """Device buffers of host arrays (copied) or byte counts, freed at the end."""
+        got = []
+        try:
+            for s in specs:
+                got.append(self.alloc(max(int(s), 1)) if isinstance(s, (int, np.integer)) else self.to_device(s))
+            yield got
+        finally:
+            for b in got:
+                self.free(b)
 
     # ---- stack / verify step -------------------------------------------------------
     def prepare_stack(self, layers: Sequence[MoeLayer], norms: Sequence[F32Tensor]) -> Stack:

@@ -3,10 +3,13 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -759,6 +762,7 @@ extern "C" int32_t tqf_hip_destroy(tqf_hip_ctx *ctx) {
     (void)hipFree(ctx->d_q4k);
     (void)hipFree(ctx->d_lm);
     (void)hipFree(ctx->d_grouped);
+    (void)hipFree(ctx->d_f8);
     (void)hipFree(ctx->d_sample);
     (void)hipFree(const_cast<const uint8_t **>(ctx->d_adhoc_mats));
     for (Slab &s : ctx->slabs) (void)hipFree(s.base);
@@ -2187,5 +2191,259 @@ extern "C" int32_t tqf_hip_profile_read(tqf_hip_ctx *ctx, int32_t kind, uint64_t
     if (launches) *launches = ctx->prof_launches[kind];
     if (total_ms) *total_ms = ctx->prof_ms[kind];
     if (algorithmic_bytes) *algorithmic_bytes = ctx->prof_bytes[kind];
+    return TQF_HIP_OK;
+}
+
+// ===========================================================================
+// e4m3 with a scale for each block of 128, and the batched router
+// ===========================================================================
+namespace {
+bool valid_f8(const tqf_hip_weights *w) { return w && w->tiles && w->format == TQF_HIP_FORMAT_F8; }
+bool valid_type(int32_t type) { return type == TQF_HIP_TYPE_F32 || type == TQF_HIP_TYPE_BF16; }
+size_t type_bytes(int32_t type) { return type == TQF_HIP_TYPE_F32 ? 4 : 2; }
+bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+bool overlap(const void *a, size_t an, const void *b, size_t bn) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+bool f8_shape_ok(uint32_t rows, uint32_t cols) { return rows && cols && rows <= kF8MaxRows && cols <= kF8MaxCols; }
+
+int32_t check_f8_shape(tqf_hip_ctx *ctx, size_t len, size_t n_scales, uint32_t rows, uint32_t cols) {
+    if (!f8_shape_ok(rows, cols))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "F8 matrix needs 1 <= rows <= 2^24 and 1 <= cols <= 65536");
+    if (len != (size_t)rows * cols) return fail(ctx, TQF_HIP_ERR_INVALID, "F8 byte length does not match rows x cols");
+    if (n_scales != f8_scale_count(f8_shape(rows, cols)))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "F8 matrix needs one scale for each block of 128 x 128");
+    return TQF_HIP_OK;
+}
+
+int32_t f8_upload_from(tqf_hip_ctx *ctx, const uint8_t *d_q, const float *d_scales, uint32_t rows, uint32_t cols,
+                       tqf_hip_weights **out) {
+    const F8Shape d = f8_shape(rows, cols);
+    tqf_hip_weights *w = new (std::nothrow) tqf_hip_weights();
+    if (!w) return fail(ctx, TQF_HIP_ERR_NOMEM, "out of host memory");
+    void *tiles = nullptr;
+    if (arena_alloc(ctx, f8_layout_bytes(d), &tiles) != hipSuccess) {
+        delete w;
+        return fail(ctx, TQF_HIP_ERR_NOMEM, "weights allocation failed");
+    }
+    w->dims = MatrixDims{};
+    w->dims.rows = rows;
+    w->dims.cols = cols;
+    w->format = TQF_HIP_FORMAT_F8;
+    w->tiles = static_cast<uint8_t *>(tiles);
+    w->bytes = f8_layout_bytes(d);
+    w->d_self = nullptr;
+    hipError_t e = launch_f8_repack(ctx->stream, d_q, d_scales, d, w->tiles);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        weights_release(ctx, w);
+        return hip_fail(ctx, "weights upload", e);
+    }
+    *out = w;
+    return TQF_HIP_OK;
+}
+
+// Grows the F8 scratch (the context's stream has drained before the old one goes).
+int32_t ensure_f8_scratch(tqf_hip_ctx *ctx, size_t bytes) {
+    if (bytes == 0 || (ctx->d_f8 && ctx->f8_bytes >= bytes)) return TQF_HIP_OK;
+    TQF_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    if (grow(ctx->d_f8, ctx->f8_bytes, bytes) != hipSuccess) {
+        ctx->d_f8 = nullptr;
+        (void)hipGetLastError();
+        return fail(ctx, TQF_HIP_ERR_NOMEM, "F8 scratch allocation failed");
+    }
+    return TQF_HIP_OK;
+}
+}  // namespace
+
+extern "C" uint64_t tqf_hip_f8_weights_bytes_for(uint32_t rows, uint32_t cols) {
+    if (!f8_shape_ok(rows, cols)) return 0;
+    return align_up(f8_layout_bytes(f8_shape(rows, cols)), kAlign);
+}
+
+extern "C" int32_t tqf_hip_f8_weights_upload(tqf_hip_ctx *ctx, const uint8_t *q, size_t len, const float *scales,
+                                             size_t n_scales, uint32_t rows, uint32_t cols, tqf_hip_weights **out) {
+    TQF_ENTER(ctx);
+    if (!q || !scales || !out) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    *out = nullptr;
+    if (int32_t rc = check_f8_shape(ctx, len, n_scales, rows, cols)) return rc;
+    const size_t at = align_up(len, kAlign);
+    if (int32_t rc = ensure_stage(ctx, at + n_scales * 4)) return rc;
+    uint8_t *stage = static_cast<uint8_t *>(ctx->d_stage);
+    TQF_HIP(ctx, hipMemcpyAsync(stage, q, len, hipMemcpyHostToDevice, ctx->stream));
+    TQF_HIP(ctx, hipMemcpyAsync(stage + at, scales, n_scales * 4, hipMemcpyHostToDevice, ctx->stream));
+    return f8_upload_from(ctx, stage, reinterpret_cast<const float *>(stage + at), rows, cols, out);
+}
+
+extern "C" int32_t tqf_hip_f8_weights_upload_device(tqf_hip_ctx *ctx, const void *d_q, size_t len, const float *d_scales,
+                                                    size_t n_scales, uint32_t rows, uint32_t cols, tqf_hip_weights **out) {
+    TQF_ENTER(ctx);
+    if (!d_q || !d_scales || !out) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    *out = nullptr;
+    if (!aligned_to(d_scales, 4)) return fail(ctx, TQF_HIP_ERR_INVALID, "scales must be aligned to 4 bytes");
+    if (int32_t rc = check_f8_shape(ctx, len, n_scales, rows, cols)) return rc;
+    return f8_upload_from(ctx, static_cast<const uint8_t *>(d_q), d_scales, rows, cols, out);
+}
+
+extern "C" int32_t tqf_hip_f8_weights_download(tqf_hip_ctx *ctx, const tqf_hip_weights *w, uint8_t *q, size_t len,
+                                               float *scales, size_t n_scales) {
+    TQF_ENTER(ctx);
+    if (!valid_f8(w) || !q || !scales) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer or not an F8 matrix");
+    const uint32_t rows = w->dims.rows, cols = w->dims.cols;
+    if (int32_t rc = check_f8_shape(ctx, len, n_scales, rows, cols)) return rc;
+    const F8Shape d = f8_shape(rows, cols);
+    std::unique_ptr<uint8_t[]> tiles(new (std::nothrow) uint8_t[w->bytes]);
+    if (!tiles) return fail(ctx, TQF_HIP_ERR_NOMEM, "out of host memory");
+    TQF_HIP(ctx, hipMemcpyAsync(tiles.get(), w->tiles, w->bytes, hipMemcpyDeviceToHost, ctx->stream));
+    TQF_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    for (uint32_t r = 0; r < rows; ++r)
+        for (uint32_t c = 0; c < cols; c += 16)
+            std::memcpy(q + (size_t)r * cols + c, tiles.get() + f8_offset(d, r, c), std::min<uint32_t>(16, cols - c));
+    std::memcpy(scales, tiles.get() + f8_tile_bytes(d), n_scales * 4);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_f8_matmul_device(tqf_hip_ctx *ctx, const tqf_hip_weights *w, const void *d_x, int32_t x_type,
+                                            uint32_t t, void *d_y, int32_t y_type) {
+    TQF_ENTER(ctx);
+    if (!w || !d_x || !d_y) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (!valid_f8(w)) return fail(ctx, TQF_HIP_ERR_INVALID, "not an F8 matrix");
+    if (!valid_type(x_type) || !valid_type(y_type)) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown element type");
+    if (t == 0 || t > TQF_HIP_F8_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "t must be in 1..65536");
+    const F8Shape d = f8_shape(w->dims.rows, w->dims.cols);
+    if ((uint64_t)t * d.kb * 128 >= (uint64_t(1) << 32))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "t * cols (rounded up to 128) must be below 2^32");
+    const size_t xb = type_bytes(x_type), yb = type_bytes(y_type);
+    if (!aligned_to(d_x, xb) || !aligned_to(d_y, yb)) return fail(ctx, TQF_HIP_ERR_INVALID, "x and y must be aligned to their elements");
+    if (overlap(d_x, (size_t)t * d.cols * xb, d_y, (size_t)t * d.rows * yb))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "x and y must not overlap");
+    if (int32_t rc = ensure_f8_scratch(ctx, f8_matmul_scratch_bytes(d, t))) return rc;
+    Prof p(ctx);
+    const hipError_t e = launch_f8_matmul(ctx->stream, w->tiles, d, d_x, x_type, t, d_y, y_type, ctx->d_f8);
+    if (e != hipSuccess) return hip_fail(ctx, "F8 product launch", e);
+    p.end(TQF_HIP_KERNEL_F8_MATMUL,
+          (double)t * d.cols * xb + (double)t * d.rows * yb + (double)d.rows * d.cols + 4.0 * f8_scale_count(d), 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_f8_experts_prepare(tqf_hip_ctx *ctx, const tqf_hip_weights *const *gate,
+                                              const tqf_hip_weights *const *up, const tqf_hip_weights *const *down,
+                                              uint32_t n_experts, tqf_hip_f8_experts **out) {
+    TQF_ENTER(ctx);
+    if (!gate || !up || !down || !out) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    *out = nullptr;
+    if (n_experts == 0 || n_experts > TQF_HIP_ROUTE_MAX_EXPERTS)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "n_experts must be in 1..1024");
+    if (!valid_f8(gate[0])) return fail(ctx, TQF_HIP_ERR_INVALID, "expert 0: not an F8 matrix");
+    const uint32_t F = gate[0]->dims.rows, H = gate[0]->dims.cols;
+    if (H > kF8MaxCols || F > kF8MaxCols) return fail(ctx, TQF_HIP_ERR_INVALID, "hidden and width must be at most 65536");
+    std::unique_ptr<const uint8_t *[]> mats(new (std::nothrow) const uint8_t *[(size_t)n_experts * 3]);
+    std::unique_ptr<tqf_hip_f8_experts> ex(new (std::nothrow) tqf_hip_f8_experts());
+    if (!mats || !ex) return fail(ctx, TQF_HIP_ERR_NOMEM, "out of host memory");
+    auto ok = [](const tqf_hip_weights *w, uint32_t r, uint32_t c) { return valid_f8(w) && w->dims.rows == r && w->dims.cols == c; };
+    for (uint32_t e = 0; e < n_experts; ++e) {
+        if (!ok(gate[e], F, H) || !ok(up[e], F, H) || !ok(down[e], H, F))
+            return fail(ctx, TQF_HIP_ERR_INVALID, "expert matrices must be F8: gate and up [width x hidden], down [hidden x width]");
+        mats[(size_t)e * 3] = gate[e]->tiles;
+        mats[(size_t)e * 3 + 1] = up[e]->tiles;
+        mats[(size_t)e * 3 + 2] = down[e]->tiles;
+    }
+    void *dm = nullptr;
+    if (arena_alloc(ctx, (size_t)n_experts * 3 * sizeof(void *), &dm) != hipSuccess)
+        return fail(ctx, TQF_HIP_ERR_NOMEM, "expert table allocation failed");
+    const hipError_t e = hipMemcpy(dm, mats.get(), (size_t)n_experts * 3 * sizeof(void *), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        arena_free(ctx, dm);
+        return hip_fail(ctx, "expert table upload", e);
+    }
+    ex->d_mats = static_cast<const uint8_t **>(dm);
+    ex->n_experts = n_experts;
+    ex->hidden = H;
+    ex->width = F;
+    *out = ex.release();
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_f8_experts_free(tqf_hip_ctx *ctx, tqf_hip_f8_experts *experts) {
+    TQF_ENTER(ctx);
+    if (!experts) return TQF_HIP_OK;
+    TQF_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    arena_free(ctx, const_cast<const uint8_t **>(experts->d_mats));
+    delete experts;
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_f8_experts_device(tqf_hip_ctx *ctx, const tqf_hip_f8_experts *experts, const void *d_x,
+                                             int32_t x_type, uint32_t t, const uint16_t *d_ids, const float *d_w,
+                                             uint32_t top_k, void *d_y, int32_t y_type, int32_t *d_status) {
+    TQF_ENTER(ctx);
+    if (!experts || !d_x || !d_ids || !d_w || !d_y) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (!valid_type(x_type) || !valid_type(y_type)) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown element type");
+    if (t == 0 || t > TQF_HIP_GROUPED_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "t must be in 1..4096");
+    if (top_k == 0 || top_k > TQF_HIP_ROUTE_MAX_TOP_K) return fail(ctx, TQF_HIP_ERR_INVALID, "top_k must be in 1..16");
+    const size_t xb = type_bytes(x_type), yb = type_bytes(y_type);
+    if (!aligned_to(d_x, xb) || !aligned_to(d_y, yb) || !aligned_to(d_ids, 2) || !aligned_to(d_w, 4) || !aligned_to(d_status, 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "buffers must be aligned to their elements");
+    const size_t n = (size_t)t * experts->hidden;
+    if (overlap(d_x, n * xb, d_y, n * yb)) return fail(ctx, TQF_HIP_ERR_INVALID, "x and y must not overlap");
+    const F8ExpertsDev ex{experts->d_mats, experts->n_experts, experts->hidden, experts->width};
+    if (int32_t rc = ensure_f8_scratch(ctx, f8_experts_scratch_bytes(ex, t, top_k))) return rc;
+    Prof p(ctx);
+    const hipError_t e = launch_f8_experts(ctx->stream, ex, d_x, x_type, t, d_ids, d_w, top_k, d_y, y_type, d_status, ctx->d_f8);
+    if (e != hipSuccess) return hip_fail(ctx, "F8 experts launch", e);
+    p.end(TQF_HIP_KERNEL_F8_EXPERTS, 0.0, 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_router_logits_device(tqf_hip_ctx *ctx, const tqf_hip_tensor *router, const void *d_x, int32_t x_type,
+                                                uint32_t t, uint32_t n_experts, uint32_t hidden, float *d_logits) {
+    TQF_ENTER(ctx);
+    if (!router || !router->data || !d_x || !d_logits) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (!valid_type(x_type)) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown element type");
+    if (t == 0 || t > TQF_HIP_F8_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "t must be in 1..65536");
+    if (n_experts == 0 || n_experts > TQF_HIP_ROUTE_MAX_EXPERTS)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "n_experts must be in 1..1024");
+    if (hidden == 0 || hidden > kF8MaxCols) return fail(ctx, TQF_HIP_ERR_INVALID, "hidden must be in 1..65536");
+    if (router->count != (size_t)n_experts * hidden) return fail(ctx, TQF_HIP_ERR_INVALID, "router must be f32 [n_experts x hidden]");
+    const size_t xb = type_bytes(x_type);
+    if (!aligned_to(d_x, xb) || !aligned_to(d_logits, 4)) return fail(ctx, TQF_HIP_ERR_INVALID, "buffers must be aligned to their elements");
+    if (overlap(d_x, (size_t)t * hidden * xb, d_logits, (size_t)t * n_experts * 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "x and logits must not overlap");
+    Prof p(ctx);
+    const hipError_t e = launch_router_logits(ctx->stream, router->data, d_x, x_type, t, n_experts, hidden, d_logits);
+    if (e != hipSuccess) return hip_fail(ctx, "router product launch", e);
+    p.end(TQF_HIP_KERNEL_ROUTER, (double)t * hidden * xb + 4.0 * n_experts * ((double)hidden + t), 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_route_tokens_device(tqf_hip_ctx *ctx, const void *d_logits, int32_t logits_type, uint32_t t,
+                                               uint32_t n_experts, const float *d_bias, const tqf_hip_route_options *options,
+                                               uint16_t *d_ids, float *d_w, int32_t *d_status) {
+    TQF_ENTER(ctx);
+    if (!d_logits || !options || !d_ids || !d_w) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    const tqf_hip_route_options &o = *options;
+    if (!valid_type(logits_type)) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown element type");
+    if (t == 0 || t > TQF_HIP_F8_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "t must be in 1..65536");
+    if (n_experts == 0 || n_experts > TQF_HIP_ROUTE_MAX_EXPERTS)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "n_experts must be in 1..1024");
+    if (o.score != TQF_HIP_SCORE_SOFTMAX && o.score != TQF_HIP_SCORE_SIGMOID) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown score");
+    if (o.n_groups == 0 || o.n_groups > 64 || n_experts % o.n_groups)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "n_groups must be in 1..64 and divide n_experts");
+    if (o.top_groups == 0 || o.top_groups > o.n_groups) return fail(ctx, TQF_HIP_ERR_INVALID, "top_groups must be in 1..n_groups");
+    if (o.group_best != 1 && o.group_best != 2) return fail(ctx, TQF_HIP_ERR_INVALID, "group_best must be 1 or 2");
+    if (o.top_k == 0 || o.top_k > TQF_HIP_ROUTE_MAX_TOP_K || o.top_k > o.top_groups * (n_experts / o.n_groups))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "top_k must be in 1..16 and at most the experts of the groups kept");
+    if (!std::isfinite(o.scale)) return fail(ctx, TQF_HIP_ERR_INVALID, "scale must be finite");
+    if (!aligned_to(d_logits, type_bytes(logits_type)) || !aligned_to(d_bias, 4) || !aligned_to(d_ids, 2) || !aligned_to(d_w, 4) ||
+        !aligned_to(d_status, 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "buffers must be aligned to their elements");
+    const size_t lb = (size_t)t * n_experts * type_bytes(logits_type), n = (size_t)t * o.top_k;
+    if (overlap(d_logits, lb, d_ids, n * 2) || overlap(d_logits, lb, d_w, n * 4) || overlap(d_ids, n * 2, d_w, n * 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "logits, ids and weights must not overlap");
+    Prof p(ctx);
+    const hipError_t e = launch_route_tokens(ctx->stream, d_logits, logits_type, t, n_experts, d_bias, o, d_ids, d_w, d_status);
+    if (e != hipSuccess) return hip_fail(ctx, "route kernel launch", e);
+    p.end(TQF_HIP_KERNEL_ROUTER, (double)lb + 6.0 * n + (d_bias ? 4.0 * n_experts : 0.0), 0, nullptr);
     return TQF_HIP_OK;
 }

@@ -1,0 +1,1036 @@
+// tqf_f8.hip -- products of e4m3 matrices with block-128 scales (gfx950).
+//
+//   f8_matmul   Y[t][n] = sum_b s_x[t][b] s_w[n / 128][b] sum_{k in b} q_x[t][k] q_w[n][k]
+//   f8_experts  y[t] = sum_k w[t][k] D_e(silu(G_e x_t) * U_e x_t),  e = ids[t][k]
+// with G, U, D products of the first kind, x and h quantised row by row in
+// blocks b of 128 (tqf_f8.h has the format and the device layout).
+//
+// Weights are the A operand (16 or 32 of their rows), activation rows the B
+// operand, so a lane's results are consecutive outputs of one activation row
+// and a block's scale is one number per lane: d = the block's product from a
+// zero start, acc = fma(d, s_x s_w, acc) in f32.
+//
+// How exact the block's product is.  The fp8 matrix instructions align the
+// products of a block to the largest before they add: against 64 bits, a
+// block of normal values is 1.3e-5 off (relative, 2-norm), 3.9e-5 with rows
+// that span 2^8; the 32-column instruction is no better.  bf16 results are
+// rounded at 2^-9 = 2e-3, so they are made of these; f32 results, and every
+// small call, widen the values to bf16 (exact) for the bf16 instructions,
+// whose products of e4m3 values came out exact in the same test.
+#include <hip/hip_runtime.h>
+
+#include "tqf_f8.h"
+
+namespace tqf {
+
+namespace {
+
+constexpr int kKB = 4096;  // bytes of a tile's K block
+
+// ---- layout ------------------------------------------------------------------
+__global__ __launch_bounds__(256) void f8_repack_kernel(const uint8_t *__restrict__ q, const float *__restrict__ scales,
+                                                        F8Shape d, uint8_t *__restrict__ out) {
+    const size_t chunks = f8_tile_bytes(d) / 16, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t ns = (size_t)(d.tiles / 4) * d.kb;
+    if (i < ns) reinterpret_cast<float *>(out + f8_tile_bytes(d))[i] = scales[i];
+    if (i >= chunks) return;
+    const uint32_t in = (uint32_t)(i & 255);  // chunk within the K block: 32 rows to each 16 columns
+    const size_t blk = i >> 8, tile = blk / d.kb;
+    const uint32_t kb = (uint32_t)(blk - tile * d.kb);
+    const size_t row = tile * 32 + (in & 31);
+    const uint32_t col = kb * 128 + (in >> 5) * 16;
+    u32x4 v = {0, 0, 0, 0};
+    if (row < d.rows && col < d.cols) {
+        const uint8_t *src = q + row * d.cols + col;
+        const uint32_t n = d.cols - col < 16 ? d.cols - col : 16;
+        if (n == 16 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+            v = *reinterpret_cast<const u32x4 *>(src);
+        } else {
+            for (uint32_t j = 0; j < n; ++j) v[j >> 2] |= (uint32_t)src[j] << (8 * (j & 3));
+        }
+    }
+    reinterpret_cast<u32x4 *>(out)[i] = v;
+}
+
+// ---- quantisation of rows ------------------------------------------------------
+// Largest magnitude over the eight lanes that hold a block of 128.
+__device__ __forceinline__ float amax8(float a) {
+    a = fmaxf(a, dpp_f<kDppXor1>(a));
+    a = fmaxf(a, dpp_f<kDppXor2>(a));
+    return fmaxf(a, dpp_f<kDppHalfMirror>(a));
+}
+// Sixteen values of a block whose eight lanes are neighbours -> their bytes;
+// *scale receives the block's.
+__device__ __forceinline__ u32x4 quantize16(const float (&v)[16], float *scale) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a = fmaxf(a, fabsf(v[i]));
+    const F8Factors f = f8_factors(amax8(a));
+    *scale = f.scale;
+    u32x4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        q[i] = f8_pack4(v[4 * i] * f.inv, v[4 * i + 1] * f.inv, v[4 * i + 2] * f.inv, v[4 * i + 3] * f.inv);
+    return q;
+}
+
+// Chunk i of x [t x cols]: the 16 columns i % (8 kb) of row i / (8 kb).  Eight
+// lanes share a block, so all of an aligned group take part or none.
+template <typename XT>
+__device__ __forceinline__ void quantize_chunk(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb, bool vec,
+                                               uint32_t i, uint8_t *__restrict__ xq, float *__restrict__ xs) {
+    const uint32_t row = i / (8 * kb), c = i - row * 8 * kb, k = c * 16;
+    const int valid = k < cols ? (int)(cols - k) : 0;
+    float v[16], s;
+    load_row<16>(x + (size_t)row * cols + k, valid, vec, v);
+    const u32x4 q = quantize16(v, &s);
+    reinterpret_cast<u32x4 *>(xq)[i] = q;
+    if ((c & 7) == 0) xs[(size_t)(c >> 3) * t + row] = s;
+}
+template <typename XT>
+__global__ __launch_bounds__(256) void f8_quantize_kernel(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb,
+                                                          uint8_t *__restrict__ xq, float *__restrict__ xs) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= t * kb * 8) return;
+    quantize_chunk(x, t, cols, kb, rows_aligned(x, cols, sizeof(XT)), i, xq, xs);
+}
+
+// ---- matrix instructions ---------------------------------------------------------
+// A policy says how a wavefront takes a K block: M weight rows by M activation
+// rows to an accumulator D; `Raw` what a lane loads of an operand, `Op` what
+// the instructions take.  a_off(l, sub, j): byte of load j in the K block of
+// the tile; b_row / b_chunk: the activation row and the 16-column chunk of load
+// j; row(l, g): the first of the four weight rows in D's group g.
+struct Fp8x32 {  // v_mfma_f32_32x32x64_f8f6f4: two to a block
+    static constexpr int M = 32, kLoads = 4, kGroups = 4;
+    typedef f32x16 D;
+    struct Raw {
+        u32x4 q[4];
+    };
+    typedef Raw Op;
+    static __device__ __forceinline__ uint32_t a_off(int l, int, int j) { return j * 1024 + l * 16; }
+    static __device__ __forceinline__ int b_row(int l) { return l & 31; }
+    static __device__ __forceinline__ int b_chunk(int l, int j) { return 2 * j + (l >> 5); }
+    static __device__ __forceinline__ int row(int l, int g) { return 8 * g + 4 * (l >> 5); }
+    static __device__ __forceinline__ const Op &op(const Raw &r) { return r; }
+    static __device__ __forceinline__ i32x8 pair(u32x4 a, u32x4 b) {
+        return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+    }
+    static __device__ __forceinline__ D mma(const Op &a, const Op &b) {
+        D d = {};
+        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(a.q[0], a.q[1]), pair(b.q[0], b.q[1]), d, 0, 0, 0, 0, 0, 0);
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(a.q[2], a.q[3]), pair(b.q[2], b.q[3]), d, 0, 0, 0, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float across(float a) { return fmaxf(a, __shfl_xor(a, 32)); }
+};
+struct Fp8x16 {  // v_mfma_f32_16x16x128_f8f6f4: one to a block
+    static constexpr int M = 16, kLoads = 2, kGroups = 1;
+    typedef f32x4 D;
+    struct Raw {
+        u32x4 q[2];
+    };
+    typedef Raw Op;
+    static __device__ __forceinline__ uint32_t a_off(int l, int sub, int j) {
+        return (4 * j + (l >> 4)) * 512 + sub * 256 + (l & 15) * 16;
+    }
+    static __device__ __forceinline__ int b_row(int l) { return l & 15; }
+    static __device__ __forceinline__ int b_chunk(int l, int j) { return 4 * j + (l >> 4); }
+    static __device__ __forceinline__ int row(int l, int) { return 4 * (l >> 4); }
+    static __device__ __forceinline__ const Op &op(const Raw &r) { return r; }
+    static __device__ __forceinline__ D mma(const Op &a, const Op &b) {
+        const D z = {0.0f, 0.0f, 0.0f, 0.0f};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Fp8x32::pair(a.q[0], a.q[1]), Fp8x32::pair(b.q[0], b.q[1]), z, 0,
+                                                                0, 0, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float across(float a) {
+        a = fmaxf(a, __shfl_xor(a, 16));
+        return fmaxf(a, __shfl_xor(a, 32));
+    }
+};
+struct Bf16x16 : Fp8x16 {  // the same tiles, widened to bf16: v_mfma_f32_16x16x32_bf16, four to a block
+    struct Op {
+        bf16x8 v[4];
+    };
+    static __device__ __forceinline__ Op op(const Raw &r) {
+        return Op{{f8_widen(r.q[0][0], r.q[0][1]), f8_widen(r.q[0][2], r.q[0][3]), f8_widen(r.q[1][0], r.q[1][1]),
+                   f8_widen(r.q[1][2], r.q[1][3])}};
+    }
+    static __device__ __forceinline__ D mma(const Op &a, const Op &b) {
+        D d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], d, 0, 0, 0);
+        return d;
+    }
+};
+
+// ---- copies to LDS -----------------------------------------------------------------
+typedef __amdgpu_buffer_rsrc_t Desc;  // loads past `bytes` return zero
+__device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+}
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ void copy16(Desc d, uint32_t voff, uint32_t soff, void *lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, soff, 0, 0);
+}
+// This wavefront's loads (those to LDS among them) and LDS reads are done, then
+// the workgroup's.
+__device__ __forceinline__ void publish() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ---- the tiled product -----------------------------------------------------------
+// A workgroup of four wavefronts: CT * M activation rows by 4 RT M weight rows.
+// Each wavefront streams its own weight rows straight to registers (nothing
+// else needs them); the activation rows of a K block are copied to LDS by all
+// four and read by each, [row][8 chunks] with chunk c of row r in slot
+// c ^ swizzle(r): the copies read whole 128-byte lines, and both the 8 and the
+// 16 lanes that LDS serves together find their chunks in different banks.
+// Two stages: a block's loads are issued when the one before is computed.
+__device__ __forceinline__ int swizzle(int r) { return (r ^ (r >> 3 & 1)) & 7; }  // by r % 16
+
+enum Mode { kDense, kGateUp, kDown };
+constexpr int kTileWaves = 4;
+
+struct TiledArgs {
+    const uint8_t *mat;              // kDense
+    const uint8_t *const *mats;      // experts
+    F8Shape d;                       // of the matrices
+    const uint8_t *xq;               // activation rows [xrows][kb 128]
+    const float *xs;                 // [kb][xrows]
+    uint32_t xrows;
+    void *y;                         // kDense: [t x rows]
+    const uint2 *tiles;              // experts: {first position, e | rows << 16}
+    const int32_t *n_tiles;
+    const int32_t *row_of_pos;       // kGateUp: the activation row of a position
+    uint8_t *hq;                     // kGateUp: h [positions][hkb 128] and its scales [hkb][hrows]
+    float *hs;
+    uint32_t hkb, hrows;
+    float *out;                      // kDown: [positions][rows]
+};
+
+template <class P, int RT, int CT, int MODE, typename YT>
+__global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8_tiled_kernel(TiledArgs a) {
+    constexpr int M = P::M, kRows = CT * M;       // activation rows of the workgroup
+    constexpr int kCopies = kRows / 32;           // copies of 1 KiB each wavefront makes for a block
+    constexpr int kG = P::kGroups;
+    static_assert(kRows % 32 == 0 || kRows == 16, "copies are dealt to four wavefronts");
+    __shared__ __attribute__((aligned(16))) uint8_t stage[2][kRows * 128];
+    __shared__ float s_max[kTileWaves][MODE == kGateUp ? kRows : 1];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    const uint32_t kb_n = a.d.kb, kp = kb_n * 128;
+
+    // which activation rows and weights
+    uint32_t first, rows, e = 0, rblock;
+    if constexpr (MODE == kDense) {
+        // neighbouring workgroups run on different XCDs: deal each XCD a
+        // contiguous share of the order (row blocks fastest), so that the ones
+        // that read the same rows of x share an L2
+        const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * M - 1) / (4 * RT * M), all = gridDim.x;
+        const uint32_t per = (all + 7) / 8, id = (blockIdx.x % 8) * per + blockIdx.x / 8;
+        if (blockIdx.x / 8 >= per || id >= all) return;
+        first = id / rbs * kRows;
+        rblock = id % rbs;
+        if (first >= a.xrows) return;
+        rows = a.xrows - first < kRows ? a.xrows - first : kRows;
+    } else {
+        if ((int)blockIdx.y >= *a.n_tiles) return;
+        const uint2 t = a.tiles[blockIdx.y];
+        first = t.x;
+        e = t.y & 0xFFFFu;
+        rows = t.y >> 16;
+        rblock = blockIdx.x;
+    }
+    // this wavefront's row tiles: bases and scales (a tile never spans two
+    // scale blocks; tiles past the matrix read its last and store nothing)
+    const uint8_t *base[RT];
+    const float *ws[RT];
+    uint32_t wrow[RT];
+    int sub[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const uint8_t *mat;
+        if constexpr (MODE == kDense) {
+            mat = a.mat;
+            wrow[r] = ((rblock * kTileWaves + wave) * RT + r) * M;
+        } else if constexpr (MODE == kGateUp) {
+            mat = a.mats[(size_t)e * 3 + (r < RT / 2 ? 0 : 1)];
+            wrow[r] = ((rblock * kTileWaves + wave) * (RT / 2) + r % (RT / 2)) * M;
+        } else {
+            mat = a.mats[(size_t)e * 3 + 2];
+            wrow[r] = ((rblock * kTileWaves + wave) * RT + r) * M;
+        }
+        uint32_t tile = wrow[r] / 32;
+        if (tile >= a.d.tiles) tile = a.d.tiles - 1;
+        sub[r] = (int)(wrow[r] / 16 & 1);
+        base[r] = mat + (size_t)tile * kb_n * kKB;
+        ws[r] = reinterpret_cast<const float *>(mat + f8_tile_bytes(a.d)) + (size_t)(tile / 4) * kb_n;
+    }
+    // activation rows: what this lane copies, and whose scale it applies
+    auto source_row = [&](uint32_t local) -> uint32_t {
+        const uint32_t p = first + (local < rows ? local : rows - 1);
+        if constexpr (MODE == kGateUp) return (uint32_t)a.row_of_pos[p];
+        else return p;
+    };
+    uint32_t xbase = 0;
+    if constexpr (MODE != kGateUp) xbase = first;
+    const Desc dx = make_desc(a.xq + (size_t)xbase * kp, (uint32_t)(((size_t)a.xrows - xbase) * kp < 0xFFFFFFFFull
+                                                                       ? ((size_t)a.xrows - xbase) * kp : 0xFFFFFFFFull));
+    constexpr int kMine = kCopies ? kCopies : 1;
+    const bool copies = kCopies > 0 || wave < 2;  // 16 rows: two wavefronts
+    uint32_t voff[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+        const int local = (wave * kMine + j) * 8 + l / 8;
+        voff[j] = copies ? (source_row((uint32_t)local) - xbase) * kp + (uint32_t)(((l & 7) ^ swizzle(local)) * 16) : 0;
+    }
+    uint32_t srow[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) srow[c] = source_row((uint32_t)(c * M + P::b_row(l)));
+    uint32_t boff[P::kLoads];
+#pragma unroll
+    for (int j = 0; j < P::kLoads; ++j) boff[j] = P::b_row(l) * 128 + ((P::b_chunk(l, j) ^ swizzle(P::b_row(l))) * 16);
+
+    typename P::D acc[RT][CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[r][c] = typename P::D{};
+
+    struct Block {
+        typename P::Raw w[RT];
+        float s[CT];
+    };
+    auto issue = [&](uint32_t kb, Block &b) {
+        if (copies) {
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) copy16(dx, voff[j], kb * 128, &stage[kb & 1][(wave * kMine + j) * 1024]);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int j = 0; j < P::kLoads; ++j)
+                b.w[r].q[j] = *reinterpret_cast<const u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) b.s[c] = a.xs[(size_t)kb * a.xrows + srow[c]];
+    };
+    auto compute = [&](uint32_t kb, const Block &b) {
+        const uint8_t *st = stage[kb & 1];
+        float sw[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) sw[r] = ws[r][kb];
+        typename P::Op aw[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) aw[r] = P::op(b.w[r]);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            if (MODE != kDense && c > 0 && (uint32_t)(c * M) >= rows) continue;  // no rows of this tile here
+            typename P::Raw raw;
+#pragma unroll
+            for (int j = 0; j < P::kLoads; ++j) raw.q[j] = *reinterpret_cast<const u32x4 *>(st + c * M * 128 + boff[j]);
+            const typename P::Op bx = P::op(raw);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const typename P::D d = P::mma(aw[r], bx);
+                const float s = b.s[c] * sw[r];
+#pragma unroll
+                for (int i = 0; i < 4 * kG; ++i) acc[r][c][i] = __builtin_fmaf(d[i], s, acc[r][c][i]);
+            }
+        }
+    };
+    Block b0, b1;
+    issue(0, b0);
+    for (uint32_t kb = 0; kb < kb_n; kb += 2) {
+        publish();
+        if (kb + 1 < kb_n) issue(kb + 1, b1);
+        compute(kb, b0);
+        if (kb + 1 >= kb_n) break;
+        publish();
+        if (kb + 2 < kb_n) issue(kb + 2, b0);
+        compute(kb + 1, b1);
+    }
+
+    if constexpr (MODE == kGateUp) {
+        // h = silu(g) u, quantised: the workgroup's 128 columns are one block
+        constexpr int HT = RT / 2;
+        float h[HT][CT][4 * kG];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            float m = 0.0f;
+#pragma unroll
+            for (int r = 0; r < HT; ++r)
+#pragma unroll
+                for (int i = 0; i < 4 * kG; ++i) {
+                    const float g = acc[r][c][i];
+                    h[r][c][i] = g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * acc[r + HT][c][i];
+                    m = fmaxf(m, fabsf(h[r][c][i]));
+                }
+            m = P::across(m);
+            if (l < M) s_max[wave][c * M + l] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const int local = c * M + P::b_row(l);
+            const float m = fmaxf(fmaxf(s_max[0][local], s_max[1][local]), fmaxf(s_max[2][local], s_max[3][local]));
+            const F8Factors f = f8_factors(m);
+            if ((uint32_t)local >= rows) continue;
+            const uint32_t pos = first + local;
+            if (wave == 0 && l < M) a.hs[(size_t)rblock * a.hrows + pos] = f.scale;
+#pragma unroll
+            for (int r = 0; r < HT; ++r)
+#pragma unroll
+                for (int g = 0; g < kG; ++g) {
+                    const float *v = &h[r][c][4 * g];
+                    *reinterpret_cast<uint32_t *>(a.hq + (size_t)pos * a.hkb * 128 + wrow[r] + P::row(l, g)) =
+                        f8_pack4(v[0] * f.inv, v[1] * f.inv, v[2] * f.inv, v[3] * f.inv);
+                }
+        }
+    } else {
+        YT *y = MODE == kDense ? static_cast<YT *>(a.y) : reinterpret_cast<YT *>(a.out);
+        const uint32_t n = a.d.rows;
+        const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const uint32_t local = (uint32_t)(c * M + P::b_row(l));
+            if (local >= rows) continue;
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int g = 0; g < kG; ++g) {
+                    const uint32_t col = wrow[r] + P::row(l, g);
+                    if (col >= n) continue;
+                    const f32x4 v = {acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
+                    store4(y + (size_t)(first + local) * n + col, (int)(n - col), vec, v);
+                }
+        }
+    }
+}
+
+// ---- few rows: the weight stream ----------------------------------------------
+// Up to 16 rows against one matrix in one launch.  Every workgroup quantises
+// the rows into LDS (they are few), then its wavefronts walk the weights: with
+// SPLIT, the eight wavefronts share a tile's K blocks and add their parts in
+// LDS in wavefront order; without, each walks tiles of its own.  SUB: 16-row
+// subtiles of a tile that a wavefront takes.
+constexpr int kRowsMax = 16;
+constexpr int kRowsWaves = 8;
+constexpr int kRowsThreads = kRowsWaves * 64;
+struct RowsLayout {
+    uint32_t stride;  // bytes of a quantised row: 16 more than its values, so that rows start in different banks
+    uint32_t scales, red, total;
+};
+__host__ __device__ inline RowsLayout rows_layout(uint32_t t, uint32_t kb) {
+    RowsLayout L;
+    L.stride = kb * 128 + 16;
+    L.scales = t * L.stride;
+    L.red = (L.scales + t * kb * 4 + 15) & ~15u;
+    L.total = L.red + kRowsWaves * 2 * 1024;
+    return L;
+}
+constexpr uint32_t kRowsLds = 128u << 10;
+
+template <int SUB, bool SPLIT, typename XT, typename YT>
+__global__ __launch_bounds__(kRowsThreads) void f8_rows_kernel(const uint8_t *__restrict__ mat, F8Shape d,
+                                                               const XT *__restrict__ x, uint32_t t, YT *__restrict__ y) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    typedef Bf16x16 P;
+    const RowsLayout L = rows_layout(t, d.kb);
+    float *xs = reinterpret_cast<float *>(lds + L.scales);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    const bool vec = rows_aligned(x, d.cols, sizeof(XT));
+    for (uint32_t i = tid; i < t * d.kb * 8; i += kRowsThreads) {
+        const uint32_t row = i / (8 * d.kb), c = i - row * 8 * d.kb, k = c * 16;
+        float v[16], s;
+        load_row<16>(x + (size_t)row * d.cols + k, k < d.cols ? (int)(d.cols - k) : 0, vec, v);
+        *reinterpret_cast<u32x4 *>(lds + row * L.stride + k) = quantize16(v, &s);
+        if ((c & 7) == 0) xs[row * d.kb + (c >> 3)] = s;
+    }
+    __syncthreads();
+
+    const uint32_t token = (uint32_t)P::b_row(l) < t ? (uint32_t)P::b_row(l) : t - 1;
+    const uint8_t *bx = lds + token * L.stride + (l >> 4) * 16;
+    const float *sx = xs + token * d.kb;
+    const float *scales = reinterpret_cast<const float *>(mat + f8_tile_bytes(d));
+    const uint32_t units = (d.rows + 16 * SUB - 1) / (16 * SUB);
+    const bool yvec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)d.rows * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
+    const uint32_t u0 = SPLIT ? blockIdx.x : blockIdx.x * kRowsWaves + wave, ustep = SPLIT ? gridDim.x : gridDim.x * kRowsWaves;
+    for (uint32_t u = u0; u < units; u += ustep) {
+        const uint32_t row0 = u * 16 * SUB, tile = row0 / 32;
+        const uint8_t *w = mat + (size_t)tile * d.kb * kKB;
+        const float *ws = scales + (size_t)(tile / 4) * d.kb;
+        const int s0 = (int)(row0 / 16 & 1);
+        f32x4 acc[SUB] = {};
+        constexpr int kAhead = 4;  // K blocks in flight
+        for (uint32_t b0 = SPLIT ? wave : 0; b0 < d.kb; b0 += kAhead * (SPLIT ? kRowsWaves : 1)) {
+            typename P::Raw raw[kAhead][SUB];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const uint32_t kb = b0 + i * (SPLIT ? kRowsWaves : 1);
+                if (kb >= d.kb) break;
+#pragma unroll
+                for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        raw[i][s].q[j] = *reinterpret_cast<const u32x4 *>(w + (size_t)kb * kKB + P::a_off(l, s0 + s, j));
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const uint32_t kb = b0 + i * (SPLIT ? kRowsWaves : 1);
+                if (kb >= d.kb) break;
+                typename P::Raw rb;
+                rb.q[0] = *reinterpret_cast<const u32x4 *>(bx + kb * 128);
+                rb.q[1] = *reinterpret_cast<const u32x4 *>(bx + kb * 128 + 64);
+                const typename P::Op b = P::op(rb);
+                const float sc = sx[kb] * ws[kb];
+#pragma unroll
+                for (int s = 0; s < SUB; ++s) {
+                    const f32x4 p = P::mma(P::op(raw[i][s]), b);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[s][v] = __builtin_fmaf(p[v], sc, acc[s][v]);
+                }
+            }
+        }
+        if constexpr (SPLIT) {
+            f32x4 *red = reinterpret_cast<f32x4 *>(lds + L.red);
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) red[(wave * SUB + s) * 64 + l] = acc[s];
+            __syncthreads();
+            if (wave < SUB) {
+                f32x4 v = red[wave * 64 + l];
+#pragma unroll
+                for (int i = 1; i < kRowsWaves; ++i) v += red[(i * SUB + wave) * 64 + l];
+                const uint32_t col = row0 + wave * 16 + P::row(l, 0);
+                if ((uint32_t)P::b_row(l) < t && col < d.rows)
+                    store4(y + (size_t)P::b_row(l) * d.rows + col, (int)(d.rows - col), yvec, v);
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+                const uint32_t col = row0 + s * 16 + P::row(l, 0);
+                if ((uint32_t)P::b_row(l) < t && col < d.rows)
+                    store4(y + (size_t)P::b_row(l) * d.rows + col, (int)(d.rows - col), yvec, acc[s]);
+            }
+        }
+    }
+}
+
+int cu_count() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+    return n > 0 ? n : 256;
+}
+
+template <typename XT, typename YT>
+hipError_t launch_rows(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT *x, uint32_t t, YT *y) {
+    const uint32_t lds = rows_layout(t, d.kb).total, cus = (uint32_t)cu_count();
+    const uint32_t per_cu = lds <= (72u << 10) ? 2 : 1;  // workgroups that fit a compute unit's LDS
+    const uint32_t tiles = (d.rows + 31) / 32, slots = cus * per_cu;
+    auto launch = [&](auto kernel, uint32_t grid) {
+        // more than 64 KiB of LDS is asked for by name
+        if (lds > (64u << 10)) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<grid, kRowsThreads, lds, s>>>(mat, d, x, t, y);
+        return hipGetLastError();
+    };
+    if (tiles >= slots * kRowsWaves) return launch(f8_rows_kernel<2, false, XT, YT>, slots);
+    if (tiles >= cus) return launch(f8_rows_kernel<2, true, XT, YT>, tiles < slots ? tiles : slots);
+    const uint32_t units = (d.rows + 15) / 16;
+    return launch(f8_rows_kernel<1, true, XT, YT>, units < slots ? units : slots);
+}
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+bool rows_path(const F8Shape &d, uint32_t t) { return t <= kRowsMax && rows_layout(t, d.kb).total <= kRowsLds; }
+
+template <typename XT>
+hipError_t quantize(hipStream_t s, const XT *x, uint32_t t, uint32_t cols, uint32_t kb, uint8_t *xq, float *xs) {
+    f8_quantize_kernel<<<(t * kb * 8 + 255) / 256, 256, 0, s>>>(x, t, cols, kb, xq, xs);
+    return hipGetLastError();
+}
+
+template <class P, int RT, int CT, typename YT>
+hipError_t launch_dense(hipStream_t s, const TiledArgs &a) {
+    constexpr uint32_t kM = P::M;
+    const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * kM - 1) / (4 * RT * kM), tbs = (a.xrows + CT * kM - 1) / (CT * kM);
+    f8_tiled_kernel<P, RT, CT, kDense, YT><<<(rbs * tbs + 7) / 8 * 8, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <typename XT, typename YT>
+hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT *x, uint32_t t, YT *y, void *scratch) {
+    if (rows_path(d, t)) return launch_rows(s, mat, d, x, t, y);
+    uint8_t *xq = static_cast<uint8_t *>(scratch);
+    float *xs = reinterpret_cast<float *>(xq + align256((size_t)t * d.kb * 128));
+    hipError_t e = quantize(s, x, t, d.cols, d.kb, xq, xs);
+    if (e != hipSuccess) return e;
+    TiledArgs a{};
+    a.mat = mat;
+    a.d = d;
+    a.xq = xq;
+    a.xs = xs;
+    a.xrows = t;
+    a.y = y;
+    if constexpr (sizeof(YT) == 4) {
+        return t <= 32 ? launch_dense<Bf16x16, 2, 2, YT>(s, a) : launch_dense<Bf16x16, 2, 4, YT>(s, a);
+    } else {
+        if (t <= 32) return launch_dense<Fp8x32, 1, 1, YT>(s, a);
+        if (t <= 64) return launch_dense<Fp8x32, 2, 2, YT>(s, a);
+        return launch_dense<Fp8x32, 2, 4, YT>(s, a);
+    }
+}
+
+// ---- the routed experts ------------------------------------------------------
+// Many pairs: `plan` sorts the (token, k) pairs by expert and cuts them into
+// tiles of one expert each (and quantises x in the workgroups after its own);
+// gate_up and down are the tiled product over those tiles; combine adds a
+// token's weighted outputs in the order of its routes.  Few pairs: two launches
+// that take every pair by itself.
+struct ExpertsArgs {
+    const uint16_t *ids;  // [t x top_k]
+    const float *w;
+    uint32_t t, top_k, n_experts;
+    int32_t *status;
+};
+constexpr int kPlanThreads = 1024;
+constexpr uint32_t kMaxF8Experts = 1024;
+
+// Positions of the pairs p = t top_k + k, by expert.  Every workgroup counts all
+// ids (in LDS: those of the pairs before its own 1024, and all of them) and so
+// needs nothing from the others; within an expert its own pairs take places in
+// the order in which their LDS atomics arrive, which no result depends on: a
+// pair's column of a product is computed alike wherever it stands.  A tile is
+// {first position, e | rows << 16} with at most tile_m rows, an expert's tiles
+// of equal size.  An id that names no expert makes *n_tiles -1: the kernels
+// after this one then do nothing.
+template <typename XT>
+__global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, uint32_t tile_m, int32_t *__restrict__ pos_of_pair,
+                                                               int32_t *__restrict__ row_of_pos, uint2 *__restrict__ tiles,
+                                                               int32_t *__restrict__ n_tiles, const XT *__restrict__ x,
+                                                               uint32_t hidden, uint32_t kb, uint8_t *__restrict__ xq,
+                                                               float *__restrict__ xs) {
+    const uint32_t pairs = a.t * a.top_k, plan_blocks = (pairs + kPlanThreads - 1) / kPlanThreads;
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    if (blockIdx.x >= plan_blocks) {
+        const uint32_t i = (blockIdx.x - plan_blocks) * kPlanThreads + tid;
+        if (i < a.t * kb * 8) quantize_chunk(x, a.t, hidden, kb, rows_aligned(x, hidden, sizeof(XT)), i, xq, xs);
+        return;
+    }
+    __shared__ int32_t before[kMaxF8Experts], total[kMaxF8Experts], place[kMaxF8Experts];
+    __shared__ int32_t s_pairs[kPlanThreads / 64], s_tiles[kPlanThreads / 64];
+    __shared__ int32_t s_bad;
+    before[tid] = total[tid] = 0;
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    const uint32_t b0 = blockIdx.x * kPlanThreads;
+    for (uint32_t r = tid; r < pairs; r += 8 * kPlanThreads) {
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = r + i * kPlanThreads < pairs ? a.ids[r + i * kPlanThreads] : TQF_HIP_NO_EXPERT;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (e[i] == TQF_HIP_NO_EXPERT) continue;
+            if (e[i] >= a.n_experts) {
+                s_bad = 1;
+                continue;
+            }
+            atomicAdd(&total[e[i]], 1);
+            if (r + i * kPlanThreads < b0) atomicAdd(&before[e[i]], 1);
+        }
+    }
+    __syncthreads();
+    if (s_bad) {
+        if (blockIdx.x == 0 && tid == 0) {
+            *n_tiles = -1;
+            if (a.status) *a.status = TQF_HIP_ERR_INVALID;
+        }
+        return;
+    }
+    // exclusive scans of pairs and tiles over the experts, one to a thread
+    const int c = total[tid], n = (c + (int)tile_m - 1) / (int)tile_m;
+    int sc = c, sn = n;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int u = __shfl_up(sc, o), v = __shfl_up(sn, o);
+        if (lane >= o) {
+            sc += u;
+            sn += v;
+        }
+    }
+    if (lane == 63) {
+        s_pairs[wave] = sc;
+        s_tiles[wave] = sn;
+    }
+    __syncthreads();
+    int base = sc - c, tbase = sn - n;
+    for (int i = 0; i < wave; ++i) {
+        base += s_pairs[i];
+        tbase += s_tiles[i];
+    }
+    place[tid] = base + before[tid];
+    if (blockIdx.x == 0) {
+        const int step = n ? (c + n - 1) / n : 0;
+        for (int i = 0; i < n; ++i) {
+            const int rows = c - i * step < step ? c - i * step : step;
+            tiles[tbase + i] = make_uint2((uint32_t)(base + i * step), (uint32_t)tid | ((uint32_t)rows << 16));
+        }
+        if (tid == kPlanThreads - 1) *n_tiles = tbase + n;
+    }
+    __syncthreads();
+    const uint32_t p = b0 + tid;
+    if (p < pairs) {
+        const uint32_t e = a.ids[p];
+        int pos = -1;
+        if (e != TQF_HIP_NO_EXPERT) {
+            pos = atomicAdd(&place[e], 1);
+            row_of_pos[pos] = (int32_t)(p / a.top_k);
+        }
+        pos_of_pair[p] = pos;
+    }
+}
+
+template <typename YT>
+__global__ __launch_bounds__(256) void f8_combine_kernel(ExpertsArgs a, const int32_t *__restrict__ pos_of_pair,
+                                                         const int32_t *__restrict__ n_tiles, const float *__restrict__ out,
+                                                         uint32_t hidden, YT *__restrict__ y) {
+    if (*n_tiles < 0) return;
+    const uint32_t t = blockIdx.y, h = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (h >= hidden) return;
+    const int valid = (int)(hidden - h);
+    const bool vec = (hidden & 3) == 0;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t k = 0; k < a.top_k; ++k) {
+        const int pos = pos_of_pair[t * a.top_k + k];
+        if (pos < 0) continue;
+        const float w = a.w[t * a.top_k + k];
+        const float *src = out + (size_t)pos * hidden + h;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vec) {
+            o = *reinterpret_cast<const f32x4 *>(src);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < valid) o[i] = src[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(w, o[i], v[i]);
+    }
+    const bool yvec = vec && (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(YT) - 1)) == 0;
+    store4(y + (size_t)t * hidden + h, valid, yvec, v);
+}
+
+// Few pairs.  A pair's row is the only column of its products, so all 16
+// columns of the operand are that row (one address for 16 lanes).
+constexpr uint32_t kPairsMax = 64;      // pairs
+constexpr uint32_t kPairsHidden = 8192, kPairsWidth = 2048;
+
+// Whether every id of the call names an expert or none (each wavefront asks).
+__device__ __forceinline__ bool ids_ok(const ExpertsArgs &a, int lane) {
+    bool bad = false;
+    for (uint32_t i = lane; i < a.t * a.top_k; i += 64) {
+        const uint32_t e = a.ids[i];
+        bad |= e != TQF_HIP_NO_EXPERT && e >= a.n_experts;
+    }
+    return __ballot(bad) == 0;
+}
+// A row of n K blocks, of which this wavefront needs b0, b0 + step, ...: their
+// values quantised to bf16 into q [kb][128] and their scales into s [kb].
+// Sixteen lanes take a block, eight values each.
+template <typename XT>
+__device__ __forceinline__ void quantize_blocks(const XT *x, uint32_t cols, bool vec, uint32_t b0, uint32_t step, uint32_t n,
+                                                int lane, uint16_t *q, float *s) {
+    for (uint32_t b = b0; b < n; b += 4 * step) {
+        const uint32_t kb = b + (lane / 16) * step, k = kb * 128 + (lane % 16) * 8;
+        float v[8], m = 0.0f;
+        load_row<8>(x + k, kb < n && k < cols ? (int)(cols - k) : 0, vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+        m = amax8(m);
+        m = fmaxf(m, dpp_f<kDppMirror>(m));
+        const F8Factors f = f8_factors(m);
+        if (kb < n) {
+            const uint32_t lo = f8_pack4(v[0] * f.inv, v[1] * f.inv, v[2] * f.inv, v[3] * f.inv);
+            const uint32_t hi = f8_pack4(v[4] * f.inv, v[5] * f.inv, v[6] * f.inv, v[7] * f.inv);
+            *reinterpret_cast<bf16x8 *>(q + k) = f8_widen(lo, hi);
+            if (lane % 16 == 0) s[kb] = f.scale;
+        }
+    }
+}
+// This lane's operand of K block kb of a row in LDS.
+__device__ __forceinline__ Bf16x16::Op pair_operand(const uint16_t *q, uint32_t kb, int lane) {
+    const bf16x8 *p = reinterpret_cast<const bf16x8 *>(q + kb * 128 + (lane >> 4) * 16);
+    return Bf16x16::Op{{p[0], p[1], p[8], p[9]}};
+}
+
+// h[pair] = silu(g) u for 16 columns; four wavefronts share the K blocks.
+template <typename XT>
+__global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, const uint8_t *const *__restrict__ mats, F8Shape d,
+                                                              const XT *__restrict__ x, float *__restrict__ h, uint32_t hstride) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    typedef Bf16x16 P;
+    uint16_t *q = reinterpret_cast<uint16_t *>(lds);
+    float *s = reinterpret_cast<float *>(lds + (size_t)d.kb * 256);
+    float *red = s + ((d.kb + 3) & ~3u);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    const uint32_t pair = blockIdx.y, e = a.ids[pair], row0 = blockIdx.x * 16;
+    if (!ids_ok(a, l)) {
+        if (blockIdx.x == 0 && pair == 0 && tid == 0 && a.status) *a.status = TQF_HIP_ERR_INVALID;
+        return;
+    }
+    if (e == TQF_HIP_NO_EXPERT) return;
+    const uint8_t *g = mats[(size_t)e * 3], *u = mats[(size_t)e * 3 + 1];
+    const uint32_t tile = row0 / 32;
+    const int sub = (int)(row0 / 16 & 1);
+    const size_t base = (size_t)tile * d.kb * kKB, sbase = f8_tile_bytes(d) + (size_t)(tile / 4) * d.kb * 4;
+    const float *gs = reinterpret_cast<const float *>(g + sbase), *us = reinterpret_cast<const float *>(u + sbase);
+    f32x4 ag = {0.0f, 0.0f, 0.0f, 0.0f}, au = ag;
+    constexpr int kAhead = 4;
+    typename P::Raw rg[kAhead], ru[kAhead];
+    auto issue = [&](uint32_t b0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t kb = b0 + 4 * i;
+            if (kb >= d.kb) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const size_t at = base + (size_t)kb * kKB + P::a_off(l, sub, j);
+                rg[i].q[j] = *reinterpret_cast<const u32x4 *>(g + at);
+                ru[i].q[j] = *reinterpret_cast<const u32x4 *>(u + at);
+            }
+        }
+    };
+    issue(wave);
+    const XT *row = x + (size_t)(pair / a.top_k) * d.cols;
+    quantize_blocks(row, d.cols, rows_aligned(x, d.cols, sizeof(XT)), wave, 4, d.kb, l, q, s);
+    __syncthreads();
+    for (uint32_t b0 = wave; b0 < d.kb; b0 += 4 * kAhead) {
+        if (b0 != (uint32_t)wave) issue(b0);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t kb = b0 + 4 * i;
+            if (kb >= d.kb) break;
+            const typename P::Op b = pair_operand(q, kb, l);
+            const f32x4 pg = P::mma(P::op(rg[i]), b), pu = P::mma(P::op(ru[i]), b);
+            const float sg = s[kb] * gs[kb], su = s[kb] * us[kb];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                ag[v] = __builtin_fmaf(pg[v], sg, ag[v]);
+                au[v] = __builtin_fmaf(pu[v], su, au[v]);
+            }
+        }
+    }
+    if ((l & 15) == 0) {
+        *reinterpret_cast<f32x4 *>(red + wave * 32 + P::row(l, 0)) = ag;
+        *reinterpret_cast<f32x4 *>(red + wave * 32 + 16 + P::row(l, 0)) = au;
+    }
+    __syncthreads();
+    if (tid < 16 && row0 + tid < d.rows) {
+        const float gv = (red[tid] + red[32 + tid]) + (red[64 + tid] + red[96 + tid]);
+        const float uv = (red[16 + tid] + red[48 + tid]) + (red[80 + tid] + red[112 + tid]);
+        h[(size_t)pair * hstride + row0 + tid] = gv / (1.0f + expf(-gv)) * uv;
+    }
+}
+
+// y[token] for 16 columns: a wavefront takes the routes k = wave, wave + 8, ...
+template <typename YT>
+__global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const uint8_t *const *__restrict__ mats, F8Shape d,
+                                                           const float *__restrict__ h, uint32_t hstride, YT *__restrict__ y) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    typedef Bf16x16 P;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    uint16_t *q = reinterpret_cast<uint16_t *>(lds + (size_t)wave * d.kb * 256);
+    float *s = reinterpret_cast<float *>(lds + (size_t)8 * d.kb * 256) + wave * d.kb;
+    float *red = reinterpret_cast<float *>(lds + (size_t)8 * d.kb * 260);  // [top_k][16]
+    const uint32_t token = blockIdx.y, row0 = blockIdx.x * 16, tile = row0 / 32;
+    const int sub = (int)(row0 / 16 & 1);
+    if (!ids_ok(a, l)) return;
+    const size_t base = (size_t)tile * d.kb * kKB, sbase = f8_tile_bytes(d) + (size_t)(tile / 4) * d.kb * 4;
+    for (uint32_t k = wave; k < a.top_k; k += 8) {
+        const uint32_t pair = token * a.top_k + k, e = a.ids[pair];
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (e != TQF_HIP_NO_EXPERT) {
+            const uint8_t *m = mats[(size_t)e * 3 + 2];
+            const float *ms = reinterpret_cast<const float *>(m + sbase);
+            constexpr int kAhead = 4;
+            typename P::Raw raw[kAhead];
+            auto issue = [&](uint32_t b0) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (b0 + i >= d.kb) break;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        raw[i].q[j] = *reinterpret_cast<const u32x4 *>(m + base + (size_t)(b0 + i) * kKB + P::a_off(l, sub, j));
+                }
+            };
+            issue(0);
+            quantize_blocks(h + (size_t)pair * hstride, d.cols, true, 0, 1, d.kb, l, q, s);
+            // this wavefront's own writes: LDS serves it in order
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (uint32_t b0 = 0; b0 < d.kb; b0 += kAhead) {
+                if (b0) issue(b0);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (b0 + i >= d.kb) break;
+                    const f32x4 p = P::mma(P::op(raw[i]), pair_operand(q, b0 + i, l));
+                    const float sc = s[b0 + i] * ms[b0 + i];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(p[v], sc, acc[v]);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // before the next route's values
+        }
+        if ((l & 15) == 0) *reinterpret_cast<f32x4 *>(red + k * 16 + P::row(l, 0)) = acc;
+    }
+    __syncthreads();
+    if (tid < 16 && row0 + tid < d.rows) {
+        float v = 0.0f;
+        for (uint32_t k = 0; k < a.top_k; ++k) {
+            const uint32_t pair = token * a.top_k + k;
+            if (a.ids[pair] != TQF_HIP_NO_EXPERT) v = __builtin_fmaf(a.w[pair], red[k * 16 + tid], v);
+        }
+        const f32x4 one = {v, 0.0f, 0.0f, 0.0f};
+        store4(y + (size_t)token * d.rows + row0 + tid, 1, false, one);
+    }
+}
+
+bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
+    return t * top_k <= kPairsMax && ex.hidden <= kPairsHidden && ex.width <= kPairsWidth;
+}
+// Rows of a tile by the pairs an expert has on average: enough to hold most
+// experts' in one tile, whose weights are then read once.
+uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
+    const uint32_t mean = t * top_k / ex.n_experts;
+    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : 128;
+}
+struct ExpertsScratch {
+    int32_t *pos_of_pair, *row_of_pos, *n_tiles;
+    uint2 *tiles;
+    uint8_t *xq, *hq;
+    float *xs, *hs, *out;
+    uint32_t max_tiles;
+    size_t total;
+};
+ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
+    const size_t P = (size_t)t * top_k, kbh = (ex.hidden + 127) / 128, kbf = (ex.width + 127) / 128;
+    const uint32_t m = tile_rows(ex, t, top_k);
+    ExpertsScratch b;
+    b.max_tiles = (uint32_t)(P / m + (P < ex.n_experts ? P : ex.n_experts));
+    uint8_t *p = static_cast<uint8_t *>(scratch);
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *at = p + off;
+        off += align256(bytes);
+        return at;
+    };
+    b.n_tiles = reinterpret_cast<int32_t *>(take(4));
+    b.pos_of_pair = reinterpret_cast<int32_t *>(take(P * 4));
+    b.row_of_pos = reinterpret_cast<int32_t *>(take(P * 4));
+    b.tiles = reinterpret_cast<uint2 *>(take((size_t)b.max_tiles * 8));
+    b.xq = take((size_t)t * kbh * 128);
+    b.xs = reinterpret_cast<float *>(take((size_t)t * kbh * 4));
+    b.hq = take(P * kbf * 128);
+    b.hs = reinterpret_cast<float *>(take(P * kbf * 4));
+    b.out = reinterpret_cast<float *>(take(P * ex.hidden * 4));
+    b.total = off;
+    return b;
+}
+
+template <class P, int RT, int CT>
+hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
+    TiledArgs a{};
+    a.mats = ex.mats;
+    a.d = f8_shape(ex.width, ex.hidden);
+    a.xq = b.xq;
+    a.xs = b.xs;
+    a.xrows = t;
+    a.tiles = b.tiles;
+    a.n_tiles = b.n_tiles;
+    a.row_of_pos = b.row_of_pos;
+    a.hq = b.hq;
+    a.hs = b.hs;
+    a.hkb = (ex.width + 127) / 128;
+    a.hrows = pairs;
+    static_assert(RT * P::M == 64, "a workgroup of gate_up makes one block of h");
+    f8_tiled_kernel<P, RT, CT, kGateUp, float><<<dim3(a.hkb, b.max_tiles), 256, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    a.d = f8_shape(ex.hidden, ex.width);
+    a.xq = b.hq;
+    a.xs = b.hs;
+    a.xrows = pairs;
+    a.out = b.out;
+    f8_tiled_kernel<P, RT, CT, kDown, float><<<dim3((ex.hidden + 255) / 256, b.max_tiles), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <typename XT, typename YT>
+hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, const ExpertsArgs &a, void *scratch) {
+    const uint32_t pairs = a.t * a.top_k;
+    const F8Shape dg = f8_shape(ex.width, ex.hidden), dd = f8_shape(ex.hidden, ex.width);
+    if (pairs_path(ex, a.t, a.top_k)) {
+        float *h = static_cast<float *>(scratch);
+        const uint32_t hstride = dd.kb * 128;
+        f8_pair_gate_up_kernel<<<dim3((ex.width + 15) / 16, pairs), 256, dg.kb * 260 + 16 + 512, s>>>(a, ex.mats, dg, x, h, hstride);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        f8_pair_down_kernel<<<dim3((ex.hidden + 15) / 16, a.t), 512, 8 * dd.kb * 260 + a.top_k * 64, s>>>(a, ex.mats, dd, h, hstride, y);
+        return hipGetLastError();
+    }
+    const ExpertsScratch b = experts_scratch(scratch, ex, a.t, a.top_k);
+    const uint32_t plan = (pairs + kPlanThreads - 1) / kPlanThreads, quant = (a.t * dg.kb * 8 + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t m = tile_rows(ex, a.t, a.top_k);
+    f8_plan_kernel<<<plan + quant, kPlanThreads, 0, s>>>(a, m, b.pos_of_pair, b.row_of_pos, b.tiles, b.n_tiles, x, ex.hidden, dg.kb,
+                                                        b.xq, b.xs);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    e = m == 16   ? launch_tiles<Fp8x16, 4, 1>(s, ex, b, a.t, pairs)
+        : m == 32 ? launch_tiles<Fp8x32, 2, 1>(s, ex, b, a.t, pairs)
+        : m == 64 ? launch_tiles<Fp8x32, 2, 2>(s, ex, b, a.t, pairs)
+                  : launch_tiles<Fp8x32, 2, 4>(s, ex, b, a.t, pairs);
+    if (e != hipSuccess) return e;
+    f8_combine_kernel<<<dim3((ex.hidden + 1023) / 1024, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, b.out, ex.hidden, y);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_f8_repack(hipStream_t s, const uint8_t *q, const float *scales, const F8Shape &d, uint8_t *out) {
+    const size_t chunks = f8_tile_bytes(d) / 16;  // more than there are scales
+    f8_repack_kernel<<<(uint32_t)((chunks + 255) / 256), 256, 0, s>>>(q, scales, d, out);
+    return hipGetLastError();
+}
+
+size_t f8_matmul_scratch_bytes(const F8Shape &d, uint32_t t) {
+    if (rows_path(d, t)) return 0;
+    return align256((size_t)t * d.kb * 128) + align256((size_t)t * d.kb * 4);
+}
+
+hipError_t launch_f8_matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const void *x, int32_t x_type, uint32_t t,
+                            void *y, int32_t y_type, void *scratch) {
+    const float *xf = static_cast<const float *>(x);
+    const uint16_t *xb = static_cast<const uint16_t *>(x);
+    float *yf = static_cast<float *>(y);
+    uint16_t *yb = static_cast<uint16_t *>(y);
+    if (x_type == TQF_HIP_TYPE_F32)
+        return y_type == TQF_HIP_TYPE_F32 ? matmul(s, mat, d, xf, t, yf, scratch) : matmul(s, mat, d, xf, t, yb, scratch);
+    return y_type == TQF_HIP_TYPE_F32 ? matmul(s, mat, d, xb, t, yf, scratch) : matmul(s, mat, d, xb, t, yb, scratch);
+}
+
+size_t f8_experts_scratch_bytes(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
+    if (pairs_path(ex, t, top_k)) return (size_t)t * top_k * ((ex.width + 127) / 128 * 128) * 4;
+    return experts_scratch(nullptr, ex, t, top_k).total;
+}
+
+hipError_t launch_f8_experts(hipStream_t s, const F8ExpertsDev &ex, const void *x, int32_t x_type, uint32_t t,
+                             const uint16_t *ids, const float *w, uint32_t top_k, void *y, int32_t y_type, int32_t *status,
+                             void *scratch) {
+    const ExpertsArgs a{ids, w, t, top_k, ex.n_experts, status};
+    const float *xf = static_cast<const float *>(x);
+    const uint16_t *xb = static_cast<const uint16_t *>(x);
+    float *yf = static_cast<float *>(y);
+    uint16_t *yb = static_cast<uint16_t *>(y);
+    if (x_type == TQF_HIP_TYPE_F32)
+        return y_type == TQF_HIP_TYPE_F32 ? experts(s, ex, xf, yf, a, scratch) : experts(s, ex, xf, yb, a, scratch);
+    return y_type == TQF_HIP_TYPE_F32 ? experts(s, ex, xb, yf, a, scratch) : experts(s, ex, xb, yb, a, scratch);
+}
+
+}  // namespace tqf

@@ -19,6 +19,8 @@
 // whose products of e4m3 values came out exact in the same test.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "tqf_f8.h"
 
 namespace tqf {
@@ -169,12 +171,20 @@ __device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
 }
 typedef __attribute__((address_space(3))) void lds_void;
+// Matrices found through a table: without the address space the compiler would
+// load through flat instructions, which also count as LDS accesses.
+typedef __attribute__((address_space(1))) const uint8_t global_u8;
+typedef __attribute__((address_space(1))) const float global_f32;
+typedef __attribute__((address_space(1))) const u32x4 global_u32x4;
 __device__ __forceinline__ void copy16(Desc d, uint32_t voff, uint32_t soff, void *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, soff, 0, 0);
 }
-// This wavefront's loads (those to LDS among them) and LDS reads are done, then
-// the workgroup's.
-__device__ __forceinline__ void publish() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// This wavefront's loads but the last N (those to LDS among them) and its LDS
+// reads are done, then the workgroup's.
+template <int N>
+__device__ __forceinline__ void publish() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
 // ---- the tiled product -----------------------------------------------------------
 // A workgroup of four wavefronts: CT * M activation rows by 4 RT M weight rows.
@@ -206,28 +216,33 @@ struct TiledArgs {
     float *out;                      // kDown: [positions][rows]
 };
 
-template <class P, int RT, int CT, int MODE, typename YT>
-__global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8_tiled_kernel(TiledArgs a) {
-    constexpr int M = P::M, kRows = CT * M;       // activation rows of the workgroup
-    constexpr int kCopies = kRows / 32;           // copies of 1 KiB each wavefront makes for a block
+template <class P, int RT, int CT, int MODE, typename YT, int NS = 2, int OCC = 2, int TW = 1>
+__global__ __launch_bounds__(256 * TW, OCC) void f8_tiled_kernel(TiledArgs a) {
+    constexpr int M = P::M, kRows = TW * CT * M;  // activation rows of the workgroup
+    constexpr int kCopies = CT * M / 32;          // copies of 1 KiB each wavefront makes for a block
     constexpr int kG = P::kGroups;
-    static_assert(kRows % 32 == 0 || kRows == 16, "copies are dealt to four wavefronts");
-    __shared__ __attribute__((aligned(16))) uint8_t stage[2][kRows * 128];
+    static_assert(CT * M % 32 == 0 || kRows == 16, "copies are dealt to the wavefronts");
+    __shared__ __attribute__((aligned(16))) uint8_t stage[NS][kRows * 128];
     __shared__ float s_max[kTileWaves][MODE == kGateUp ? kRows : 1];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    const int tid = threadIdx.x, all_wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    const int wave = all_wave % kTileWaves;  // which weight rows
     const uint32_t kb_n = a.d.kb, kp = kb_n * 128;
 
     // which activation rows and weights
     uint32_t first, rows, e = 0, rblock;
     if constexpr (MODE == kDense) {
-        // neighbouring workgroups run on different XCDs: deal each XCD a
-        // contiguous share of the order (row blocks fastest), so that the ones
-        // that read the same rows of x share an L2
-        const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * M - 1) / (4 * RT * M), all = gridDim.x;
-        const uint32_t per = (all + 7) / 8, id = (blockIdx.x % 8) * per + blockIdx.x / 8;
-        if (blockIdx.x / 8 >= per || id >= all) return;
-        first = id / rbs * kRows;
-        rblock = id % rbs;
+        // Neighbouring workgroups run on different XCDs: each XCD is dealt a
+        // contiguous share of an order in which four blocks of activation rows
+        // take turns, then the next block of weight rows, so that the 32
+        // workgroups that an XCD runs at a time share both in its L2.
+        const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * M - 1) / (4 * RT * M), tbs = (a.xrows + kRows - 1) / kRows;
+        const uint32_t per = gridDim.x / 8, id = (blockIdx.x % 8) * per + blockIdx.x / 8;
+        const uint32_t four = id / (4 * rbs) * 4, left = tbs > four ? tbs - four : 0, turn = left < 4 ? left : 4;
+        if (turn == 0) return;
+        const uint32_t in = id - four * rbs;
+        first = (four + in % turn) * kRows;
+        rblock = in / turn;
+        if (rblock >= rbs) return;
         if (first >= a.xrows) return;
         rows = a.xrows - first < kRows ? a.xrows - first : kRows;
     } else {
@@ -240,8 +255,8 @@ __global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8
     }
     // this wavefront's row tiles: bases and scales (a tile never spans two
     // scale blocks; tiles past the matrix read its last and store nothing)
-    const uint8_t *base[RT];
-    const float *ws[RT];
+    global_u8 *base[RT];
+    global_f32 *ws[RT];
     uint32_t wrow[RT];
     int sub[RT];
 #pragma unroll
@@ -260,8 +275,15 @@ __global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8
         uint32_t tile = wrow[r] / 32;
         if (tile >= a.d.tiles) tile = a.d.tiles - 1;
         sub[r] = (int)(wrow[r] / 16 & 1);
-        base[r] = mat + (size_t)tile * kb_n * kKB;
-        ws[r] = reinterpret_cast<const float *>(mat + f8_tile_bytes(a.d)) + (size_t)(tile / 4) * kb_n;
+        base[r] = (global_u8 *)mat + (size_t)tile * kb_n * kKB;
+        ws[r] = (global_f32 *)(mat + f8_tile_bytes(a.d)) + (size_t)(tile / 4) * kb_n;
+    }
+    // this wavefront's activation rows: with two sets of four, each takes half
+    uint32_t row0 = 0, mine = rows;
+    if constexpr (TW == 2) {
+        const uint32_t half = ((rows + 1) / 2 + M - 1) / M * M;
+        row0 = all_wave / kTileWaves ? half : 0;
+        mine = row0 ? (rows > half ? rows - half : 0) : (rows < half ? rows : half);
     }
     // activation rows: what this lane copies, and whose scale it applies
     auto source_row = [&](uint32_t local) -> uint32_t {
@@ -271,19 +293,19 @@ __global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8
     };
     uint32_t xbase = 0;
     if constexpr (MODE != kGateUp) xbase = first;
-    const Desc dx = make_desc(a.xq + (size_t)xbase * kp, (uint32_t)(((size_t)a.xrows - xbase) * kp < 0xFFFFFFFFull
-                                                                       ? ((size_t)a.xrows - xbase) * kp : 0xFFFFFFFFull));
+    // (f8_matmul and f8_experts keep rows times kp below 2^32)
+    const Desc dx = make_desc(a.xq + (size_t)xbase * kp, (a.xrows - xbase) * kp);
     constexpr int kMine = kCopies ? kCopies : 1;
-    const bool copies = kCopies > 0 || wave < 2;  // 16 rows: two wavefronts
+    const bool copies = kCopies > 0 || all_wave < 2;  // 16 rows: two wavefronts
     uint32_t voff[kMine];
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-        const int local = (wave * kMine + j) * 8 + l / 8;
+        const int local = (all_wave * kMine + j) * 8 + l / 8;
         voff[j] = copies ? (source_row((uint32_t)local) - xbase) * kp + (uint32_t)(((l & 7) ^ swizzle(local)) * 16) : 0;
     }
     uint32_t srow[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) srow[c] = source_row((uint32_t)(c * M + P::b_row(l)));
+    for (int c = 0; c < CT; ++c) srow[c] = source_row(row0 + (uint32_t)(c * M + P::b_row(l)));
     uint32_t boff[P::kLoads];
 #pragma unroll
     for (int j = 0; j < P::kLoads; ++j) boff[j] = P::b_row(l) * 128 + ((P::b_chunk(l, j) ^ swizzle(P::b_row(l))) * 16);
@@ -294,57 +316,92 @@ __global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[r][c] = typename P::D{};
 
-    struct Block {
-        typename P::Raw w[RT];
-        float s[CT];
-    };
-    auto issue = [&](uint32_t kb, Block &b) {
-        if (copies) {
+    // The K loop over N of the CT tiles of activation rows (an expert's rows may
+    // fill fewer).  All that a block needs from memory is asked for together:
+    // loads return in order, so one asked for later would wait for the next
+    // block's.  A ring of NS blocks, NS - 1 ahead (past the end the last block
+    // again, so that no branch splits the loop).
+    auto k_loop = [&](auto tiles_used) {
+        constexpr int N = decltype(tiles_used)::value;
+        struct Block {
+            typename P::Raw w[RT];
+            float s[N], sw[RT];
+        };
+        Block b[NS];
+        auto issue = [&](uint32_t block, int u) {
+            // kept in a scalar register: a copy whose offset the compiler put in
+            // a vector register would be wrapped in a loop over its values
+            const uint32_t kb = (uint32_t)__builtin_amdgcn_readfirstlane((int)(block < kb_n ? block : kb_n - 1));
+            if (copies) {
 #pragma unroll
-            for (int j = 0; j < kMine; ++j) copy16(dx, voff[j], kb * 128, &stage[kb & 1][(wave * kMine + j) * 1024]);
-        }
+                for (int j = 0; j < kMine; ++j) copy16(dx, voff[j], kb * 128, &stage[u][(all_wave * kMine + j) * 1024]);
+            }
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int j = 0; j < P::kLoads; ++j)
-                b.w[r].q[j] = *reinterpret_cast<const u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
+                for (int j = 0; j < P::kLoads; ++j)
+                    b[u].w[r].q[j] = *reinterpret_cast<const global_u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
 #pragma unroll
-        for (int c = 0; c < CT; ++c) b.s[c] = a.xs[(size_t)kb * a.xrows + srow[c]];
-    };
-    auto compute = [&](uint32_t kb, const Block &b) {
-        const uint8_t *st = stage[kb & 1];
-        float sw[RT];
+            for (int c = 0; c < N; ++c) b[u].s[c] = a.xs[(size_t)kb * a.xrows + srow[c]];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) sw[r] = ws[r][kb];
-        typename P::Op aw[RT];
+            for (int r = 0; r < RT; ++r) b[u].sw[r] = ws[r][kb];
+        };
+        // The instructions of a tile are issued ahead of the fmas that take the
+        // tile before it, so that the vector ALU works while they run.
+        auto compute = [&](int u) {
+            const uint8_t *st = stage[u] + row0 * 128;
+            typename P::Op aw[RT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) aw[r] = P::op(b.w[r]);
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            if (MODE != kDense && c > 0 && (uint32_t)(c * M) >= rows) continue;  // no rows of this tile here
-            typename P::Raw raw;
-#pragma unroll
-            for (int j = 0; j < P::kLoads; ++j) raw.q[j] = *reinterpret_cast<const u32x4 *>(st + c * M * 128 + boff[j]);
-            const typename P::Op bx = P::op(raw);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const typename P::D d = P::mma(aw[r], bx);
-                const float s = b.s[c] * sw[r];
+            for (int r = 0; r < RT; ++r) aw[r] = P::op(b[u].w[r]);
+            auto add = [&](int r, int c, const typename P::D &d) {
+                const float s = b[u].s[c] * b[u].sw[r];
 #pragma unroll
                 for (int i = 0; i < 4 * kG; ++i) acc[r][c][i] = __builtin_fmaf(d[i], s, acc[r][c][i]);
+            };
+            typename P::D d;
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                typename P::Raw raw;
+#pragma unroll
+                for (int j = 0; j < P::kLoads; ++j) raw.q[j] = *reinterpret_cast<const u32x4 *>(st + c * M * 128 + boff[j]);
+                const typename P::Op bx = P::op(raw);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const typename P::D next = P::mma(aw[r], bx);
+                    if (c || r) add(r ? r - 1 : RT - 1, r ? c : c - 1, d);
+                    d = next;
+                }
             }
+            add(RT - 1, N - 1, d);
+        };
+        // Of the loads after a block's copies at least the copies and weights of
+        // the NS - 2 blocks after it may be in flight.
+        constexpr int kLater = (NS - 2) * (kMine * (kCopies > 0) + RT * P::kLoads);
+        auto step = [&](uint32_t kb, int u) {
+            publish<kLater>();
+            issue(kb + NS - 1, (u + NS - 1) % NS);
+            compute(u);
+        };
+#pragma unroll
+        for (int u = 0; u < NS - 1; ++u) issue(u, u);
+        uint32_t kb = 0;
+        for (; kb + NS <= kb_n; kb += NS) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u) step(kb + u, u);
         }
+#pragma unroll
+        for (int u = 0; u < NS - 1; ++u)
+            if (kb + u < kb_n) step(kb + u, u);
+        publish<0>();  // no copy is under way when the workgroup's LDS goes to another
     };
-    Block b0, b1;
-    issue(0, b0);
-    for (uint32_t kb = 0; kb < kb_n; kb += 2) {
-        publish();
-        if (kb + 1 < kb_n) issue(kb + 1, b1);
-        compute(kb, b0);
-        if (kb + 1 >= kb_n) break;
-        publish();
-        if (kb + 2 < kb_n) issue(kb + 2, b0);
-        compute(kb + 1, b1);
+    if constexpr (MODE == kDense) {
+        k_loop(std::integral_constant<int, CT>{});
+    } else {
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane((int)((mine + M - 1) / M));
+        if (CT >= 4 && n >= 4) k_loop(std::integral_constant<int, CT < 4 ? CT : 4>{});
+        else if (CT >= 3 && n >= 3) k_loop(std::integral_constant<int, CT < 3 ? CT : 3>{});
+        else if (CT >= 2 && n >= 2) k_loop(std::integral_constant<int, CT < 2 ? CT : 2>{});
+        else k_loop(std::integral_constant<int, 1>{});
     }
 
     if constexpr (MODE == kGateUp) {
@@ -363,15 +420,15 @@ __global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8
                     m = fmaxf(m, fabsf(h[r][c][i]));
                 }
             m = P::across(m);
-            if (l < M) s_max[wave][c * M + l] = m;
+            if (l < M && (uint32_t)(c * M + l) < mine) s_max[wave][row0 + c * M + l] = m;
         }
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const int local = c * M + P::b_row(l);
+            const uint32_t in = (uint32_t)(c * M + P::b_row(l)), local = row0 + in;
+            if (in >= mine) continue;
             const float m = fmaxf(fmaxf(s_max[0][local], s_max[1][local]), fmaxf(s_max[2][local], s_max[3][local]));
             const F8Factors f = f8_factors(m);
-            if ((uint32_t)local >= rows) continue;
             const uint32_t pos = first + local;
             if (wave == 0 && l < M) a.hs[(size_t)rblock * a.hrows + pos] = f.scale;
 #pragma unroll
@@ -389,8 +446,8 @@ __global__ __launch_bounds__(256, RT * CT * P::M * P::M >= 8192 ? 1 : 2) void f8
         const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const uint32_t local = (uint32_t)(c * M + P::b_row(l));
-            if (local >= rows) continue;
+            const uint32_t in = (uint32_t)(c * M + P::b_row(l)), local = row0 + in;
+            if (in >= mine) continue;
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -548,11 +605,11 @@ hipError_t quantize(hipStream_t s, const XT *x, uint32_t t, uint32_t cols, uint3
     return hipGetLastError();
 }
 
-template <class P, int RT, int CT, typename YT>
+template <class P, int RT, int CT, typename YT, int NS = 2, int OCC = 2, int TW = 1>
 hipError_t launch_dense(hipStream_t s, const TiledArgs &a) {
     constexpr uint32_t kM = P::M;
-    const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * kM - 1) / (4 * RT * kM), tbs = (a.xrows + CT * kM - 1) / (CT * kM);
-    f8_tiled_kernel<P, RT, CT, kDense, YT><<<(rbs * tbs + 7) / 8 * 8, 256, 0, s>>>(a);
+    const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * kM - 1) / (4 * RT * kM), tbs = (a.xrows + TW * CT * kM - 1) / (TW * CT * kM);
+    f8_tiled_kernel<P, RT, CT, kDense, YT, NS, OCC, TW><<<(rbs * tbs + 7) / 8 * 8, 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -575,7 +632,7 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     } else {
         if (t <= 32) return launch_dense<Fp8x32, 1, 1, YT>(s, a);
         if (t <= 64) return launch_dense<Fp8x32, 2, 2, YT>(s, a);
-        return launch_dense<Fp8x32, 2, 4, YT>(s, a);
+        return launch_dense<Fp8x32, 2, 3, YT>(s, a);
     }
 }
 
@@ -777,11 +834,11 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
         return;
     }
     if (e == TQF_HIP_NO_EXPERT) return;
-    const uint8_t *g = mats[(size_t)e * 3], *u = mats[(size_t)e * 3 + 1];
+    global_u8 *g = (global_u8 *)mats[(size_t)e * 3], *u = (global_u8 *)mats[(size_t)e * 3 + 1];
     const uint32_t tile = row0 / 32;
     const int sub = (int)(row0 / 16 & 1);
     const size_t base = (size_t)tile * d.kb * kKB, sbase = f8_tile_bytes(d) + (size_t)(tile / 4) * d.kb * 4;
-    const float *gs = reinterpret_cast<const float *>(g + sbase), *us = reinterpret_cast<const float *>(u + sbase);
+    global_f32 *gs = (global_f32 *)(g + sbase), *us = (global_f32 *)(u + sbase);
     f32x4 ag = {0.0f, 0.0f, 0.0f, 0.0f}, au = ag;
     constexpr int kAhead = 4;
     typename P::Raw rg[kAhead], ru[kAhead];
@@ -793,8 +850,8 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const size_t at = base + (size_t)kb * kKB + P::a_off(l, sub, j);
-                rg[i].q[j] = *reinterpret_cast<const u32x4 *>(g + at);
-                ru[i].q[j] = *reinterpret_cast<const u32x4 *>(u + at);
+                rg[i].q[j] = *reinterpret_cast<const global_u32x4 *>(g + at);
+                ru[i].q[j] = *reinterpret_cast<const global_u32x4 *>(u + at);
             }
         }
     };
@@ -848,8 +905,8 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
         const uint32_t pair = token * a.top_k + k, e = a.ids[pair];
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         if (e != TQF_HIP_NO_EXPERT) {
-            const uint8_t *m = mats[(size_t)e * 3 + 2];
-            const float *ms = reinterpret_cast<const float *>(m + sbase);
+            global_u8 *m = (global_u8 *)mats[(size_t)e * 3 + 2];
+            global_f32 *ms = (global_f32 *)(m + sbase);
             constexpr int kAhead = 4;
             typename P::Raw raw[kAhead];
             auto issue = [&](uint32_t b0) {
@@ -858,7 +915,7 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
                     if (b0 + i >= d.kb) break;
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
-                        raw[i].q[j] = *reinterpret_cast<const u32x4 *>(m + base + (size_t)(b0 + i) * kKB + P::a_off(l, sub, j));
+                        raw[i].q[j] = *reinterpret_cast<const global_u32x4 *>(m + base + (size_t)(b0 + i) * kKB + P::a_off(l, sub, j));
                 }
             };
             issue(0);
@@ -899,7 +956,8 @@ bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
 // experts' in one tile, whose weights are then read once.
 uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
     const uint32_t mean = t * top_k / ex.n_experts;
-    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : 128;
+    static const int var = getenv("V") ? atoi(getenv("V")) : 0;
+    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : var == 0 ? 192 : 96;
 }
 struct ExpertsScratch {
     int32_t *pos_of_pair, *row_of_pos, *n_tiles;
@@ -934,7 +992,7 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     return b;
 }
 
-template <class P, int RT, int CT>
+template <class P, int RT, int CT, int NS = 2, int OCC = 2, int TW = 1>
 hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
     TiledArgs a{};
     a.mats = ex.mats;
@@ -950,7 +1008,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.hkb = (ex.width + 127) / 128;
     a.hrows = pairs;
     static_assert(RT * P::M == 64, "a workgroup of gate_up makes one block of h");
-    f8_tiled_kernel<P, RT, CT, kGateUp, float><<<dim3(a.hkb, b.max_tiles), 256, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kGateUp, float, NS, OCC, TW><<<dim3(a.hkb, b.max_tiles), 256 * TW, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     a.d = f8_shape(ex.hidden, ex.width);
@@ -958,7 +1016,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.xs = b.hs;
     a.xrows = pairs;
     a.out = b.out;
-    f8_tiled_kernel<P, RT, CT, kDown, float><<<dim3((ex.hidden + 255) / 256, b.max_tiles), 256, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kDown, float, NS, OCC, TW><<<dim3((ex.hidden + 255) / 256, b.max_tiles), 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -982,10 +1040,12 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
                                                         b.xq, b.xs);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    static const int var = getenv("V") ? atoi(getenv("V")) : 0;
     e = m == 16   ? launch_tiles<Fp8x16, 4, 1>(s, ex, b, a.t, pairs)
         : m == 32 ? launch_tiles<Fp8x32, 2, 1>(s, ex, b, a.t, pairs)
         : m == 64 ? launch_tiles<Fp8x32, 2, 2>(s, ex, b, a.t, pairs)
-                  : launch_tiles<Fp8x32, 2, 4>(s, ex, b, a.t, pairs);
+                  : var == 0 ? launch_tiles<Fp8x32, 2, 3, 2, 2, 2>(s, ex, b, a.t, pairs)
+                  : launch_tiles<Fp8x32, 2, 3, 2, 2, 1>(s, ex, b, a.t, pairs);
     if (e != hipSuccess) return e;
     f8_combine_kernel<<<dim3((ex.hidden + 1023) / 1024, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, b.out, ex.hidden, y);
     return hipGetLastError();

@@ -76,24 +76,29 @@ __device__ __forceinline__ u32x4 quantize16(const float (&v)[16], float *scale) 
     return q;
 }
 
-// Chunk i of x [t x cols]: the 16 columns i % (8 kb) of row i / (8 kb).  Eight
-// lanes share a block, so all of an aligned group take part or none.
+// Quantised rows are kept by K block, [kb][t][128]: the tiled product reads many
+// rows of one block at a time, which in rows of kb 128 bytes would lie kb 128
+// apart, for most widths all in a few of the L2's channels.
+// Chunk i of x [t x cols]: 16 columns; eight lanes share a block of a row (so all
+// of an aligned group take part or none), a wavefront has eight rows.
+__host__ __device__ __forceinline__ uint32_t quantize_chunks(uint32_t t, uint32_t kb) { return (t + 7) / 8 * 64 * kb; }
 template <typename XT>
 __device__ __forceinline__ void quantize_chunk(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb, bool vec,
                                                uint32_t i, uint8_t *__restrict__ xq, float *__restrict__ xs) {
-    const uint32_t row = i / (8 * kb), c = i - row * 8 * kb, k = c * 16;
+    const uint32_t rows8 = i / (64 * kb), block = i / 64 - rows8 * kb, row = rows8 * 8 + i / 8 % 8, k = block * 128 + i % 8 * 16;
+    if (row >= t) return;
     const int valid = k < cols ? (int)(cols - k) : 0;
     float v[16], s;
     load_row<16>(x + (size_t)row * cols + k, valid, vec, v);
     const u32x4 q = quantize16(v, &s);
-    reinterpret_cast<u32x4 *>(xq)[i] = q;
-    if ((c & 7) == 0) xs[(size_t)(c >> 3) * t + row] = s;
+    const size_t at = (size_t)block * t + row;
+    reinterpret_cast<u32x4 *>(xq)[at * 8 + i % 8] = q;
+    if (i % 8 == 0) xs[at] = s;
 }
 template <typename XT>
 __global__ __launch_bounds__(256) void f8_quantize_kernel(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb,
                                                           uint8_t *__restrict__ xq, float *__restrict__ xs) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= t * kb * 8) return;
     quantize_chunk(x, t, cols, kb, rows_aligned(x, cols, sizeof(XT)), i, xq, xs);
 }
 
@@ -118,10 +123,10 @@ struct Fp8x32 {  // v_mfma_f32_32x32x64_f8f6f4: two to a block
     static __device__ __forceinline__ i32x8 pair(u32x4 a, u32x4 b) {
         return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
     }
-    static __device__ __forceinline__ D mma(const Op &a, const Op &b) {
-        D d = {};
-        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(a.q[0], a.q[1]), pair(b.q[0], b.q[1]), d, 0, 0, 0, 0, 0, 0);
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(a.q[2], a.q[3]), pair(b.q[2], b.q[3]), d, 0, 0, 0, 0, 0, 0);
+    static constexpr int kParts = 2;
+    static __device__ __forceinline__ D part(const Op &a, const Op &b, const D &d, int i) {
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(a.q[2 * i], a.q[2 * i + 1]), pair(b.q[2 * i], b.q[2 * i + 1]), d, 0, 0,
+                                                               0, 0, 0, 0);
     }
     static __device__ __forceinline__ float across(float a) { return fmaxf(a, __shfl_xor(a, 32)); }
 };
@@ -139,9 +144,9 @@ struct Fp8x16 {  // v_mfma_f32_16x16x128_f8f6f4: one to a block
     static __device__ __forceinline__ int b_chunk(int l, int j) { return 4 * j + (l >> 4); }
     static __device__ __forceinline__ int row(int l, int) { return 4 * (l >> 4); }
     static __device__ __forceinline__ const Op &op(const Raw &r) { return r; }
-    static __device__ __forceinline__ D mma(const Op &a, const Op &b) {
-        const D z = {0.0f, 0.0f, 0.0f, 0.0f};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Fp8x32::pair(a.q[0], a.q[1]), Fp8x32::pair(b.q[0], b.q[1]), z, 0,
+    static constexpr int kParts = 1;
+    static __device__ __forceinline__ D part(const Op &a, const Op &b, const D &d, int) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Fp8x32::pair(a.q[0], a.q[1]), Fp8x32::pair(b.q[0], b.q[1]), d, 0,
                                                                 0, 0, 0, 0, 0);
     }
     static __device__ __forceinline__ float across(float a) {
@@ -157,10 +162,14 @@ struct Bf16x16 : Fp8x16 {  // the same tiles, widened to bf16: v_mfma_f32_16x16x
         return Op{{f8_widen(r.q[0][0], r.q[0][1]), f8_widen(r.q[0][2], r.q[0][3]), f8_widen(r.q[1][0], r.q[1][1]),
                    f8_widen(r.q[1][2], r.q[1][3])}};
     }
+    static constexpr int kParts = 4;
+    static __device__ __forceinline__ D part(const Op &a, const Op &b, const D &d, int i) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], d, 0, 0, 0);
+    }
     static __device__ __forceinline__ D mma(const Op &a, const Op &b) {
         D d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], d, 0, 0, 0);
+        for (int i = 0; i < 4; ++i) d = part(a, b, d, i);
         return d;
     }
 };
@@ -173,17 +182,20 @@ __device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
 typedef __attribute__((address_space(3))) void lds_void;
 // Matrices found through a table: without the address space the compiler would
 // load through flat instructions, which also count as LDS accesses.
+typedef __attribute__((address_space(1))) void global_void;
 typedef __attribute__((address_space(1))) const uint8_t global_u8;
 typedef __attribute__((address_space(1))) const float global_f32;
 typedef __attribute__((address_space(1))) const u32x4 global_u32x4;
 __device__ __forceinline__ void copy16(Desc d, uint32_t voff, uint32_t soff, void *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, soff, 0, 0);
 }
-// This wavefront's loads but the last N (those to LDS among them) and its LDS
-// reads are done, then the workgroup's.
-template <int N>
+__device__ __forceinline__ void copy4(Desc d, uint32_t voff, uint32_t soff, void *lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 4, voff, soff, 0, 0);
+}
+// This wavefront's loads (those to LDS among them) and LDS reads are done, then
+// the workgroup's.
 __device__ __forceinline__ void publish() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // ---- the tiled product -----------------------------------------------------------
@@ -203,30 +215,41 @@ struct TiledArgs {
     const uint8_t *mat;              // kDense
     const uint8_t *const *mats;      // experts
     F8Shape d;                       // of the matrices
-    const uint8_t *xq;               // activation rows [xrows][kb 128]
+    const uint8_t *xq;               // activation rows [kb][xrows][128]
     const float *xs;                 // [kb][xrows]
     uint32_t xrows;
     void *y;                         // kDense: [t x rows]
     const uint2 *tiles;              // experts: {first position, e | rows << 16}
     const int32_t *n_tiles;
+    uint32_t rblocks;                // experts: workgroups to a tile
     const int32_t *row_of_pos;       // kGateUp: the activation row of a position
-    uint8_t *hq;                     // kGateUp: h [positions][hkb 128] and its scales [hkb][hrows]
+    uint8_t *hq;                     // kGateUp: h [hkb][hrows][128] and its scales [hkb][hrows]
     float *hs;
     uint32_t hkb, hrows;
     float *out;                      // kDown: [positions][rows]
 };
 
-template <class P, int RT, int CT, int MODE, typename YT, int NS = 2, int OCC = 2, int TW = 1>
-__global__ __launch_bounds__(256 * TW, OCC) void f8_tiled_kernel(TiledArgs a) {
+template <class P, int RT, int CT, int MODE, typename YT, int TW = 1, bool WL = false>
+__global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     constexpr int M = P::M, kRows = TW * CT * M;  // activation rows of the workgroup
     constexpr int kCopies = CT * M / 32;          // copies of 1 KiB each wavefront makes for a block
     constexpr int kG = P::kGroups;
     static_assert(CT * M % 32 == 0 || kRows == 16, "copies are dealt to the wavefronts");
-    __shared__ __attribute__((aligned(16))) uint8_t stage[NS][kRows * 128];
+    constexpr int kWBytes = WL ? kTileWaves * RT * kKB : 16;
+    static_assert(!WL || M == 32, "a tile in LDS is one of the matrix's");
+    constexpr int kScaleRows = (kRows + 63) / 64 * 64;  // a copy fills 64
+    // A variable to each stage: a read of one is then known not to wait for the
+    // copies that are under way to another.
+    __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * 128], x1[kRows * 128];
+    __shared__ __attribute__((aligned(16))) uint8_t w0[kWBytes], w1[kWBytes];
+    __shared__ float s0[kScaleRows], s1[kScaleRows], s_w[2][kF8MaxCols / 128];
+    auto stage_x = [&](int u) { return u % 2 ? x1 : x0; };
+    auto stage_s = [&](int u) { return u % 2 ? s1 : s0; };
+    auto stage_w = [&](int u) { return u % 2 ? w1 : w0; };
     __shared__ float s_max[kTileWaves][MODE == kGateUp ? kRows : 1];
     const int tid = threadIdx.x, all_wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
     const int wave = all_wave % kTileWaves;  // which weight rows
-    const uint32_t kb_n = a.d.kb, kp = kb_n * 128;
+    const uint32_t kb_n = a.d.kb;
 
     // which activation rows and weights
     uint32_t first, rows, e = 0, rblock;
@@ -246,37 +269,51 @@ __global__ __launch_bounds__(256 * TW, OCC) void f8_tiled_kernel(TiledArgs a) {
         if (first >= a.xrows) return;
         rows = a.xrows - first < kRows ? a.xrows - first : kRows;
     } else {
-        if ((int)blockIdx.y >= *a.n_tiles) return;
-        const uint2 t = a.tiles[blockIdx.y];
+        // Neighbouring workgroups run on different XCDs: the blocks of weight
+        // rows of one tile, which share its activation rows, are given to one.
+        const uint32_t in = blockIdx.x / 8, tile = in / a.rblocks * 8 + blockIdx.x % 8;
+        if ((int)tile >= *a.n_tiles) return;
+        const uint2 t = a.tiles[tile];
         first = t.x;
         e = t.y & 0xFFFFu;
         rows = t.y >> 16;
-        rblock = blockIdx.x;
+        rblock = in % a.rblocks;
     }
-    // this wavefront's row tiles: bases and scales (a tile never spans two
-    // scale blocks; tiles past the matrix read its last and store nothing)
-    global_u8 *base[RT];
-    global_f32 *ws[RT];
+    // row tile r of weight wavefront w: its first row, and where it is (a tile
+    // never spans two scale blocks; tiles past the matrix read its last and
+    // store nothing)
+    auto tile_row = [&](int w, int r) -> uint32_t {
+        if constexpr (MODE == kGateUp) return ((rblock * kTileWaves + w) * (RT / 2) + r % (RT / 2)) * M;
+        else return ((rblock * kTileWaves + w) * RT + r) * M;
+    };
+    auto tile_mat = [&](int r) -> const uint8_t * {
+        if constexpr (MODE == kDense) return a.mat;
+        else return a.mats[(size_t)e * 3 + (MODE == kDown ? 2 : r < RT / 2 ? 0 : 1)];
+    };
+    auto tile_index = [&](uint32_t row) { return row / 32 < a.d.tiles ? row / 32 : a.d.tiles - 1; };
+    global_u8 *base[RT];  // of this wavefront's tiles; with WL, of the ones that it copies
     uint32_t wrow[RT];
     int sub[RT];
+    constexpr int kWMine = WL ? RT / TW : RT;
+    Desc dw[kWMine];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        const uint8_t *mat;
-        if constexpr (MODE == kDense) {
-            mat = a.mat;
-            wrow[r] = ((rblock * kTileWaves + wave) * RT + r) * M;
-        } else if constexpr (MODE == kGateUp) {
-            mat = a.mats[(size_t)e * 3 + (r < RT / 2 ? 0 : 1)];
-            wrow[r] = ((rblock * kTileWaves + wave) * (RT / 2) + r % (RT / 2)) * M;
-        } else {
-            mat = a.mats[(size_t)e * 3 + 2];
-            wrow[r] = ((rblock * kTileWaves + wave) * RT + r) * M;
-        }
-        uint32_t tile = wrow[r] / 32;
-        if (tile >= a.d.tiles) tile = a.d.tiles - 1;
+        wrow[r] = tile_row(wave, r);
         sub[r] = (int)(wrow[r] / 16 & 1);
-        base[r] = (global_u8 *)mat + (size_t)tile * kb_n * kKB;
-        ws[r] = (global_f32 *)(mat + f8_tile_bytes(a.d)) + (size_t)(tile / 4) * kb_n;
+    }
+#pragma unroll
+    for (int i = 0; i < kWMine; ++i) {
+        const int q = WL ? all_wave * kWMine + i : i, w = WL ? q / RT : wave, r = WL ? q % RT : i;
+        base[i] = (global_u8 *)tile_mat(r) + (size_t)tile_index(tile_row(w, r)) * kb_n * kKB;
+        if constexpr (WL) dw[i] = make_desc(tile_mat(r) + (size_t)tile_index(tile_row(w, r)) * kb_n * kKB, kb_n * kKB);
+    }
+    // The weights' scales, for the whole of K: gate's and up's, or those of the
+    // two scale blocks that the workgroup's rows span.
+    constexpr int kSetRows = MODE == kGateUp ? 0 : 128;
+    auto scale_set = [&](int r) { return MODE == kGateUp ? (r < RT / 2 ? 0 : 1) : (int)((wave * RT + r) * M / 128); };
+    for (uint32_t i = tid; i < 2 * kb_n; i += 256 * TW) {
+        const uint32_t set = i / kb_n, row = tile_row(0, 0) + set * kSetRows;
+        s_w[set][i - set * kb_n] = ((global_f32 *)(tile_mat(set ? RT - 1 : 0) + f8_tile_bytes(a.d)))[(size_t)(tile_index(row) / 4) * kb_n + (i - set * kb_n)];
     }
     // this wavefront's activation rows: with two sets of four, each takes half
     uint32_t row0 = 0, mine = rows;
@@ -293,19 +330,23 @@ __global__ __launch_bounds__(256 * TW, OCC) void f8_tiled_kernel(TiledArgs a) {
     };
     uint32_t xbase = 0;
     if constexpr (MODE != kGateUp) xbase = first;
-    // (f8_matmul and f8_experts keep rows times kp below 2^32)
-    const Desc dx = make_desc(a.xq + (size_t)xbase * kp, (a.xrows - xbase) * kp);
+    // (f8_matmul and f8_experts keep the bytes of a call's rows below 2^32)
+    const uint32_t xblock = a.xrows * 128;
+    const Desc dx = make_desc(a.xq + (size_t)xbase * 128, kb_n * xblock - xbase * 128);
+    // (where there are fewer copies than wavefronts, several make the same one:
+    // a branch would split the K loop)
     constexpr int kMine = kCopies ? kCopies : 1;
-    const bool copies = kCopies > 0 || all_wave < 2;  // 16 rows: two wavefronts
     uint32_t voff[kMine];
+    int at[kMine];
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-        const int local = (all_wave * kMine + j) * 8 + l / 8;
-        voff[j] = copies ? (source_row((uint32_t)local) - xbase) * kp + (uint32_t)(((l & 7) ^ swizzle(local)) * 16) : 0;
+        at[j] = (all_wave * kMine + j) * 8 % kRows;
+        const int local = at[j] + l / 8;
+        voff[j] = (source_row((uint32_t)local) - xbase) * 128 + (uint32_t)(((l & 7) ^ swizzle(local)) * 16);
     }
-    uint32_t srow[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) srow[c] = source_row(row0 + (uint32_t)(c * M + P::b_row(l)));
+    const int scale0 = all_wave * 64 % kScaleRows;
+    const uint32_t srow = source_row((uint32_t)(scale0 + l)) * 4;
+    const Desc ds = make_desc(a.xs, 0xFFFFFFFFu);
     uint32_t boff[P::kLoads];
 #pragma unroll
     for (int j = 0; j < P::kLoads; ++j) boff[j] = P::b_row(l) * 128 + ((P::b_chunk(l, j) ^ swizzle(P::b_row(l))) * 16);
@@ -317,82 +358,104 @@ __global__ __launch_bounds__(256 * TW, OCC) void f8_tiled_kernel(TiledArgs a) {
         for (int c = 0; c < CT; ++c) acc[r][c] = typename P::D{};
 
     // The K loop over N of the CT tiles of activation rows (an expert's rows may
-    // fill fewer).  All that a block needs from memory is asked for together:
-    // loads return in order, so one asked for later would wait for the next
-    // block's.  A ring of NS blocks, NS - 1 ahead (past the end the last block
-    // again, so that no branch splits the loop).
+    // fill fewer).  A block is asked for while the one before is computed (past
+    // the end the last one again, so that no branch splits the loop; two blocks
+    // ahead for the weights measured no gain).  Scales go through LDS
+    // too: in registers they would have to be waited for with the blocks asked
+    // for after them.
     auto k_loop = [&](auto tiles_used) {
         constexpr int N = decltype(tiles_used)::value;
-        struct Block {
-            typename P::Raw w[RT];
-            float s[N], sw[RT];
-        };
-        Block b[NS];
+        typename P::Raw b[2][WL ? 1 : RT];  // weights in registers
+        // kept in a scalar register: a copy whose offset the compiler put in a
+        // vector register would be wrapped in a loop over its values
+        const uint32_t last = kb_n - 1;
+        auto clamped = [&](uint32_t block) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(block < last ? block : last)); };
         auto issue = [&](uint32_t block, int u) {
-            // kept in a scalar register: a copy whose offset the compiler put in
-            // a vector register would be wrapped in a loop over its values
-            const uint32_t kb = (uint32_t)__builtin_amdgcn_readfirstlane((int)(block < kb_n ? block : kb_n - 1));
-            if (copies) {
+            const uint32_t kb = clamped(block);
 #pragma unroll
-                for (int j = 0; j < kMine; ++j) copy16(dx, voff[j], kb * 128, &stage[u][(all_wave * kMine + j) * 1024]);
-            }
+            for (int j = 0; j < kMine; ++j) copy16(dx, voff[j], kb * xblock, stage_x(u) + at[j] * 128);
+            copy4(ds, srow + kb * a.xrows * 4, 0, stage_s(u) + scale0);
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+            for (int r = 0; r < kWMine; ++r)
 #pragma unroll
-                for (int j = 0; j < P::kLoads; ++j)
-                    b[u].w[r].q[j] = *reinterpret_cast<const global_u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
-#pragma unroll
-            for (int c = 0; c < N; ++c) b[u].s[c] = a.xs[(size_t)kb * a.xrows + srow[c]];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) b[u].sw[r] = ws[r][kb];
+                for (int j = 0; j < P::kLoads; ++j) {
+                    if constexpr (WL) copy16(dw[r], l * 16, kb * kKB + j * 1024, stage_w(u) + (all_wave * kWMine + r) * kKB + j * 1024);
+                    else b[u % 2][r].q[j] = *reinterpret_cast<const global_u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
+                }
         };
-        // The instructions of a tile are issued ahead of the fmas that take the
-        // tile before it, so that the vector ALU works while they run.
-        auto compute = [&](int u) {
-            const uint8_t *st = stage[u] + row0 * 128;
+        // A wavefront issues in order, and an instruction of the matrix cores
+        // waits there for the one before it: so the fmas that take a tile are
+        // dealt out behind the matrix instructions of the next one.
+        auto compute = [&](uint32_t kb, int u) {
+            const uint8_t *st = stage_x(u) + row0 * 128;
             typename P::Op aw[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) aw[r] = P::op(b[u].w[r]);
-            auto add = [&](int r, int c, const typename P::D &d) {
-                const float s = b[u].s[c] * b[u].sw[r];
+            for (int r = 0; r < RT; ++r) {
+                if constexpr (WL) {
+                    typename P::Raw raw;
 #pragma unroll
-                for (int i = 0; i < 4 * kG; ++i) acc[r][c][i] = __builtin_fmaf(d[i], s, acc[r][c][i]);
-            };
-            typename P::D d;
-#pragma unroll
-            for (int c = 0; c < N; ++c) {
+                    for (int j = 0; j < P::kLoads; ++j)
+                        raw.q[j] = *reinterpret_cast<const u32x4 *>(stage_w(u) + (wave * RT + r) * kKB + P::a_off(l, 0, j));
+                    aw[r] = P::op(raw);
+                } else {
+                    aw[r] = P::op(b[u % 2][r]);
+                }
+            }
+            auto load_b = [&](int c) {
                 typename P::Raw raw;
 #pragma unroll
                 for (int j = 0; j < P::kLoads; ++j) raw.q[j] = *reinterpret_cast<const u32x4 *>(st + c * M * 128 + boff[j]);
+                return raw;
+            };
+            constexpr int kD = 4 * kG, kChunk = (kD + P::kParts - 1) / P::kParts;
+            // chunk i of tile n's fmas
+            auto add = [&](int n, const typename P::D &d, float scale, int i) {
+#pragma unroll
+                for (int v = i * kChunk; v < (i + 1) * kChunk && v < kD; ++v)
+                    acc[n % RT][n / RT][v] = __builtin_fmaf(d[v], scale, acc[n % RT][n / RT][v]);
+            };
+            typename P::D d = {};
+            float scale = 0.0f, sx[N], sw[RT];
+            typename P::Raw raw = load_b(0);
+#pragma unroll
+            for (int c = 0; c < N; ++c) sx[c] = stage_s(u)[row0 + c * M + P::b_row(l)];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) sw[r] = s_w[scale_set(r)][kb];
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
                 const typename P::Op bx = P::op(raw);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    const typename P::D next = P::mma(aw[r], bx);
-                    if (c || r) add(r ? r - 1 : RT - 1, r ? c : c - 1, d);
+                    const int n = c * RT + r;
+                    typename P::D next = {};
+#pragma unroll
+                    for (int i = 0; i < P::kParts; ++i) {
+                        next = P::part(aw[r], bx, next, i);
+                        if (r == RT - 1 && i == 0 && c + 1 < N) raw = load_b(c + 1);
+                        if constexpr (P::kParts == 2) __builtin_amdgcn_sched_barrier(0);
+                        if (n) add(n - 1, d, scale, i);
+                        if constexpr (P::kParts == 2) __builtin_amdgcn_sched_barrier(0);
+                    }
                     d = next;
+                    scale = sx[c] * sw[r];
                 }
             }
-            add(RT - 1, N - 1, d);
+#pragma unroll
+            for (int i = 0; i < P::kParts; ++i) add(N * RT - 1, d, scale, i);
         };
-        // Of the loads after a block's copies at least the copies and weights of
-        // the NS - 2 blocks after it may be in flight.
-        constexpr int kLater = (NS - 2) * (kMine * (kCopies > 0) + RT * P::kLoads);
         auto step = [&](uint32_t kb, int u) {
-            publish<kLater>();
-            issue(kb + NS - 1, (u + NS - 1) % NS);
-            compute(u);
+            publish();
+            issue(kb + 1, u + 1);
+            compute(kb, u);
         };
-#pragma unroll
-        for (int u = 0; u < NS - 1; ++u) issue(u, u);
+        issue(0, 0);
         uint32_t kb = 0;
-        for (; kb + NS <= kb_n; kb += NS) {
-#pragma unroll
-            for (int u = 0; u < NS; ++u) step(kb + u, u);
+        for (; kb + 2 <= kb_n; kb += 2) {
+            step(kb, 0);
+            step(kb + 1, 1);
         }
-#pragma unroll
-        for (int u = 0; u < NS - 1; ++u)
-            if (kb + u < kb_n) step(kb + u, u);
-        publish<0>();  // no copy is under way when the workgroup's LDS goes to another
+        if (kb < kb_n) step(kb, 0);
+        publish();  // no copy is under way when the workgroup's LDS goes to another
     };
     if constexpr (MODE == kDense) {
         k_loop(std::integral_constant<int, CT>{});
@@ -436,7 +499,7 @@ __global__ __launch_bounds__(256 * TW, OCC) void f8_tiled_kernel(TiledArgs a) {
 #pragma unroll
                 for (int g = 0; g < kG; ++g) {
                     const float *v = &h[r][c][4 * g];
-                    *reinterpret_cast<uint32_t *>(a.hq + (size_t)pos * a.hkb * 128 + wrow[r] + P::row(l, g)) =
+                    *reinterpret_cast<uint32_t *>(a.hq + ((size_t)rblock * a.hrows + pos) * 128 + wrow[r] % 128 + P::row(l, g)) =
                         f8_pack4(v[0] * f.inv, v[1] * f.inv, v[2] * f.inv, v[3] * f.inv);
                 }
         }
@@ -601,15 +664,15 @@ bool rows_path(const F8Shape &d, uint32_t t) { return t <= kRowsMax && rows_layo
 
 template <typename XT>
 hipError_t quantize(hipStream_t s, const XT *x, uint32_t t, uint32_t cols, uint32_t kb, uint8_t *xq, float *xs) {
-    f8_quantize_kernel<<<(t * kb * 8 + 255) / 256, 256, 0, s>>>(x, t, cols, kb, xq, xs);
+    f8_quantize_kernel<<<(quantize_chunks(t, kb) + 255) / 256, 256, 0, s>>>(x, t, cols, kb, xq, xs);
     return hipGetLastError();
 }
 
-template <class P, int RT, int CT, typename YT, int NS = 2, int OCC = 2, int TW = 1>
+template <class P, int RT, int CT, typename YT, int TW = 1, bool WL = false>
 hipError_t launch_dense(hipStream_t s, const TiledArgs &a) {
     constexpr uint32_t kM = P::M;
     const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * kM - 1) / (4 * RT * kM), tbs = (a.xrows + TW * CT * kM - 1) / (TW * CT * kM);
-    f8_tiled_kernel<P, RT, CT, kDense, YT, NS, OCC, TW><<<(rbs * tbs + 7) / 8 * 8, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kDense, YT, TW, WL><<<(rbs * tbs + 7) / 8 * 8, 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -632,7 +695,7 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     } else {
         if (t <= 32) return launch_dense<Fp8x32, 1, 1, YT>(s, a);
         if (t <= 64) return launch_dense<Fp8x32, 2, 2, YT>(s, a);
-        return launch_dense<Fp8x32, 2, 3, YT>(s, a);
+        return launch_dense<Fp8x32, 2, 4, YT, 2, true>(s, a);
     }
 }
 
@@ -669,7 +732,7 @@ __global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, ui
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     if (blockIdx.x >= plan_blocks) {
         const uint32_t i = (blockIdx.x - plan_blocks) * kPlanThreads + tid;
-        if (i < a.t * kb * 8) quantize_chunk(x, a.t, hidden, kb, rows_aligned(x, hidden, sizeof(XT)), i, xq, xs);
+        quantize_chunk(x, a.t, hidden, kb, rows_aligned(x, hidden, sizeof(XT)), i, xq, xs);
         return;
     }
     __shared__ int32_t before[kMaxF8Experts], total[kMaxF8Experts], place[kMaxF8Experts];
@@ -956,8 +1019,7 @@ bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
 // experts' in one tile, whose weights are then read once.
 uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
     const uint32_t mean = t * top_k / ex.n_experts;
-    static const int var = getenv("V") ? atoi(getenv("V")) : 0;
-    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : var == 0 ? 192 : 96;
+    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : 192;
 }
 struct ExpertsScratch {
     int32_t *pos_of_pair, *row_of_pos, *n_tiles;
@@ -992,7 +1054,7 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     return b;
 }
 
-template <class P, int RT, int CT, int NS = 2, int OCC = 2, int TW = 1>
+template <class P, int RT, int CT, int TW = 1, bool WL = false>
 hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
     TiledArgs a{};
     a.mats = ex.mats;
@@ -1007,8 +1069,9 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.hs = b.hs;
     a.hkb = (ex.width + 127) / 128;
     a.hrows = pairs;
+    a.rblocks = a.hkb;
     static_assert(RT * P::M == 64, "a workgroup of gate_up makes one block of h");
-    f8_tiled_kernel<P, RT, CT, kGateUp, float, NS, OCC, TW><<<dim3(a.hkb, b.max_tiles), 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kGateUp, float, TW, WL><<<(b.max_tiles + 7) / 8 * 8 * a.rblocks, 256 * TW, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     a.d = f8_shape(ex.hidden, ex.width);
@@ -1016,7 +1079,8 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.xs = b.hs;
     a.xrows = pairs;
     a.out = b.out;
-    f8_tiled_kernel<P, RT, CT, kDown, float, NS, OCC, TW><<<dim3((ex.hidden + 255) / 256, b.max_tiles), 256 * TW, 0, s>>>(a);
+    a.rblocks = (ex.hidden + 255) / 256;
+    f8_tiled_kernel<P, RT, CT, kDown, float, TW, WL><<<(b.max_tiles + 7) / 8 * 8 * a.rblocks, 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1034,18 +1098,16 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
         return hipGetLastError();
     }
     const ExpertsScratch b = experts_scratch(scratch, ex, a.t, a.top_k);
-    const uint32_t plan = (pairs + kPlanThreads - 1) / kPlanThreads, quant = (a.t * dg.kb * 8 + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t plan = (pairs + kPlanThreads - 1) / kPlanThreads, quant = (quantize_chunks(a.t, dg.kb) + kPlanThreads - 1) / kPlanThreads;
     const uint32_t m = tile_rows(ex, a.t, a.top_k);
     f8_plan_kernel<<<plan + quant, kPlanThreads, 0, s>>>(a, m, b.pos_of_pair, b.row_of_pos, b.tiles, b.n_tiles, x, ex.hidden, dg.kb,
                                                         b.xq, b.xs);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    static const int var = getenv("V") ? atoi(getenv("V")) : 0;
     e = m == 16   ? launch_tiles<Fp8x16, 4, 1>(s, ex, b, a.t, pairs)
         : m == 32 ? launch_tiles<Fp8x32, 2, 1>(s, ex, b, a.t, pairs)
         : m == 64 ? launch_tiles<Fp8x32, 2, 2>(s, ex, b, a.t, pairs)
-                  : var == 0 ? launch_tiles<Fp8x32, 2, 3, 2, 2, 2>(s, ex, b, a.t, pairs)
-                  : launch_tiles<Fp8x32, 2, 3, 2, 2, 1>(s, ex, b, a.t, pairs);
+                  : launch_tiles<Fp8x32, 2, 3, 2, true>(s, ex, b, a.t, pairs);
     if (e != hipSuccess) return e;
     f8_combine_kernel<<<dim3((ex.hidden + 1023) / 1024, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, b.out, ex.hidden, y);
     return hipGetLastError();

@@ -61,6 +61,36 @@ def test_logits(be, kind, t, n, hidden, offset):
     be.free_tensor(w)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("hidden", [32, 256, 320, 327])
+def test_logits_of_every_tile_size(be, kind, hidden):
+    """Row and expert counts on both sides of each change of tile: near 64 bits, and bit by bit the same number for a
+    row and an expert whatever stands beside them (the order of the sum does not depend on the tile)."""
+    rng = np.random.default_rng(hidden)
+    t, n = 4096, 259
+    x, r = rng.standard_normal((t, hidden)).astype(np.float32), rng.standard_normal((n, hidden)).astype(np.float32)
+    bits = ref.to_bf16(x) if kind == "bf16" else x
+    xv = (ref.from_bf16(bits) if kind == "bf16" else x).astype(np.float64)
+    want, mag = xv @ r.astype(np.float64).T, np.abs(xv) @ np.abs(r.astype(np.float64)).T
+    tol = (hidden + 24) * 2.0 ** -23 * mag  # as above
+    d_x = be.to_device(bits)
+    whole = None
+    for rows, experts in ((t, n), (t, 17), (1969, 259), (1921, 256), (1025, 256), (1000, 256), (513, 256), (481, 259), (9, 259), (t, 1)):
+        w = be.upload_f32(r[:experts])
+        guard = np.full(rows * experts + 16, 7.0, np.float32)
+        d_l = be.to_device(guard)
+        be.router_logits_device(w, d_x, rows, experts, hidden, d_l, x_type=kind)
+        got = be.read(d_l, np.float32, guard.shape)
+        assert np.array_equal(got[rows * experts:], guard[rows * experts:])
+        got = got[:rows * experts].reshape(rows, experts)
+        assert np.all(np.abs(got - want[:rows, :experts]) <= tol[:rows, :experts])
+        whole = got if whole is None else whole
+        assert np.array_equal(got, whole[:rows, :experts])
+        be.free(d_l)
+        be.free_tensor(w)
+    be.free(d_x)
+
+
 def test_logits_are_near_f32(be):
     """Far from the worst case, both paths are as near to 64 bits as a rounding or two of an f32 sum."""
     rng = np.random.default_rng(5)

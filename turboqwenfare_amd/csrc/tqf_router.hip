@@ -60,9 +60,12 @@ __global__ __launch_bounds__(256) void logits_few_kernel(const float *__restrict
 // last pieces vanish), so R = R0 + R1 + R2, and for bf16 x three products give
 // every bit of x R; f32 x is split as well, and of the nine products the six
 // above 2^-24 of the largest are taken.  The f32 instructions would take five
-// times as long.  Wavefronts split K (8 ways) and take their operands straight
-// from memory: 16 ET experts by 16 TT rows each, no LDS until their sums are
-// added, pairwise.
+// times as long.  A workgroup has 16 ET experts by 16 TT rows; its wavefronts
+// split K (8 ways, a step of 32 columns each in turn) and add their sums in LDS,
+// pairwise, in the same order for every tile size.  4096 bf16 rows of 2048 by 256
+// experts: 19 us, where the three products alone would take 8.6 at the rate of a
+// large library product; the vector units, which split the router's rows anew in
+// every workgroup, and the matrix cores take turns.
 struct Split3 {
     bf16x8 p[3];
 };
@@ -81,95 +84,161 @@ __device__ __forceinline__ Split3 split3(const float (&v)[8]) {
 }
 constexpr int kLogitWaves = 8;
 
-template <int ET, int TT, typename XT>
+// A step's 32 columns of 16 N rows on their way to a wavefront.  A lane that
+// loaded its own operands (row l % 16) would make every one of them a cache
+// access of its own, and the accesses, one a cycle, would bound the kernel: so
+// neighbouring lanes load neighbouring 16 bytes of a row, and the wavefront
+// passes them through an LDS tile that only it uses.  Chunks of a 128-byte line
+// (one f32 row or two bf16 ones) are permuted by the line, so that neither side
+// meets a bank twice.
+template <typename T, int N>
+struct Stage {
+    static constexpr int kRowChunks = 2 * (int)sizeof(T), kLoads = N * kRowChunks / 4, kBytes = kLoads * 1024;
+    u32x4 q[kLoads];
+    const uint8_t *base;   // of the first row
+    uint32_t off[kLoads];  // from there: below 64 rows
+    static __device__ __forceinline__ int slot(int row, int chunk) {
+        const int i = row * kRowChunks + chunk, line = i / 8;
+        return (line * 8 + ((i ^ line) & 7)) * 16;
+    }
+    __device__ __forceinline__ void begin(const T *p, uint32_t hidden, uint32_t row0, uint32_t rows, int l) {
+        base = reinterpret_cast<const uint8_t *>(p + (size_t)row0 * hidden);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const uint32_t row = (j * 64 + l) / kRowChunks;
+            off[j] = (row0 + row < rows ? row : rows - 1 - row0) * hidden * (uint32_t)sizeof(T) + l % kRowChunks * 16;
+        }
+    }
+    __device__ __forceinline__ void ask(uint32_t step) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) q[j] = *reinterpret_cast<const u32x4 *>(base + (size_t)step * 32 * sizeof(T) + off[j]);
+    }
+    __device__ __forceinline__ void put(uint8_t *lds, int l) const {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4 *>(lds + slot((j * 64 + l) / kRowChunks, l % kRowChunks)) = q[j];
+    }
+    // the eight columns 8 g of row 16 i + r
+    static __device__ __forceinline__ Split3 get(const uint8_t *lds, int i, int r, int g) {
+        Split3 s;
+        if constexpr (sizeof(T) == 2) {
+            s.p[0] = *reinterpret_cast<const bf16x8 *>(lds + slot(16 * i + r, g));
+        } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(lds + slot(16 * i + r, 2 * g));
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(lds + slot(16 * i + r, 2 * g + 1));
+            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            s = split3(v);
+        }
+        return s;
+    }
+};
+
+template <int ET, int TT, bool WHOLE, typename XT>
 __global__ __launch_bounds__(64 * kLogitWaves) void logits_kernel(const float *__restrict__ router, const XT *__restrict__ x,
                                                                   uint32_t t, uint32_t n_experts, uint32_t hidden,
                                                                   float *__restrict__ logits) {
-    __shared__ f32x4 red[kLogitWaves / 2][ET * TT][64];
+    // a wavefront's stage, then its sums
+    constexpr int kStage = WHOLE ? Stage<float, ET>::kBytes + Stage<XT, TT>::kBytes : 0, kSums = ET * TT * 1024;
+    constexpr int kMine = kStage > kSums ? kStage : kSums;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kLogitWaves][kMine];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l & 15, g = l >> 4;
-    const uint32_t e0 = blockIdx.x * 16 * ET, t0 = blockIdx.y * 16 * TT;
-    const bool wvec = rows_aligned(router, hidden, 4), xvec = rows_aligned(x, hidden, sizeof(XT));
-    const float *wrow[ET];
-    const XT *xrow[TT];
-#pragma unroll
-    for (int i = 0; i < ET; ++i) {
-        const uint32_t e = e0 + i * 16 + r;
-        wrow[i] = router + (size_t)(e < n_experts ? e : n_experts - 1) * hidden;
-    }
-#pragma unroll
-    for (int i = 0; i < TT; ++i) {
-        const uint32_t row = t0 + i * 16 + r;
-        xrow[i] = x + (size_t)(row < t ? row : t - 1) * hidden;
-    }
+    uint8_t *mine = lds[wave];
+    // neighbouring workgroups run on different XCDs: those of the same rows are
+    // given to one, whose L2 then loads them once
+    const uint32_t ebs = (n_experts + 16 * ET - 1) / (16 * ET), in = blockIdx.x / 8;
+    const uint32_t e0 = in % ebs * 16 * ET, t0 = (in / ebs * 8 + blockIdx.x % 8) * 16 * TT;
+    if (t0 >= t) return;
     f32x4 acc[ET][TT] = {};
+    // a piece of every row tile before the next piece: neighbouring instructions
+    // then add to different sums and need not wait for each other
+    auto multiply = [&](int e, const Split3 &w, const Split3 (&xs)[TT]) {
+        auto add = [&](int wp, int xp) {
+#pragma unroll
+            for (int i = 0; i < TT; ++i) acc[e][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[wp], xs[i].p[xp], acc[e][i], 0, 0, 0);
+        };
+        if constexpr (sizeof(XT) == 2) {
+            add(2, 0);
+            add(1, 0);
+            add(0, 0);
+        } else {
+            add(2, 0);
+            add(1, 1);
+            add(0, 2);
+            add(1, 0);
+            add(0, 1);
+            add(0, 0);
+        }
+    };
     const uint32_t steps = (hidden + 31) / 32;
-    for (uint32_t st = wave; st < steps; st += kLogitWaves) {
-        const uint32_t k = st * 32 + g * 8;
-        const int valid = k < hidden ? (int)(hidden - k) : 0;
-        Split3 xs[TT];
+    if constexpr (WHOLE) {
+        // a step's operands are asked for while the one before is computed
+        Stage<float, ET> ws;
+        Stage<XT, TT> xs;
+        ws.begin(router, hidden, e0, n_experts, l);
+        xs.begin(x, hidden, t0, t, l);
+        uint8_t *wt = mine, *xt = mine + ws.kBytes;
+        auto ask = [&](uint32_t st) {
+            st = st < steps ? st : steps - 1;
+            ws.ask(st);
+            xs.ask(st);
+        };
+        ask(wave);
+        for (uint32_t st = wave; st < steps; st += kLogitWaves) {
+            ws.put(wt, l);
+            xs.put(xt, l);
+            ask(st + kLogitWaves);
+            Split3 xp[TT];
+#pragma unroll
+            for (int i = 0; i < TT; ++i) xp[i] = xs.get(xt, i, r, g);
+#pragma unroll
+            for (int e = 0; e < ET; ++e) {
+                multiply(e, ws.get(wt, e, r, g), xp);
+                if constexpr (sizeof(XT) == 4) __builtin_amdgcn_sched_barrier(0);  // or the next tiles' pieces take all registers
+            }
+        }
+    } else {
+        const bool wvec = rows_aligned(router, hidden, 4), xvec = rows_aligned(x, hidden, sizeof(XT));
+        const float *wrow[ET];
+        const XT *xrow[TT];
+#pragma unroll
+        for (int i = 0; i < ET; ++i) {
+            const uint32_t e = e0 + i * 16 + r;
+            wrow[i] = router + (size_t)(e < n_experts ? e : n_experts - 1) * hidden;
+        }
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-            float v[8];
-            load_row<8>(xrow[i] + k, valid, xvec, v);
-            if constexpr (sizeof(XT) == 2) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) xs[i].p[0][j] = (__bf16)v[j];
-            } else {
-                xs[i] = split3(v);
-            }
+            const uint32_t row = t0 + i * 16 + r;
+            xrow[i] = x + (size_t)(row < t ? row : t - 1) * hidden;
         }
-#pragma unroll
-        for (int e = 0; e < ET; ++e) {
-            float v[8];
-            load_row<8>(wrow[e] + k, valid, wvec, v);
-            const Split3 w = split3(v);
+        for (uint32_t st = wave; st < steps; st += kLogitWaves) {
+            const uint32_t k = st * 32 + g * 8;
+            const int valid = k < hidden ? (int)(hidden - k) : 0;
+            Split3 xs[TT];
 #pragma unroll
             for (int i = 0; i < TT; ++i) {
-                f32x4 a = acc[e][i];
-                auto add = [&](int wp, int xp) { a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[wp], xs[i].p[xp], a, 0, 0, 0); };
-                if constexpr (sizeof(XT) == 2) {
-                    add(2, 0);
-                    add(1, 0);
-                    add(0, 0);
-                } else {
-                    add(2, 0);
-                    add(1, 1);
-                    add(0, 2);
-                    add(1, 0);
-                    add(0, 1);
-                    add(0, 0);
-                }
-                acc[e][i] = a;
+                float v[8];
+                load_row<8>(xrow[i] + k, valid, xvec, v);
+                xs[i] = split3(v);
+            }
+#pragma unroll
+            for (int e = 0; e < ET; ++e) {
+                float v[8];
+                load_row<8>(wrow[e] + k, valid, wvec, v);
+                multiply(e, split3(v), xs);
             }
         }
     }
-    for (int half = kLogitWaves / 2; half >= 1; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
 #pragma unroll
-            for (int e = 0; e < ET; ++e)
+    for (int e = 0; e < ET; ++e)
 #pragma unroll
-                for (int i = 0; i < TT; ++i) red[wave - half][e * TT + i][l] = acc[e][i];
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int e = 0; e < ET; ++e)
-#pragma unroll
-                for (int i = 0; i < TT; ++i) acc[e][i] += red[wave][e * TT + i][l];
-        }
-        __syncthreads();
-    }
-    if (wave) return;
+        for (int i = 0; i < TT; ++i) reinterpret_cast<f32x4 *>(mine)[(e * TT + i) * 64 + l] = acc[e][i];
+    __syncthreads();
     const bool vec = ((reinterpret_cast<uintptr_t>(logits) | (uint64_t)n_experts * 4) & 15) == 0;
-#pragma unroll
-    for (int i = 0; i < TT; ++i) {
-        const uint32_t row = t0 + i * 16 + r;
-        if (row >= t) continue;
-#pragma unroll
-        for (int e = 0; e < ET; ++e) {
-            const uint32_t col = e0 + e * 16 + 4 * g;
-            if (col < n_experts) store4(logits + (size_t)row * n_experts + col, (int)(n_experts - col), vec, acc[e][i]);
-        }
+    for (int tile = wave; tile < ET * TT; tile += kLogitWaves) {
+        auto sum = [&](int w) { return reinterpret_cast<const f32x4 *>(lds[w])[tile * 64 + l]; };
+        auto two = [&](int w) { return sum(w) + sum(w + 4); };
+        const f32x4 v = (two(0) + two(2)) + (two(1) + two(3));
+        const uint32_t row = t0 + tile % TT * 16 + r, col = e0 + tile / TT * 16 + 4 * g;
+        if (row < t && col < n_experts) store4(logits + (size_t)row * n_experts + col, (int)(n_experts - col), vec, v);
     }
 }
 
@@ -316,15 +385,35 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs64 a, const LT *__r
     if (bad && lane == 0 && a.status) *a.status = TQF_HIP_ERR_ROUTER;
 }
 
+template <int ET, int TT, typename XT>
+void logits_many(hipStream_t s, const float *router, const XT *x, uint32_t t, uint32_t n, uint32_t hidden, float *logits) {
+    const uint32_t ebs = (n + 16 * ET - 1) / (16 * ET), tbs = (t + 16 * TT - 1) / (16 * TT), grid = (tbs + 7) / 8 * 8 * ebs;
+    const bool whole = hidden % 32 == 0 && rows_aligned(router, hidden, 4) && rows_aligned(x, hidden, sizeof(XT));
+    if (whole) logits_kernel<ET, TT, true, XT><<<grid, 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
+    else logits_kernel<ET, TT, false, XT><<<grid, 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
+}
 template <typename XT>
 hipError_t logits_launch(hipStream_t s, const float *router, const XT *x, uint32_t t, uint32_t n, uint32_t hidden, float *logits) {
     if (t <= kFewRows) {
         logits_few_kernel<<<n, 256, 0, s>>>(router, x, t, n, hidden, logits);
-    } else if (t <= 512) {
-        logits_kernel<1, 2, XT><<<dim3((n + 15) / 16, (t + 31) / 32), 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
-    } else {
-        logits_kernel<4, 4, XT><<<dim3((n + 63) / 64, (t + 63) / 64), 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
+        return hipGetLastError();
     }
+    // The larger a workgroup's tile, the fewer pieces are split and bytes loaded
+    // for a product; the smaller, the sooner its eight wavefronts are through
+    // their steps.  With 2048 columns and 256 experts, bf16 rows, us:
+    //               1 x 2   2 x 2   2 x 4   2 x 8   4 x 4
+    //   512 rows      7.9                    16.2    18
+    //   1024 rows    10.7    11.0    12.2    16.4    18.1
+    //   4096 rows    35.6    30.7    24.6    19.5    21.7
+    // and f32 rows (2 x 8 would not fit the registers)
+    //   1024 rows    19.8    16.2    22.4            30.5
+    //   4096 rows    62.5    47.9    45.7            36.2
+    const uint64_t tiles = (uint64_t)((n + 15) / 16) * ((t + 15) / 16);
+    if (tiles <= 512) logits_many<1, 2>(s, router, x, t, n, hidden, logits);
+    else if (tiles <= 1024) logits_many<2, 2>(s, router, x, t, n, hidden, logits);
+    else if (tiles <= 2048) logits_many<2, 4>(s, router, x, t, n, hidden, logits);
+    else if constexpr (sizeof(XT) == 2) logits_many<2, 8>(s, router, x, t, n, hidden, logits);
+    else logits_many<4, 4>(s, router, x, t, n, hidden, logits);
     return hipGetLastError();
 }
 

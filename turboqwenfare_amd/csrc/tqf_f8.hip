@@ -242,6 +242,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     // copies that are under way to another.
     __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * 128], x1[kRows * 128];
     __shared__ __attribute__((aligned(16))) uint8_t w0[kWBytes], w1[kWBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t out_lds[MODE != kGateUp && M == 32 && !WL ? kTileWaves * 4096 : 16];
     __shared__ float s0[kScaleRows], s1[kScaleRows], s_w[2][kF8MaxCols / 128];
     auto stage_x = [&](int u) { return u % 2 ? x1 : x0; };
     auto stage_s = [&](int u) { return u % 2 ? s1 : s0; };
@@ -467,6 +468,10 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         else k_loop(std::integral_constant<int, 1>{});
     }
 
+    // Results go to memory through LDS (the stages are free now): a lane has a
+    // few columns of one row, and stored from there every lane's would be a cache
+    // access of its own; passed through LDS, neighbouring lanes store neighbouring
+    // 16 bytes.  Chunks are permuted by the row as the activations' are.
     if constexpr (MODE == kGateUp) {
         // h = silu(g) u, quantised: the workgroup's 128 columns are one block
         constexpr int HT = RT / 2;
@@ -499,27 +504,74 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
 #pragma unroll
                 for (int g = 0; g < kG; ++g) {
                     const float *v = &h[r][c][4 * g];
-                    *reinterpret_cast<uint32_t *>(a.hq + ((size_t)rblock * a.hrows + pos) * 128 + wrow[r] % 128 + P::row(l, g)) =
+                    const uint32_t byte = wrow[r] % 128 + P::row(l, g);
+                    *reinterpret_cast<uint32_t *>(x0 + local * 128 + ((byte / 16 ^ (local & 7)) * 16) + byte % 16) =
                         f8_pack4(v[0] * f.inv, v[1] * f.inv, v[2] * f.inv, v[3] * f.inv);
                 }
         }
+        __syncthreads();
+        for (uint32_t i = tid; i < rows * 8; i += 256 * TW)
+            reinterpret_cast<u32x4 *>(a.hq + ((size_t)rblock * a.hrows + first) * 128)[i] =
+                *reinterpret_cast<const u32x4 *>(x0 + i / 8 * 128 + ((i ^ i / 8) & 7) * 16);
     } else {
         YT *y = MODE == kDense ? static_cast<YT *>(a.y) : reinterpret_cast<YT *>(a.out);
         const uint32_t n = a.d.rows;
-        const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
+        if constexpr (M == 32) {
+            // 32 rows of this wavefront's at a time, a line (128 bytes, or what the
+            // wavefront has) of each
+            constexpr int kEach = 16 / sizeof(YT), kFit = 32 / (int)sizeof(YT) / 8, kTiles = RT < kFit ? RT : kFit;
+            constexpr int kLine = kTiles * 32 * (int)sizeof(YT), kChunks = kLine / 16;
+            uint8_t *mine_lds = (WL ? w0 : out_lds) + all_wave * 4096;
+            const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & 15) == 0;
+            const int row = P::b_row(l);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            const uint32_t in = (uint32_t)(c * M + P::b_row(l)), local = row0 + in;
-            if (in >= mine) continue;
+            for (int c = 0; c < CT; ++c) {
+                if ((uint32_t)(c * 32) >= mine) break;
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+                for (int r0 = 0; r0 < RT; r0 += kTiles) {
 #pragma unroll
-                for (int g = 0; g < kG; ++g) {
-                    const uint32_t col = wrow[r] + P::row(l, g);
-                    if (col >= n) continue;
-                    const f32x4 v = {acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
-                    store4(y + (size_t)(first + local) * n + col, (int)(n - col), vec, v);
+                    for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+                        for (int g = 0; g < kG; ++g) {
+                            const int byte = (r * 32 + P::row(l, g)) * (int)sizeof(YT);
+                            const f32x4 v = {acc[r0 + r][c][4 * g], acc[r0 + r][c][4 * g + 1], acc[r0 + r][c][4 * g + 2], acc[r0 + r][c][4 * g + 3]};
+                            store4(reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16), 4, true, v);
+                        }
+#pragma unroll
+                    for (int j = 0; j < kChunks / 2; ++j) {
+                        const int at = (j * 64 + l) / kChunks, chunk = l % kChunks;
+                        const u32x4 v = *reinterpret_cast<const u32x4 *>(mine_lds + at * kLine + ((chunk ^ at) & (kChunks - 1)) * 16);
+                        const uint32_t in = (uint32_t)(c * 32 + at), col = wrow[r0] + chunk * kEach;
+                        if (in >= mine || col >= n) continue;
+                        YT *to = y + (size_t)(first + row0 + in) * n + col;
+                        if (vec) {
+                            *reinterpret_cast<u32x4 *>(to) = v;
+                        } else {
+                            YT each[kEach];
+                            __builtin_memcpy(each, &v, 16);
+#pragma unroll
+                            for (int k = 0; k < kEach; ++k)
+                                if (col + k < n) to[k] = each[k];
+                        }
+                    }
                 }
+            }
+        } else {
+            const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const uint32_t in = (uint32_t)(c * M + P::b_row(l)), local = row0 + in;
+                if (in >= mine) continue;
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int g = 0; g < kG; ++g) {
+                        const uint32_t col = wrow[r] + P::row(l, g);
+                        if (col >= n) continue;
+                        const f32x4 v = {acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
+                        store4(y + (size_t)(first + local) * n + col, (int)(n - col), vec, v);
+                    }
+            }
         }
     }
 }

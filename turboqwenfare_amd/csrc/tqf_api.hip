@@ -2388,7 +2388,7 @@ extern "C" int32_t tqf_hip_f8_experts_device(tqf_hip_ctx *ctx, const tqf_hip_f8_
     const size_t n = (size_t)t * experts->hidden;
     if (overlap(d_x, n * xb, d_y, n * yb)) return fail(ctx, TQF_HIP_ERR_INVALID, "x and y must not overlap");
     const F8ExpertsDev ex{experts->d_mats, experts->n_experts, experts->hidden, experts->width};
-    if (int32_t rc = ensure_f8_scratch(ctx, f8_experts_scratch_bytes(ex, t, top_k))) return rc;
+    if (int32_t rc = ensure_f8_scratch(ctx, f8_experts_scratch_bytes(ex, t, top_k, y_type))) return rc;
     Prof p(ctx);
     const hipError_t e = launch_f8_experts(ctx->stream, ex, d_x, x_type, t, d_ids, d_w, top_k, d_y, y_type, d_status, ctx->d_f8);
     if (e != hipSuccess) return hip_fail(ctx, "F8 experts launch", e);

@@ -226,8 +226,23 @@ struct TiledArgs {
     uint8_t *hq;                     // kGateUp: h [hkb][hrows][128] and its scales [hkb][hrows]
     float *hs;
     uint32_t hkb, hrows;
-    float *out;                      // kDown: [positions][rows]
+    void *out;                       // kDown: [positions][rows], f32 or Out16
+    float *out_scales;               // Out16's: [positions][rows / 64]
 };
+// The outputs of a pair wait in memory for their weighted sum: as f32, or, where
+// there are many and y is bf16, as 16-bit integers times a scale for each 64
+// columns (one wavefront's).  That halves the bytes written and read again, and
+// costs at most 2^-16 of the largest of the 64, where bf16 y itself is rounded by
+// 2^-9 of the value.  kNotFinite stands for an infinity or NaN.
+typedef int16_t Out16;
+constexpr int kOutBlock = 64, kNotFinite = -32768;
+
+// Two outputs in steps of the scale; inv: one over the block's largest.
+__device__ __forceinline__ uint32_t out16(float a, float b, float inv) {
+    const uint32_t q = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(a * inv, b * inv));
+    const uint32_t lo = fabsf(a) < __builtin_inff() ? q & 0xFFFFu : 0x8000u, hi = fabsf(b) < __builtin_inff() ? q >> 16 : 0x8000u;
+    return lo | hi << 16;
+}
 
 template <class P, int RT, int CT, int MODE, typename YT, int TW = 1, bool WL = false>
 __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
@@ -514,8 +529,10 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
             reinterpret_cast<u32x4 *>(a.hq + ((size_t)rblock * a.hrows + first) * 128)[i] =
                 *reinterpret_cast<const u32x4 *>(x0 + i / 8 * 128 + ((i ^ i / 8) & 7) * 16);
     } else {
-        YT *y = MODE == kDense ? static_cast<YT *>(a.y) : reinterpret_cast<YT *>(a.out);
-        const uint32_t n = a.d.rows;
+        constexpr bool kOut16 = std::is_same<YT, Out16>::value;
+        static_assert(!kOut16 || (MODE == kDown && RT * M == kOutBlock), "a wavefront's columns share a scale");
+        YT *y = MODE == kDense ? static_cast<YT *>(a.y) : static_cast<YT *>(a.out);
+        const uint32_t blocks = (a.d.rows + kOutBlock - 1) / kOutBlock, n = kOut16 ? blocks * kOutBlock : a.d.rows;
         if constexpr (M == 32) {
             // 32 rows of this wavefront's at a time, a line (128 bytes, or what the
             // wavefront has) of each
@@ -527,6 +544,23 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 if ((uint32_t)(c * 32) >= mine) break;
+                float inv = 0.0f;
+                if constexpr (kOut16) {
+                    float m = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4 * kG; ++i) {
+                            const float v = fabsf(acc[r][c][i]);
+                            m = fmaxf(m, v < __builtin_inff() ? v : 0.0f);
+                        }
+                    m = P::across(m);
+                    if (m < 0x1p-100f) m = 0.0f;
+                    inv = m > 0.0f ? 1.0f / m : 0.0f;
+                    const uint32_t in = (uint32_t)(c * 32 + row);
+                    if (l < 32 && in < mine && wrow[0] < n)
+                        a.out_scales[(size_t)(first + row0 + in) * blocks + wrow[0] / kOutBlock] = m * (1.0f / 32767.0f);
+                }
 #pragma unroll
                 for (int r0 = 0; r0 < RT; r0 += kTiles) {
 #pragma unroll
@@ -535,7 +569,9 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                         for (int g = 0; g < kG; ++g) {
                             const int byte = (r * 32 + P::row(l, g)) * (int)sizeof(YT);
                             const f32x4 v = {acc[r0 + r][c][4 * g], acc[r0 + r][c][4 * g + 1], acc[r0 + r][c][4 * g + 2], acc[r0 + r][c][4 * g + 3]};
-                            store4(reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16), 4, true, v);
+                            YT *to = reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16);
+                            if constexpr (kOut16) *reinterpret_cast<uint2 *>(to) = make_uint2(out16(v[0], v[1], inv), out16(v[2], v[3], inv));
+                            else store4(to, 4, true, v);
                         }
 #pragma unroll
                     for (int j = 0; j < kChunks / 2; ++j) {
@@ -890,6 +926,37 @@ __global__ __launch_bounds__(256) void f8_combine_kernel(ExpertsArgs a, const in
     store4(y + (size_t)t * hidden + h, valid, yvec, v);
 }
 
+// The same from Out16: eight columns to a thread.
+__global__ __launch_bounds__(256) void f8_combine16_kernel(ExpertsArgs a, const int32_t *__restrict__ pos_of_pair,
+                                                           const int32_t *__restrict__ n_tiles, const Out16 *__restrict__ out,
+                                                           const float *__restrict__ scales, uint32_t hidden, bool vec,
+                                                           uint16_t *__restrict__ y) {
+    if (*n_tiles < 0) return;
+    const uint32_t t = blockIdx.y, h = (blockIdx.x * 256 + threadIdx.x) * 8, blocks = (hidden + kOutBlock - 1) / kOutBlock;
+    if (h >= hidden) return;
+    float v[8] = {};
+    for (uint32_t k = 0; k < a.top_k; ++k) {
+        const int pos = pos_of_pair[t * a.top_k + k];
+        if (pos < 0) continue;
+        const u32x4 q = *reinterpret_cast<const u32x4 *>(out + (size_t)pos * blocks * kOutBlock + h);
+        const float w = a.w[t * a.top_k + k], scale = scales[(size_t)pos * blocks + h / kOutBlock];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int n = (int16_t)(q[i / 2] >> i % 2 * 16);
+            const float o = n == kNotFinite ? __builtin_nanf("") : (float)n * scale;
+            v[i] = __builtin_fmaf(w, o, v[i]);
+        }
+    }
+    const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+    uint16_t *to = y + (size_t)t * hidden + h;
+    if (vec) {
+        *reinterpret_cast<u32x4 *>(to) = u32x4{bf16_bits2(lo[0], lo[1]), bf16_bits2(lo[2], lo[3]), bf16_bits2(hi[0], hi[1]), bf16_bits2(hi[2], hi[3])};
+    } else {
+        store4(to, (int)(hidden - h), false, lo);
+        store4(to + 4, (int)(hidden - h) - 4, false, hi);
+    }
+}
+
 // Few pairs.  A pair's row is the only column of its products, so all 16
 // columns of the operand are that row (one address for 16 lanes).
 constexpr uint32_t kPairsMax = 64;      // pairs
@@ -1077,11 +1144,13 @@ struct ExpertsScratch {
     int32_t *pos_of_pair, *row_of_pos, *n_tiles;
     uint2 *tiles;
     uint8_t *xq, *hq;
-    float *xs, *hs, *out;
+    float *xs, *hs, *out_scales;
+    void *out;
+    bool out16;
     uint32_t max_tiles;
     size_t total;
 };
-ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
+ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t, uint32_t top_k, int32_t y_type) {
     const size_t P = (size_t)t * top_k, kbh = (ex.hidden + 127) / 128, kbf = (ex.width + 127) / 128;
     const uint32_t m = tile_rows(ex, t, top_k);
     ExpertsScratch b;
@@ -1101,12 +1170,15 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     b.xs = reinterpret_cast<float *>(take((size_t)t * kbh * 4));
     b.hq = take(P * kbf * 128);
     b.hs = reinterpret_cast<float *>(take(P * kbf * 4));
-    b.out = reinterpret_cast<float *>(take(P * ex.hidden * 4));
+    const size_t blocks = (ex.hidden + kOutBlock - 1) / kOutBlock;
+    b.out16 = m >= 64 && y_type == TQF_HIP_TYPE_BF16;
+    b.out = take(b.out16 ? P * blocks * kOutBlock * 2 : P * ex.hidden * 4);
+    b.out_scales = reinterpret_cast<float *>(take(b.out16 ? P * blocks * 4 : 0));
     b.total = off;
     return b;
 }
 
-template <class P, int RT, int CT, int TW = 1, bool WL = false>
+template <class P, int RT, int CT, typename OT, int TW = 1, bool WL = false>
 hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
     TiledArgs a{};
     a.mats = ex.mats;
@@ -1131,8 +1203,9 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.xs = b.hs;
     a.xrows = pairs;
     a.out = b.out;
+    a.out_scales = b.out_scales;
     a.rblocks = (ex.hidden + 255) / 256;
-    f8_tiled_kernel<P, RT, CT, kDown, float, TW, WL><<<(b.max_tiles + 7) / 8 * 8 * a.rblocks, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kDown, OT, TW, WL><<<(b.max_tiles + 7) / 8 * 8 * a.rblocks, 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1149,19 +1222,30 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
         f8_pair_down_kernel<<<dim3((ex.hidden + 15) / 16, a.t), 512, 8 * dd.kb * 260 + a.top_k * 64, s>>>(a, ex.mats, dd, h, hstride, y);
         return hipGetLastError();
     }
-    const ExpertsScratch b = experts_scratch(scratch, ex, a.t, a.top_k);
+    const ExpertsScratch b = experts_scratch(scratch, ex, a.t, a.top_k, sizeof(YT) == 2 ? TQF_HIP_TYPE_BF16 : TQF_HIP_TYPE_F32);
     const uint32_t plan = (pairs + kPlanThreads - 1) / kPlanThreads, quant = (quantize_chunks(a.t, dg.kb) + kPlanThreads - 1) / kPlanThreads;
     const uint32_t m = tile_rows(ex, a.t, a.top_k);
     f8_plan_kernel<<<plan + quant, kPlanThreads, 0, s>>>(a, m, b.pos_of_pair, b.row_of_pos, b.tiles, b.n_tiles, x, ex.hidden, dg.kb,
                                                         b.xq, b.xs);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    e = m == 16   ? launch_tiles<Fp8x16, 4, 1>(s, ex, b, a.t, pairs)
-        : m == 32 ? launch_tiles<Fp8x32, 2, 1>(s, ex, b, a.t, pairs)
-        : m == 64 ? launch_tiles<Fp8x32, 2, 2>(s, ex, b, a.t, pairs)
-                  : launch_tiles<Fp8x32, 2, 3, 2, true>(s, ex, b, a.t, pairs);
+    if (m == 16) {
+        e = launch_tiles<Fp8x16, 4, 1, float>(s, ex, b, a.t, pairs);
+    } else if (m == 32) {
+        e = launch_tiles<Fp8x32, 2, 1, float>(s, ex, b, a.t, pairs);
+    } else {
+        typedef typename std::conditional<sizeof(YT) == 2, Out16, float>::type OT;
+        e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT, 2, true>(s, ex, b, a.t, pairs);
+    }
     if (e != hipSuccess) return e;
-    f8_combine_kernel<<<dim3((ex.hidden + 1023) / 1024, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, b.out, ex.hidden, y);
+    const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)ex.hidden * sizeof(YT)) & 15) == 0;
+    if (sizeof(YT) == 2 && b.out16) {
+        f8_combine16_kernel<<<dim3((ex.hidden + 2047) / 2048, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, static_cast<const Out16 *>(b.out),
+                                                                                b.out_scales, ex.hidden, vec, reinterpret_cast<uint16_t *>(y));
+    } else {
+        f8_combine_kernel<<<dim3((ex.hidden + 1023) / 1024, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, static_cast<const float *>(b.out),
+                                                                              ex.hidden, y);
+    }
     return hipGetLastError();
 }
 
@@ -1189,9 +1273,9 @@ hipError_t launch_f8_matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d,
     return y_type == TQF_HIP_TYPE_F32 ? matmul(s, mat, d, xb, t, yf, scratch) : matmul(s, mat, d, xb, t, yb, scratch);
 }
 
-size_t f8_experts_scratch_bytes(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
+size_t f8_experts_scratch_bytes(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k, int32_t y_type) {
     if (pairs_path(ex, t, top_k)) return (size_t)t * top_k * ((ex.width + 127) / 128 * 128) * 4;
-    return experts_scratch(nullptr, ex, t, top_k).total;
+    return experts_scratch(nullptr, ex, t, top_k, y_type).total;
 }
 
 hipError_t launch_f8_experts(hipStream_t s, const F8ExpertsDev &ex, const void *x, int32_t x_type, uint32_t t,

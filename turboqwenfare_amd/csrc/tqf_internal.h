@@ -594,7 +594,7 @@ struct F8ExpertsDev {
     const uint8_t *const *mats;
     uint32_t n_experts, hidden, width;
 };
-size_t f8_experts_scratch_bytes(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k);
+size_t f8_experts_scratch_bytes(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k, int32_t y_type);
 hipError_t launch_f8_experts(hipStream_t s, const F8ExpertsDev &ex, const void *x, int32_t x_type, uint32_t t,
                              const uint16_t *ids, const float *w, uint32_t top_k, void *y, int32_t y_type, int32_t *status,
                              void *scratch);

@@ -211,16 +211,21 @@ __device__ __forceinline__ int swizzle(int r) { return (r ^ (r >> 3 & 1)) & 7; }
 enum Mode { kDense, kGateUp, kDown };
 constexpr int kTileWaves = 4;
 
+// Rows of one expert, with its matrices, so that a workgroup finds all it needs
+// in one load.  No rows: nothing to do.
+struct Tile {
+    uint32_t first, rows;  // positions
+    const uint8_t *gate, *up, *down;
+};
+
 struct TiledArgs {
     const uint8_t *mat;              // kDense
-    const uint8_t *const *mats;      // experts
     F8Shape d;                       // of the matrices
     const uint8_t *xq;               // activation rows [kb][xrows][128]
     const float *xs;                 // [kb][xrows]
     uint32_t xrows;
     void *y;                         // kDense: [t x rows]
-    const uint2 *tiles;              // experts: {first position, e | rows << 16}
-    const int32_t *n_tiles;
+    const Tile *tiles;               // experts
     uint32_t rblocks;                // experts: workgroups to a tile
     const int32_t *row_of_pos;       // kGateUp: the activation row of a position
     uint8_t *hq;                     // kGateUp: h [hkb][hrows][128] and its scales [hkb][hrows]
@@ -268,7 +273,8 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     const uint32_t kb_n = a.d.kb;
 
     // which activation rows and weights
-    uint32_t first, rows, e = 0, rblock;
+    uint32_t first, rows, rblock;
+    const uint8_t *mat0, *mat1;  // of the first and second half of a wavefront's row tiles
     if constexpr (MODE == kDense) {
         // Neighbouring workgroups run on different XCDs: each XCD is dealt a
         // contiguous share of an order in which four blocks of activation rows
@@ -284,16 +290,20 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         if (rblock >= rbs) return;
         if (first >= a.xrows) return;
         rows = a.xrows - first < kRows ? a.xrows - first : kRows;
+        mat0 = mat1 = a.mat;
     } else {
         // Neighbouring workgroups run on different XCDs: the blocks of weight
-        // rows of one tile, which share its activation rows, are given to one.
-        const uint32_t in = blockIdx.x / 8, tile = in / a.rblocks * 8 + blockIdx.x % 8;
-        if ((int)tile >= *a.n_tiles) return;
-        const uint2 t = a.tiles[tile];
-        first = t.x;
-        e = t.y & 0xFFFFu;
-        rows = t.y >> 16;
-        rblock = in % a.rblocks;
+        // rows of one tile, which share its activation rows, are given to one,
+        // and with them those of a neighbouring tile, which is often the same
+        // expert's and finds its weights in that XCD's L2.
+        const uint32_t in = blockIdx.x / 8, tile = in / a.rblocks / 2 * 16 + blockIdx.x % 8 * 2 + in % 2;
+        const Tile t = a.tiles[tile];
+        if (t.rows == 0) return;
+        first = t.first;
+        rows = t.rows;
+        mat0 = MODE == kGateUp ? t.gate : t.down;
+        mat1 = MODE == kGateUp ? t.up : t.down;
+        rblock = in / 2 % a.rblocks;
     }
     // row tile r of weight wavefront w: its first row, and where it is (a tile
     // never spans two scale blocks; tiles past the matrix read its last and
@@ -302,10 +312,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         if constexpr (MODE == kGateUp) return ((rblock * kTileWaves + w) * (RT / 2) + r % (RT / 2)) * M;
         else return ((rblock * kTileWaves + w) * RT + r) * M;
     };
-    auto tile_mat = [&](int r) -> const uint8_t * {
-        if constexpr (MODE == kDense) return a.mat;
-        else return a.mats[(size_t)e * 3 + (MODE == kDown ? 2 : r < RT / 2 ? 0 : 1)];
-    };
+    auto tile_mat = [&](int r) { return MODE == kGateUp && r >= RT / 2 ? mat1 : mat0; };
     auto tile_index = [&](uint32_t row) { return row / 32 < a.d.tiles ? row / 32 : a.d.tiles - 1; };
     global_u8 *base[RT];  // of this wavefront's tiles; with WL, of the ones that it copies
     uint32_t wrow[RT];
@@ -327,10 +334,23 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     // two scale blocks that the workgroup's rows span.
     constexpr int kSetRows = MODE == kGateUp ? 0 : 128;
     auto scale_set = [&](int r) { return MODE == kGateUp ? (r < RT / 2 ? 0 : 1) : (int)((wave * RT + r) * M / 128); };
-    for (uint32_t i = tid; i < 2 * kb_n; i += 256 * TW) {
-        const uint32_t set = i / kb_n, row = tile_row(0, 0) + set * kSetRows;
-        s_w[set][i - set * kb_n] = ((global_f32 *)(tile_mat(set ? RT - 1 : 0) + f8_tile_bytes(a.d)))[(size_t)(tile_index(row) / 4) * kb_n + (i - set * kb_n)];
+    // Asked for here, before the first block's copies, and kept when those are
+    // under way.
+    constexpr int kScaleLoads = 2 * (kF8MaxCols / 128) / (256 * TW);
+    float w_scale[kScaleLoads];
+#pragma unroll
+    for (int j = 0; j < kScaleLoads; ++j) {
+        const uint32_t i = j * 256 * TW + tid, set = i < kb_n ? 0 : 1, block = i - set * kb_n, row = tile_row(0, 0) + set * kSetRows;
+        if (i < 2 * kb_n)
+            w_scale[j] = ((global_f32 *)((set ? tile_mat(RT - 1) : tile_mat(0)) + f8_tile_bytes(a.d)))[(size_t)(tile_index(row) / 4) * kb_n + block];
     }
+    auto keep_scales = [&] {
+#pragma unroll
+        for (int j = 0; j < kScaleLoads; ++j) {
+            const uint32_t i = j * 256 * TW + tid, set = i < kb_n ? 0 : 1;
+            if (i < 2 * kb_n) s_w[set][i - set * kb_n] = w_scale[j];
+        }
+    };
     // this wavefront's activation rows: with two sets of four, each takes half
     uint32_t row0 = 0, mine = rows;
     if constexpr (TW == 2) {
@@ -386,11 +406,14 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         // vector register would be wrapped in a loop over its values
         const uint32_t last = kb_n - 1;
         auto clamped = [&](uint32_t block) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(block < last ? block : last)); };
-        auto issue = [&](uint32_t block, int u) {
+        auto issue_x = [&](uint32_t block, int u) {
             const uint32_t kb = clamped(block);
 #pragma unroll
             for (int j = 0; j < kMine; ++j) copy16(dx, voff[j], kb * xblock, stage_x(u) + at[j] * 128);
             copy4(ds, srow + kb * a.xrows * 4, 0, stage_s(u) + scale0);
+        };
+        auto issue_w = [&](uint32_t block, int u) {
+            const uint32_t kb = clamped(block);
 #pragma unroll
             for (int r = 0; r < kWMine; ++r)
 #pragma unroll
@@ -461,10 +484,13 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         };
         auto step = [&](uint32_t kb, int u) {
             publish();
-            issue(kb + 1, u + 1);
+            issue_x(kb + 1, u + 1);
+            issue_w(kb + 1, u + 1);
             compute(kb, u);
         };
-        issue(0, 0);
+        issue_w(0, 0);  // first, as it needs no row_of_pos
+        issue_x(0, 0);
+        keep_scales();
         uint32_t kb = 0;
         for (; kb + 2 <= kb_n; kb += 2) {
             step(kb, 0);
@@ -807,12 +833,13 @@ constexpr uint32_t kMaxF8Experts = 1024;
 // needs nothing from the others; within an expert its own pairs take places in
 // the order in which their LDS atomics arrive, which no result depends on: a
 // pair's column of a product is computed alike wherever it stands.  A tile is
-// {first position, e | rows << 16} with at most tile_m rows, an expert's tiles
-// of equal size.  An id that names no expert makes *n_tiles -1: the kernels
-// after this one then do nothing.
+// at most tile_m rows of one expert, an expert's tiles of equal size; those behind
+// the last have no rows.  An id that names no expert makes *n_tiles -1 and leaves
+// no tile with rows: the kernels after this one then do nothing.
 template <typename XT>
 __global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, uint32_t tile_m, int32_t *__restrict__ pos_of_pair,
-                                                               int32_t *__restrict__ row_of_pos, uint2 *__restrict__ tiles,
+                                                               int32_t *__restrict__ row_of_pos, Tile *__restrict__ tiles,
+                                                               uint32_t max_tiles, const uint8_t *const *__restrict__ mats,
                                                                int32_t *__restrict__ n_tiles, const XT *__restrict__ x,
                                                                uint32_t hidden, uint32_t kb, uint8_t *__restrict__ xq,
                                                                float *__restrict__ xs) {
@@ -847,9 +874,12 @@ __global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, ui
     }
     __syncthreads();
     if (s_bad) {
-        if (blockIdx.x == 0 && tid == 0) {
-            *n_tiles = -1;
-            if (a.status) *a.status = TQF_HIP_ERR_INVALID;
+        if (blockIdx.x == 0) {
+            for (uint32_t i = tid; i < max_tiles; i += kPlanThreads) tiles[i].rows = 0;
+            if (tid == 0) {
+                *n_tiles = -1;
+                if (a.status) *a.status = TQF_HIP_ERR_INVALID;
+            }
         }
         return;
     }
@@ -879,9 +909,13 @@ __global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, ui
         const int step = n ? (c + n - 1) / n : 0;
         for (int i = 0; i < n; ++i) {
             const int rows = c - i * step < step ? c - i * step : step;
-            tiles[tbase + i] = make_uint2((uint32_t)(base + i * step), (uint32_t)tid | ((uint32_t)rows << 16));
+            tiles[tbase + i] = Tile{(uint32_t)(base + i * step), (uint32_t)rows, mats[3 * tid], mats[3 * tid + 1], mats[3 * tid + 2]};
         }
-        if (tid == kPlanThreads - 1) *n_tiles = tbase + n;
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < kPlanThreads / 64; ++i) all += s_tiles[i];
+        for (uint32_t i = all + tid; i < max_tiles; i += kPlanThreads) tiles[i].rows = 0;
+        if (tid == 0) *n_tiles = all;
     }
     __syncthreads();
     const uint32_t p = b0 + tid;
@@ -1135,14 +1169,19 @@ bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
     return t * top_k <= kPairsMax && ex.hidden <= kPairsHidden && ex.width <= kPairsWidth;
 }
 // Rows of a tile by the pairs an expert has on average: enough to hold most
-// experts' in one tile, whose weights are then read once.
+// experts' in one tile, whose weights are then read once; but no more than 96, so
+// that a compute unit has two workgroups, of which one computes while the other
+// starts or stores (256 experts, hidden 2048, width 512, top 8, us for tiles of
+// 64 / 96 / 192 rows, the last with weights in LDS: 1100 tokens 181 / 181 / 211,
+// 2048 229 / 204 / 235, 4096 318 / 277 / 285, and 315 / 287 / 329 for a skewed
+// choice of experts).
 uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
     const uint32_t mean = t * top_k / ex.n_experts;
-    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : 192;
+    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : 96;
 }
 struct ExpertsScratch {
     int32_t *pos_of_pair, *row_of_pos, *n_tiles;
-    uint2 *tiles;
+    Tile *tiles;
     uint8_t *xq, *hq;
     float *xs, *hs, *out_scales;
     void *out;
@@ -1154,7 +1193,7 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     const size_t P = (size_t)t * top_k, kbh = (ex.hidden + 127) / 128, kbf = (ex.width + 127) / 128;
     const uint32_t m = tile_rows(ex, t, top_k);
     ExpertsScratch b;
-    b.max_tiles = (uint32_t)(P / m + (P < ex.n_experts ? P : ex.n_experts));
+    b.max_tiles = (uint32_t)(P / m + (P < ex.n_experts ? P : ex.n_experts) + 15) / 16 * 16;  // launched by eights
     uint8_t *p = static_cast<uint8_t *>(scratch);
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -1165,7 +1204,7 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     b.n_tiles = reinterpret_cast<int32_t *>(take(4));
     b.pos_of_pair = reinterpret_cast<int32_t *>(take(P * 4));
     b.row_of_pos = reinterpret_cast<int32_t *>(take(P * 4));
-    b.tiles = reinterpret_cast<uint2 *>(take((size_t)b.max_tiles * 8));
+    b.tiles = reinterpret_cast<Tile *>(take((size_t)b.max_tiles * sizeof(Tile)));
     b.xq = take((size_t)t * kbh * 128);
     b.xs = reinterpret_cast<float *>(take((size_t)t * kbh * 4));
     b.hq = take(P * kbf * 128);
@@ -1181,13 +1220,11 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
 template <class P, int RT, int CT, typename OT, int TW = 1, bool WL = false>
 hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
     TiledArgs a{};
-    a.mats = ex.mats;
     a.d = f8_shape(ex.width, ex.hidden);
     a.xq = b.xq;
     a.xs = b.xs;
     a.xrows = t;
     a.tiles = b.tiles;
-    a.n_tiles = b.n_tiles;
     a.row_of_pos = b.row_of_pos;
     a.hq = b.hq;
     a.hs = b.hs;
@@ -1195,7 +1232,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.hrows = pairs;
     a.rblocks = a.hkb;
     static_assert(RT * P::M == 64, "a workgroup of gate_up makes one block of h");
-    f8_tiled_kernel<P, RT, CT, kGateUp, float, TW, WL><<<(b.max_tiles + 7) / 8 * 8 * a.rblocks, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kGateUp, float, TW, WL><<<b.max_tiles * a.rblocks, 256 * TW, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     a.d = f8_shape(ex.hidden, ex.width);
@@ -1205,7 +1242,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.out = b.out;
     a.out_scales = b.out_scales;
     a.rblocks = (ex.hidden + 255) / 256;
-    f8_tiled_kernel<P, RT, CT, kDown, OT, TW, WL><<<(b.max_tiles + 7) / 8 * 8 * a.rblocks, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kDown, OT, TW, WL><<<b.max_tiles * a.rblocks, 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1225,7 +1262,7 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
     const ExpertsScratch b = experts_scratch(scratch, ex, a.t, a.top_k, sizeof(YT) == 2 ? TQF_HIP_TYPE_BF16 : TQF_HIP_TYPE_F32);
     const uint32_t plan = (pairs + kPlanThreads - 1) / kPlanThreads, quant = (quantize_chunks(a.t, dg.kb) + kPlanThreads - 1) / kPlanThreads;
     const uint32_t m = tile_rows(ex, a.t, a.top_k);
-    f8_plan_kernel<<<plan + quant, kPlanThreads, 0, s>>>(a, m, b.pos_of_pair, b.row_of_pos, b.tiles, b.n_tiles, x, ex.hidden, dg.kb,
+    f8_plan_kernel<<<plan + quant, kPlanThreads, 0, s>>>(a, m, b.pos_of_pair, b.row_of_pos, b.tiles, b.max_tiles, ex.mats, b.n_tiles, x, ex.hidden, dg.kb,
                                                         b.xq, b.xs);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1235,7 +1272,7 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
         e = launch_tiles<Fp8x32, 2, 1, float>(s, ex, b, a.t, pairs);
     } else {
         typedef typename std::conditional<sizeof(YT) == 2, Out16, float>::type OT;
-        e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT, 2, true>(s, ex, b, a.t, pairs);
+        e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT>(s, ex, b, a.t, pairs);
     }
     if (e != hipSuccess) return e;
     const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)ex.hidden * sizeof(YT)) & 15) == 0;

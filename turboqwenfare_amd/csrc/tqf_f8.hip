@@ -1045,12 +1045,11 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
     float *red = s + ((d.kb + 3) & ~3u);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
     const uint32_t pair = blockIdx.y, e = a.ids[pair], row0 = blockIdx.x * 16;
-    if (!ids_ok(a, l)) {
-        if (blockIdx.x == 0 && pair == 0 && tid == 0 && a.status) *a.status = TQF_HIP_ERR_INVALID;
-        return;
-    }
-    if (e == TQF_HIP_NO_EXPERT) return;
-    global_u8 *g = (global_u8 *)mats[(size_t)e * 3], *u = (global_u8 *)mats[(size_t)e * 3 + 1];
+    if (e == TQF_HIP_NO_EXPERT) return;  // (a bad id is reported by its own pair among others)
+    // one trip to memory after another, id, table, weights and scales: everything
+    // else comes behind them.  An id out of range reads expert 0's until it is seen.
+    const size_t m0 = (size_t)(e < a.n_experts ? e : 0) * 3;
+    global_u8 *g = (global_u8 *)mats[m0], *u = (global_u8 *)mats[m0 + 1];
     const uint32_t tile = row0 / 32;
     const int sub = (int)(row0 / 16 & 1);
     const size_t base = (size_t)tile * d.kb * kKB, sbase = f8_tile_bytes(d) + (size_t)(tile / 4) * d.kb * 4;
@@ -1058,6 +1057,7 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
     f32x4 ag = {0.0f, 0.0f, 0.0f, 0.0f}, au = ag;
     constexpr int kAhead = 4;
     typename P::Raw rg[kAhead], ru[kAhead];
+    float sg[kAhead], su[kAhead];
     auto issue = [&](uint32_t b0) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
@@ -1069,9 +1069,15 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
                 rg[i].q[j] = *reinterpret_cast<const global_u32x4 *>(g + at);
                 ru[i].q[j] = *reinterpret_cast<const global_u32x4 *>(u + at);
             }
+            sg[i] = gs[kb];
+            su[i] = us[kb];
         }
     };
     issue(wave);
+    if (!ids_ok(a, l)) {
+        if (blockIdx.x == 0 && tid == 0 && a.status) *a.status = TQF_HIP_ERR_INVALID;
+        return;
+    }
     const XT *row = x + (size_t)(pair / a.top_k) * d.cols;
     quantize_blocks(row, d.cols, rows_aligned(x, d.cols, sizeof(XT)), wave, 4, d.kb, l, q, s);
     __syncthreads();
@@ -1083,11 +1089,11 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
             if (kb >= d.kb) break;
             const typename P::Op b = pair_operand(q, kb, l);
             const f32x4 pg = P::mma(P::op(rg[i]), b), pu = P::mma(P::op(ru[i]), b);
-            const float sg = s[kb] * gs[kb], su = s[kb] * us[kb];
+            const float gscale = s[kb] * sg[i], uscale = s[kb] * su[i];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                ag[v] = __builtin_fmaf(pg[v], sg, ag[v]);
-                au[v] = __builtin_fmaf(pu[v], su, au[v]);
+                ag[v] = __builtin_fmaf(pg[v], gscale, ag[v]);
+                au[v] = __builtin_fmaf(pu[v], uscale, au[v]);
             }
         }
     }
@@ -1115,20 +1121,21 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
     float *red = reinterpret_cast<float *>(lds + (size_t)8 * d.kb * 260);  // [top_k][16]
     const uint32_t token = blockIdx.y, row0 = blockIdx.x * 16, tile = row0 / 32;
     const int sub = (int)(row0 / 16 & 1);
-    if (!ids_ok(a, l)) return;
     const size_t base = (size_t)tile * d.kb * kKB, sbase = f8_tile_bytes(d) + (size_t)(tile / 4) * d.kb * 4;
     for (uint32_t k = wave; k < a.top_k; k += 8) {
         const uint32_t pair = token * a.top_k + k, e = a.ids[pair];
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         if (e != TQF_HIP_NO_EXPERT) {
-            global_u8 *m = (global_u8 *)mats[(size_t)e * 3 + 2];
+            global_u8 *m = (global_u8 *)mats[(size_t)(e < a.n_experts ? e : 0) * 3 + 2];
             global_f32 *ms = (global_f32 *)(m + sbase);
             constexpr int kAhead = 4;
             typename P::Raw raw[kAhead];
+            float sm[kAhead];
             auto issue = [&](uint32_t b0) {
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
                     if (b0 + i >= d.kb) break;
+                    sm[i] = ms[b0 + i];
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         raw[i].q[j] = *reinterpret_cast<const global_u32x4 *>(m + base + (size_t)(b0 + i) * kKB + P::a_off(l, sub, j));
@@ -1144,7 +1151,7 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
                 for (int i = 0; i < kAhead; ++i) {
                     if (b0 + i >= d.kb) break;
                     const f32x4 p = P::mma(P::op(raw[i]), pair_operand(q, b0 + i, l));
-                    const float sc = s[b0 + i] * ms[b0 + i];
+                    const float sc = s[b0 + i] * sm[i];
 #pragma unroll
                     for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(p[v], sc, acc[v]);
                 }
@@ -1153,8 +1160,9 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
         }
         if ((l & 15) == 0) *reinterpret_cast<f32x4 *>(red + k * 16 + P::row(l, 0)) = acc;
     }
+    const bool ok = ids_ok(a, l);  // last, as it waits for nothing that the weights wait for
     __syncthreads();
-    if (tid < 16 && row0 + tid < d.rows) {
+    if (ok && tid < 16 && row0 + tid < d.rows) {
         float v = 0.0f;
         for (uint32_t k = 0; k < a.top_k; ++k) {
             const uint32_t pair = token * a.top_k + k;

@@ -356,13 +356,21 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs64 a, const LT *__r
             val = more ? s[i] : val;
         }
         const uint32_t hi = wave_umax((uint32_t)(best >> 32));
-        const uint32_t lo = wave_umax((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-        if ((hi | lo) == 0) break;
+        if (hi == 0) break;  // (a key that is not 0 has bits above its 32nd)
+        // one lane with the largest upper half has won; several compare the lower
+        // halves, and equals their experts
+        bool won = (uint32_t)(best >> 32) == hi;
+        uint64_t who = __ballot(won);
         const uint32_t e = e0 + at * a.lanes;
-        const bool cand = best == (((uint64_t)hi << 32) | lo);
-        const uint32_t win = ~wave_umax(cand ? ~e : 0u);
-        const bool won = cand && e == win;
-        const int from = (int)__builtin_ctzll(__ballot(won));
+        if (who & (who - 1)) {
+            const uint32_t lo = wave_umax(won ? (uint32_t)best : 0u);
+            won = won && (uint32_t)best == lo;
+            const uint32_t first = ~wave_umax(won ? ~e : 0u);
+            won = won && e == first;
+            who = __ballot(won);
+        }
+        const int from = (int)__builtin_ctzll(who);
+        const uint32_t win = (uint32_t)__builtin_amdgcn_readlane((int)e, from);
         const double sv = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(val), from),
                                            __builtin_amdgcn_readlane(__double2loint(val), from));
         if ((uint32_t)lane == k) {

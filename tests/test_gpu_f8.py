@@ -380,6 +380,50 @@ def test_rows_do_not_see_each_other(small, t):
     assert np.array_equal(shuffled, got[p], equal_nan=True)
 
 
+@pytest.mark.parametrize("y_kind", ["f32", "bf16"])
+@pytest.mark.parametrize("t", [5, 20, 40, 130, 400])
+def test_outputs_of_very_different_sizes(be, t, y_kind):
+    """Columns of one scale block that differ by 2^16, and one that is no number: each as near as it would be alone."""
+    rng = np.random.default_rng(t)
+    n, hidden, width, k = 3, 200, 130, 2
+    mats = [[ref.random_matrix(rng, *shape, spread=1) for shape in ((width, hidden), (width, hidden), (hidden, width))] for _ in range(n)]
+    for e in range(n):
+        q = mats[e][2][0]
+        small_rows = rng.permutation(hidden)[: hidden // 2]
+        q[small_rows] = (q[small_rows] & 0x87) | 0x08  # 2^-6 and above
+        q[small_rows[0]] = (q[small_rows[0]] & 0x86) | 0x78  # 2^8 and above
+    mats[1][2][0][77, 5] = 0x7F  # NaN in one row of expert 1's down matrix
+    layer = Layer.__new__(Layer)
+    layer.be, layer.n, layer.hidden, layer.width = be, n, hidden, width
+    layer.handles = [[be.upload_f8(*m[i]) for m in mats] for i in range(3)]
+    layer.mats = [tuple(ref.values(*m) for m in e) for e in mats]
+    layer.ex = be.prepare_f8_experts(*layer.handles)
+    bits = rows_of(rng, t, hidden, "bf16")
+    ids, w = layer.routes(rng, t, k)
+    got, st = layer.run(bits, "bf16", ids, w, y_kind)
+    assert st == 0
+    got = values_of(got, y_kind).astype(np.float64)
+    hit = (ids == 1).any(1)
+    assert hit.any() and not hit.all()
+    assert np.isnan(got[hit, 77]).all() and not np.isnan(np.delete(got[hit], 77, 1)).any() and not np.isnan(got[~hit]).any()
+    layer.mats[1][2][77] = 0.0
+    want, tol = ref.experts(values_of(bits, "bf16"), ids, w, layer.mats, t * k > 64, y_kind)
+    # pair outputs of many rows may wait as f16: 2^-11 of each, and the sum of a row's pairs is at most the tolerance's sum
+    mag = np.zeros_like(want)
+    for e in range(n):
+        rows, slot = np.nonzero(ids == e)
+        part, _ = ref.experts(values_of(bits, "bf16")[rows], np.full((len(rows), 1), e, np.uint16), w[rows, slot][:, None], layer.mats, t * k > 64, "f32")
+        np.add.at(mag, rows, np.abs(part))
+    tol = tol + (2.0 ** -11 * mag if y_kind == "bf16" else 0)
+    ok = np.ones_like(want, bool)
+    ok[:, 77] = ~hit
+    assert np.all((np.abs(got - want) <= tol + 1e-35)[ok])
+    # the small columns are there, not rounded away beside the large ones: off by far less than their own size
+    err = np.linalg.norm((got - want)[:, ok.all(0)], axis=0) / np.linalg.norm(want[:, ok.all(0)], axis=0)
+    assert err.max() <= 2.0 ** -4, err.max()  # e4m3's half step: h's rounding may move a value by as much
+    layer.close()
+
+
 def test_calls_of_different_sizes_in_turn(small, odd):
     """The scratch of a large call is a smaller one's too, and another layer's."""
     for layer, t, k in ((small, 300, 8), (small, 3, 2), (odd, 100, 5), (small, 40, 8), (odd, 1, 1), (small, 300, 8)):

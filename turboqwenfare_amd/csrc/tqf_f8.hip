@@ -235,18 +235,14 @@ struct TiledArgs {
     float *out_scales;               // Out16's: [positions][rows / 64]
 };
 // The outputs of a pair wait in memory for their weighted sum: as f32, or, where
-// there are many and y is bf16, as 16-bit integers times a scale for each 64
-// columns (one wavefront's).  That halves the bytes written and read again, and
-// costs at most 2^-16 of the largest of the 64, where bf16 y itself is rounded by
-// 2^-9 of the value.  kNotFinite stands for an infinity or NaN.
-typedef int16_t Out16;
-constexpr int kOutBlock = 64, kNotFinite = -32768;
-
-// Two outputs in steps of the scale; inv: one over the block's largest.
-__device__ __forceinline__ uint32_t out16(float a, float b, float inv) {
-    const uint32_t q = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(a * inv, b * inv));
-    const uint32_t lo = fabsf(a) < __builtin_inff() ? q & 0xFFFFu : 0x8000u, hi = fabsf(b) < __builtin_inff() ? q >> 16 : 0x8000u;
-    return lo | hi << 16;
+// there are many and y is bf16, as f16 times a power of two for each 64 columns
+// (one wavefront's) that brings the largest of them below 2^15.  That halves the
+// bytes written and read again; it rounds by 2^-11 of the value (2^-39 of the
+// largest for the smallest ones), where bf16 y itself is rounded by 2^-8.
+typedef _Float16 Out16;
+constexpr int kOutBlock = 64;
+__device__ __forceinline__ uint32_t out16(float a, float b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
 }
 
 template <class P, int RT, int CT, int MODE, typename YT, int TW = 1, bool WL = false>
@@ -581,11 +577,11 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                             m = fmaxf(m, v < __builtin_inff() ? v : 0.0f);
                         }
                     m = P::across(m);
-                    if (m < 0x1p-100f) m = 0.0f;
-                    inv = m > 0.0f ? 1.0f / m : 0.0f;
+                    const uint32_t p = m < 0x1p-100f ? 0 : __float_as_uint(m) & 0x7F800000u;  // 2^e <= m
+                    inv = p ? __uint_as_float((268u << 23) - p) : 0.0f;                // 2^(14 - e)
                     const uint32_t in = (uint32_t)(c * 32 + row);
                     if (l < 32 && in < mine && wrow[0] < n)
-                        a.out_scales[(size_t)(first + row0 + in) * blocks + wrow[0] / kOutBlock] = m * (1.0f / 32767.0f);
+                        a.out_scales[(size_t)(first + row0 + in) * blocks + wrow[0] / kOutBlock] = __uint_as_float(p) * 0x1p-14f;
                 }
 #pragma unroll
                 for (int r0 = 0; r0 < RT; r0 += kTiles) {
@@ -596,7 +592,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                             const int byte = (r * 32 + P::row(l, g)) * (int)sizeof(YT);
                             const f32x4 v = {acc[r0 + r][c][4 * g], acc[r0 + r][c][4 * g + 1], acc[r0 + r][c][4 * g + 2], acc[r0 + r][c][4 * g + 3]};
                             YT *to = reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16);
-                            if constexpr (kOut16) *reinterpret_cast<uint2 *>(to) = make_uint2(out16(v[0], v[1], inv), out16(v[2], v[3], inv));
+                            if constexpr (kOut16) *reinterpret_cast<uint2 *>(to) = make_uint2(out16(v[0] * inv, v[1] * inv), out16(v[2] * inv, v[3] * inv));
                             else store4(to, 4, true, v);
                         }
 #pragma unroll
@@ -976,8 +972,7 @@ __global__ __launch_bounds__(256) void f8_combine16_kernel(ExpertsArgs a, const 
         const float w = a.w[t * a.top_k + k], scale = scales[(size_t)pos * blocks + h / kOutBlock];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int n = (int16_t)(q[i / 2] >> i % 2 * 16);
-            const float o = n == kNotFinite ? __builtin_nanf("") : (float)n * scale;
+            const float o = (float)__builtin_bit_cast(_Float16, (uint16_t)(q[i / 2] >> i % 2 * 16)) * scale;
             v[i] = __builtin_fmaf(w, o, v[i]);
         }
     }

@@ -130,34 +130,25 @@ struct Fp8x32 {  // v_mfma_f32_32x32x64_f8f6f4: two to a block
     }
     static __device__ __forceinline__ float across(float a) { return fmaxf(a, __shfl_xor(a, 32)); }
 };
-struct Fp8x16 {  // v_mfma_f32_16x16x128_f8f6f4: one to a block
+struct Bf16x16 {  // widened to bf16: v_mfma_f32_16x16x32_bf16, four to a block
     static constexpr int M = 16, kLoads = 2, kGroups = 1;
     typedef f32x4 D;
     struct Raw {
         u32x4 q[2];
     };
-    typedef Raw Op;
+    struct Op {
+        bf16x8 v[4];
+    };
     static __device__ __forceinline__ uint32_t a_off(int l, int sub, int j) {
         return (4 * j + (l >> 4)) * 512 + sub * 256 + (l & 15) * 16;
     }
     static __device__ __forceinline__ int b_row(int l) { return l & 15; }
     static __device__ __forceinline__ int b_chunk(int l, int j) { return 4 * j + (l >> 4); }
     static __device__ __forceinline__ int row(int l, int) { return 4 * (l >> 4); }
-    static __device__ __forceinline__ const Op &op(const Raw &r) { return r; }
-    static constexpr int kParts = 1;
-    static __device__ __forceinline__ D part(const Op &a, const Op &b, const D &d, int) {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Fp8x32::pair(a.q[0], a.q[1]), Fp8x32::pair(b.q[0], b.q[1]), d, 0,
-                                                                0, 0, 0, 0, 0);
-    }
     static __device__ __forceinline__ float across(float a) {
         a = fmaxf(a, __shfl_xor(a, 16));
         return fmaxf(a, __shfl_xor(a, 32));
     }
-};
-struct Bf16x16 : Fp8x16 {  // the same tiles, widened to bf16: v_mfma_f32_16x16x32_bf16, four to a block
-    struct Op {
-        bf16x8 v[4];
-    };
     static __device__ __forceinline__ Op op(const Raw &r) {
         return Op{{f8_widen(r.q[0][0], r.q[0][1]), f8_widen(r.q[0][2], r.q[0][3]), f8_widen(r.q[1][0], r.q[1][1]),
                    f8_widen(r.q[1][2], r.q[1][3])}};
@@ -1270,9 +1261,9 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (m == 16) {
-        e = launch_tiles<Fp8x16, 4, 1, float>(s, ex, b, a.t, pairs);
+        e = launch_tiles<Bf16x16, 4, 1, float>(s, ex, b, a.t, pairs);
     } else if (m == 32) {
-        e = launch_tiles<Fp8x32, 2, 1, float>(s, ex, b, a.t, pairs);
+        e = launch_tiles<Bf16x16, 4, 2, float>(s, ex, b, a.t, pairs);
     } else {
         typedef typename std::conditional<sizeof(YT) == 2, Out16, float>::type OT;
         e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT>(s, ex, b, a.t, pairs);

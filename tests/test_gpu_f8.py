@@ -120,6 +120,14 @@ def test_matmul_many_rows(be, t, rows, cols):
         check_matmul(be, t, rows, cols, "f32", y_kind)
 
 
+@pytest.mark.parametrize("kind,y_kind", TYPES)
+@pytest.mark.parametrize("t,rows,cols", [
+    (17, 32768, 140), (17, 32769, 140), (32, 33000, 257), (33, 33001, 129), (64, 32800, 100), (65, 32769, 130), (300, 16500, 700), (257, 40000, 77)])
+def test_matmul_on_both_sides_of_the_split(be, t, rows, cols, kind, y_kind):
+    """Matrices about as large as those from which on tiles take over from wavefronts that split K."""
+    check_matmul(be, t, rows, cols, kind, y_kind)
+
+
 def test_matmul_is_as_exact_as_f32(be):
     """Far from the worst case: f32 results are as near to 64 bits as random roundings of an f32 sum are (a bf16 one as its rounding)."""
     for t in (1, 16, 100):

@@ -82,7 +82,11 @@ __device__ __forceinline__ u32x4 quantize16(const float (&v)[16], float *scale) 
 // Chunk i of x [t x cols]: 16 columns; eight lanes share a block of a row (so all
 // of an aligned group take part or none), a wavefront has eight rows.
 __host__ __device__ __forceinline__ uint32_t quantize_chunks(uint32_t t, uint32_t kb) { return (t + 7) / 8 * 64 * kb; }
-template <typename XT>
+// TILED: by K block in tiles of 32 rows laid out as the weights', so that a
+// wavefront loads an operand of 32 rows as 1 KiB that lies together; scales as
+// [kb][tiles 32].
+constexpr __host__ __device__ uint32_t pad32(uint32_t t) { return (t + 31) / 32 * 32; }
+template <bool TILED, typename XT>
 __device__ __forceinline__ void quantize_chunk(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb, bool vec,
                                                uint32_t i, uint8_t *__restrict__ xq, float *__restrict__ xs) {
     const uint32_t rows8 = i / (64 * kb), block = i / 64 - rows8 * kb, row = rows8 * 8 + i / 8 % 8, k = block * 128 + i % 8 * 16;
@@ -91,15 +95,15 @@ __device__ __forceinline__ void quantize_chunk(const XT *__restrict__ x, uint32_
     float v[16], s;
     load_row<16>(x + (size_t)row * cols + k, valid, vec, v);
     const u32x4 q = quantize16(v, &s);
-    const size_t at = (size_t)block * t + row;
-    reinterpret_cast<u32x4 *>(xq)[at * 8 + i % 8] = q;
+    const size_t at = (size_t)block * (TILED ? pad32(t) : t) + row;
+    reinterpret_cast<u32x4 *>(xq)[TILED ? (at - row % 32) * 8 + i % 8 * 32 + row % 32 : at * 8 + i % 8] = q;
     if (i % 8 == 0) xs[at] = s;
 }
-template <typename XT>
+template <bool TILED, typename XT>
 __global__ __launch_bounds__(256) void f8_quantize_kernel(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb,
                                                           uint8_t *__restrict__ xq, float *__restrict__ xs) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    quantize_chunk(x, t, cols, kb, rows_aligned(x, cols, sizeof(XT)), i, xq, xs);
+    quantize_chunk<TILED>(x, t, cols, kb, rows_aligned(x, cols, sizeof(XT)), i, xq, xs);
 }
 
 // ---- matrix instructions ---------------------------------------------------------
@@ -763,9 +767,102 @@ hipError_t launch_rows(hipStream_t s, const uint8_t *mat, const F8Shape &d, cons
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 bool rows_path(const F8Shape &d, uint32_t t) { return t <= kRowsMax && rows_layout(t, d.kb).total <= kRowsLds; }
 
-template <typename XT>
+// ---- a few hundred rows: K split over the wavefronts -----------------------------
+// Where the tiles of the product above would leave most compute units without
+// work.  A workgroup takes one tile of 32 weight rows by 32 NT activation rows;
+// its eight wavefronts take the K blocks in turn, straight from memory to
+// registers (both operands lie as the instructions take them), a block ahead,
+// and add their sums in LDS, pairwise.
+constexpr int kSplitWaves = 8;
+
+template <class P, int NT, typename YT>
+__global__ __launch_bounds__(64 * kSplitWaves) void f8_split_kernel(const uint8_t *__restrict__ mat, F8Shape d,
+                                                                    const uint8_t *__restrict__ xq, const float *__restrict__ xs,
+                                                                    uint32_t t, YT *__restrict__ y) {
+    constexpr int M = P::M, RT = 32 / M, CT = 32 * NT / M, kG = P::kGroups, kQuads = RT * CT * kG;
+    __shared__ f32x4 red[kSplitWaves][kQuads][64];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    // neighbouring workgroups run on different XCDs: those of one tile of weights
+    // are given to one
+    const uint32_t chunks = (t + 32 * NT - 1) / (32 * NT), in = blockIdx.x / 8, tile = in / chunks * 8 + blockIdx.x % 8;
+    const uint32_t t0 = in % chunks * 32 * NT, t_tiles = pad32(t) / 32;
+    if (tile * 32 >= d.rows) return;
+    const uint8_t *w = mat + (size_t)tile * d.kb * kKB;
+    const float *ws = reinterpret_cast<const float *>(mat + f8_tile_bytes(d)) + (size_t)(tile / 4) * d.kb;
+    uint32_t x_tile[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x_tile[n] = t0 / 32 + n < t_tiles ? t0 / 32 + n : t_tiles - 1;
+
+    typename P::D acc[RT][CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[r][c] = typename P::D{};
+    typename P::Raw a[2][RT], b[2][CT];
+    float sx[2][CT], sw[2];
+    auto ask = [&](uint32_t block, int u) {
+        const uint32_t kb = block < d.kb ? block : d.kb - 1;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int j = 0; j < P::kLoads; ++j) a[u][r].q[j] = *reinterpret_cast<const u32x4 *>(w + (size_t)kb * kKB + P::a_off(l, r, j));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const size_t at = (size_t)kb * t_tiles + x_tile[c * M / 32];
+#pragma unroll
+            for (int j = 0; j < P::kLoads; ++j) b[u][c].q[j] = *reinterpret_cast<const u32x4 *>(xq + at * kKB + P::a_off(l, c % RT, j));
+            sx[u][c] = xs[at * 32 + c % RT * M + P::b_row(l)];
+        }
+        sw[u] = ws[kb];
+    };
+    auto compute = [&](int u) {
+        typename P::Op aw[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) aw[r] = P::op(a[u][r]);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const typename P::Op bx = P::op(b[u][c]);
+            const float scale = sx[u][c] * sw[u];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                typename P::D p = {};
+#pragma unroll
+                for (int i = 0; i < P::kParts; ++i) p = P::part(aw[r], bx, p, i);
+#pragma unroll
+                for (int v = 0; v < 4 * kG; ++v) acc[r][c][v] = __builtin_fmaf(p[v], scale, acc[r][c][v]);
+            }
+        }
+    };
+    ask(wave, 0);
+    for (uint32_t kb = wave; kb < d.kb; kb += 2 * kSplitWaves) {
+        ask(kb + kSplitWaves, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(0);
+        ask(kb + 2 * kSplitWaves, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kb + kSplitWaves < d.kb) compute(1);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int g = 0; g < kG; ++g)
+                red[wave][(r * CT + c) * kG + g][l] = f32x4{acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
+    __syncthreads();
+    const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)d.rows * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
+    for (int q = wave; q < kQuads; q += kSplitWaves) {
+        const int g = q % kG, c = q / kG % CT, r = q / kG / CT;
+        auto two = [&](int i) { return red[i][q][l] + red[i + 4][q][l]; };
+        const f32x4 v = (two(0) + two(2)) + (two(1) + two(3));
+        const uint32_t row = t0 + c * M + P::b_row(l), col = tile * 32 + r * M + P::row(l, g);
+        if (row < t && col < d.rows) store4(y + (size_t)row * d.rows + col, (int)(d.rows - col), vec, v);
+    }
+}
+
+template <bool TILED, typename XT>
 hipError_t quantize(hipStream_t s, const XT *x, uint32_t t, uint32_t cols, uint32_t kb, uint8_t *xq, float *xs) {
-    f8_quantize_kernel<<<(quantize_chunks(t, kb) + 255) / 256, 256, 0, s>>>(x, t, cols, kb, xq, xs);
+    f8_quantize_kernel<TILED><<<(quantize_chunks(t, kb) + 255) / 256, 256, 0, s>>>(x, t, cols, kb, xq, xs);
     return hipGetLastError();
 }
 
@@ -777,12 +874,42 @@ hipError_t launch_dense(hipStream_t s, const TiledArgs &a) {
     return hipGetLastError();
 }
 
+template <class P, int NT, typename YT>
+hipError_t launch_split(hipStream_t s, const uint8_t *mat, const F8Shape &d, const uint8_t *xq, const float *xs, uint32_t t, YT *y) {
+    const uint32_t tiles = (d.rows + 31) / 32, chunks = (t + 32 * NT - 1) / (32 * NT);
+    f8_split_kernel<P, NT, YT><<<(tiles + 7) / 8 * 8 * chunks, 64 * kSplitWaves, 0, s>>>(mat, d, xq, xs, t, y);
+    return hipGetLastError();
+}
+
+// A workgroup's activation rows where K is split; 0: the tiled product is faster,
+// as it is once its larger tiles (which load less for a product) fill the card.
+// us, split / tiled: 64 bf16 rows of 4096 by 8192 12.2 / 26.4, 256 26.5 / 50, 512
+// (1024 workgroups) 45 / 52, 1024 88 / 56, 256 by 20000 (1250) 59 / 53; f32 rows of
+// the same by 8192, 64 rows 13 / 32, 512 56 / 46.  f32 takes 32 rows always (256
+// rows 31, in steps of 64 33, of 128 40).
+uint32_t split_rows(const F8Shape &d, uint32_t t, bool f32) {
+    const uint32_t rows = f32 || t <= 32 ? 32 : t <= 64 ? 64 : 128;
+    return (uint64_t)((d.rows + 31) / 32) * ((t + rows - 1) / rows) <= 1024 ? rows : 0;
+}
+
 template <typename XT, typename YT>
 hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT *x, uint32_t t, YT *y, void *scratch) {
     if (rows_path(d, t)) return launch_rows(s, mat, d, x, t, y);
     uint8_t *xq = static_cast<uint8_t *>(scratch);
-    float *xs = reinterpret_cast<float *>(xq + align256((size_t)t * d.kb * 128));
-    hipError_t e = quantize(s, x, t, d.cols, d.kb, xq, xs);
+    float *xs = reinterpret_cast<float *>(xq + align256((size_t)pad32(t) * d.kb * 128));
+    constexpr bool kF32 = sizeof(YT) == 4;
+    if (const uint32_t rows = split_rows(d, t, kF32)) {
+        hipError_t e = quantize<true>(s, x, t, d.cols, d.kb, xq, xs);
+        if (e != hipSuccess) return e;
+        if constexpr (kF32) {
+            return launch_split<Bf16x16, 1, YT>(s, mat, d, xq, xs, t, y);
+        } else {
+            return rows == 32   ? launch_split<Fp8x32, 1, YT>(s, mat, d, xq, xs, t, y)
+                   : rows == 64 ? launch_split<Fp8x32, 2, YT>(s, mat, d, xq, xs, t, y)
+                                : launch_split<Fp8x32, 4, YT>(s, mat, d, xq, xs, t, y);
+        }
+    }
+    hipError_t e = quantize<false>(s, x, t, d.cols, d.kb, xq, xs);
     if (e != hipSuccess) return e;
     TiledArgs a{};
     a.mat = mat;
@@ -791,7 +918,7 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     a.xs = xs;
     a.xrows = t;
     a.y = y;
-    if constexpr (sizeof(YT) == 4) {
+    if constexpr (kF32) {
         return t <= 32 ? launch_dense<Bf16x16, 2, 2, YT>(s, a) : launch_dense<Bf16x16, 2, 4, YT>(s, a);
     } else {
         if (t <= 32) return launch_dense<Fp8x32, 1, 1, YT>(s, a);
@@ -834,7 +961,7 @@ __global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, ui
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     if (blockIdx.x >= plan_blocks) {
         const uint32_t i = (blockIdx.x - plan_blocks) * kPlanThreads + tid;
-        quantize_chunk(x, a.t, hidden, kb, rows_aligned(x, hidden, sizeof(XT)), i, xq, xs);
+        quantize_chunk<false>(x, a.t, hidden, kb, rows_aligned(x, hidden, sizeof(XT)), i, xq, xs);
         return;
     }
     __shared__ int32_t before[kMaxF8Experts], total[kMaxF8Experts], place[kMaxF8Experts];
@@ -1290,7 +1417,7 @@ hipError_t launch_f8_repack(hipStream_t s, const uint8_t *q, const float *scales
 
 size_t f8_matmul_scratch_bytes(const F8Shape &d, uint32_t t) {
     if (rows_path(d, t)) return 0;
-    return align256((size_t)t * d.kb * 128) + align256((size_t)t * d.kb * 4);
+    return align256((size_t)pad32(t) * d.kb * 128) + align256((size_t)pad32(t) * d.kb * 4);
 }
 
 hipError_t launch_f8_matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const void *x, int32_t x_type, uint32_t t,

@@ -109,9 +109,26 @@ struct Stage {
             off[j] = (row0 + row < rows ? row : rows - 1 - row0) * hidden * (uint32_t)sizeof(T) + l % kRowChunks * 16;
         }
     }
-    __device__ __forceinline__ void ask(uint32_t step) {
+    // Rows may begin anywhere (an odd number of columns): the loads need no
+    // alignment but the type's.  TAIL: the last step is no whole one; its columns
+    // are taken one by one.
+    template <bool TAIL>
+    __device__ __forceinline__ void ask(uint32_t step, uint32_t hidden, int l) {
+        const uint8_t *p = base + (size_t)step * 32 * sizeof(T);
+        if (!TAIL || (step + 1) * 32 <= hidden) {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) q[j] = *reinterpret_cast<const u32x4 *>(base + (size_t)step * 32 * sizeof(T) + off[j]);
+            for (int j = 0; j < kLoads; ++j) __builtin_memcpy(&q[j], __builtin_assume_aligned(p + off[j], sizeof(T)), 16);
+        } else {
+            constexpr int kEach = 16 / sizeof(T);
+            const uint32_t k = step * 32 + l % kRowChunks * kEach;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                T v[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) v[i] = k + i < hidden ? reinterpret_cast<const T *>(p + off[j])[i] : T{};
+                __builtin_memcpy(&q[j], v, 16);
+            }
+        }
     }
     __device__ __forceinline__ void put(uint8_t *lds, int l) const {
 #pragma unroll
@@ -132,12 +149,12 @@ struct Stage {
     }
 };
 
-template <int ET, int TT, bool WHOLE, typename XT>
+template <int ET, int TT, bool TAIL, typename XT>
 __global__ __launch_bounds__(64 * kLogitWaves) void logits_kernel(const float *__restrict__ router, const XT *__restrict__ x,
                                                                   uint32_t t, uint32_t n_experts, uint32_t hidden,
                                                                   float *__restrict__ logits) {
     // a wavefront's stage, then its sums
-    constexpr int kStage = WHOLE ? Stage<float, ET>::kBytes + Stage<XT, TT>::kBytes : 0, kSums = ET * TT * 1024;
+    constexpr int kStage = Stage<float, ET>::kBytes + Stage<XT, TT>::kBytes, kSums = ET * TT * 1024;
     constexpr int kMine = kStage > kSums ? kStage : kSums;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kLogitWaves][kMine];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l & 15, g = l >> 4;
@@ -169,62 +186,36 @@ __global__ __launch_bounds__(64 * kLogitWaves) void logits_kernel(const float *_
         }
     };
     const uint32_t steps = (hidden + 31) / 32;
-    if constexpr (WHOLE) {
-        // a step's operands are asked for while the one before is computed
-        Stage<float, ET> ws;
-        Stage<XT, TT> xs;
-        ws.begin(router, hidden, e0, n_experts, l);
-        xs.begin(x, hidden, t0, t, l);
-        uint8_t *wt = mine, *xt = mine + ws.kBytes;
-        auto ask = [&](uint32_t st) {
+    // a step's operands are asked for while the one before is computed
+    Stage<float, ET> ws;
+    Stage<XT, TT> xs;
+    ws.begin(router, hidden, e0, n_experts, l);
+    xs.begin(x, hidden, t0, t, l);
+    uint8_t *wt = mine, *xt = mine + ws.kBytes;
+    auto ask = [&](uint32_t st) {
+        // behind the last step nothing is loaded, or, where the branch costs more
+        // than the load (4096 rows 20.5 us, 19 without it; 512 rows 7.1, and 8.1
+        // without it), the last step again
+        if (TAIL || ET * TT <= 4) {
+            if (st >= steps) return;
+        } else {
             st = st < steps ? st : steps - 1;
-            ws.ask(st);
-            xs.ask(st);
-        };
-        ask(wave);
-        for (uint32_t st = wave; st < steps; st += kLogitWaves) {
-            ws.put(wt, l);
-            xs.put(xt, l);
-            ask(st + kLogitWaves);
-            Split3 xp[TT];
-#pragma unroll
-            for (int i = 0; i < TT; ++i) xp[i] = xs.get(xt, i, r, g);
-#pragma unroll
-            for (int e = 0; e < ET; ++e) {
-                multiply(e, ws.get(wt, e, r, g), xp);
-                if constexpr (sizeof(XT) == 4) __builtin_amdgcn_sched_barrier(0);  // or the next tiles' pieces take all registers
-            }
         }
-    } else {
-        const bool wvec = rows_aligned(router, hidden, 4), xvec = rows_aligned(x, hidden, sizeof(XT));
-        const float *wrow[ET];
-        const XT *xrow[TT];
+        ws.template ask<TAIL>(st, hidden, l);
+        xs.template ask<TAIL>(st, hidden, l);
+    };
+    ask(wave);
+    for (uint32_t st = wave; st < steps; st += kLogitWaves) {
+        ws.put(wt, l);
+        xs.put(xt, l);
+        ask(st + kLogitWaves);
+        Split3 xp[TT];
 #pragma unroll
-        for (int i = 0; i < ET; ++i) {
-            const uint32_t e = e0 + i * 16 + r;
-            wrow[i] = router + (size_t)(e < n_experts ? e : n_experts - 1) * hidden;
-        }
+        for (int i = 0; i < TT; ++i) xp[i] = xs.get(xt, i, r, g);
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-            const uint32_t row = t0 + i * 16 + r;
-            xrow[i] = x + (size_t)(row < t ? row : t - 1) * hidden;
-        }
-        for (uint32_t st = wave; st < steps; st += kLogitWaves) {
-            const uint32_t k = st * 32 + g * 8;
-            const int valid = k < hidden ? (int)(hidden - k) : 0;
-            Split3 xs[TT];
-#pragma unroll
-            for (int i = 0; i < TT; ++i) {
-                float v[8];
-                load_row<8>(xrow[i] + k, valid, xvec, v);
-                xs[i] = split3(v);
-            }
-#pragma unroll
-            for (int e = 0; e < ET; ++e) {
-                float v[8];
-                load_row<8>(wrow[e] + k, valid, wvec, v);
-                multiply(e, split3(v), xs);
-            }
+        for (int e = 0; e < ET; ++e) {
+            multiply(e, ws.get(wt, e, r, g), xp);
+            if constexpr (sizeof(XT) == 4) __builtin_amdgcn_sched_barrier(0);  // or the next tiles' pieces take all registers
         }
     }
 #pragma unroll
@@ -396,9 +387,8 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs64 a, const LT *__r
 template <int ET, int TT, typename XT>
 void logits_many(hipStream_t s, const float *router, const XT *x, uint32_t t, uint32_t n, uint32_t hidden, float *logits) {
     const uint32_t ebs = (n + 16 * ET - 1) / (16 * ET), tbs = (t + 16 * TT - 1) / (16 * TT), grid = (tbs + 7) / 8 * 8 * ebs;
-    const bool whole = hidden % 32 == 0 && rows_aligned(router, hidden, 4) && rows_aligned(x, hidden, sizeof(XT));
-    if (whole) logits_kernel<ET, TT, true, XT><<<grid, 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
-    else logits_kernel<ET, TT, false, XT><<<grid, 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
+    if (hidden % 32 == 0) logits_kernel<ET, TT, false, XT><<<grid, 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
+    else logits_kernel<ET, TT, true, XT><<<grid, 64 * kLogitWaves, 0, s>>>(router, x, t, n, hidden, logits);
 }
 template <typename XT>
 hipError_t logits_launch(hipStream_t s, const float *router, const XT *x, uint32_t t, uint32_t n, uint32_t hidden, float *logits) {
@@ -410,12 +400,12 @@ hipError_t logits_launch(hipStream_t s, const float *router, const XT *x, uint32
     // for a product; the smaller, the sooner its eight wavefronts are through
     // their steps.  With 2048 columns and 256 experts, bf16 rows, us:
     //               1 x 2   2 x 2   2 x 4   2 x 8   4 x 4
-    //   512 rows      7.9                    16.2    18
-    //   1024 rows    10.7    11.0    12.2    16.4    18.1
-    //   4096 rows    35.6    30.7    24.6    19.5    21.7
+    //   512 rows      7.1                    16.2    18
+    //   1024 rows    10.7    10.5    12.2    16.4    18.1
+    //   4096 rows    35.6    30.7    24.6    19.3    21.7
     // and f32 rows (2 x 8 would not fit the registers)
-    //   1024 rows    19.8    16.2    22.4            30.5
-    //   4096 rows    62.5    47.9    45.7            36.2
+    //   1024 rows    19.8    16.1    22.4            30.5
+    //   4096 rows    62.5    47.9    45.7            35.2
     const uint64_t tiles = (uint64_t)((n + 15) / 16) * ((t + 15) / 16);
     if (tiles <= 512) logits_many<1, 2>(s, router, x, t, n, hidden, logits);
     else if (tiles <= 1024) logits_many<2, 2>(s, router, x, t, n, hidden, logits);

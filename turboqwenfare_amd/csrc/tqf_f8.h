@@ -58,30 +58,25 @@ __device__ __forceinline__ bf16x8 f8_widen(uint32_t lo, uint32_t hi) {
 }
 
 // ---- elements of the callers' types ------------------------------------------
-// N consecutive elements at p as f32, the first `valid` of them (0 past that);
-// `vec`: p is 16-byte aligned, so that whole groups may be loaded wide.
+// N consecutive elements at p as f32, the first `valid` of them (0 past that).
+// The wide loads need no alignment but the elements'.
 template <int N>
-__device__ __forceinline__ void load_row(const float *p, int valid, bool vec, float (&v)[N]) {
-    if (vec && valid >= N) {
+__device__ __forceinline__ void load_row(const float *p, int valid, float (&v)[N]) {
+    if (valid >= N) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const f32x4 f = *reinterpret_cast<const f32x4 *>(p + i);
-            v[i] = f[0];
-            v[i + 1] = f[1];
-            v[i + 2] = f[2];
-            v[i + 3] = f[3];
-        }
+        for (int i = 0; i < N; i += 4) __builtin_memcpy(&v[i], p + i, 16);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = i < valid ? p[i] : 0.0f;
     }
 }
 template <int N>
-__device__ __forceinline__ void load_row(const uint16_t *p, int valid, bool vec, float (&v)[N]) {
-    if (vec && valid >= N) {
+__device__ __forceinline__ void load_row(const uint16_t *p, int valid, float (&v)[N]) {
+    if (valid >= N) {
 #pragma unroll
         for (int i = 0; i < N; i += 8) {
-            const u32x4 f = *reinterpret_cast<const u32x4 *>(p + i);
+            u32x4 f;
+            __builtin_memcpy(&f, p + i, 16);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 v[i + 2 * j] = __uint_as_float(f[j] << 16);
@@ -92,11 +87,6 @@ __device__ __forceinline__ void load_row(const uint16_t *p, int valid, bool vec,
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = i < valid ? __uint_as_float((uint32_t)p[i] << 16) : 0.0f;
     }
-}
-// Whether rows of `cols` elements of sz bytes at p can be loaded 16 bytes at a
-// time from every multiple of 16 elements.
-__host__ __device__ inline bool rows_aligned(const void *p, uint32_t cols, uint32_t sz) {
-    return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)cols * sz) & 15) == 0;
 }
 
 // Four consecutive outputs at p, the first `valid` of them; `vec`: p is aligned

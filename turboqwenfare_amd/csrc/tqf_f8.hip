@@ -87,13 +87,13 @@ __host__ __device__ __forceinline__ uint32_t quantize_chunks(uint32_t t, uint32_
 // [kb][tiles 32].
 constexpr __host__ __device__ uint32_t pad32(uint32_t t) { return (t + 31) / 32 * 32; }
 template <bool TILED, typename XT>
-__device__ __forceinline__ void quantize_chunk(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb, bool vec,
+__device__ __forceinline__ void quantize_chunk(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb,
                                                uint32_t i, uint8_t *__restrict__ xq, float *__restrict__ xs) {
     const uint32_t rows8 = i / (64 * kb), block = i / 64 - rows8 * kb, row = rows8 * 8 + i / 8 % 8, k = block * 128 + i % 8 * 16;
     if (row >= t) return;
     const int valid = k < cols ? (int)(cols - k) : 0;
     float v[16], s;
-    load_row<16>(x + (size_t)row * cols + k, valid, vec, v);
+    load_row<16>(x + (size_t)row * cols + k, valid, v);
     const u32x4 q = quantize16(v, &s);
     const size_t at = (size_t)block * (TILED ? pad32(t) : t) + row;
     reinterpret_cast<u32x4 *>(xq)[TILED ? (at - row % 32) * 8 + i % 8 * 32 + row % 32 : at * 8 + i % 8] = q;
@@ -103,7 +103,7 @@ template <bool TILED, typename XT>
 __global__ __launch_bounds__(256) void f8_quantize_kernel(const XT *__restrict__ x, uint32_t t, uint32_t cols, uint32_t kb,
                                                           uint8_t *__restrict__ xq, float *__restrict__ xs) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    quantize_chunk<TILED>(x, t, cols, kb, rows_aligned(x, cols, sizeof(XT)), i, xq, xs);
+    quantize_chunk<TILED>(x, t, cols, kb, i, xq, xs);
 }
 
 // ---- matrix instructions ---------------------------------------------------------
@@ -660,11 +660,10 @@ __global__ __launch_bounds__(kRowsThreads) void f8_rows_kernel(const uint8_t *__
     const RowsLayout L = rows_layout(t, d.kb);
     float *xs = reinterpret_cast<float *>(lds + L.scales);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
-    const bool vec = rows_aligned(x, d.cols, sizeof(XT));
     for (uint32_t i = tid; i < t * d.kb * 8; i += kRowsThreads) {
         const uint32_t row = i / (8 * d.kb), c = i - row * 8 * d.kb, k = c * 16;
         float v[16], s;
-        load_row<16>(x + (size_t)row * d.cols + k, k < d.cols ? (int)(d.cols - k) : 0, vec, v);
+        load_row<16>(x + (size_t)row * d.cols + k, k < d.cols ? (int)(d.cols - k) : 0, v);
         *reinterpret_cast<u32x4 *>(lds + row * L.stride + k) = quantize16(v, &s);
         if ((c & 7) == 0) xs[row * d.kb + (c >> 3)] = s;
     }
@@ -961,7 +960,7 @@ __global__ __launch_bounds__(kPlanThreads) void f8_plan_kernel(ExpertsArgs a, ui
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     if (blockIdx.x >= plan_blocks) {
         const uint32_t i = (blockIdx.x - plan_blocks) * kPlanThreads + tid;
-        quantize_chunk<false>(x, a.t, hidden, kb, rows_aligned(x, hidden, sizeof(XT)), i, xq, xs);
+        quantize_chunk<false>(x, a.t, hidden, kb, i, xq, xs);
         return;
     }
     __shared__ int32_t before[kMaxF8Experts], total[kMaxF8Experts], place[kMaxF8Experts];
@@ -1122,12 +1121,12 @@ __device__ __forceinline__ bool ids_ok(const ExpertsArgs &a, int lane) {
 // values quantised to bf16 into q [kb][128] and their scales into s [kb].
 // Sixteen lanes take a block, eight values each.
 template <typename XT>
-__device__ __forceinline__ void quantize_blocks(const XT *x, uint32_t cols, bool vec, uint32_t b0, uint32_t step, uint32_t n,
+__device__ __forceinline__ void quantize_blocks(const XT *x, uint32_t cols, uint32_t b0, uint32_t step, uint32_t n,
                                                 int lane, uint16_t *q, float *s) {
     for (uint32_t b = b0; b < n; b += 4 * step) {
         const uint32_t kb = b + (lane / 16) * step, k = kb * 128 + (lane % 16) * 8;
         float v[8], m = 0.0f;
-        load_row<8>(x + k, kb < n && k < cols ? (int)(cols - k) : 0, vec, v);
+        load_row<8>(x + k, kb < n && k < cols ? (int)(cols - k) : 0, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
         m = amax8(m);
@@ -1192,7 +1191,7 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
         return;
     }
     const XT *row = x + (size_t)(pair / a.top_k) * d.cols;
-    quantize_blocks(row, d.cols, rows_aligned(x, d.cols, sizeof(XT)), wave, 4, d.kb, l, q, s);
+    quantize_blocks(row, d.cols, wave, 4, d.kb, l, q, s);
     __syncthreads();
     for (uint32_t b0 = wave; b0 < d.kb; b0 += 4 * kAhead) {
         if (b0 != (uint32_t)wave) issue(b0);
@@ -1255,7 +1254,7 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
                 }
             };
             issue(0);
-            quantize_blocks(h + (size_t)pair * hstride, d.cols, true, 0, 1, d.kb, l, q, s);
+            quantize_blocks(h + (size_t)pair * hstride, d.cols, 0, 1, d.kb, l, q, s);
             // this wavefront's own writes: LDS serves it in order
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             for (uint32_t b0 = 0; b0 < d.kb; b0 += kAhead) {

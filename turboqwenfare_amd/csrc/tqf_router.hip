@@ -29,16 +29,15 @@ __global__ __launch_bounds__(256) void logits_few_kernel(const float *__restrict
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
     const uint32_t e = blockIdx.x;
     const float *r = router + (size_t)e * hidden;
-    const bool wvec = rows_aligned(router, hidden, 4), xvec = rows_aligned(x, hidden, sizeof(XT));
     double acc[kFewRows] = {};
     for (uint32_t k = tid * 8; k < hidden; k += 2048) {
         float w[8];
-        load_row<8>(r + k, (int)(hidden - k), wvec, w);
+        load_row<8>(r + k, (int)(hidden - k), w);
 #pragma unroll
         for (uint32_t i = 0; i < kFewRows; ++i) {
             if (i >= t) break;
             float v[8];
-            load_row<8>(x + (size_t)i * hidden + k, (int)(hidden - k), xvec, v);
+            load_row<8>(x + (size_t)i * hidden + k, (int)(hidden - k), v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[i] = __builtin_fma((double)w[j], (double)v[j], acc[i]);
         }

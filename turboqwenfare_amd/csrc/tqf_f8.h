@@ -89,23 +89,24 @@ __device__ __forceinline__ void load_row(const uint16_t *p, int valid, float (&v
     }
 }
 
-// Four consecutive outputs at p, the first `valid` of them; `vec`: p is aligned
-// to four elements.  bf16 is rounded to nearest, ties to even.
+// Four consecutive outputs at p, the first `valid` of them, at any alignment.
+// bf16 is rounded to nearest, ties to even.
 __device__ __forceinline__ uint32_t bf16_bits2(float a, float b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
 }
-__device__ __forceinline__ void store4(float *p, int valid, bool vec, f32x4 v) {
-    if (vec && valid >= 4) {
-        *reinterpret_cast<f32x4 *>(p) = v;
+__device__ __forceinline__ void store4(float *p, int valid, f32x4 v) {
+    if (valid >= 4) {
+        __builtin_memcpy(p, &v, 16);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < valid) p[i] = v[i];
     }
 }
-__device__ __forceinline__ void store4(uint16_t *p, int valid, bool vec, f32x4 v) {
-    if (vec && valid >= 4) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(bf16_bits2(v[0], v[1]), bf16_bits2(v[2], v[3]));
+__device__ __forceinline__ void store4(uint16_t *p, int valid, f32x4 v) {
+    if (valid >= 4) {
+        const uint2 b = make_uint2(bf16_bits2(v[0], v[1]), bf16_bits2(v[2], v[3]));
+        __builtin_memcpy(p, &b, 8);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)

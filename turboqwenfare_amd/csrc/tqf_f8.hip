@@ -556,7 +556,6 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
             constexpr int kEach = 16 / sizeof(YT), kFit = 32 / (int)sizeof(YT) / 8, kTiles = RT < kFit ? RT : kFit;
             constexpr int kLine = kTiles * 32 * (int)sizeof(YT), kChunks = kLine / 16;
             uint8_t *mine_lds = (WL ? w0 : out_lds) + all_wave * 4096;
-            const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & 15) == 0;
             const int row = P::b_row(l);
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
@@ -588,7 +587,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                             const f32x4 v = {acc[r0 + r][c][4 * g], acc[r0 + r][c][4 * g + 1], acc[r0 + r][c][4 * g + 2], acc[r0 + r][c][4 * g + 3]};
                             YT *to = reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16);
                             if constexpr (kOut16) *reinterpret_cast<uint2 *>(to) = make_uint2(out16(v[0] * inv, v[1] * inv), out16(v[2] * inv, v[3] * inv));
-                            else store4(to, 4, true, v);
+                            else store4(static_cast<YT *>(__builtin_assume_aligned(to, 4 * sizeof(YT))), 4, v);
                         }
 #pragma unroll
                     for (int j = 0; j < kChunks / 2; ++j) {
@@ -597,8 +596,8 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                         const uint32_t in = (uint32_t)(c * 32 + at), col = wrow[r0] + chunk * kEach;
                         if (in >= mine || col >= n) continue;
                         YT *to = y + (size_t)(first + row0 + in) * n + col;
-                        if (vec) {
-                            *reinterpret_cast<u32x4 *>(to) = v;
+                        if (col + kEach <= n) {
+                            __builtin_memcpy(to, &v, 16);
                         } else {
                             YT each[kEach];
                             __builtin_memcpy(each, &v, 16);
@@ -610,7 +609,6 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                 }
             }
         } else {
-            const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)n * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 const uint32_t in = (uint32_t)(c * M + P::b_row(l)), local = row0 + in;
@@ -622,7 +620,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                         const uint32_t col = wrow[r] + P::row(l, g);
                         if (col >= n) continue;
                         const f32x4 v = {acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
-                        store4(y + (size_t)(first + local) * n + col, (int)(n - col), vec, v);
+                        store4(y + (size_t)(first + local) * n + col, (int)(n - col), v);
                     }
             }
         }
@@ -674,7 +672,6 @@ __global__ __launch_bounds__(kRowsThreads) void f8_rows_kernel(const uint8_t *__
     const float *sx = xs + token * d.kb;
     const float *scales = reinterpret_cast<const float *>(mat + f8_tile_bytes(d));
     const uint32_t units = (d.rows + 16 * SUB - 1) / (16 * SUB);
-    const bool yvec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)d.rows * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
     const uint32_t u0 = SPLIT ? blockIdx.x : blockIdx.x * kRowsWaves + wave, ustep = SPLIT ? gridDim.x : gridDim.x * kRowsWaves;
     for (uint32_t u = u0; u < units; u += ustep) {
         const uint32_t row0 = u * 16 * SUB, tile = row0 / 32;
@@ -723,7 +720,7 @@ __global__ __launch_bounds__(kRowsThreads) void f8_rows_kernel(const uint8_t *__
                 for (int i = 1; i < kRowsWaves; ++i) v += red[(i * SUB + wave) * 64 + l];
                 const uint32_t col = row0 + wave * 16 + P::row(l, 0);
                 if ((uint32_t)P::b_row(l) < t && col < d.rows)
-                    store4(y + (size_t)P::b_row(l) * d.rows + col, (int)(d.rows - col), yvec, v);
+                    store4(y + (size_t)P::b_row(l) * d.rows + col, (int)(d.rows - col), v);
             }
             __syncthreads();
         } else {
@@ -731,7 +728,7 @@ __global__ __launch_bounds__(kRowsThreads) void f8_rows_kernel(const uint8_t *__
             for (int s = 0; s < SUB; ++s) {
                 const uint32_t col = row0 + s * 16 + P::row(l, 0);
                 if ((uint32_t)P::b_row(l) < t && col < d.rows)
-                    store4(y + (size_t)P::b_row(l) * d.rows + col, (int)(d.rows - col), yvec, acc[s]);
+                    store4(y + (size_t)P::b_row(l) * d.rows + col, (int)(d.rows - col), acc[s]);
             }
         }
     }
@@ -849,13 +846,12 @@ __global__ __launch_bounds__(64 * kSplitWaves) void f8_split_kernel(const uint8_
             for (int g = 0; g < kG; ++g)
                 red[wave][(r * CT + c) * kG + g][l] = f32x4{acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
     __syncthreads();
-    const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)d.rows * sizeof(YT)) & (4 * sizeof(YT) - 1)) == 0;
     for (int q = wave; q < kQuads; q += kSplitWaves) {
         const int g = q % kG, c = q / kG % CT, r = q / kG / CT;
         auto two = [&](int i) { return red[i][q][l] + red[i + 4][q][l]; };
         const f32x4 v = (two(0) + two(2)) + (two(1) + two(3));
         const uint32_t row = t0 + c * M + P::b_row(l), col = tile * 32 + r * M + P::row(l, g);
-        if (row < t && col < d.rows) store4(y + (size_t)row * d.rows + col, (int)(d.rows - col), vec, v);
+        if (row < t && col < d.rows) store4(y + (size_t)row * d.rows + col, (int)(d.rows - col), v);
     }
 }
 
@@ -1051,32 +1047,23 @@ __global__ __launch_bounds__(256) void f8_combine_kernel(ExpertsArgs a, const in
     const uint32_t t = blockIdx.y, h = (blockIdx.x * 256 + threadIdx.x) * 4;
     if (h >= hidden) return;
     const int valid = (int)(hidden - h);
-    const bool vec = (hidden & 3) == 0;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t k = 0; k < a.top_k; ++k) {
         const int pos = pos_of_pair[t * a.top_k + k];
         if (pos < 0) continue;
         const float w = a.w[t * a.top_k + k];
-        const float *src = out + (size_t)pos * hidden + h;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (vec) {
-            o = *reinterpret_cast<const f32x4 *>(src);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < valid) o[i] = src[i];
-        }
+        float o[4];
+        load_row<4>(out + (size_t)pos * hidden + h, valid, o);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(w, o[i], v[i]);
     }
-    const bool yvec = vec && (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(YT) - 1)) == 0;
-    store4(y + (size_t)t * hidden + h, valid, yvec, v);
+    store4(y + (size_t)t * hidden + h, valid, v);
 }
 
 // The same from Out16: eight columns to a thread.
 __global__ __launch_bounds__(256) void f8_combine16_kernel(ExpertsArgs a, const int32_t *__restrict__ pos_of_pair,
                                                            const int32_t *__restrict__ n_tiles, const Out16 *__restrict__ out,
-                                                           const float *__restrict__ scales, uint32_t hidden, bool vec,
+                                                           const float *__restrict__ scales, uint32_t hidden,
                                                            uint16_t *__restrict__ y) {
     if (*n_tiles < 0) return;
     const uint32_t t = blockIdx.y, h = (blockIdx.x * 256 + threadIdx.x) * 8, blocks = (hidden + kOutBlock - 1) / kOutBlock;
@@ -1095,11 +1082,12 @@ __global__ __launch_bounds__(256) void f8_combine16_kernel(ExpertsArgs a, const 
     }
     const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
     uint16_t *to = y + (size_t)t * hidden + h;
-    if (vec) {
-        *reinterpret_cast<u32x4 *>(to) = u32x4{bf16_bits2(lo[0], lo[1]), bf16_bits2(lo[2], lo[3]), bf16_bits2(hi[0], hi[1]), bf16_bits2(hi[2], hi[3])};
+    if (hidden - h >= 8) {
+        const u32x4 b = {bf16_bits2(lo[0], lo[1]), bf16_bits2(lo[2], lo[3]), bf16_bits2(hi[0], hi[1]), bf16_bits2(hi[2], hi[3])};
+        __builtin_memcpy(to, &b, 16);
     } else {
-        store4(to, (int)(hidden - h), false, lo);
-        store4(to + 4, (int)(hidden - h) - 4, false, hi);
+        store4(to, (int)(hidden - h), lo);
+        store4(to + 4, (int)(hidden - h) - 4, hi);
     }
 }
 
@@ -1281,7 +1269,7 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
             if (a.ids[pair] != TQF_HIP_NO_EXPERT) v = __builtin_fmaf(a.w[pair], red[k * 16 + tid], v);
         }
         const f32x4 one = {v, 0.0f, 0.0f, 0.0f};
-        store4(y + (size_t)token * d.rows + row0 + tid, 1, false, one);
+        store4(y + (size_t)token * d.rows + row0 + tid, 1, one);
     }
 }
 
@@ -1395,10 +1383,9 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
         e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT>(s, ex, b, a.t, pairs);
     }
     if (e != hipSuccess) return e;
-    const bool vec = ((reinterpret_cast<uintptr_t>(y) | (uint64_t)ex.hidden * sizeof(YT)) & 15) == 0;
     if (sizeof(YT) == 2 && b.out16) {
         f8_combine16_kernel<<<dim3((ex.hidden + 2047) / 2048, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, static_cast<const Out16 *>(b.out),
-                                                                                b.out_scales, ex.hidden, vec, reinterpret_cast<uint16_t *>(y));
+                                                                                b.out_scales, ex.hidden, reinterpret_cast<uint16_t *>(y));
     } else {
         f8_combine_kernel<<<dim3((ex.hidden + 1023) / 1024, a.t), 256, 0, s>>>(a, b.pos_of_pair, b.n_tiles, static_cast<const float *>(b.out),
                                                                               ex.hidden, y);

@@ -222,13 +222,12 @@ __global__ __launch_bounds__(64 * kLogitWaves) void logits_kernel(const float *_
 #pragma unroll
         for (int i = 0; i < TT; ++i) reinterpret_cast<f32x4 *>(mine)[(e * TT + i) * 64 + l] = acc[e][i];
     __syncthreads();
-    const bool vec = ((reinterpret_cast<uintptr_t>(logits) | (uint64_t)n_experts * 4) & 15) == 0;
     for (int tile = wave; tile < ET * TT; tile += kLogitWaves) {
         auto sum = [&](int w) { return reinterpret_cast<const f32x4 *>(lds[w])[tile * 64 + l]; };
         auto two = [&](int w) { return sum(w) + sum(w + 4); };
         const f32x4 v = (two(0) + two(2)) + (two(1) + two(3));
         const uint32_t row = t0 + tile % TT * 16 + r, col = e0 + tile / TT * 16 + 4 * g;
-        if (row < t && col < n_experts) store4(logits + (size_t)row * n_experts + col, (int)(n_experts - col), vec, v);
+        if (row < t && col < n_experts) store4(logits + (size_t)row * n_experts + col, (int)(n_experts - col), v);
     }
 }
 

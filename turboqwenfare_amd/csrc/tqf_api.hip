@@ -15,6 +15,7 @@
 
 #include "../../include/tqf_hip.h"
 #include "../../include/tqf_hip_synth.h"
+#include "tqf_batch.h"
 #include "tqf_internal.h"
 
 using namespace tqf;
@@ -762,7 +763,6 @@ extern "C" int32_t tqf_hip_destroy(tqf_hip_ctx *ctx) {
     (void)hipFree(ctx->d_q4k);
     (void)hipFree(ctx->d_lm);
     (void)hipFree(ctx->d_grouped);
-    (void)hipFree(ctx->d_f8);
     (void)hipFree(ctx->d_sample);
     (void)hipFree(const_cast<const uint8_t **>(ctx->d_adhoc_mats));
     for (Slab &s : ctx->slabs) (void)hipFree(s.base);
@@ -2244,12 +2244,14 @@ int32_t f8_upload_from(tqf_hip_ctx *ctx, const uint8_t *d_q, const float *d_scal
     return TQF_HIP_OK;
 }
 
-// Grows the F8 scratch (the context's stream has drained before the old one goes).
+// Grows the scratch that the F8 products share with the grouped ones (on the one
+// stream, each call is done with it before the next begins; the stream has drained
+// before the old one goes).
 int32_t ensure_f8_scratch(tqf_hip_ctx *ctx, size_t bytes) {
-    if (bytes == 0 || (ctx->d_f8 && ctx->f8_bytes >= bytes)) return TQF_HIP_OK;
+    if (bytes == 0 || (ctx->d_grouped && ctx->grouped_bytes >= bytes)) return TQF_HIP_OK;
     TQF_HIP(ctx, hipStreamSynchronize(ctx->stream));
-    if (grow(ctx->d_f8, ctx->f8_bytes, bytes) != hipSuccess) {
-        ctx->d_f8 = nullptr;
+    if (grow(ctx->d_grouped, ctx->grouped_bytes, bytes) != hipSuccess) {
+        ctx->d_grouped = nullptr;
         (void)hipGetLastError();
         return fail(ctx, TQF_HIP_ERR_NOMEM, "F8 scratch allocation failed");
     }
@@ -2320,7 +2322,7 @@ extern "C" int32_t tqf_hip_f8_matmul_device(tqf_hip_ctx *ctx, const tqf_hip_weig
         return fail(ctx, TQF_HIP_ERR_INVALID, "x and y must not overlap");
     if (int32_t rc = ensure_f8_scratch(ctx, f8_matmul_scratch_bytes(d, t))) return rc;
     Prof p(ctx);
-    const hipError_t e = launch_f8_matmul(ctx->stream, w->tiles, d, d_x, x_type, t, d_y, y_type, ctx->d_f8);
+    const hipError_t e = launch_f8_matmul(ctx->stream, w->tiles, d, d_x, x_type, t, d_y, y_type, ctx->d_grouped);
     if (e != hipSuccess) return hip_fail(ctx, "F8 product launch", e);
     p.end(TQF_HIP_KERNEL_F8_MATMUL,
           (double)t * d.cols * xb + (double)t * d.rows * yb + (double)d.rows * d.cols + 4.0 * f8_scale_count(d), 0, nullptr);
@@ -2390,7 +2392,7 @@ extern "C" int32_t tqf_hip_f8_experts_device(tqf_hip_ctx *ctx, const tqf_hip_f8_
     const F8ExpertsDev ex{experts->d_mats, experts->n_experts, experts->hidden, experts->width};
     if (int32_t rc = ensure_f8_scratch(ctx, f8_experts_scratch_bytes(ex, t, top_k, y_type))) return rc;
     Prof p(ctx);
-    const hipError_t e = launch_f8_experts(ctx->stream, ex, d_x, x_type, t, d_ids, d_w, top_k, d_y, y_type, d_status, ctx->d_f8);
+    const hipError_t e = launch_f8_experts(ctx->stream, ex, d_x, x_type, t, d_ids, d_w, top_k, d_y, y_type, d_status, ctx->d_grouped);
     if (e != hipSuccess) return hip_fail(ctx, "F8 experts launch", e);
     p.end(TQF_HIP_KERNEL_F8_EXPERTS, 0.0, 0, nullptr);
     return TQF_HIP_OK;

@@ -16,7 +16,7 @@
 #pragma once
 
 #include "tqf_device.h"
-#include "tqf_internal.h"
+#include "tqf_batch.h"
 
 namespace tqf {
 

@@ -256,7 +256,7 @@ __device__ __forceinline__ float logit_of(const float *p, size_t i) { return p[i
 __device__ __forceinline__ float logit_of(const uint16_t *p, size_t i) { return __uint_as_float((uint32_t)p[i] << 16); }
 
 template <int N, typename LT>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs64 a, const LT *__restrict__ logits) {
+__global__ __launch_bounds__(256) void pick_routes_kernel(RouteArgs64 a, const LT *__restrict__ logits) {
     const int lane = threadIdx.x % 64;
     const uint32_t row = blockIdx.x * 4 + threadIdx.x / 64;
     if (row >= a.t) return;
@@ -416,12 +416,12 @@ hipError_t logits_launch(hipStream_t s, const float *router, const XT *x, uint32
 template <typename LT>
 hipError_t route_launch(hipStream_t s, const RouteArgs64 &a, const LT *logits) {
     const uint32_t n = (a.per + a.lanes - 1) / a.lanes, grid = (a.t + 3) / 4;
-    if (n <= 1) route_kernel<1><<<grid, 256, 0, s>>>(a, logits);
-    else if (n <= 2) route_kernel<2><<<grid, 256, 0, s>>>(a, logits);
-    else if (n <= 4) route_kernel<4><<<grid, 256, 0, s>>>(a, logits);
-    else if (n <= 8) route_kernel<8><<<grid, 256, 0, s>>>(a, logits);
-    else if (n <= 16) route_kernel<16><<<grid, 256, 0, s>>>(a, logits);
-    else if (n <= 32) route_kernel<32><<<grid, 256, 0, s>>>(a, logits);
+    if (n <= 1) pick_routes_kernel<1><<<grid, 256, 0, s>>>(a, logits);
+    else if (n <= 2) pick_routes_kernel<2><<<grid, 256, 0, s>>>(a, logits);
+    else if (n <= 4) pick_routes_kernel<4><<<grid, 256, 0, s>>>(a, logits);
+    else if (n <= 8) pick_routes_kernel<8><<<grid, 256, 0, s>>>(a, logits);
+    else if (n <= 16) pick_routes_kernel<16><<<grid, 256, 0, s>>>(a, logits);
+    else if (n <= 32) pick_routes_kernel<32><<<grid, 256, 0, s>>>(a, logits);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }

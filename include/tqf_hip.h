@@ -475,11 +475,13 @@ int32_t tqf_hip_f8_weights_upload_device(tqf_hip_ctx *ctx, const void *d_q, size
 int32_t tqf_hip_f8_weights_download(tqf_hip_ctx *ctx, const tqf_hip_weights *w, uint8_t *q, size_t len,
                                     float *scales, size_t n_scales);
 /* y [t x rows] = Q(x [t x cols]) W^T, 1 <= t <= TQF_HIP_F8_MAX_TOKENS and
- * t * cols (rounded up to 128) < 2^32.  Blocks are summed in f32 in the order
- * of K.  With an f32 y (and, up to 16 rows, a bf16 y too) the products within a
- * block are exact and only their f32 sums round; a larger bf16 y uses the fp8
- * matrix cores, whose sum of a block is about 1.3e-5 of it off, 1/150 of the
- * rounding to bf16.  x and y must not overlap. */
+ * t * cols (rounded up to 128) < 2^32.  Blocks are summed in f32, in an order
+ * that t and the shape decide and nothing else, so a row's result does not
+ * depend on the other rows.  With an f32 y (and, up to 16 rows whose quantised
+ * values take less than 128 KiB, a bf16 y too) the products within a block are
+ * exact and only their f32 sums round; a larger bf16 y uses the fp8 matrix
+ * cores, whose sum of a block is about 1.3e-5 of it off, 1/150 of the rounding
+ * to bf16.  x and y must not overlap. */
 #define TQF_HIP_F8_MAX_TOKENS 65536
 int32_t tqf_hip_f8_matmul_device(tqf_hip_ctx *ctx, const tqf_hip_weights *w, const void *d_x, int32_t x_type,
                                  uint32_t t, void *d_y, int32_t y_type);
@@ -499,10 +501,13 @@ int32_t tqf_hip_f8_experts_free(tqf_hip_ctx *ctx, tqf_hip_f8_experts *experts);
  * gives zeros.  The same expert may stand in several slots.  Any other id
  * >= n_experts: *d_status (may be NULL, zeroed by the caller) is set to
  * TQF_HIP_ERR_INVALID and y is not written.  1 <= t <=
- * TQF_HIP_GROUPED_MAX_TOKENS, 1 <= top_k <= TQF_HIP_ROUTE_MAX_TOP_K.  A row's
- * result does not depend on the other rows, but for the choice of path by t and
- * top_k (up to 64 slots, and above that by the mean slots of an expert).  x
- * and y must not overlap.  The counterpart for this format of
+ * TQF_HIP_GROUPED_MAX_TOKENS, 1 <= top_k <= TQF_HIP_ROUTE_MAX_TOP_K, and t *
+ * top_k * width (rounded up to 128) < 2^32.  A row's result does not depend on
+ * the other rows, but for the choice of path by t and top_k: up to 64 slots, or
+ * up to 14 to an expert on average, block products are exact as above; beyond,
+ * they are those of the fp8 cores, and from 15 on a bf16 y's terms are rounded
+ * to f16 (2^-11 of each, under a scale for 64 columns) before their sum.  y must
+ * not overlap x, ids or w.  The counterpart for this format of
  * tqf_hip_grouped_gemm_device. */
 #define TQF_HIP_NO_EXPERT 0xFFFFu
 #define TQF_HIP_ROUTE_MAX_EXPERTS 1024

@@ -464,6 +464,33 @@ def test_experts_refusals(small, be, hip):
 
 
 # ---- a step of a batch: router, routes, experts, head, acceptance ---------------------------
+def test_experts_refuse_buffers_that_overlap_and_sizes_past_32_bits(be, small, hip):
+    n = small.hidden
+    whole = be.alloc(4 * 4 * n + 4096)
+    x = be.view(whole, 0, 4 * 2 * n)
+    y = be.view(whole, 4 * 2 * n, 4 * 2 * n)
+    ids, w = be.view(whole, 4 * 4 * n, 64), be.view(whole, 4 * 4 * n + 64, 64)
+    inside = be.view(whole, 4 * 2 * n + 16, 64)
+    for bad in ((x, ids, w, x), (x, inside, w, y), (x, ids, inside, y)):
+        with pytest.raises(hip.HipError) as e:
+            be.f8_experts_device(small.ex, bad[0], 2, bad[1], bad[2], 2, bad[3])
+        assert e.value.status == _lib.ERR_INVALID
+    be.free(whole)
+    # one expert as wide as any: t * top_k * width of 2^32
+    wide = [be.upload_f8(np.zeros(s, np.uint8), np.ones((-(-s[0] // 128), -(-s[1] // 128)), np.float32))
+            for s in ((65536, 4), (65536, 4), (4, 65536))]
+    ex = be.prepare_f8_experts(*([m] for m in wide))
+    bufs = [be.alloc(4096 * 4 * 4), be.alloc(4096 * 16 * 2), be.alloc(4096 * 16 * 4), be.alloc(4096 * 4 * 4)]
+    with pytest.raises(hip.HipError) as e:
+        be.f8_experts_device(ex, bufs[0], 4096, bufs[1], bufs[2], 16, bufs[3])
+    assert e.value.status == _lib.ERR_INVALID
+    be.free_f8_experts(ex)
+    for m in wide:
+        be.free_weights(m)
+    for b in bufs:
+        be.free(b)
+
+
 def test_a_batch_from_rows_to_tokens(be, wide):
     """Three sequences of four verify rows through the router, the experts and an F8 head on the device, then each
     sequence's acceptance: as the definitions have it, and as the host forms of the same calls."""

@@ -2387,8 +2387,11 @@ extern "C" int32_t tqf_hip_f8_experts_device(tqf_hip_ctx *ctx, const tqf_hip_f8_
     const size_t xb = type_bytes(x_type), yb = type_bytes(y_type);
     if (!aligned_to(d_x, xb) || !aligned_to(d_y, yb) || !aligned_to(d_ids, 2) || !aligned_to(d_w, 4) || !aligned_to(d_status, 4))
         return fail(ctx, TQF_HIP_ERR_INVALID, "buffers must be aligned to their elements");
-    const size_t n = (size_t)t * experts->hidden;
-    if (overlap(d_x, n * xb, d_y, n * yb)) return fail(ctx, TQF_HIP_ERR_INVALID, "x and y must not overlap");
+    const size_t n = (size_t)t * experts->hidden, slots = (size_t)t * top_k;
+    if (overlap(d_x, n * xb, d_y, n * yb) || overlap(d_ids, slots * 2, d_y, n * yb) || overlap(d_w, slots * 4, d_y, n * yb))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "y must not overlap x, ids or weights");
+    if ((uint64_t)slots * f8_shape(1, experts->width).kb * 128 >= (uint64_t(1) << 32))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "t * top_k * width (rounded up to 128) must be below 2^32");
     const F8ExpertsDev ex{experts->d_mats, experts->n_experts, experts->hidden, experts->width};
     if (int32_t rc = ensure_f8_scratch(ctx, f8_experts_scratch_bytes(ex, t, top_k, y_type))) return rc;
     Prof p(ctx);
@@ -2441,8 +2444,10 @@ extern "C" int32_t tqf_hip_route_tokens_device(tqf_hip_ctx *ctx, const void *d_l
         !aligned_to(d_status, 4))
         return fail(ctx, TQF_HIP_ERR_INVALID, "buffers must be aligned to their elements");
     const size_t lb = (size_t)t * n_experts * type_bytes(logits_type), n = (size_t)t * o.top_k;
-    if (overlap(d_logits, lb, d_ids, n * 2) || overlap(d_logits, lb, d_w, n * 4) || overlap(d_ids, n * 2, d_w, n * 4))
-        return fail(ctx, TQF_HIP_ERR_INVALID, "logits, ids and weights must not overlap");
+    const size_t bb = d_bias ? (size_t)n_experts * 4 : 0;
+    if (overlap(d_logits, lb, d_ids, n * 2) || overlap(d_logits, lb, d_w, n * 4) || overlap(d_ids, n * 2, d_w, n * 4) ||
+        (bb && (overlap(d_bias, bb, d_ids, n * 2) || overlap(d_bias, bb, d_w, n * 4))))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "logits, bias, ids and weights must not overlap");
     Prof p(ctx);
     const hipError_t e = launch_route_tokens(ctx->stream, d_logits, logits_type, t, n_experts, d_bias, o, d_ids, d_w, d_status);
     if (e != hipSuccess) return hip_fail(ctx, "route kernel launch", e);

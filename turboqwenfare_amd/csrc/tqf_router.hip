@@ -95,7 +95,7 @@ struct Stage {
     static constexpr int kRowChunks = 2 * (int)sizeof(T), kLoads = N * kRowChunks / 4, kBytes = kLoads * 1024;
     u32x4 q[kLoads];
     const uint8_t *base;   // of the first row
-    uint32_t off[kLoads];  // from there: below 64 rows
+    uint32_t off[kLoads];  // from there
     static __device__ __forceinline__ int slot(int row, int chunk) {
         const int i = row * kRowChunks + chunk, line = i / 8;
         return (line * 8 + ((i ^ line) & 7)) * 16;

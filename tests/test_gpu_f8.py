@@ -465,6 +465,8 @@ def test_experts_refusals(small, be, hip):
 
 # ---- a step of a batch: router, routes, experts, head, acceptance ---------------------------
 def test_experts_refuse_buffers_that_overlap_and_sizes_past_32_bits(be, small, hip):
+    from turboqwenfare_amd import _lib
+
     n = small.hidden
     whole = be.alloc(4 * 4 * n + 4096)
     x = be.view(whole, 0, 4 * 2 * n)

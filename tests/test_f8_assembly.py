@@ -65,6 +65,27 @@ def test_copies_to_lds_are_not_looped(assembly):
     assert seen
 
 
+def test_barriers_wait_for_the_block_they_publish(assembly):
+    """The tiled product's barrier lets the newest N loads be under way, those of the block after the one that is
+    needed: at least so many must have been issued since the barrier before."""
+    seen = 0
+    for name, body in kernels(assembly["tqf_f8.hip"]).items():
+        lines = [line.split(";")[0].strip() for line in body.split("\n")]
+        loads = None
+        for line, after in zip(lines, lines[1:]):
+            wait = re.match(r"s_waitcnt vmcnt\((\d+)\) lgkmcnt\(0\)$", line)
+            if wait and after == "s_barrier":
+                if loads is not None and int(wait[1]):
+                    assert loads >= int(wait[1]), name
+                    seen += 1
+                loads = 0
+            elif re.match(r"(buffer|global)_load", line):
+                loads = None if loads is None else loads + 1
+            elif re.match(r"\.LBB|s_c?branch", line):
+                loads = None  # another path may lead here, or this one elsewhere
+    assert seen
+
+
 def test_no_register_spills(assembly):
     for src in SOURCES:
         assert set(re.findall(r"; ScratchSize: (\d+)", assembly[src])) == {"0"}

@@ -187,10 +187,11 @@ __device__ __forceinline__ void copy16(Desc d, uint32_t voff, uint32_t soff, voi
 __device__ __forceinline__ void copy4(Desc d, uint32_t voff, uint32_t soff, void *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 4, voff, soff, 0, 0);
 }
-// This wavefront's loads (those to LDS among them) and LDS reads are done, then
-// the workgroup's.
+// This wavefront's loads (those to LDS among them) but the last N, and its LDS
+// reads, are done, then the workgroup's.
+template <int N>
 __device__ __forceinline__ void publish() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 // ---- the tiled product -----------------------------------------------------------
@@ -240,7 +241,7 @@ __device__ __forceinline__ uint32_t out16(float a, float b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
 }
 
-template <class P, int RT, int CT, int MODE, typename YT, int TW = 1, bool WL = false>
+template <class P, int RT, int CT, int MODE, typename YT, int TW = 1, bool WL = false, int AHEAD = 1>
 __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     constexpr int M = P::M, kRows = TW * CT * M;  // activation rows of the workgroup
     constexpr int kCopies = CT * M / 32;          // copies of 1 KiB each wavefront makes for a block
@@ -251,12 +252,14 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     constexpr int kScaleRows = (kRows + 63) / 64 * 64;  // a copy fills 64
     // A variable to each stage: a read of one is then known not to wait for the
     // copies that are under way to another.
-    __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * 128], x1[kRows * 128];
+    __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * 128], x1[kRows * 128], x2[AHEAD == 2 ? kRows * 128 : 16];
     __shared__ __attribute__((aligned(16))) uint8_t w0[kWBytes], w1[kWBytes];
     __shared__ __attribute__((aligned(16))) uint8_t out_lds[MODE != kGateUp && M == 32 && !WL ? kTileWaves * 4096 : 16];
-    __shared__ float s0[kScaleRows], s1[kScaleRows], s_w[2][kF8MaxCols / 128];
-    auto stage_x = [&](int u) { return u % 2 ? x1 : x0; };
-    auto stage_s = [&](int u) { return u % 2 ? s1 : s0; };
+    __shared__ float s0[kScaleRows], s1[kScaleRows], s2[AHEAD == 2 ? kScaleRows : 1], s_w[2][kF8MaxCols / 128];
+    constexpr int kStages = AHEAD + 1;
+    auto stage_x = [&](int u) { return u % kStages == 2 ? x2 : u % kStages ? x1 : x0; };
+    auto stage_s = [&](int u) { return u % kStages == 2 ? s2 : u % kStages ? s1 : s0; };
+    static_assert(!WL || AHEAD == 1, "two stages of weights in LDS");
     auto stage_w = [&](int u) { return u % 2 ? w1 : w0; };
     __shared__ float s_max[kTileWaves][MODE == kGateUp ? kRows : 1];
     const int tid = threadIdx.x, all_wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
@@ -385,14 +388,16 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         for (int c = 0; c < CT; ++c) acc[r][c] = typename P::D{};
 
     // The K loop over N of the CT tiles of activation rows (an expert's rows may
-    // fill fewer).  A block is asked for while the one before is computed (past
-    // the end the last one again, so that no branch splits the loop; two blocks
-    // ahead for the weights measured no gain).  Scales go through LDS
-    // too: in registers they would have to be waited for with the blocks asked
+    // fill fewer).  Blocks are asked for AHEAD steps before they are computed
+    // (past the end the last one again, so that no branch splits the loop): two
+    // where the registers hold another block of weights, for a step is as long as
+    // a trip to memory if nothing else fills it (experts of 512 tokens 177 us with
+    // one, 162 with two; 16 tokens of 8 experts 29.5 and 25.6).  Scales go through
+    // LDS too: in registers they would have to be waited for with the blocks asked
     // for after them.
     auto k_loop = [&](auto tiles_used) {
         constexpr int N = decltype(tiles_used)::value;
-        typename P::Raw b[2][WL ? 1 : RT];  // weights in registers
+        typename P::Raw b[kStages][WL ? 1 : RT];  // weights in registers
         // kept in a scalar register: a copy whose offset the compiler put in a
         // vector register would be wrapped in a loop over its values
         const uint32_t last = kb_n - 1;
@@ -410,7 +415,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
 #pragma unroll
                 for (int j = 0; j < P::kLoads; ++j) {
                     if constexpr (WL) copy16(dw[r], l * 16, kb * kKB + j * 1024, stage_w(u) + (all_wave * kWMine + r) * kKB + j * 1024);
-                    else b[u % 2][r].q[j] = *reinterpret_cast<const global_u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
+                    else b[u % kStages][r].q[j] = *reinterpret_cast<const global_u32x4 *>(base[r] + (size_t)kb * kKB + P::a_off(l, sub[r], j));
                 }
         };
         // A wavefront issues in order, and an instruction of the matrix cores
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                         raw.q[j] = *reinterpret_cast<const u32x4 *>(stage_w(u) + (wave * RT + r) * kKB + P::a_off(l, 0, j));
                     aw[r] = P::op(raw);
                 } else {
-                    aw[r] = P::op(b[u % 2][r]);
+                    aw[r] = P::op(b[u % kStages][r]);
                 }
             }
             auto load_b = [&](int c) {
@@ -473,22 +478,34 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
 #pragma unroll
             for (int i = 0; i < P::kParts; ++i) add(N * RT - 1, d, scale, i);
         };
+        // The loads of a block, which may be under way when the one before is
+        // needed.  (All are issued: what the loop asks for is used in it or after
+        // it.  A count that is too large would let a copy be read too soon.)
+        constexpr int kLoads = kMine + 1 + (WL ? kWMine : RT) * P::kLoads;
         auto step = [&](uint32_t kb, int u) {
-            publish();
-            issue_x(kb + 1, u + 1);
-            issue_w(kb + 1, u + 1);
+            publish<(AHEAD - 1) * kLoads>();
+            issue_x(kb + AHEAD, u + AHEAD);
+            issue_w(kb + AHEAD, u + AHEAD);
             compute(kb, u);
         };
         issue_w(0, 0);  // first, as it needs no row_of_pos
         issue_x(0, 0);
         keep_scales();
-        uint32_t kb = 0;
-        for (; kb + 2 <= kb_n; kb += 2) {
-            step(kb, 0);
-            step(kb + 1, 1);
+        if constexpr (AHEAD == 2) {
+            issue_x(1, 1);
+            issue_w(1, 1);
         }
-        if (kb < kb_n) step(kb, 0);
-        publish();  // no copy is under way when the workgroup's LDS goes to another
+        uint32_t kb = 0;
+        for (; kb + kStages <= kb_n; kb += kStages) {
+#pragma unroll
+            for (int u = 0; u < kStages; ++u) step(kb + u, u);
+        }
+        // the blocks that are left are all under way
+        publish<0>();
+#pragma unroll
+        for (int u = 0; u < kStages - 1; ++u)
+            if (kb + u < kb_n) compute(kb + u, u);
+        publish<0>();  // no copy is under way when the workgroup's LDS goes to another
     };
     if constexpr (MODE == kDense) {
         k_loop(std::integral_constant<int, CT>{});
@@ -1325,7 +1342,7 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     return b;
 }
 
-template <class P, int RT, int CT, typename OT, int TW = 1, bool WL = false>
+template <class P, int RT, int CT, typename OT, int AHEAD>
 hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
     TiledArgs a{};
     a.d = f8_shape(ex.width, ex.hidden);
@@ -1340,7 +1357,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.hrows = pairs;
     a.rblocks = a.hkb;
     static_assert(RT * P::M == 64, "a workgroup of gate_up makes one block of h");
-    f8_tiled_kernel<P, RT, CT, kGateUp, float, TW, WL><<<b.max_tiles * a.rblocks, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kGateUp, float, 1, false, AHEAD><<<b.max_tiles * a.rblocks, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     a.d = f8_shape(ex.hidden, ex.width);
@@ -1350,7 +1367,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.out = b.out;
     a.out_scales = b.out_scales;
     a.rblocks = (ex.hidden + 255) / 256;
-    f8_tiled_kernel<P, RT, CT, kDown, OT, TW, WL><<<b.max_tiles * a.rblocks, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kDown, OT, 1, false, AHEAD><<<b.max_tiles * a.rblocks, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1375,12 +1392,12 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (m == 16) {
-        e = launch_tiles<Bf16x16, 4, 1, float>(s, ex, b, a.t, pairs);
+        e = launch_tiles<Bf16x16, 4, 1, float, 2>(s, ex, b, a.t, pairs);
     } else if (m == 32) {
-        e = launch_tiles<Bf16x16, 4, 2, float>(s, ex, b, a.t, pairs);
+        e = launch_tiles<Bf16x16, 4, 2, float, 2>(s, ex, b, a.t, pairs);
     } else {
         typedef typename std::conditional<sizeof(YT) == 2, Out16, float>::type OT;
-        e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT>(s, ex, b, a.t, pairs);
+        e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT, 2>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT, 1>(s, ex, b, a.t, pairs);
     }
     if (e != hipSuccess) return e;
     if (sizeof(YT) == 2 && b.out16) {

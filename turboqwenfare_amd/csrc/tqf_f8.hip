@@ -1296,13 +1296,16 @@ bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
 // Rows of a tile by the pairs an expert has on average: enough to hold most
 // experts' in one tile, whose weights are then read once; but no more than 96, so
 // that a compute unit has two workgroups, of which one computes while the other
-// starts or stores (256 experts, hidden 2048, width 512, top 8, us for tiles of
-// 64 / 96 / 192 rows, the last with weights in LDS: 1100 tokens 181 / 181 / 211,
-// 2048 229 / 204 / 235, 4096 318 / 277 / 285, and 315 / 287 / 329 for a skewed
-// choice of experts).
+// starts or stores.  Experts that fill several tiles anyway take 64 rows until
+// those of 96 would give every compute unit a workgroup of gate_up.  us for tiles
+// of 32 / 64 / 96 rows, hidden 2048, width 512, top 8: 256 experts, 1100 tokens
+// (mean 34) - / 173 / 180, 2048 (64) - / 218 / 203, 4096 - / 301 / 279; 60
+// experts, 128 tokens (17) 47.3 / 45.1 / 46.9, 512 (68) 82 / 65 / 53; 8 experts,
+// 256 tokens 40 / 33 / 38, 512 62 / 41 / 44, 1000 99 / 66 / 66.
 uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
     const uint32_t mean = t * top_k / ex.n_experts;
-    return mean <= 6 ? 16 : mean <= 14 ? 32 : mean <= 32 ? 64 : 96;
+    if (mean <= 40) return mean <= 6 ? 16 : mean <= 14 ? 32 : 64;
+    return mean > 96 && t * top_k / 96 * ((ex.width + 127) / 128) < 256 ? 64 : 96;
 }
 struct ExpertsScratch {
     int32_t *pos_of_pair, *row_of_pos, *n_tiles;

@@ -335,6 +335,26 @@ def test_experts_of_model_width(wide, t, k):
     wide.check(t, k, "f32", "f32")
 
 
+@pytest.mark.parametrize("kind,y_kind", TYPES)
+@pytest.mark.parametrize("t,k", [(16, 4), (17, 3), (17, 1), (32, 2), (64, 1), (65, 1), (43, 1), (40, 1), (41, 1)])
+def test_few_experts(be, t, k, kind, y_kind):
+    """One and two experts: exact products up to 64 slots whatever an expert's mean, and each size of tile after them."""
+    for n in (1, 2):
+        layer = Layer(be, n, 200, 130, 5)
+        layer.check(t, min(k, n), kind, y_kind)
+        layer.close()
+
+
+@pytest.mark.parametrize("t", [90, 97, 200, 700])
+def test_tiles_of_one_expert(be, t):
+    """One to many tiles of an expert, in numbers that do not pair, whole and not."""
+    layer = Layer(be, 1, 300, 520, 6)
+    for y_kind in ("f32", "bf16"):
+        layer.check(t, 1, "bf16", y_kind, empty=0.0)
+        layer.check(t, 1, "f32", y_kind)
+    layer.close()
+
+
 @pytest.mark.parametrize("t", [2, 20, 90, 400])
 def test_uneven_routes(small, t):
     """One expert for every row; a popular one; the same expert in several slots; most rows empty; one row in use."""

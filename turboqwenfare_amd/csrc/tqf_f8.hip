@@ -19,6 +19,7 @@
 // whose products of e4m3 values came out exact in the same test.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "tqf_f8.h"
@@ -1109,8 +1110,11 @@ __global__ __launch_bounds__(256) void f8_combine16_kernel(ExpertsArgs a, const 
 }
 
 // Few pairs.  A pair's row is the only column of its products, so all 16
-// columns of the operand are that row (one address for 16 lanes).
-constexpr uint32_t kPairsMax = 64;      // pairs
+// columns of the operand are that row (one address for 16 lanes).  Down has a
+// workgroup for each token and 16 columns, so many tokens of few routes are left
+// to the tiles (us by pairs / by tiles: 16 tokens of 1 route 20.5 / 24.1, of 4
+// 42 / 43, 32 of 1 35 / 31, 64 of 1 63 / 43, 8 of 8 39 / 46).
+constexpr uint32_t kPairsMax = 64, kPairsTokens = 16;
 constexpr uint32_t kPairsHidden = 8192, kPairsWidth = 2048;
 
 // Whether every id of the call names an expert or none (each wavefront asks).
@@ -1291,7 +1295,7 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
 }
 
 bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
-    return t * top_k <= kPairsMax && ex.hidden <= kPairsHidden && ex.width <= kPairsWidth;
+    return t <= kPairsTokens && t * top_k <= kPairsMax && ex.hidden <= kPairsHidden && ex.width <= kPairsWidth;
 }
 // Rows of a tile by the pairs an expert has on average: enough to hold most
 // experts' in one tile, whose weights are then read once; but no more than 96, so
@@ -1301,9 +1305,10 @@ bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
 // of 32 / 64 / 96 rows, hidden 2048, width 512, top 8: 256 experts, 1100 tokens
 // (mean 34) - / 173 / 180, 2048 (64) - / 218 / 203, 4096 - / 301 / 279; 60
 // experts, 128 tokens (17) 47.3 / 45.1 / 46.9, 512 (68) 82 / 65 / 53; 8 experts,
-// 256 tokens 40 / 33 / 38, 512 62 / 41 / 44, 1000 99 / 66 / 66.
+// 256 tokens 40 / 33 / 38, 512 62 / 41 / 44, 1000 99 / 66 / 66.  Up to 64 pairs
+// stay on the tiles whose products are exact, as the path for few pairs is.
 uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
-    const uint32_t mean = t * top_k / ex.n_experts;
+    const uint32_t mean = t * top_k <= kPairsMax ? std::min(t * top_k / ex.n_experts, 14u) : t * top_k / ex.n_experts;
     if (mean <= 40) return mean <= 6 ? 16 : mean <= 14 ? 32 : 64;
     return mean > 96 && t * top_k / 96 * ((ex.width + 127) / 128) < 256 ? 64 : 96;
 }

@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     // copies that are under way to another.
     __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * 128], x1[kRows * 128], x2[AHEAD == 2 ? kRows * 128 : 16];
     __shared__ __attribute__((aligned(16))) uint8_t w0[kWBytes], w1[kWBytes];
-    __shared__ __attribute__((aligned(16))) uint8_t out_lds[MODE != kGateUp && M == 32 && !WL ? kTileWaves * 4096 : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t out_lds[MODE != kGateUp && !WL ? kTileWaves * M * 128 : 16];
     __shared__ float s0[kScaleRows], s1[kScaleRows], s2[AHEAD == 2 ? kScaleRows : 1], s_w[2][kF8MaxCols / 128];
     constexpr int kStages = AHEAD + 1;
     auto stage_x = [&](int u) { return u % kStages == 2 ? x2 : u % kStages ? x1 : x0; };
@@ -568,78 +568,61 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         static_assert(!kOut16 || (MODE == kDown && RT * M == kOutBlock), "a wavefront's columns share a scale");
         YT *y = MODE == kDense ? static_cast<YT *>(a.y) : static_cast<YT *>(a.out);
         const uint32_t blocks = (a.d.rows + kOutBlock - 1) / kOutBlock, n = kOut16 ? blocks * kOutBlock : a.d.rows;
-        if constexpr (M == 32) {
-            // 32 rows of this wavefront's at a time, a line (128 bytes, or what the
-            // wavefront has) of each
-            constexpr int kEach = 16 / sizeof(YT), kFit = 32 / (int)sizeof(YT) / 8, kTiles = RT < kFit ? RT : kFit;
-            constexpr int kLine = kTiles * 32 * (int)sizeof(YT), kChunks = kLine / 16;
-            uint8_t *mine_lds = (WL ? w0 : out_lds) + all_wave * 4096;
-            const int row = P::b_row(l);
+        // M rows of this wavefront's at a time, a line (128 bytes, or what the
+        // wavefront has) of each
+        constexpr int kEach = 16 / sizeof(YT), kFit = 128 / (M * (int)sizeof(YT)), kTiles = RT < kFit ? RT : kFit;
+        constexpr int kLine = kTiles * M * (int)sizeof(YT), kChunks = kLine / 16;
+        uint8_t *mine_lds = (WL ? w0 : out_lds) + all_wave * M * 128;
+        const int row = P::b_row(l);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                if ((uint32_t)(c * 32) >= mine) break;
-                float inv = 0.0f;
-                if constexpr (kOut16) {
-                    float m = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int i = 0; i < 4 * kG; ++i) {
-                            const float v = fabsf(acc[r][c][i]);
-                            m = fmaxf(m, v < __builtin_inff() ? v : 0.0f);
-                        }
-                    m = P::across(m);
-                    const uint32_t p = m < 0x1p-100f ? 0 : __float_as_uint(m) & 0x7F800000u;  // 2^e <= m
-                    inv = p ? __uint_as_float((268u << 23) - p) : 0.0f;                // 2^(14 - e)
-                    const uint32_t in = (uint32_t)(c * 32 + row);
-                    if (l < 32 && in < mine && wrow[0] < n)
-                        a.out_scales[(size_t)(first + row0 + in) * blocks + wrow[0] / kOutBlock] = __uint_as_float(p) * 0x1p-14f;
-                }
-#pragma unroll
-                for (int r0 = 0; r0 < RT; r0 += kTiles) {
-#pragma unroll
-                    for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-                        for (int g = 0; g < kG; ++g) {
-                            const int byte = (r * 32 + P::row(l, g)) * (int)sizeof(YT);
-                            const f32x4 v = {acc[r0 + r][c][4 * g], acc[r0 + r][c][4 * g + 1], acc[r0 + r][c][4 * g + 2], acc[r0 + r][c][4 * g + 3]};
-                            YT *to = reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16);
-                            if constexpr (kOut16) *reinterpret_cast<uint2 *>(to) = make_uint2(out16(v[0] * inv, v[1] * inv), out16(v[2] * inv, v[3] * inv));
-                            else store4(static_cast<YT *>(__builtin_assume_aligned(to, 4 * sizeof(YT))), 4, v);
-                        }
-#pragma unroll
-                    for (int j = 0; j < kChunks / 2; ++j) {
-                        const int at = (j * 64 + l) / kChunks, chunk = l % kChunks;
-                        const u32x4 v = *reinterpret_cast<const u32x4 *>(mine_lds + at * kLine + ((chunk ^ at) & (kChunks - 1)) * 16);
-                        const uint32_t in = (uint32_t)(c * 32 + at), col = wrow[r0] + chunk * kEach;
-                        if (in >= mine || col >= n) continue;
-                        YT *to = y + (size_t)(first + row0 + in) * n + col;
-                        if (col + kEach <= n) {
-                            __builtin_memcpy(to, &v, 16);
-                        } else {
-                            YT each[kEach];
-                            __builtin_memcpy(each, &v, 16);
-#pragma unroll
-                            for (int k = 0; k < kEach; ++k)
-                                if (col + k < n) to[k] = each[k];
-                        }
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const uint32_t in = (uint32_t)(c * M + P::b_row(l)), local = row0 + in;
-                if (in >= mine) continue;
+        for (int c = 0; c < CT; ++c) {
+            if ((uint32_t)(c * M) >= mine) break;
+            float inv = 0.0f;
+            if constexpr (kOut16) {
+                float m = 0.0f;
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int g = 0; g < kG; ++g) {
-                        const uint32_t col = wrow[r] + P::row(l, g);
-                        if (col >= n) continue;
-                        const f32x4 v = {acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]};
-                        store4(y + (size_t)(first + local) * n + col, (int)(n - col), v);
+                    for (int i = 0; i < 4 * kG; ++i) {
+                        const float v = fabsf(acc[r][c][i]);
+                        m = fmaxf(m, v < __builtin_inff() ? v : 0.0f);
                     }
+                m = P::across(m);
+                const uint32_t p = m < 0x1p-100f ? 0 : __float_as_uint(m) & 0x7F800000u;  // 2^e <= m
+                inv = p ? __uint_as_float((268u << 23) - p) : 0.0f;                // 2^(14 - e)
+                const uint32_t in = (uint32_t)(c * M + row);
+                if (l < M && in < mine && wrow[0] < n)
+                    a.out_scales[(size_t)(first + row0 + in) * blocks + wrow[0] / kOutBlock] = __uint_as_float(p) * 0x1p-14f;
+            }
+#pragma unroll
+            for (int r0 = 0; r0 < RT; r0 += kTiles) {
+#pragma unroll
+                for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+                    for (int g = 0; g < kG; ++g) {
+                        const int byte = (r * M + P::row(l, g)) * (int)sizeof(YT);
+                        const f32x4 v = {acc[r0 + r][c][4 * g], acc[r0 + r][c][4 * g + 1], acc[r0 + r][c][4 * g + 2], acc[r0 + r][c][4 * g + 3]};
+                        YT *to = reinterpret_cast<YT *>(mine_lds + row * kLine + ((byte / 16 ^ row) & (kChunks - 1)) * 16 + byte % 16);
+                        if constexpr (kOut16) *reinterpret_cast<uint2 *>(to) = make_uint2(out16(v[0] * inv, v[1] * inv), out16(v[2] * inv, v[3] * inv));
+                        else store4(static_cast<YT *>(__builtin_assume_aligned(to, 4 * sizeof(YT))), 4, v);
+                    }
+#pragma unroll
+                for (int j = 0; j < M * kChunks / 64; ++j) {
+                    const int at = (j * 64 + l) / kChunks, chunk = l % kChunks;
+                    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine_lds + at * kLine + ((chunk ^ at) & (kChunks - 1)) * 16);
+                    const uint32_t in = (uint32_t)(c * M + at), col = wrow[r0] + chunk * kEach;
+                    if (in >= mine || col >= n) continue;
+                    YT *to = y + (size_t)(first + row0 + in) * n + col;
+                    if (col + kEach <= n) {
+                        __builtin_memcpy(to, &v, 16);
+                    } else {
+                        YT each[kEach];
+                        __builtin_memcpy(each, &v, 16);
+#pragma unroll
+                        for (int k = 0; k < kEach; ++k)
+                            if (col + k < n) to[k] = each[k];
+                    }
+                }
             }
         }
     }

@@ -862,11 +862,11 @@ hipError_t quantize(hipStream_t s, const XT *x, uint32_t t, uint32_t cols, uint3
     return hipGetLastError();
 }
 
-template <class P, int RT, int CT, typename YT, int TW = 1, bool WL = false>
+template <class P, int RT, int CT, int AHEAD, typename YT, int TW = 1, bool WL = false>
 hipError_t launch_dense(hipStream_t s, const TiledArgs &a) {
     constexpr uint32_t kM = P::M;
     const uint32_t rbs = (a.d.tiles * 32 + 4 * RT * kM - 1) / (4 * RT * kM), tbs = (a.xrows + TW * CT * kM - 1) / (TW * CT * kM);
-    f8_tiled_kernel<P, RT, CT, kDense, YT, TW, WL><<<(rbs * tbs + 7) / 8 * 8, 256 * TW, 0, s>>>(a);
+    f8_tiled_kernel<P, RT, CT, kDense, YT, TW, WL, AHEAD><<<(rbs * tbs + 7) / 8 * 8, 256 * TW, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -915,11 +915,11 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     a.xrows = t;
     a.y = y;
     if constexpr (kF32) {
-        return t <= 32 ? launch_dense<Bf16x16, 2, 2, YT>(s, a) : launch_dense<Bf16x16, 2, 4, YT>(s, a);
+        return t <= 32 ? launch_dense<Bf16x16, 2, 2, 2, YT>(s, a) : launch_dense<Bf16x16, 2, 4, 2, YT>(s, a);
     } else {
-        if (t <= 32) return launch_dense<Fp8x32, 1, 1, YT>(s, a);
-        if (t <= 64) return launch_dense<Fp8x32, 2, 2, YT>(s, a);
-        return launch_dense<Fp8x32, 2, 4, YT, 2, true>(s, a);
+        if (t <= 32) return launch_dense<Fp8x32, 1, 1, 2, YT>(s, a);
+        if (t <= 64) return launch_dense<Fp8x32, 2, 2, 2, YT>(s, a);
+        return launch_dense<Fp8x32, 2, 4, 1, YT, 2, true>(s, a);
     }
 }
 

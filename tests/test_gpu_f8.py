@@ -122,7 +122,8 @@ def test_matmul_many_rows(be, t, rows, cols):
 
 @pytest.mark.parametrize("kind,y_kind", TYPES)
 @pytest.mark.parametrize("t,rows,cols", [
-    (17, 32768, 140), (17, 32769, 140), (32, 33000, 257), (33, 33001, 129), (64, 32800, 100), (65, 32769, 130), (300, 16500, 700), (257, 40000, 77)])
+    (17, 32768, 140), (17, 32769, 140), (32, 33000, 257), (33, 33001, 129), (64, 32800, 100), (65, 32769, 130), (300, 16500, 700), (257, 40000, 77),
+    (250, 65000, 300), (300, 60000, 70), (130, 33000, 450), (256, 60001, 130)])
 def test_matmul_on_both_sides_of_the_split(be, t, rows, cols, kind, y_kind):
     """Matrices about as large as those from which on tiles take over from wavefronts that split K."""
     check_matmul(be, t, rows, cols, kind, y_kind)
@@ -155,6 +156,29 @@ def test_a_row_that_is_no_number_is_alone(be, t, y_kind):
     assert np.isnan(got[:, 7]).all() and np.isfinite(np.delete(got, 7, 1)).all()
     for h in (w, w2):
         be.free_weights(h)
+
+
+def test_how_the_fp8_cores_cut_products(be):
+    """Two products of 448 x 448 that cancel, and a small one in the same eight or another: what is left of it.  The
+    tolerances for large bf16 results stand on this: at most 7 * 2^-13 of the magnitudes is lost."""
+    small = np.array([448.0, 16.0, 8.0, 4.0, 1.0])
+    code = [int(np.flatnonzero(ref.TABLE == v)[0]) for v in (448.0, -448.0, *small)]
+    x = np.zeros((40, 128), np.float32)  # more rows than the exact path takes
+    x[:, :2] = 448
+    x[:, [2, 4, 7, 8, 16, 64, 127]] = 1
+    for at in (2, 4, 7, 8, 16, 64, 127):
+        q = np.zeros((len(small), 128), np.uint8)
+        q[:, 0], q[:, 1], q[:, at] = code[0], code[1], code[2:]
+        w = be.upload_f8(q, np.ones((1, 1), np.float32))
+        d_x, d_y = be.to_device(ref.to_bf16(x)), be.to_device(np.zeros((40, len(small)), np.uint16))
+        be.f8_matmul_device(w, d_x, 40, d_y, x_type="bf16", y_type="bf16")
+        got = ref.from_bf16(be.read(d_y, np.uint16, (40, len(small))))
+        # 448 = 1.75 * 2^8: the larger products count as 2^16, and 2^-13 of that is 8
+        kept = np.where((small < 8) & (at < 8), 0, small)
+        assert (got == kept).all() or (got == small).all(), (at, got[0])
+        for b in (d_x, d_y):
+            be.free(b)
+        be.free_weights(w)
 
 
 def test_values_at_the_borders(be):

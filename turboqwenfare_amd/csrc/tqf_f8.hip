@@ -10,10 +10,11 @@
 // and a block's scale is one number per lane: d = the block's product from a
 // zero start, acc = fma(d, s_x s_w, acc) in f32.
 //
-// How exact the block's product is.  The fp8 matrix instructions align the
-// products of a block to the largest before they add: against 64 bits, a
-// block of normal values is 1.3e-5 off (relative, 2-norm), 3.9e-5 with rows
-// that span 2^8; the 32-column instruction is no better.  bf16 results are
+// How exact the block's product is.  The fp8 matrix instructions take eight
+// products at a time and cut each to 2^-13 of the largest one's power of two
+// (measured, tests/test_gpu_f8.py): a block loses less than 7 * 2^-13 of its
+// magnitudes; against 64 bits, one of normal values is 1.3e-5 off (relative,
+// 2-norm), 3.9e-5 with rows that span 2^8.  bf16 results are
 // rounded at 2^-9 = 2e-3, so they are made of these; f32 results, and every
 // small call, widen the values to bf16 (exact) for the bf16 instructions,
 // whose products of e4m3 values came out exact in the same test.
@@ -879,9 +880,9 @@ hipError_t launch_split(hipStream_t s, const uint8_t *mat, const F8Shape &d, con
 
 // A workgroup's activation rows where K is split; 0: the tiled product is faster,
 // as it is once its larger tiles (which load less for a product) fill the card.
-// us, split / tiled: 64 bf16 rows of 4096 by 8192 12.2 / 26.4, 256 26.5 / 50, 512
-// (1024 workgroups) 45 / 52, 1024 88 / 56, 256 by 20000 (1250) 59 / 53; f32 rows of
-// the same by 8192, 64 rows 13 / 32, 512 56 / 46.  f32 takes 32 rows always (256
+// us, split / tiled: 64 bf16 rows of 4096 by 8192 12.2 / 26, 256 26.5 / 50, 512
+// (1024 workgroups) 45 / 45, 1024 88 / 45, 256 by 20000 (1250) 59 / 53; f32 rows of
+// the same by 8192, 64 rows 13 / 32, 512 56 / 41.  f32 takes 32 rows always (256
 // rows 31, in steps of 64 33, of 128 40).
 uint32_t split_rows(const F8Shape &d, uint32_t t, bool f32) {
     const uint32_t rows = f32 || t <= 32 ? 32 : t <= 64 ? 64 : 128;
@@ -919,7 +920,15 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     } else {
         if (t <= 32) return launch_dense<Fp8x32, 1, 1, 2, YT>(s, a);
         if (t <= 64) return launch_dense<Fp8x32, 2, 2, 2, YT>(s, a);
-        return launch_dense<Fp8x32, 2, 4, 1, YT, 2, true>(s, a);
+        // Tiles of 256 rows where they leave little of the card without work in
+        // their last round (a compute unit holds one), else of 64 where all run
+        // at once (two to a unit), else of 96.  us for tiles of 64 / 96 / 256 rows:
+        // 4096 by 8192, K 4096 172 / 160 / 143, 2048 by 6000 (0.73 of a round) 65 /
+        // 78 / 60; 2048 by 4096 (0.5) 46 / 50 / 60, 1024 by 8192 45 / 48 / 55; 2560
+        // by 8192, K 2048 (0.63 of two) 57 / 56 / 65.
+        const uint64_t rbs = (d.rows + 255) / 256, rounds = (rbs * ((t + 255) / 256) + 255) / 256;
+        if ((uint64_t)d.rows * t * 10 >= rounds * 7 * 256 * 256 * 256) return launch_dense<Fp8x32, 2, 4, 1, YT, 2, true>(s, a);
+        return rbs * ((t + 63) / 64) <= 512 ? launch_dense<Fp8x32, 2, 2, 2, YT>(s, a) : launch_dense<Fp8x32, 2, 3, 1, YT>(s, a);
     }
 }
 

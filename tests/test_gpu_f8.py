@@ -583,3 +583,84 @@ def test_a_batch_from_rows_to_tokens(be, wide):
         be.free(b)
     be.free_weights(head)
     be.free_tensor(router)
+
+
+def test_calls_that_share_scratch(be, small):
+    """The grouped product of a Q4_0 layer and the F8 calls have one scratch: each gives the same whatever came before,
+    when the scratch grows and when it does not."""
+    from turboqwenfare_amd import synth
+
+    rng = np.random.default_rng(21)
+    H, F, E, own = 256, 256, 256, 24  # (a layer has 256 experts; they take turns with 24 matrices)
+    mats = [(be.synth_q4_0(F, H, 3 * e, 5), be.synth_q4_0(F, H, 3 * e + 1, 5), be.synth_q4_0(H, F, 3 * e + 2, 5)) for e in range(own + 1)]
+    tensors = [be.upload_f32(synth.normal((E, H), seed=1, std=H ** -0.5)), be.upload_f32(synth.normal((H,), seed=2, std=H ** -0.5))]
+    layer = be.prepare_moe_layer(tensors[0], tensors[1], mats[own], *([mats[e % own][i] for e in range(E)] for i in range(3)))
+    w8 = be.upload_f8(*ref.random_matrix(rng, 300, 260))
+    cases = []
+    for t in (3, 40, 700):
+        ids, w = synth.zipf_routes(t, E, seed=t)
+        cases.append(("grouped", (synth.bf16_round(synth.normal((t, H), seed=t)), ids, w)))
+        ids, w = small.routes(rng, t, 8)
+        cases.append(("experts", (rows_of(rng, t, small.hidden, "bf16"), ids, w)))
+        cases.append(("matmul", (rng.standard_normal((t, 260)).astype(np.float32),)))
+
+    def run(kind, args):
+        if kind == "grouped":
+            return be.grouped_gemm(layer, *args)
+        if kind == "matmul":
+            return be.f8_matmul(w8, *args)
+        y, st = small.run(args[0], "bf16", args[1], args[2], "bf16")
+        assert st == 0
+        return y
+
+    first = [run(*c) for c in cases]
+    for at in rng.permutation(np.repeat(np.arange(len(cases)), 3)):
+        assert np.array_equal(run(*cases[at]), first[at]), (cases[at][0], at)
+    be.free_moe_layer(layer)
+    for m in mats:
+        for w in m:
+            be.free_weights(w)
+    for t in tensors:
+        be.free_tensor(t)
+    be.free_weights(w8)
+
+
+def test_a_chunk_from_rows_to_logits(be):
+    """A prompt chunk of bf16 rows, some of them padding (a row of masked logits), through the routes, the experts and a
+    projection on the device, twice without a wait: as the definitions have it at each stage."""
+    rng = np.random.default_rng(31)
+    n, H, F, t, k = 12, 256, 200, 700, 4
+    layer = Layer(be, n, H, F, 7)
+    x = ref.to_bf16(rng.standard_normal((t, H)).astype(np.float32))
+    router = (rng.standard_normal((n, H)) / 16).astype(np.float32)
+    bias = rng.standard_normal(n).astype(np.float32) * 0.05
+    hq, hs = ref.random_matrix(rng, 520, H)
+    r, head = be.upload_f32(router), be.upload_f8(hq, hs)
+    lg0 = be.to_device(np.zeros((t, n), np.float32))
+    be.router_logits_device(r, be.to_device(x), t, n, H, lg0, x_type="bf16")
+    lg = be.read(lg0, np.float32, (t, n))
+    pad = rng.random(t) < 0.1
+    lg[pad] = -np.inf
+    d = {key: be.to_device(a) for key, a in dict(x=x, lg=lg, bias=bias, ids=np.zeros((t, k), np.uint16), w=np.zeros((t, k), np.float32),
+                                                 y=np.zeros((t, H), np.uint16), out=np.zeros((t, 520), np.uint16), st=np.zeros(2, np.int32)).items()}
+    for _ in range(2):
+        be.route_tokens_device(d["lg"], t, n, k, d["ids"], d["w"], score="sigmoid", d_bias=d["bias"], n_groups=3, top_groups=2, group_best=2, scale=2.0,
+                               d_status=d["st"])
+        be.f8_experts_device(layer.ex, d["x"], t, d["ids"], d["w"], k, d["y"], x_type="bf16", y_type="bf16", d_status=be.view(d["st"], 4, 4))
+        be.f8_matmul_device(head, d["y"], t, d["out"], x_type="bf16", y_type="bf16")
+    ids, w, y, out = (be.read(d[key], a, s) for key, a, s in (("ids", np.uint16, (t, k)), ("w", np.float32, (t, k)), ("y", np.uint16, (t, H)),
+                                                             ("out", np.uint16, (t, 520))))
+    assert (be.read(d["st"], np.int32, (2,)) == 0).all()
+    want, p, _ = ref.route(lg, k, "sigmoid", bias, 3, 2, 2, True, 2.0)
+    assert np.array_equal(ids, want) and np.allclose(w, p, rtol=2.0 ** -23, atol=0) and (ids[pad] == ref.NONE).all()
+    want, tol = ref.experts(values_of(x, "bf16"), ids, w, layer.mats, True, "bf16")
+    part = sum(np.abs(ref.experts(values_of(x, "bf16"), ids[:, i:i + 1], w[:, i:i + 1], layer.mats, True, "f32")[0]) for i in range(k))
+    got = values_of(y, "bf16").astype(np.float64)
+    assert np.all(np.abs(got - want) <= tol + 2.0 ** -11 * part + 1e-35) and (got[pad] == 0).all()  # terms wait as f16
+    want, tol = ref.matmul(values_of(y, "bf16"), ref.values(hq, hs), True)
+    assert np.all(np.abs(values_of(out, "bf16") - want) <= tol + 2.0 ** -8 * (np.abs(want) + tol) + 1e-35)
+    for b in (*d.values(), lg0):
+        be.free(b)
+    be.free_weights(head)
+    be.free_tensor(r)
+    layer.close()

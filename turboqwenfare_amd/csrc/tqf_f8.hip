@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     // copies that are under way to another.
     __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * 128], x1[kRows * 128], x2[AHEAD == 2 ? kRows * 128 : 16];
     __shared__ __attribute__((aligned(16))) uint8_t w0[kWBytes], w1[kWBytes];
-    __shared__ __attribute__((aligned(16))) uint8_t out_lds[MODE != kGateUp && !WL ? kTileWaves * M * 128 : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t out_lds[MODE != kGateUp && !WL ? TW * kTileWaves * M * 128 : 16];
     __shared__ float s0[kScaleRows], s1[kScaleRows], s2[AHEAD == 2 ? kScaleRows : 1], s_w[2][kF8MaxCols / 128];
     constexpr int kStages = AHEAD + 1;
     auto stage_x = [&](int u) { return u % kStages == 2 ? x2 : u % kStages ? x1 : x0; };

@@ -1109,25 +1109,35 @@ __global__ __launch_bounds__(256) void f8_combine16_kernel(ExpertsArgs a, const 
 constexpr uint32_t kPairsMax = 64, kPairsTokens = 16;
 constexpr uint32_t kPairsHidden = 8192, kPairsWidth = 2048;
 
-// Whether every id of the call names an expert or none (each wavefront asks).
-__device__ __forceinline__ bool ids_ok(const ExpertsArgs &a, int lane) {
-    bool bad = false;
-    for (uint32_t i = lane; i < a.t * a.top_k; i += 64) {
-        const uint32_t e = a.ids[i];
-        bad |= e != TQF_HIP_NO_EXPERT && e >= a.n_experts;
-    }
-    return __ballot(bad) == 0;
+// One trip to memory after another is what these two cost: id, table (or pointer),
+// weights.  Loads return in the order they are issued, so all that does not wait
+// for another load is asked for before the weights, which everything after them
+// would have to wait for.
+
+// Whether every id of the call names an expert or none (each wavefront asks; at
+// most kPairsMax = 64 of them).
+__device__ __forceinline__ uint32_t load_id(const ExpertsArgs &a, int lane) {
+    return (uint32_t)lane < a.t * a.top_k ? a.ids[lane] : TQF_HIP_NO_EXPERT;
+}
+__device__ __forceinline__ bool ids_ok(const ExpertsArgs &a, uint32_t id) {
+    return __ballot(id != TQF_HIP_NO_EXPERT && id >= a.n_experts) == 0;
 }
 // A row of n K blocks, of which this wavefront needs b0, b0 + step, ...: their
 // values quantised to bf16 into q [kb][128] and their scales into s [kb].
-// Sixteen lanes take a block, eight values each.
+// Sixteen lanes take a block, eight values each, four blocks at a time; those of
+// the first four are asked for by load_blocks.
 template <typename XT>
-__device__ __forceinline__ void quantize_blocks(const XT *x, uint32_t cols, uint32_t b0, uint32_t step, uint32_t n,
-                                                int lane, uint16_t *q, float *s) {
+__device__ __forceinline__ void load_blocks(const XT *x, uint32_t cols, uint32_t b, uint32_t step, uint32_t n, int lane, float (&v)[8]) {
+    const uint32_t kb = b + (lane / 16) * step, k = kb * 128 + (lane % 16) * 8;
+    load_row<8>(x + k, kb < n && k < cols ? (int)(cols - k) : 0, v);
+}
+template <typename XT>
+__device__ __forceinline__ void quantize_blocks(const XT *x, uint32_t cols, uint32_t b0, uint32_t step, uint32_t n, int lane,
+                                                float (&v)[8], uint16_t *q, float *s) {
     for (uint32_t b = b0; b < n; b += 4 * step) {
+        if (b != b0) load_blocks(x, cols, b, step, n, lane, v);
         const uint32_t kb = b + (lane / 16) * step, k = kb * 128 + (lane % 16) * 8;
-        float v[8], m = 0.0f;
-        load_row<8>(x + k, kb < n && k < cols ? (int)(cols - k) : 0, v);
+        float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
         m = amax8(m);
@@ -1150,7 +1160,8 @@ __device__ __forceinline__ Bf16x16::Op pair_operand(const uint16_t *q, uint32_t 
 // h[pair] = silu(g) u for 16 columns; four wavefronts share the K blocks.
 template <typename XT>
 __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, const uint8_t *const *__restrict__ mats, F8Shape d,
-                                                              const XT *__restrict__ x, float *__restrict__ h, uint32_t hstride) {
+                                                              const XT *__restrict__ x, float *__restrict__ h, uint32_t hstride,
+                                                              const uint8_t **__restrict__ downs) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     typedef Bf16x16 P;
     uint16_t *q = reinterpret_cast<uint16_t *>(lds);
@@ -1158,10 +1169,17 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
     float *red = s + ((d.kb + 3) & ~3u);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
     const uint32_t pair = blockIdx.y, e = a.ids[pair], row0 = blockIdx.x * 16;
+    const XT *row = x + (size_t)(pair / a.top_k) * d.cols;
+    const uint32_t id = load_id(a, l);
+    float xv[8];
+    load_blocks(row, d.cols, wave, 4, d.kb, l, xv);
+    __builtin_amdgcn_sched_barrier(0);
+    // An id out of range reads expert 0's matrices until all ids are seen; down
+    // finds its matrix without the table.
+    const bool named = e < a.n_experts;
+    const size_t m0 = (size_t)(named ? e : 0) * 3;
+    if (blockIdx.x == 0 && tid == 0) downs[pair] = named ? mats[m0 + 2] : nullptr;
     if (e == TQF_HIP_NO_EXPERT) return;  // (a bad id is reported by its own pair among others)
-    // one trip to memory after another, id, table, weights and scales: everything
-    // else comes behind them.  An id out of range reads expert 0's until it is seen.
-    const size_t m0 = (size_t)(e < a.n_experts ? e : 0) * 3;
     global_u8 *g = (global_u8 *)mats[m0], *u = (global_u8 *)mats[m0 + 1];
     const uint32_t tile = row0 / 32;
     const int sub = (int)(row0 / 16 & 1);
@@ -1187,12 +1205,11 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
         }
     };
     issue(wave);
-    if (!ids_ok(a, l)) {
+    if (!ids_ok(a, id)) {
         if (blockIdx.x == 0 && tid == 0 && a.status) *a.status = TQF_HIP_ERR_INVALID;
         return;
     }
-    const XT *row = x + (size_t)(pair / a.top_k) * d.cols;
-    quantize_blocks(row, d.cols, wave, 4, d.kb, l, q, s);
+    quantize_blocks(row, d.cols, wave, 4, d.kb, l, xv, q, s);
     __syncthreads();
     for (uint32_t b0 = wave; b0 < d.kb; b0 += 4 * kAhead) {
         if (b0 != (uint32_t)wave) issue(b0);
@@ -1223,10 +1240,13 @@ __global__ __launch_bounds__(256) void f8_pair_gate_up_kernel(ExpertsArgs a, con
 }
 
 // y[token] for 16 columns: a wavefront takes the routes k = wave, wave + 8, ...
+// downs: the matrix of each pair, null for an empty slot.
 template <typename YT>
-__global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const uint8_t *const *__restrict__ mats, F8Shape d,
+__global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const uint8_t *const *__restrict__ downs, F8Shape d,
                                                            const float *__restrict__ h, uint32_t hstride, YT *__restrict__ y) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ float weight[TQF_HIP_ROUTE_MAX_TOP_K];
+    __shared__ bool used[TQF_HIP_ROUTE_MAX_TOP_K];
     typedef Bf16x16 P;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
     uint16_t *q = reinterpret_cast<uint16_t *>(lds + (size_t)wave * d.kb * 256);
@@ -1235,11 +1255,17 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
     const uint32_t token = blockIdx.y, row0 = blockIdx.x * 16, tile = row0 / 32;
     const int sub = (int)(row0 / 16 & 1);
     const size_t base = (size_t)tile * d.kb * kKB, sbase = f8_tile_bytes(d) + (size_t)(tile / 4) * d.kb * 4;
+    const uint32_t id = load_id(a, l);
     for (uint32_t k = wave; k < a.top_k; k += 8) {
-        const uint32_t pair = token * a.top_k + k, e = a.ids[pair];
+        const uint32_t pair = token * a.top_k + k;
+        const float *row = h + (size_t)pair * hstride;
+        const float w = a.w[pair];
+        float hv[8];
+        load_blocks(row, d.cols, 0, 1, d.kb, l, hv);
+        __builtin_amdgcn_sched_barrier(0);
+        global_u8 *m = (global_u8 *)downs[pair];
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (e != TQF_HIP_NO_EXPERT) {
-            global_u8 *m = (global_u8 *)mats[(size_t)(e < a.n_experts ? e : 0) * 3 + 2];
+        if (m) {
             global_f32 *ms = (global_f32 *)(m + sbase);
             constexpr int kAhead = 4;
             typename P::Raw raw[kAhead];
@@ -1255,7 +1281,7 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
                 }
             };
             issue(0);
-            quantize_blocks(h + (size_t)pair * hstride, d.cols, 0, 1, d.kb, l, q, s);
+            quantize_blocks(row, d.cols, 0, 1, d.kb, l, hv, q, s);
             // this wavefront's own writes: LDS serves it in order
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             for (uint32_t b0 = 0; b0 < d.kb; b0 += kAhead) {
@@ -1272,15 +1298,17 @@ __global__ __launch_bounds__(512) void f8_pair_down_kernel(ExpertsArgs a, const 
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // before the next route's values
         }
         if ((l & 15) == 0) *reinterpret_cast<f32x4 *>(red + k * 16 + P::row(l, 0)) = acc;
+        if (l == 0) {
+            weight[k] = w;
+            used[k] = m != nullptr;
+        }
     }
-    const bool ok = ids_ok(a, l);  // last, as it waits for nothing that the weights wait for
+    const bool ok = ids_ok(a, id);
     __syncthreads();
     if (ok && tid < 16 && row0 + tid < d.rows) {
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.top_k; ++k) {
-            const uint32_t pair = token * a.top_k + k;
-            if (a.ids[pair] != TQF_HIP_NO_EXPERT) v = __builtin_fmaf(a.w[pair], red[k * 16 + tid], v);
-        }
+        for (uint32_t k = 0; k < a.top_k; ++k)
+            if (used[k]) v = __builtin_fmaf(weight[k], red[k * 16 + tid], v);
         const f32x4 one = {v, 0.0f, 0.0f, 0.0f};
         store4(y + (size_t)token * d.rows + row0 + tid, 1, one);
     }
@@ -1376,12 +1404,13 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
     const uint32_t pairs = a.t * a.top_k;
     const F8Shape dg = f8_shape(ex.width, ex.hidden), dd = f8_shape(ex.hidden, ex.width);
     if (pairs_path(ex, a.t, a.top_k)) {
-        float *h = static_cast<float *>(scratch);
+        const uint8_t **downs = static_cast<const uint8_t **>(scratch);
+        float *h = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + kPairsMax * sizeof(void *));
         const uint32_t hstride = dd.kb * 128;
-        f8_pair_gate_up_kernel<<<dim3((ex.width + 15) / 16, pairs), 256, dg.kb * 260 + 16 + 512, s>>>(a, ex.mats, dg, x, h, hstride);
+        f8_pair_gate_up_kernel<<<dim3((ex.width + 15) / 16, pairs), 256, dg.kb * 260 + 16 + 512, s>>>(a, ex.mats, dg, x, h, hstride, downs);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        f8_pair_down_kernel<<<dim3((ex.hidden + 15) / 16, a.t), 512, 8 * dd.kb * 260 + a.top_k * 64, s>>>(a, ex.mats, dd, h, hstride, y);
+        f8_pair_down_kernel<<<dim3((ex.hidden + 15) / 16, a.t), 512, 8 * dd.kb * 260 + a.top_k * 64, s>>>(a, downs, dd, h, hstride, y);
         return hipGetLastError();
     }
     const ExpertsScratch b = experts_scratch(scratch, ex, a.t, a.top_k, sizeof(YT) == 2 ? TQF_HIP_TYPE_BF16 : TQF_HIP_TYPE_F32);
@@ -1435,7 +1464,7 @@ hipError_t launch_f8_matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d,
 }
 
 size_t f8_experts_scratch_bytes(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k, int32_t y_type) {
-    if (pairs_path(ex, t, top_k)) return (size_t)t * top_k * ((ex.width + 127) / 128 * 128) * 4;
+    if (pairs_path(ex, t, top_k)) return kPairsMax * sizeof(void *) + (size_t)t * top_k * ((ex.width + 127) / 128 * 128) * 4;
     return experts_scratch(nullptr, ex, t, top_k, y_type).total;
 }
 

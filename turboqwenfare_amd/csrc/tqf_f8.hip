@@ -888,10 +888,10 @@ hipError_t launch_split(hipStream_t s, const uint8_t *mat, const F8Shape &d, con
 // as it is once its larger tiles (which load less for a product) fill the card.
 // us, split / tiled: 64 bf16 rows of 4096 by 8192 12.2 / 26, 256 26.5 / 50, 512
 // (1024 workgroups) 45 / 45, 1024 88 / 45, 256 by 20000 (1250) 59 / 53; f32 rows of
-// the same by 8192, 64 rows 13 / 32, 512 56 / 41.  f32 takes 32 rows always (256
-// rows 31, in steps of 64 33, of 128 40).
-uint32_t split_rows(const F8Shape &d, uint32_t t, bool f32) {
-    const uint32_t rows = f32 || t <= 32 ? 32 : t <= 64 ? 64 : 128;
+// the same by 8192, 64 rows 13 / 32, 512 56 / 41.  The bf16 instructions take 32
+// rows always (256 rows 31, in steps of 64 33, of 128 40).
+uint32_t split_rows(const F8Shape &d, uint32_t t, bool exact) {
+    const uint32_t rows = exact || t <= 32 ? 32 : t <= 64 ? 64 : 128;
     return (uint64_t)((d.rows + 31) / 32) * ((t + rows - 1) / rows) <= 1024 ? rows : 0;
 }
 
@@ -901,12 +901,13 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     uint8_t *xq = static_cast<uint8_t *>(scratch);
     float *xs = reinterpret_cast<float *>(xq + align256((size_t)pad32(t) * d.kb * 128));
     constexpr bool kF32 = sizeof(YT) == 4;
-    if (const uint32_t rows = split_rows(d, t, kF32)) {
+    // up to 16 rows have exact products, also those that are too wide for a workgroup's LDS
+    const bool exact = kF32 || t <= kRowsMax;
+    if (const uint32_t rows = split_rows(d, t, exact)) {
         hipError_t e = quantize<true>(s, x, t, d.cols, d.kb, xq, xs);
         if (e != hipSuccess) return e;
-        if constexpr (kF32) {
-            return launch_split<Bf16x16, 1, YT>(s, mat, d, xq, xs, t, y);
-        } else {
+        if (exact) return launch_split<Bf16x16, 1, YT>(s, mat, d, xq, xs, t, y);
+        if constexpr (!kF32) {
             return rows == 32   ? launch_split<Fp8x32, 1, YT>(s, mat, d, xq, xs, t, y)
                    : rows == 64 ? launch_split<Fp8x32, 2, YT>(s, mat, d, xq, xs, t, y)
                                 : launch_split<Fp8x32, 4, YT>(s, mat, d, xq, xs, t, y);
@@ -924,6 +925,7 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
     if constexpr (kF32) {
         return t <= 32 ? launch_dense<Bf16x16, 2, 2, 2, YT>(s, a) : launch_dense<Bf16x16, 2, 4, 2, YT>(s, a);
     } else {
+        if (exact) return launch_dense<Bf16x16, 2, 2, 2, YT>(s, a);
         if (t <= 32) return launch_dense<Fp8x32, 1, 1, 2, YT>(s, a);
         if (t <= 64) return launch_dense<Fp8x32, 2, 2, 2, YT>(s, a);
         // Tiles of 256 rows where they leave little of the card without work in

@@ -14,13 +14,16 @@
 // products at a time and cut each to 2^-13 of the largest one's power of two
 // (measured, tests/test_gpu_f8.py): a block loses less than 7 * 2^-13 of its
 // magnitudes; against 64 bits, one of normal values is 1.3e-5 off (relative,
-// 2-norm), 3.9e-5 with rows that span 2^8.  bf16 results are
-// rounded at 2^-9 = 2e-3, so they are made of these; f32 results, and every
-// small call, widen the values to bf16 (exact) for the bf16 instructions,
-// whose products of e4m3 values came out exact in the same test.
+// 2-norm), 3.9e-5 with rows that span 2^8.  Rounding to bf16
+// costs 1.7e-3, so bf16 results of large calls are made of these (f8_matmul's,
+// and the down products of f8_experts).  f32 results, the experts' gate and up
+// products, whose error the quantisation of h would make larger, and every small
+// call widen the values to bf16 (exact) for the bf16 instructions, whose products
+// of e4m3 values came out exact in the same test.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "tqf_f8.h"
@@ -519,7 +522,9 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
         k_loop(std::integral_constant<int, CT>{});
     } else {
         const uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane((int)((mine + M - 1) / M));
-        if (CT >= 4 && n >= 4) k_loop(std::integral_constant<int, CT < 4 ? CT : 4>{});
+        if (CT >= 6 && n >= 6) k_loop(std::integral_constant<int, CT < 6 ? CT : 6>{});
+        else if (CT >= 5 && n >= 5) k_loop(std::integral_constant<int, CT < 5 ? CT : 5>{});
+        else if (CT >= 4 && n >= 4) k_loop(std::integral_constant<int, CT < 4 ? CT : 4>{});
         else if (CT >= 3 && n >= 3) k_loop(std::integral_constant<int, CT < 3 ? CT : 3>{});
         else if (CT >= 2 && n >= 2) k_loop(std::integral_constant<int, CT < 2 ? CT : 2>{});
         else k_loop(std::integral_constant<int, 1>{});
@@ -742,10 +747,15 @@ __global__ __launch_bounds__(kRowsThreads) void f8_rows_kernel(const uint8_t *__
     }
 }
 
+// Compute units of the current device (asked for once).
 int cu_count() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
-    return n > 0 ? n : 256;
+    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 template <typename XT, typename YT>
@@ -1329,16 +1339,22 @@ bool pairs_path(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
 // experts' in one tile, whose weights are then read once; but no more than 96, so
 // that a compute unit has two workgroups, of which one computes while the other
 // starts or stores.  Experts that fill several tiles anyway take 64 rows until
-// those of 96 would give every compute unit a workgroup of gate_up.  us for tiles
-// of 32 / 64 / 96 rows, hidden 2048, width 512, top 8: 256 experts, 1100 tokens
-// (mean 34) - / 173 / 180, 2048 (64) - / 218 / 203, 4096 - / 301 / 279; 60
-// experts, 128 tokens (17) 47.3 / 45.1 / 46.9, 512 (68) 82 / 65 / 53; 8 experts,
-// 256 tokens 40 / 33 / 38, 512 62 / 41 / 44, 1000 99 / 66 / 66.  Up to 64 pairs
-// stay on the tiles whose products are exact, as the path for few pairs is.
+// those of 96 would give every compute unit two workgroups of gate_up, and 32
+// where those of 64 would give one to fewer than half of them.  us for tiles of 32
+// / 64 / 96 rows, bf16 y, hidden 2048, width 512, top 8: 256 experts, 512 tokens
+// (mean 16) 175 / 163 / 180, 1100 (34) 220 / 191 / 197, 2048 (64) 282 / 226 / 210,
+// 4096 475 / 328 / 305; 60 experts, 300 tokens (40) 65 / 55 / 58, 512 (68) 86 / 76
+// / 62, 800 (107) 118 / 82 / 83, 2048 222 / 159 / 146; 8 experts, 16 tokens 28.5 /
+// 30.5 / 39, 64 34 / 39 / 43, 128 35 / 40 / 43, 256 41 / 42 / 50, 512 63 / 50 / 57,
+// 1000 101 / 78 / 86, 4096 334 / 240 / 237.  Up to 64 pairs stay on the tiles whose
+// products are all exact, as the path for few pairs is.
 uint32_t tile_rows(const F8ExpertsDev &ex, uint32_t t, uint32_t top_k) {
-    const uint32_t mean = t * top_k <= kPairsMax ? std::min(t * top_k / ex.n_experts, 14u) : t * top_k / ex.n_experts;
-    if (mean <= 40) return mean <= 6 ? 16 : mean <= 14 ? 32 : 64;
-    return mean > 96 && t * top_k / 96 * ((ex.width + 127) / 128) < 256 ? 64 : 96;
+    const uint32_t pairs = t * top_k, mean = pairs <= kPairsMax ? std::min(pairs / ex.n_experts, 14u) : pairs / ex.n_experts;
+    const uint32_t blocks = (ex.width + 127) / 128, cus = (uint32_t)cu_count();
+    if (mean <= 14) return mean <= 6 ? 16 : 32;
+    if (ex.n_experts * ((mean + 63) / 64) * blocks < cus / 2) return 32;
+    if (mean <= 40) return 64;
+    return mean > 96 && pairs / 96 * blocks < 2 * cus ? 64 : 96;
 }
 struct ExpertsScratch {
     int32_t *pos_of_pair, *row_of_pos, *n_tiles;
@@ -1378,8 +1394,16 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     return b;
 }
 
-template <class P, int RT, int CT, typename OT, int AHEAD>
+// G, D: how gate_up and down take tiles of ROWS rows.
+template <class P_, int RT_, int CT_, int AHEAD_>
+struct TileForm {
+    typedef P_ P;
+    static constexpr int RT = RT_, CT = CT_, AHEAD = AHEAD_, kRows = CT_ * P_::M;
+};
+template <class G, class D, typename OT>
 hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScratch &b, uint32_t t, uint32_t pairs) {
+    static_assert(G::kRows == D::kRows, "gate_up and down take the same tiles");
+    static_assert(G::RT * G::P::M == 64, "a workgroup of gate_up makes one block of h");
     TiledArgs a{};
     a.d = f8_shape(ex.width, ex.hidden);
     a.xq = b.xq;
@@ -1392,8 +1416,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.hkb = (ex.width + 127) / 128;
     a.hrows = pairs;
     a.rblocks = a.hkb;
-    static_assert(RT * P::M == 64, "a workgroup of gate_up makes one block of h");
-    f8_tiled_kernel<P, RT, CT, kGateUp, float, 1, false, AHEAD><<<b.max_tiles * a.rblocks, 256, 0, s>>>(a);
+    f8_tiled_kernel<typename G::P, G::RT, G::CT, kGateUp, float, 1, false, G::AHEAD><<<b.max_tiles * a.rblocks, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     a.d = f8_shape(ex.hidden, ex.width);
@@ -1403,7 +1426,7 @@ hipError_t launch_tiles(hipStream_t s, const F8ExpertsDev &ex, const ExpertsScra
     a.out = b.out;
     a.out_scales = b.out_scales;
     a.rblocks = (ex.hidden + 255) / 256;
-    f8_tiled_kernel<P, RT, CT, kDown, OT, 1, false, AHEAD><<<b.max_tiles * a.rblocks, 256, 0, s>>>(a);
+    f8_tiled_kernel<typename D::P, D::RT, D::CT, kDown, OT, 1, false, D::AHEAD><<<b.max_tiles * a.rblocks, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1428,13 +1451,24 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
                                                         b.xq, b.xs);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    // gate_up always takes the bf16 instructions: its error would move values of h
+    // across a rounding step (fp8 ones: 2.1e-3 to 2.3e-3 of y instead of the 1.7e-3
+    // that bf16 rounding costs, and an f32 y no nearer than a bf16 one).  down takes
+    // the fp8 ones where its results are rounded to bf16 next; 4096 tokens
+    // take 305 us so, and 277 with gate_up on the fp8 ones too.
+    typedef TileForm<Bf16x16, 4, 1, 2> T16;
+    typedef TileForm<Bf16x16, 4, 2, 2> T32;
+    typedef TileForm<Bf16x16, 4, 4, 2> T64;
+    typedef TileForm<Bf16x16, 4, 6, 1> T96;
     if (m == 16) {
-        e = launch_tiles<Bf16x16, 4, 1, float, 2>(s, ex, b, a.t, pairs);
+        e = launch_tiles<T16, T16, float>(s, ex, b, a.t, pairs);
     } else if (m == 32) {
-        e = launch_tiles<Bf16x16, 4, 2, float, 2>(s, ex, b, a.t, pairs);
+        e = launch_tiles<T32, T32, float>(s, ex, b, a.t, pairs);
+    } else if constexpr (sizeof(YT) == 4) {
+        e = m == 64 ? launch_tiles<T64, T64, float>(s, ex, b, a.t, pairs) : launch_tiles<T96, T96, float>(s, ex, b, a.t, pairs);
     } else {
-        typedef typename std::conditional<sizeof(YT) == 2, Out16, float>::type OT;
-        e = m == 64 ? launch_tiles<Fp8x32, 2, 2, OT, 2>(s, ex, b, a.t, pairs) : launch_tiles<Fp8x32, 2, 3, OT, 1>(s, ex, b, a.t, pairs);
+        e = m == 64 ? launch_tiles<T64, TileForm<Fp8x32, 2, 2, 2>, Out16>(s, ex, b, a.t, pairs)
+                    : launch_tiles<T96, TileForm<Fp8x32, 2, 3, 1>, Out16>(s, ex, b, a.t, pairs);
     }
     if (e != hipSuccess) return e;
     if (sizeof(YT) == 2 && b.out16) {

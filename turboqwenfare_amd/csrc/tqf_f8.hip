@@ -600,8 +600,10 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
                         m = fmaxf(m, v < __builtin_inff() ? v : 0.0f);
                     }
                 m = P::across(m);
-                const uint32_t p = m < 0x1p-100f ? 0 : __float_as_uint(m) & 0x7F800000u;  // 2^e <= m
-                inv = p ? __uint_as_float((268u << 23) - p) : 0.0f;                // 2^(14 - e)
+                // 2^e <= m, but no less than 2^-100: 2^(14 - e) stays finite, and an
+                // infinity beside zeros an infinity
+                const uint32_t p = __float_as_uint(fmaxf(m, 0x1p-100f)) & 0x7F800000u;
+                inv = __uint_as_float((268u << 23) - p);  // 2^(14 - e)
                 const uint32_t in = (uint32_t)(c * M + row);
                 if (l < M && in < mine && wrow[0] < n)
                     a.out_scales[(size_t)(first + row0 + in) * blocks + wrow[0] / kOutBlock] = __uint_as_float(p) * 0x1p-14f;

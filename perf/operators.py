@@ -181,21 +181,20 @@ class _Kept:
 
 
 def _experts_handle(c, index):
-    """The prepared experts of a layer, kept with its weights."""
+    """The prepared experts of a layer, with their matrices: laid out once for a geometry, and given back when neither
+    a state nor this module, which keeps those of the newest geometry, has them."""
     be, key = _backend(), (c["experts"], c["hidden"], c["width"], index)
     if _HANDLES and next(iter(_HANDLES))[:3] != key[:3]:
-        for prepared, mats in _HANDLES.values():
-            be.free_f8_experts(prepared)
-            for m in mats:
-                be.free_weights(m)
         _HANDLES.clear()
     if key not in _HANDLES:
         layer = _layer(c, index)
         torch.cuda.synchronize()
         mats = [[be.upload_f8_device(_buf(q[e]), _buf(s[e]), q.shape[1], q.shape[2]) for e in range(q.shape[0])]
                 for q, s in layer]
-        _HANDLES[key] = be.prepare_f8_experts(*mats), [m for g in mats for m in g]
-    return _HANDLES[key][0]
+        prepared = be.prepare_f8_experts(*mats)
+        _HANDLES[key] = _Kept([prepared, *mats[0], *mats[1], *mats[2]],
+                              lambda h: be.free_f8_experts(h) if h is prepared else be.free_weights(h))
+    return _HANDLES[key]
 
 
 def prepare(case, seed):
@@ -343,8 +342,8 @@ def run(st):
     if kind == "matmul":
         be.f8_matmul_device(st["kept"].handles[0], b["x"], c["t"], b["out"], x_type=c["x"], y_type=c["y"])
         return st["out"]
-    for i, handle in enumerate(st["handles"]):
-        be.f8_experts_device(handle, b["x"][i], c["t"], b["ids"][i], b["w"][i], c["top_k"], b["out"][i], x_type=c["x"],
+    for i, kept in enumerate(st["handles"]):
+        be.f8_experts_device(kept.handles[0], b["x"][i], c["t"], b["ids"][i], b["w"][i], c["top_k"], b["out"][i], x_type=c["x"],
                              y_type="bf16", d_status=b["status"])
     return st["out"]
 

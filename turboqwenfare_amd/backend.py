@@ -50,6 +50,14 @@ def _hold(what: str, *needs) -> None:
             raise ValueError(f"{what}: a buffer of {buf.nbytes} bytes, {nbytes} needed")
 
 
+def _integers(what: str, a, dtype, low: int, high: int) -> np.ndarray:
+    """`a` as `dtype`, if it holds integers of low..high (negative ones wrap); other numbers would be cut."""
+    a = np.asarray(a)
+    if a.dtype != dtype and (a.dtype.kind not in "iu" or (a.size and (int(a.min()) < low or int(a.max()) > high))):
+        raise ValueError(f"{what}: integers of {low}..{high}")
+    return np.ascontiguousarray(a).astype(dtype, copy=False)
+
+
 @dataclass
 class Q4Weights:
     handle: int
@@ -502,7 +510,7 @@ class HipBackend:
 
     def upload_f8(self, q: np.ndarray, scales: np.ndarray) -> F8Weights:
         """q [rows, cols] u8 (e4m3 bytes), scales [ceil(rows / 128), ceil(cols / 128)] f32."""
-        q = np.ascontiguousarray(q, dtype=np.uint8)
+        q = _integers("upload_f8: the e4m3 bytes", q, np.uint8, -128, 255)
         s = np.ascontiguousarray(scales, dtype=np.float32)
         if q.ndim != 2 or s.shape != (-(-q.shape[0] // 128), -(-q.shape[1] // 128)):
             raise ValueError("upload_f8: q [rows, cols] and one scale for each block of 128 x 128")
@@ -569,9 +577,9 @@ class HipBackend:
                                                        d_y.ptr, yt, d_status.ptr if d_status else None))
 
     def f8_experts(self, ex: F8Experts, x: np.ndarray, ids: np.ndarray, w: np.ndarray) -> np.ndarray:
-        """Host form: x [t, hidden] f32, ids [t, k] u16, w [t, k] f32 -> [t, hidden] f32."""
+        """Host form: x [t, hidden] f32, ids [t, k] u16 (-1: an empty slot), w [t, k] f32 -> [t, hidden] f32."""
         x = np.ascontiguousarray(x, dtype=np.float32)
-        ids = np.ascontiguousarray(ids, dtype=np.uint16)
+        ids = _integers("f8_experts: ids", ids, np.uint16, -1, 0xFFFF)
         w = np.ascontiguousarray(w, dtype=np.float32)
         if x.ndim != 2 or x.shape[1] != ex.hidden or ids.ndim != 2 or ids.shape[0] != x.shape[0] or w.shape != ids.shape:
             raise ValueError("f8_experts: x [t, hidden], ids and w [t, top_k]")

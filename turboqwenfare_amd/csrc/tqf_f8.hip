@@ -899,12 +899,12 @@ hipError_t launch_split(hipStream_t s, const uint8_t *mat, const F8Shape &d, con
 // A workgroup's activation rows where K is split; 0: the tiled product is faster,
 // as it is once its larger tiles (which load less for a product) fill the card.
 // us, split / tiled: 64 bf16 rows of 4096 by 8192 12.2 / 26, 256 26.5 / 50, 512
-// (1024 workgroups) 45 / 45, 1024 88 / 45, 256 by 20000 (1250) 59 / 53; f32 rows of
-// the same by 8192, 64 rows 13 / 32, 512 56 / 41.  The bf16 instructions take 32
-// rows always (256 rows 31, in steps of 64 33, of 128 40).
+// (1024 workgroups, four to a compute unit) 45 / 45, 1024 88 / 45, 256 by 20000
+// (1250) 59 / 53; f32 rows of the same by 8192, 64 rows 13 / 32, 512 56 / 41.  The
+// bf16 instructions take 32 rows always (256 rows 31, in steps of 64 33, of 128 40).
 uint32_t split_rows(const F8Shape &d, uint32_t t, bool exact) {
     const uint32_t rows = exact || t <= 32 ? 32 : t <= 64 ? 64 : 128;
-    return (uint64_t)((d.rows + 31) / 32) * ((t + rows - 1) / rows) <= 1024 ? rows : 0;
+    return (uint64_t)((d.rows + 31) / 32) * ((t + rows - 1) / rows) <= 4u * (uint32_t)cu_count() ? rows : 0;
 }
 
 template <typename XT, typename YT>
@@ -946,9 +946,9 @@ hipError_t matmul(hipStream_t s, const uint8_t *mat, const F8Shape &d, const XT 
         // 4096 by 8192, K 4096 172 / 160 / 143, 2048 by 6000 (0.73 of a round) 65 /
         // 78 / 60; 2048 by 4096 (0.5) 46 / 50 / 60, 1024 by 8192 45 / 48 / 55; 2560
         // by 8192, K 2048 (0.63 of two) 57 / 56 / 65.
-        const uint64_t rbs = (d.rows + 255) / 256, rounds = (rbs * ((t + 255) / 256) + 255) / 256;
-        if ((uint64_t)d.rows * t * 10 >= rounds * 7 * 256 * 256 * 256) return launch_dense<Fp8x32, 2, 4, 1, YT, 2, true>(s, a);
-        return rbs * ((t + 63) / 64) <= 512 ? launch_dense<Fp8x32, 2, 2, 2, YT>(s, a) : launch_dense<Fp8x32, 2, 3, 1, YT>(s, a);
+        const uint64_t cus = (uint64_t)cu_count(), rbs = (d.rows + 255) / 256, rounds = (rbs * ((t + 255) / 256) + cus - 1) / cus;
+        if ((uint64_t)d.rows * t * 10 >= rounds * 7 * cus * 256 * 256) return launch_dense<Fp8x32, 2, 4, 1, YT, 2, true>(s, a);
+        return rbs * ((t + 63) / 64) <= 2 * cus ? launch_dense<Fp8x32, 2, 2, 2, YT>(s, a) : launch_dense<Fp8x32, 2, 3, 1, YT>(s, a);
     }
 }
 

@@ -176,3 +176,31 @@ def test_large_tiles(be):
         y, st = layer.run(x, "f32", ids, w, y_kind)
         assert st == 1 and (y == (0x4242 if y_kind == "bf16" else 7)).all()
     layer.close()
+
+
+@pytest.mark.parametrize("hidden,width", [(65536, 5), (5, 65536)])
+def test_as_wide_as_any(be, hidden, width):
+    """512 blocks of K, by few slots and by tiles."""
+    from test_gpu_f8 import Layer
+
+    layer = Layer(be, 2, hidden, width, 3)
+    for t, k in ((1, 2), (17, 2), (130, 1)):
+        layer.check(t, k, "bf16", "f32")
+        layer.check(t, k, "f32", "bf16")
+    layer.close()
+
+
+def test_as_many_experts_as_any(be):
+    """1024 experts (that take turns with 16 matrices each), one slot to an expert and 64."""
+    from test_gpu_f8 import Layer
+
+    few = Layer(be, 16, 130, 70, 4)
+    n = 1024
+    many = Layer.__new__(Layer)
+    many.be, many.n, many.hidden, many.width = be, n, few.hidden, few.width
+    many.mats = [few.mats[e % 16] for e in range(n)]
+    many.ex = be.prepare_f8_experts(*([g[e % 16] for e in range(n)] for g in few.handles))
+    for t, k in ((1, 16), (64, 16), (4096, 5), (4096, 16)):
+        many.check(t, k, "bf16", "bf16")
+    be.free_f8_experts(many.ex)
+    few.close()

@@ -457,7 +457,8 @@ int32_t tqf_hip_lm_head_logits_device(tqf_hip_ctx *ctx, const tqf_hip_weights *w
  * of 128: with a the block's largest magnitude, scale = a / 448 and
  * q = e4m3(x * (448 / a)), both quotients and the product rounded to f32, the
  * conversion to nearest with ties to even; a block with a < 2^-100 is zero.  A
- * row with a NaN or an infinity gives NaN; other rows do not see it.
+ * row with a NaN or an infinity gives NaN; other rows do not see it.  A block's
+ * two scales are multiplied first, in f32: their product should be finite.
  * Element types of rows (`*_type`): */
 #define TQF_HIP_TYPE_F32 0
 #define TQF_HIP_TYPE_BF16 1
@@ -524,7 +525,9 @@ int32_t tqf_hip_f8_experts_device(tqf_hip_ctx *ctx, const tqf_hip_f8_experts *ex
  * logits [t x n_experts] f32.  1 <= n_experts <= TQF_HIP_ROUTE_MAX_EXPERTS, 1 <=
  * hidden <= 65536.  Up to 8 rows the products are summed in 64 bits; above that
  * every product of a bf16 x is exact (of an f32 x to 2^-24 of it), sums are f32,
- * and an f32 magnitude above 3.39e38 (the largest bf16) counts as infinite. */
+ * and an f32 magnitude above 3.39e38 (the largest bf16) counts as infinite.  A
+ * row with an infinity or a NaN has no finite logit (above 8 rows NaN also where
+ * the sum would be infinite); other rows do not see it. */
 int32_t tqf_hip_router_logits_device(tqf_hip_ctx *ctx, const tqf_hip_tensor *router, const void *d_x,
                                      int32_t x_type, uint32_t t, uint32_t n_experts, uint32_t hidden,
                                      float *d_logits);
@@ -652,8 +655,8 @@ int32_t tqf_hip_recovery_counts(tqf_hip_ctx *ctx, uint64_t *stack_reruns, uint64
 int32_t tqf_hip_profile_enable(tqf_hip_ctx *ctx, int32_t enable);
 /* Synchronises, then reports launches, summed kernel milliseconds and the
  * summed algorithmic HBM bytes of those launches for one kind (0 for the
- * grouped GEMM kinds, whose bytes depend on the routes: the caller, who holds
- * the ids, counts the distinct experts). */
+ * grouped GEMM kinds and the F8 experts, whose bytes depend on the routes: the
+ * caller, who holds the ids, counts the distinct experts). */
 int32_t tqf_hip_profile_read(tqf_hip_ctx *ctx, int32_t kind, uint64_t *launches,
                              double *total_ms, double *algorithmic_bytes);
 

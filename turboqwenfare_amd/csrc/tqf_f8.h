@@ -11,8 +11,12 @@
 // l % 16 of chunks 4 j + l / 16 for the 16-row ones (the order in which an
 // MFMA takes its K elements is free, so long as both operands have the same).
 //
-// Rows of activations are quantised in blocks of 128 (f8_block below) and kept
-// row-major, [row][128 K blocks] bytes, with their scales [K block][row].
+// Rows of activations are quantised in blocks of 128 (f8_factors, f8_pack4) and kept
+// by K block, for the form that reads them (t rows, t32: rounded up to 32):
+//   tiles         [K block][t][128 bytes], scales [K block][t]; so is h, by position
+//   split K       [K block][t32 / 32][8 chunks][32 rows][16 bytes], the matrices'
+//                 order, scales [K block][t32]
+// The forms for up to 16 rows and for few slots keep them in LDS.
 #pragma once
 
 #include "tqf_device.h"

@@ -58,13 +58,15 @@ __global__ __launch_bounds__(256) void logits_few_kernel(const float *__restrict
 // three bf16 (8 bits each; exact for magnitudes above 2^-102, below which the
 // last pieces vanish), so R = R0 + R1 + R2, and for bf16 x three products give
 // every bit of x R; f32 x is split as well, and of the nine products the six
-// above 2^-24 of the largest are taken.  The f32 instructions would take five
-// times as long.  A workgroup has 16 ET experts by 16 TT rows; its wavefronts
-// split K (8 ways, a step of 32 columns each in turn) and add their sums in LDS,
-// pairwise, in the same order for every tile size.  4096 bf16 rows of 2048 by 256
-// experts: 19 us, where the three products alone would take 8.6 at the rate of a
-// large library product; the vector units, which split the router's rows anew in
-// every workgroup, and the matrix cores take turns.
+// above 2^-24 of the largest are taken.  A workgroup has 16 ET experts by 16 TT
+// rows; its wavefronts split K (8 ways, a step of 32 columns each in turn) and add
+// their sums in LDS, pairwise, in the same order for every tile size.  4096 rows of
+// 2048 by 256 experts: 19 us with bf16 x and 35 with f32, where the products alone
+// would take 8.6 and 17 at the rate of a large library product; the vector units,
+// which split the router's rows anew in every workgroup, and the matrix cores take
+// turns.  The f32 instructions (157 TFLOP/s from registers) need 27 us for the
+// product alone: more than the bf16 form takes, less than the f32 one does; a
+// kernel of them was not built.
 struct Split3 {
     bf16x8 p[3];
 };

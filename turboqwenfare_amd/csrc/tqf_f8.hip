@@ -402,9 +402,9 @@ __global__ __launch_bounds__(256 * TW, 2) void f8_tiled_kernel(TiledArgs a) {
     // fill fewer).  Blocks are asked for AHEAD steps before they are computed
     // (past the end the last one again, so that no branch splits the loop): two
     // where the registers hold another block of weights, for a step is as long as
-    // a trip to memory if nothing else fills it (experts of 512 tokens 177 us with
-    // one, 162 with two; 16 tokens of 8 experts 29.5 and 25.6).  Scales go through
-    // LDS too: in registers they would have to be waited for with the blocks asked
+    // a trip to memory if nothing else fills it (both kernels of 512 tokens of
+    // experts on the fp8 cores: 177 us with one, 162 with two).  Scales go through LDS
+    // too: in registers they would have to be waited for with the blocks asked
     // for after them.
     auto k_loop = [&](auto tiles_used) {
         constexpr int N = decltype(tiles_used)::value;

@@ -14,12 +14,12 @@
 // products at a time and cut each to 2^-13 of the largest one's power of two
 // (measured, tests/test_gpu_f8.py): a block loses less than 7 * 2^-13 of its
 // magnitudes; against 64 bits, one of normal values is 1.3e-5 off (relative,
-// 2-norm), 3.9e-5 with rows that span 2^8.  Rounding to bf16
-// costs 1.7e-3, so bf16 results of large calls are made of these (f8_matmul's,
-// and the down products of f8_experts).  f32 results, the experts' gate and up
-// products, whose error the quantisation of h would make larger, and every small
-// call widen the values to bf16 (exact) for the bf16 instructions, whose products
-// of e4m3 values came out exact in the same test.
+// 2-norm), 3.9e-5 with rows that span 2^8.  Rounding to bf16 costs 1.7e-3, so bf16
+// results of large calls are made of these (f8_matmul's, and the down products of
+// f8_experts).  f32 results, the experts' gate and up products, whose error the
+// quantisation of h would make larger, and every small call widen the values to
+// bf16 (exact) for the bf16 instructions, whose products of e4m3 values came out
+// exact in the same test.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1396,7 +1396,7 @@ ExpertsScratch experts_scratch(void *scratch, const F8ExpertsDev &ex, uint32_t t
     return b;
 }
 
-// G, D: how gate_up and down take tiles of ROWS rows.
+// How a kernel takes tiles of kRows rows; G: gate_up, D: down.
 template <class P_, int RT_, int CT_, int AHEAD_>
 struct TileForm {
     typedef P_ P;
@@ -1456,8 +1456,8 @@ hipError_t experts(hipStream_t s, const F8ExpertsDev &ex, const XT *x, YT *y, co
     // gate_up always takes the bf16 instructions: its error would move values of h
     // across a rounding step (fp8 ones: 2.1e-3 to 2.3e-3 of y instead of the 1.7e-3
     // that bf16 rounding costs, and an f32 y no nearer than a bf16 one).  down takes
-    // the fp8 ones where its results are rounded to bf16 next; 4096 tokens
-    // take 305 us so, and 277 with gate_up on the fp8 ones too.
+    // the fp8 ones where its results are rounded to bf16 next; 4096 tokens take 305
+    // us so, and 277 with gate_up on the fp8 ones too.
     typedef TileForm<Bf16x16, 4, 1, 2> T16;
     typedef TileForm<Bf16x16, 4, 2, 2> T32;
     typedef TileForm<Bf16x16, 4, 4, 2> T64;

@@ -558,6 +558,110 @@ int32_t tqf_hip_route_tokens_device(tqf_hip_ctx *ctx, const void *d_logits, int3
                                     const tqf_hip_route_options *options, uint16_t *d_ids, float *d_w,
                                     int32_t *d_status);
 
+/* ---- attention: the half of a decoder layer between two MoE tails ---------------
+ * The role of the reference's BF16 full attention (model/qwen36/attention.rs) for
+ * the rows of a prompt and for the verify rows of many sequences; the cache is
+ * this backend's own.  A layer runs: projection (e.g. tqf_hip_f8_matmul_device),
+ * tqf_hip_qk_rope_device, then tqf_hip_attn_prompt_device over a prompt's packed
+ * rows or tqf_hip_attn_paged_device over the cache, projection,
+ * tqf_hip_add_rows_device. */
+#define TQF_HIP_ATTN_MAX_TOKENS (1u << 20) /* query rows of a call           */
+#define TQF_HIP_ATTN_MAX_SEQS 16384        /* sequences of a call            */
+typedef struct tqf_hip_heads {
+    uint32_t q_heads;  /* 1..256, a multiple of kv_heads: query head h reads key head h / (q_heads / kv_heads) */
+    uint32_t kv_heads; /* 1..q_heads                                          */
+    uint32_t head_dim; /* 64, 128 or 256                                      */
+} tqf_hip_heads;
+/* Heads of rows that stand anywhere (among others in a projection's output):
+ * element (t, h, i) is data[t * row_stride + h * head_stride + i].  Strides in
+ * elements, multiples of 8 below 2^24; data aligned to 16 bytes.  Heads may
+ * interleave, but rows must not: row_stride >= head_dim where there are several rows. */
+typedef struct tqf_hip_head_rows {
+    const void *data;
+    uint64_t row_stride, head_stride;
+} tqf_hip_head_rows;
+/* A layer's cache, in device memory of the caller: pages of page_size tokens,
+ * keys and values [n_pages x kv_heads x page_size x head_dim], either bf16
+ * (TQF_HIP_TYPE_BF16) or e4m3 (TQF_HIP_TYPE_F8) with an f32 scale for each token
+ * and head [n_pages x kv_heads x page_size]: value = e4m3 * scale.  Slot s is token
+ * s % page_size of page s / page_size.  page_size is 16, 32, 64, 128 or 256,
+ * n_pages * page_size < 2^31; all four pointers aligned to 16 bytes. */
+#define TQF_HIP_TYPE_F8 2 /* of caches only */
+typedef struct tqf_hip_kv_cache {
+    void *d_k, *d_v;
+    float *d_k_scales, *d_v_scales; /* F8 only */
+    int32_t type;
+    uint32_t n_pages, page_size, kv_heads, head_dim;
+} tqf_hip_kv_cache;
+/* The rotation's frequencies (radians a position), one a pair of elements, 8..128
+ * pairs, a multiple of 8.  Angles are taken in 64 bits. */
+typedef struct tqf_hip_rope tqf_hip_rope;
+int32_t tqf_hip_rope_prepare(tqf_hip_ctx *ctx, const double *frequencies, uint32_t pairs, tqf_hip_rope **out);
+int32_t tqf_hip_rope_free(tqf_hip_ctx *ctx, tqf_hip_rope *rope);
+typedef struct tqf_hip_qk_options {
+    const tqf_hip_tensor *q_norm, *k_norm; /* [head_dim] each; NULL: that norm is left out */
+    float eps;                             /* >= 0, of the norms                           */
+    const tqf_hip_rope *rope;              /* 2 pairs <= head_dim; NULL: no rotation       */
+    int32_t neighbours; /* 0: pairs (i, i + pairs); 1: (2 i, 2 i + 1).  What is past 2 pairs stays */
+} tqf_hip_qk_options;
+/* For each of t rows (1..TQF_HIP_F8_MAX_TOKENS) and each head of q and k:
+ * x / sqrt(mean(x^2) + eps) * w, then each pair (a, b) becomes (a cos - b sin,
+ * b cos + a sin) of the angle positions[t] * frequency; sums f32, rounded once.
+ * q, k, v have x_type.  q goes to d_q_out [t x q_heads x head_dim], k to d_k_out
+ * and v (as it is) to d_v_out [t x kv_heads x head_dim] (either may be NULL), all
+ * bf16.  With a cache, k and v also go to slot d_slots[t] (-1: not cached, as for
+ * padding rows; two rows must not have one slot); in e4m3 a head's scale is its largest
+ * magnitude / 448 (below 2^-100: all zero) and a head with a NaN or an infinity
+ * reads back as NaN.  Any other slot outside the cache is left out and sets
+ * *d_status (may be NULL, zeroed by the caller) to TQF_HIP_ERR_INVALID.  cache and
+ * d_slots are both given or both NULL.  Outputs overlap neither one another nor
+ * the inputs. */
+int32_t tqf_hip_qk_rope_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, const tqf_hip_qk_options *options,
+                               const tqf_hip_head_rows *q, const tqf_hip_head_rows *k, const tqf_hip_head_rows *v,
+                               int32_t x_type, uint32_t t, const int32_t *d_positions, uint16_t *d_q_out,
+                               uint16_t *d_k_out, uint16_t *d_v_out, const tqf_hip_kv_cache *cache,
+                               const int32_t *d_slots, int32_t *d_status);
+/* Causal attention of packed prompts, all bf16.  Sequence s has the query rows
+ * cu_q[s]..cu_q[s + 1] and the keys cu_k[s]..cu_k[s + 1] (cu_* [n_seqs + 1] on the
+ * device, ascending, at most total_q and total_k); its last query is at its last
+ * key, so query i sees the keys j <= i + (keys - queries): a prompt has as many of
+ * both, a chunk of one more keys.
+ *   y[i][h] = sum_j softmax_j(scale q[i][h] . k[j]) v[j] * sigmoid(gate[i][h])
+ * (gate NULL: no factor), y [total_q x q_heads x head_dim].  Rows that see no key
+ * are 0; keys that a row does not see do not change it, NaN or not; rows of y
+ * outside every sequence stay as they are.  Scores, maxima and sums are f32,
+ * weights are rounded to bf16 for their product with v.  A sequence whose bounds
+ * are out of order or range is left out and sets *d_status (may be NULL, zeroed by the
+ * caller) to TQF_HIP_ERR_INVALID; y is then undefined.  scale > 0.  1 <= total_q <=
+ * TQF_HIP_ATTN_MAX_TOKENS, total_k < 2^31 (0: k and v are not read), 1 <= n_seqs <=
+ * TQF_HIP_ATTN_MAX_SEQS.  y must not overlap the inputs. */
+int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale,
+                                   const tqf_hip_head_rows *q, const tqf_hip_head_rows *k, const tqf_hip_head_rows *v,
+                                   const tqf_hip_head_rows *gate, const int32_t *d_cu_q, const int32_t *d_cu_k,
+                                   uint32_t n_seqs, uint32_t total_q, uint32_t total_k, uint16_t *d_y,
+                                   int32_t *d_status);
+/* Attention of the last `rows` (1..TQF_HIP_MAX_TOKENS) tokens of every sequence
+ * over its cache: 1 for decoding, k + 1 for verify rows.  lens[s] counts a
+ * sequence's cached tokens, these rows among them; token j is at slot
+ * pages[s][j / page_size] * page_size + j % page_size (pages [n_seqs x max_pages]);
+ * row i of the sequence is q row s * rows + i and sees the first lens[s] - rows + 1 + i
+ * tokens (none: 0).  The formula and the precision are the prompt's, e4m3 values
+ * are exact; q and gate bf16, y [n_seqs * rows x q_heads x head_dim].  The order of
+ * a sequence's sums depends on the lengths of all.  Page numbers behind a sequence's
+ * last token are not read.  A sequence with a page outside the cache, or with a length
+ * below 0 or above max_pages * page_size, gives NaN rows and sets *d_status (may be
+ * NULL, zeroed by the caller) to TQF_HIP_ERR_INVALID.  1 <= n_seqs <=
+ * TQF_HIP_ATTN_MAX_SEQS, 1 <= max_pages, max_pages * page_size < 2^31.  y must not
+ * overlap the inputs. */
+int32_t tqf_hip_attn_paged_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale,
+                                  const tqf_hip_head_rows *q, const tqf_hip_head_rows *gate, uint32_t n_seqs,
+                                  uint32_t rows, const tqf_hip_kv_cache *cache, const int32_t *d_pages,
+                                  uint32_t max_pages, const int32_t *d_lens, uint16_t *d_y, int32_t *d_status);
+/* d_out[i] = d_a[i] + d_b[i], n f32 values: a block's result onto the residual
+ * (the Metal tqf_residual_add, backend/metal/kernels.rs:372-379).  d_out may be d_a or d_b; any other
+ * overlap of it with them is not allowed. */
+int32_t tqf_hip_add_rows_device(tqf_hip_ctx *ctx, const float *d_a, const float *d_b, size_t n, float *d_out);
+
 /* ---- the decode loop's row kernels ------------------------------------------
  * Embedding rows (Qwen36Runtime::decode_step's embedding.row,
  * model/qwen36/runtime.rs:403; the row decoded per its dtype as
@@ -649,14 +753,18 @@ int32_t tqf_hip_recovery_counts(tqf_hip_ctx *ctx, uint64_t *stack_reruns, uint64
 #define TQF_HIP_KERNEL_F8_MATMUL 13      /* e4m3 matrix product, with its quantisation */
 #define TQF_HIP_KERNEL_F8_EXPERTS 14     /* e4m3 routed experts, all launches of a call */
 #define TQF_HIP_KERNEL_ROUTER 15         /* batched router: logits, routes            */
-#define TQF_HIP_KERNEL_KINDS 16
+#define TQF_HIP_KERNEL_QK_ROPE 16        /* heads: norms, rotation, cache                */
+#define TQF_HIP_KERNEL_ATTN_PROMPT 17    /* attention of packed prompts                  */
+#define TQF_HIP_KERNEL_ATTN_PAGED 18     /* attention over the cache, all launches of a call */
+#define TQF_HIP_KERNEL_KINDS 19
 /* While enabled, eager (non-graph) launches of each kind are bracketed by HIP
  * events on the context stream.  Enabling clears the totals. */
 int32_t tqf_hip_profile_enable(tqf_hip_ctx *ctx, int32_t enable);
 /* Synchronises, then reports launches, summed kernel milliseconds and the
  * summed algorithmic HBM bytes of those launches for one kind (0 for the
  * grouped GEMM kinds and the F8 experts, whose bytes depend on the routes: the
- * caller, who holds the ids, counts the distinct experts). */
+ * caller, who holds the ids, counts the distinct experts; and for the paged
+ * attention, whose bytes depend on the lengths). */
 int32_t tqf_hip_profile_read(tqf_hip_ctx *ctx, int32_t kind, uint64_t *launches,
                              double *total_ms, double *algorithmic_bytes);
 

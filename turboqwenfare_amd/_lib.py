@@ -35,7 +35,10 @@ KERNEL_SAMPLE = 12
 KERNEL_F8_MATMUL = 13
 KERNEL_F8_EXPERTS = 14
 KERNEL_ROUTER = 15
-KERNEL_KINDS = 16
+KERNEL_QK_ROPE = 16
+KERNEL_ATTN_PROMPT = 17
+KERNEL_ATTN_PAGED = 18
+KERNEL_KINDS = 19
 VARIANT_PERSISTENT = 0
 VARIANT_Q4K_FOLD = 1
 VARIANT_GRAPHS = 2
@@ -48,12 +51,15 @@ FORMAT_F8 = 3
 GROUPED_MAX_TOKENS = 4096
 TYPE_F32 = 0
 TYPE_BF16 = 1
+TYPE_F8 = 2  # of caches only
 F8_MAX_TOKENS = 65536
 NO_EXPERT = 0xFFFF
 ROUTE_MAX_EXPERTS = 1024
 ROUTE_MAX_TOP_K = 16
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
+ATTN_MAX_TOKENS = 1 << 20
+ATTN_MAX_SEQS = 16384
 
 _vp = C.c_void_p
 _i32 = C.c_int32
@@ -95,6 +101,42 @@ class RouteOptions(C.Structure):
         ("scale", _f32),
     ]
 
+
+class Heads(C.Structure):
+    """``tqf_hip_heads``."""
+
+    _fields_ = [("q_heads", _u32), ("kv_heads", _u32), ("head_dim", _u32)]
+
+
+class HeadRows(C.Structure):
+    """``tqf_hip_head_rows``."""
+
+    _fields_ = [("data", _vp), ("row_stride", _u64), ("head_stride", _u64)]
+
+
+class KvCache(C.Structure):
+    """``tqf_hip_kv_cache``."""
+
+    _fields_ = [
+        ("d_k", _vp),
+        ("d_v", _vp),
+        ("d_k_scales", _vp),
+        ("d_v_scales", _vp),
+        ("type", _i32),
+        ("n_pages", _u32),
+        ("page_size", _u32),
+        ("kv_heads", _u32),
+        ("head_dim", _u32),
+    ]
+
+
+class QkOptions(C.Structure):
+    """``tqf_hip_qk_options``."""
+
+    _fields_ = [("q_norm", _vp), ("k_norm", _vp), ("eps", _f32), ("rope", _vp), ("neighbours", _i32)]
+
+
+_hr = C.POINTER(HeadRows)
 
 # name -> (restype, argtypes); every exported symbol of include/tqf_hip.h and
 # include/tqf_hip_synth.h.
@@ -167,6 +209,16 @@ SIGNATURES = {
     "tqf_hip_router_logits_device": (_i32, [_vp, _vp, _vp, _i32, _u32, _u32, _u32, _vp]),
     "tqf_hip_route_tokens_device": (
         _i32, [_vp, _vp, _i32, _u32, _u32, _vp, C.POINTER(RouteOptions), _vp, _vp, _vp]),
+    "tqf_hip_rope_prepare": (_i32, [_vp, _vp, _u32, _pp]),
+    "tqf_hip_rope_free": (_i32, [_vp, _vp]),
+    "tqf_hip_qk_rope_device": (
+        _i32, [_vp, C.POINTER(Heads), C.POINTER(QkOptions), _hr, _hr, _hr, _i32, _u32, _vp, _vp, _vp, _vp,
+               C.POINTER(KvCache), _vp, _vp]),
+    "tqf_hip_attn_prompt_device": (
+        _i32, [_vp, C.POINTER(Heads), _f32, _hr, _hr, _hr, _hr, _vp, _vp, _u32, _u32, _u32, _vp, _vp]),
+    "tqf_hip_attn_paged_device": (
+        _i32, [_vp, C.POINTER(Heads), _f32, _hr, _hr, _u32, _u32, C.POINTER(KvCache), _vp, _u32, _vp, _vp, _vp]),
+    "tqf_hip_add_rows_device": (_i32, [_vp, _vp, _vp, _sz, _vp]),
     "tqf_hip_embed_rows_device": (_i32, [_vp, _vp, _vp, _u32, _vp, _vp, _vp]),
     "tqf_hip_rmsnorm_rows_device": (_i32, [_vp, _vp, _u32, _u32, _vp, _vp]),
     "tqf_hip_verify_step_device": (

@@ -34,6 +34,8 @@ def _ptr(a: np.ndarray) -> int:
 
 
 _TYPES = {"f32": _lib.TYPE_F32, "bf16": _lib.TYPE_BF16}
+_CACHE_TYPES = {"bf16": _lib.TYPE_BF16, "f8": _lib.TYPE_F8}
+_PAIRS = {"half": 0, "neighbours": 1}
 _TYPE_BYTES = {_lib.TYPE_F32: 4, _lib.TYPE_BF16: 2}
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
@@ -110,6 +112,33 @@ class F32Tensor:
 class DeviceBuffer:
     ptr: int
     nbytes: int
+
+
+@dataclass
+class Rope:
+    """The frequencies of a rotation on the device."""
+    handle: int
+    pairs: int
+
+
+@dataclass
+class KvCache:
+    """A layer's paged cache: keys and values [n_pages, kv_heads, page_size, head_dim], "bf16" or "f8" (e4m3, with
+    scales [n_pages, kv_heads, page_size])."""
+    d_k: DeviceBuffer
+    d_v: DeviceBuffer
+    n_pages: int
+    kv_heads: int
+    page_size: int
+    head_dim: int
+    type: str = "bf16"
+    d_k_scales: DeviceBuffer | None = None
+    d_v_scales: DeviceBuffer | None = None
+
+    def as_struct(self) -> _lib.KvCache:
+        p = lambda b: b.ptr if b else None  # noqa: E731
+        return _lib.KvCache(p(self.d_k), p(self.d_v), p(self.d_k_scales), p(self.d_v_scales), _CACHE_TYPES[self.type],
+                            self.n_pages, self.page_size, self.kv_heads, self.head_dim)
 
 
 class MoeLayer:
@@ -641,6 +670,120 @@ class HipBackend:
         if st:
             raise HipError(st, "route_tokens: a row's routing fails (NaN or +inf)")
         return ids, w
+
+    # ---- attention -----------------------------------------------------------------
+    # heads: (q_heads, kv_heads, head_dim).  strides: (row, head) in elements, where rows do not stand packed.
+    def prepare_rope(self, frequencies) -> Rope:
+        """A rotation's frequencies, radians a position, one a pair of elements."""
+        f = np.ascontiguousarray(frequencies, dtype=np.float64)
+        if f.ndim != 1:
+            raise ValueError("prepare_rope: one frequency for each pair")
+        h = C.c_void_p()
+        self._check(self.lib.tqf_hip_rope_prepare(self.ctx, _ptr(f), f.size, C.byref(h)))
+        return Rope(h.value, f.size)
+
+    def free_rope(self, rope: Rope) -> None:
+        self._check(self.lib.tqf_hip_rope_free(self.ctx, rope.handle))
+
+    def kv_cache(self, d_k: DeviceBuffer, d_v: DeviceBuffer, n_pages: int, kv_heads: int, page_size: int, head_dim: int,
+                 type: str = "bf16", d_k_scales: DeviceBuffer | None = None,
+                 d_v_scales: DeviceBuffer | None = None) -> KvCache:
+        """A cache in buffers of the caller."""
+        if type not in _CACHE_TYPES:
+            raise ValueError('cache types are "bf16" and "f8"')
+        n = n_pages * kv_heads * page_size
+        size = 1 if type == "f8" else 2
+        if type == "f8" and not (d_k_scales and d_v_scales):
+            raise ValueError("kv_cache: an f8 cache needs scales")
+        _hold("kv_cache", (d_k, n * head_dim * size), (d_v, n * head_dim * size),
+              *([(d_k_scales, 4 * n), (d_v_scales, 4 * n)] if type == "f8" else []))
+        return KvCache(d_k, d_v, n_pages, kv_heads, page_size, head_dim, type, d_k_scales, d_v_scales)
+
+    def alloc_kv_cache(self, n_pages: int, kv_heads: int, page_size: int, head_dim: int, type: str = "bf16") -> KvCache:
+        """A cache in buffers of its own (free_kv_cache gives them back)."""
+        n = n_pages * kv_heads * page_size
+        size = 1 if type == "f8" else 2
+        sizes = [n * head_dim * size] * 2 + ([4 * n] * 2 if type == "f8" else [])
+        got = []
+        try:
+            for b in sizes:
+                got.append(self.alloc(b))
+        except HipError:
+            for b in got:
+                self.free(b)
+            raise
+        return self.kv_cache(got[0], got[1], n_pages, kv_heads, page_size, head_dim, type, *got[2:])
+
+    def free_kv_cache(self, c: KvCache) -> None:
+        for b in (c.d_k, c.d_v, c.d_k_scales, c.d_v_scales):
+            if b:
+                self.free(b)
+
+    @staticmethod
+    def _head_rows(what: str, buf: DeviceBuffer, t: int, heads: int, dim: int, strides, nbytes: int) -> _lib.HeadRows:
+        row, head = strides if strides is not None else (heads * dim, dim)
+        if row < 0 or head < 0:
+            raise ValueError(f"{what}: strides must not be negative")
+        if t > 0:
+            _hold(what, (buf, ((t - 1) * row + (heads - 1) * head + dim) * nbytes))
+        return _lib.HeadRows(buf.ptr, row, head)
+
+    def qk_rope_device(self, d_q: DeviceBuffer, d_k: DeviceBuffer, d_v: DeviceBuffer, t: int, heads, d_positions: DeviceBuffer | None,
+                       d_q_out: DeviceBuffer, d_k_out: DeviceBuffer | None = None, d_v_out: DeviceBuffer | None = None,
+                       x_type: str = "f32", strides=(None, None, None), q_norm: F32Tensor | None = None,
+                       k_norm: F32Tensor | None = None, eps: float = 1e-6, rope: Rope | None = None, pairs: str = "half",
+                       cache: KvCache | None = None, d_slots: DeviceBuffer | None = None,
+                       d_status: DeviceBuffer | None = None) -> None:
+        """Norms and rotation of q and k heads; bf16 rows out, k and v into the cache (tqf_hip_qk_rope_device)."""
+        if pairs not in _PAIRS:
+            raise ValueError('pairs are "half" or "neighbours"')
+        xt, (nq, nk, dim) = _row_type(x_type), heads
+        size, what = _TYPE_BYTES[xt], "qk_rope_device"
+        rows = [self._head_rows(what, b, t, n, dim, s, size) for b, n, s in zip((d_q, d_k, d_v), (nq, nk, nk), strides)]
+        _hold(what, (d_q_out, 2 * t * nq * dim), *[(b, 2 * t * nk * dim) for b in (d_k_out, d_v_out) if b],
+              *[(b, 4 * t) for b in (d_positions, d_slots) if b])
+        p = lambda b: b.ptr if b else None  # noqa: E731
+        o = _lib.QkOptions(q_norm.handle if q_norm else None, k_norm.handle if k_norm else None, float(eps),
+                           rope.handle if rope else None, _PAIRS[pairs])
+        self._check(self.lib.tqf_hip_qk_rope_device(
+            self.ctx, C.byref(_lib.Heads(*heads)), C.byref(o), *[C.byref(r) for r in rows], xt, t, p(d_positions), d_q_out.ptr,
+            p(d_k_out), p(d_v_out), C.byref(cache.as_struct()) if cache else None, p(d_slots), p(d_status)))
+
+    def attn_prompt_device(self, d_q: DeviceBuffer, d_k: DeviceBuffer, d_v: DeviceBuffer, heads, d_cu_q: DeviceBuffer,
+                           d_cu_k: DeviceBuffer, n_seqs: int, total_q: int, total_k: int, d_y: DeviceBuffer,
+                           scale: float | None = None, strides=(None, None, None), d_gate: DeviceBuffer | None = None,
+                           gate_strides=None, d_status: DeviceBuffer | None = None) -> None:
+        """Causal attention of packed sequences, bf16 (tqf_hip_attn_prompt_device); scale: head_dim^-1/2 unless given."""
+        nq, nk, dim = heads
+        what = "attn_prompt_device"
+        q, k, v = [self._head_rows(what, b, n, h, dim, s, 2)
+                   for b, n, h, s in zip((d_q, d_k, d_v), (total_q, total_k, total_k), (nq, nk, nk), strides)]
+        gate = self._head_rows(what, d_gate, total_q, nq, dim, gate_strides, 2) if d_gate else None
+        _hold(what, (d_y, 2 * total_q * nq * dim), (d_cu_q, 4 * (n_seqs + 1)), (d_cu_k, 4 * (n_seqs + 1)))
+        self._check(self.lib.tqf_hip_attn_prompt_device(
+            self.ctx, C.byref(_lib.Heads(*heads)), dim ** -0.5 if scale is None else float(scale), C.byref(q), C.byref(k),
+            C.byref(v), C.byref(gate) if gate else None, d_cu_q.ptr, d_cu_k.ptr, n_seqs, total_q, total_k, d_y.ptr,
+            d_status.ptr if d_status else None))
+
+    def attn_paged_device(self, d_q: DeviceBuffer, heads, n_seqs: int, rows: int, cache: KvCache, d_pages: DeviceBuffer,
+                          max_pages: int, d_lens: DeviceBuffer, d_y: DeviceBuffer, scale: float | None = None, q_strides=None,
+                          d_gate: DeviceBuffer | None = None, gate_strides=None,
+                          d_status: DeviceBuffer | None = None) -> None:
+        """Attention of the last `rows` tokens of every sequence over its cache (tqf_hip_attn_paged_device)."""
+        nq, _, dim = heads
+        t, what = n_seqs * rows, "attn_paged_device"
+        q = self._head_rows(what, d_q, t, nq, dim, q_strides, 2)
+        gate = self._head_rows(what, d_gate, t, nq, dim, gate_strides, 2) if d_gate else None
+        _hold(what, (d_y, 2 * t * nq * dim), (d_pages, 4 * n_seqs * max_pages), (d_lens, 4 * n_seqs))
+        self._check(self.lib.tqf_hip_attn_paged_device(
+            self.ctx, C.byref(_lib.Heads(*heads)), dim ** -0.5 if scale is None else float(scale), C.byref(q),
+            C.byref(gate) if gate else None, n_seqs, rows, C.byref(cache.as_struct()), d_pages.ptr, max_pages, d_lens.ptr, d_y.ptr,
+            d_status.ptr if d_status else None))
+
+    def add_rows_device(self, d_a: DeviceBuffer, d_b: DeviceBuffer, n: int, d_out: DeviceBuffer) -> None:
+        """d_out[i] = d_a[i] + d_b[i], n f32 values; d_out may be one of them."""
+        _hold("add_rows_device", (d_a, 4 * n), (d_b, 4 * n), (d_out, 4 * n))
+        self._check(self.lib.tqf_hip_add_rows_device(self.ctx, d_a.ptr, d_b.ptr, n, d_out.ptr))
 
     @contextlib.contextmanager
     def _buffers(self, *specs):

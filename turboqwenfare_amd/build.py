@@ -21,7 +21,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libtqf_hip.so"
 SOURCES = ["tqf_q4.hip", "tqf_q4k.hip", "tqf_q6k.hip", "tqf_stack.hip", "tqf_grouped.hip",
            "tqf_accept.hip", "tqf_sample.hip", "tqf_experts.hip", "tqf_synth.hip", "tqf_loop.hip",
-           "tqf_f8.hip", "tqf_router.hip", "tqf_api.hip"]
+           "tqf_f8.hip", "tqf_router.hip", "tqf_rope.hip", "tqf_prompt.hip", "tqf_paged.hip", "tqf_api.hip"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
@@ -31,11 +31,13 @@ HIPCC_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
 ]
-# Per-source additions.  The grouped GEMM and the e4m3 products keep MFMA
-# results in VGPRs (the per-block fp32 scaling reads every result; accumulators
-# in AGPRs would cost a v_accvgpr_read per value).
+# Per-source additions.  The grouped GEMM, the e4m3 products and the attention
+# keep MFMA results in VGPRs (the per-block fp32 scaling and the softmax read
+# every result; accumulators in AGPRs would cost a v_accvgpr_read per value).
 EXTRA_FLAGS = {"tqf_grouped.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-               "tqf_f8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+               "tqf_f8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "tqf_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "tqf_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def hipcc_path() -> str:

@@ -16,6 +16,7 @@
 #include "../../include/tqf_hip.h"
 #include "../../include/tqf_hip_synth.h"
 #include "tqf_batch.h"
+#include "tqf_attn.h"
 #include "tqf_internal.h"
 
 using namespace tqf;
@@ -2452,5 +2453,274 @@ extern "C" int32_t tqf_hip_route_tokens_device(tqf_hip_ctx *ctx, const void *d_l
     const hipError_t e = launch_route_tokens(ctx->stream, d_logits, logits_type, t, n_experts, d_bias, o, d_ids, d_w, d_status);
     if (e != hipSuccess) return hip_fail(ctx, "route kernel launch", e);
     p.end(TQF_HIP_KERNEL_ROUTER, (double)lb + 6.0 * n + (d_bias ? 4.0 * n_experts : 0.0), 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+// ===========================================================================
+// attention
+// ===========================================================================
+namespace {
+constexpr uint64_t kMaxStride = uint64_t(1) << 24;
+
+int32_t check_heads(tqf_hip_ctx *ctx, const tqf_hip_heads *h) {
+    if (!h) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (h->q_heads == 0 || h->q_heads > 256 || h->kv_heads == 0 || h->q_heads % h->kv_heads)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "q_heads must be in 1..256 and a multiple of kv_heads");
+    if (h->head_dim != 64 && h->head_dim != 128 && h->head_dim != 256)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "head_dim must be 64, 128 or 256");
+    return TQF_HIP_OK;
+}
+
+int32_t check_rows(tqf_hip_ctx *ctx, const tqf_hip_head_rows *r, uint64_t t, uint32_t heads, uint32_t dim) {
+    if (!r || !r->data) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (!aligned_to(r->data, 16) || r->row_stride % 8 || r->head_stride % 8)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "rows of heads must be aligned to 16 bytes and their strides be multiples of 8");
+    if (r->row_stride >= kMaxStride || r->head_stride >= kMaxStride)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "strides must be below 2^24");
+    if (t > 1 && r->row_stride < dim) return fail(ctx, TQF_HIP_ERR_INVALID, "row_stride must be at least head_dim");
+    (void)heads;
+    return TQF_HIP_OK;
+}
+// Bytes from the first element of the rows to behind the last.
+size_t span(const tqf_hip_head_rows &r, uint64_t t, uint32_t heads, uint32_t dim, size_t bytes) {
+    return t ? ((t - 1) * r.row_stride + (uint64_t)(heads - 1) * r.head_stride + dim) * bytes : 0;
+}
+
+int32_t check_cache(tqf_hip_ctx *ctx, const tqf_hip_kv_cache *c, const tqf_hip_heads &h) {
+    if (!c || !c->d_k || !c->d_v) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (c->type != TQF_HIP_TYPE_BF16 && c->type != TQF_HIP_TYPE_F8) return fail(ctx, TQF_HIP_ERR_INVALID, "a cache is bf16 or e4m3");
+    const bool f8 = c->type == TQF_HIP_TYPE_F8;
+    if (f8 && (!c->d_k_scales || !c->d_v_scales)) return fail(ctx, TQF_HIP_ERR_INVALID, "an e4m3 cache needs scales");
+    if (!aligned_to(c->d_k, 16) || !aligned_to(c->d_v, 16) || (f8 && (!aligned_to(c->d_k_scales, 16) || !aligned_to(c->d_v_scales, 16))))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "a cache must be aligned to 16 bytes");
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "page_size must be 16, 32, 64, 128 or 256");
+    if (c->n_pages == 0 || (uint64_t)c->n_pages * c->page_size >= (uint64_t(1) << 31))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "a cache needs pages, and fewer than 2^31 slots");
+    if (c->kv_heads != h.kv_heads || c->head_dim != h.head_dim)
+        return fail(ctx, TQF_HIP_ERR_INVALID, "the cache has other heads");
+    return TQF_HIP_OK;
+}
+size_t cache_bytes(const tqf_hip_kv_cache &c) {
+    return (size_t)c.n_pages * c.page_size * c.kv_heads * c.head_dim * (c.type == TQF_HIP_TYPE_F8 ? 1 : 2);
+}
+size_t cache_scale_bytes(const tqf_hip_kv_cache &c) {
+    return c.type == TQF_HIP_TYPE_F8 ? (size_t)c.n_pages * c.page_size * c.kv_heads * 4 : 0;
+}
+KvCache cache_of(const tqf_hip_kv_cache &c) {
+    const bool f8 = c.type == TQF_HIP_TYPE_F8;
+    return KvCache{c.d_k, c.d_v, f8 ? c.d_k_scales : nullptr, f8 ? c.d_v_scales : nullptr, f8, c.n_pages, c.page_size, c.kv_heads, c.head_dim};
+}
+HeadRows rows_of(const tqf_hip_head_rows *r) { return r ? HeadRows{r->data, r->row_stride, r->head_stride} : HeadRows{nullptr, 0, 0}; }
+
+struct Range {
+    const void *p;
+    size_t n;
+};
+bool any_overlap(const Range &out, std::initializer_list<Range> with) {
+    for (const Range &r : with)
+        if (out.p && r.p && out.n && r.n && overlap(out.p, out.n, r.p, r.n)) return true;
+    return false;
+}
+}  // namespace
+
+extern "C" int32_t tqf_hip_rope_prepare(tqf_hip_ctx *ctx, const double *frequencies, uint32_t pairs, tqf_hip_rope **out) {
+    TQF_ENTER(ctx);
+    if (!frequencies || !out) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    *out = nullptr;
+    if (pairs == 0 || pairs > 128 || pairs % 8) return fail(ctx, TQF_HIP_ERR_INVALID, "pairs must be a multiple of 8 in 8..128");
+    double turns[128];
+    for (uint32_t i = 0; i < pairs; ++i) {
+        if (!std::isfinite(frequencies[i])) return fail(ctx, TQF_HIP_ERR_INVALID, "frequencies must be finite");
+        turns[i] = frequencies[i] / 6.28318530717958647692528676655900577;
+    }
+    std::unique_ptr<tqf_hip_rope> r(new (std::nothrow) tqf_hip_rope());
+    if (!r) return fail(ctx, TQF_HIP_ERR_NOMEM, "out of host memory");
+    void *d = nullptr;
+    if (arena_alloc(ctx, pairs * sizeof(double), &d) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(ctx, TQF_HIP_ERR_NOMEM, "rotation allocation failed");
+    }
+    hipError_t e = hipMemcpyAsync(d, turns, pairs * sizeof(double), hipMemcpyHostToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        arena_free(ctx, d);
+        return hip_fail(ctx, "rotation upload", e);
+    }
+    r->d_turns = static_cast<double *>(d);
+    r->pairs = pairs;
+    *out = r.release();
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_rope_free(tqf_hip_ctx *ctx, tqf_hip_rope *rope) {
+    TQF_ENTER(ctx);
+    if (!rope) return TQF_HIP_OK;
+    TQF_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    arena_free(ctx, rope->d_turns);
+    delete rope;
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_qk_rope_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, const tqf_hip_qk_options *options,
+                                          const tqf_hip_head_rows *q, const tqf_hip_head_rows *k, const tqf_hip_head_rows *v,
+                                          int32_t x_type, uint32_t t, const int32_t *d_positions, uint16_t *d_q_out,
+                                          uint16_t *d_k_out, uint16_t *d_v_out, const tqf_hip_kv_cache *cache,
+                                          const int32_t *d_slots, int32_t *d_status) {
+    TQF_ENTER(ctx);
+    if (int32_t rc = check_heads(ctx, heads)) return rc;
+    if (!options || !d_q_out) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    const uint32_t D = heads->head_dim, nq = heads->q_heads, nk = heads->kv_heads;
+    if (!valid_type(x_type)) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown element type");
+    if (t == 0 || t > TQF_HIP_F8_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "t must be in 1..65536");
+    if (int32_t rc = check_rows(ctx, q, t, nq, D)) return rc;
+    if (int32_t rc = check_rows(ctx, k, t, nk, D)) return rc;
+    if (int32_t rc = check_rows(ctx, v, t, nk, D)) return rc;
+    if ((options->q_norm && (!options->q_norm->data || options->q_norm->count != D)) ||
+        (options->k_norm && (!options->k_norm->data || options->k_norm->count != D)))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "a norm's weights must be f32 [head_dim]");
+    if (!(options->eps >= 0.0f) || !std::isfinite(options->eps)) return fail(ctx, TQF_HIP_ERR_INVALID, "eps must be finite and not negative");
+    if (options->neighbours != 0 && options->neighbours != 1) return fail(ctx, TQF_HIP_ERR_INVALID, "neighbours must be 0 or 1");
+    if (options->rope && options->rope->pairs * 2 > D) return fail(ctx, TQF_HIP_ERR_INVALID, "the rotation has more pairs than a head");
+    if (options->rope && !d_positions) return fail(ctx, TQF_HIP_ERR_INVALID, "a rotation needs positions");
+    if ((cache != nullptr) != (d_slots != nullptr)) return fail(ctx, TQF_HIP_ERR_INVALID, "cache and slots go together");
+    if (cache)
+        if (int32_t rc = check_cache(ctx, cache, *heads)) return rc;
+    if (!aligned_to(d_q_out, 16) || !aligned_to(d_k_out, 16) || !aligned_to(d_v_out, 16) || !aligned_to(d_positions, 4) ||
+        !aligned_to(d_slots, 4) || !aligned_to(d_status, 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "outputs must be aligned to 16 bytes, integers to 4");
+    const size_t xb = type_bytes(x_type), no = (size_t)t * nk * D * 2;
+    const Range in[5] = {{q->data, span(*q, t, nq, D, xb)}, {k->data, span(*k, t, nk, D, xb)}, {v->data, span(*v, t, nk, D, xb)},
+                         {d_positions, d_positions ? (size_t)t * 4 : 0}, {d_slots, d_slots ? (size_t)t * 4 : 0}};
+    const Range out[7] = {{d_q_out, (size_t)t * nq * D * 2}, {d_k_out, d_k_out ? no : 0}, {d_v_out, d_v_out ? no : 0},
+                          {cache ? cache->d_k : nullptr, cache ? cache_bytes(*cache) : 0},
+                          {cache ? cache->d_v : nullptr, cache ? cache_bytes(*cache) : 0},
+                          {cache && cache->type == TQF_HIP_TYPE_F8 ? cache->d_k_scales : nullptr, cache ? cache_scale_bytes(*cache) : 0},
+                          {cache && cache->type == TQF_HIP_TYPE_F8 ? cache->d_v_scales : nullptr, cache ? cache_scale_bytes(*cache) : 0}};
+    for (int i = 0; i < 7; ++i) {
+        if (any_overlap(out[i], {in[0], in[1], in[2], in[3], in[4]}))
+            return fail(ctx, TQF_HIP_ERR_INVALID, "outputs must not overlap inputs");
+        for (int j = 0; j < i; ++j)
+            if (any_overlap(out[i], {out[j]})) return fail(ctx, TQF_HIP_ERR_INVALID, "outputs must not overlap");
+    }
+    RopeArgs a{};
+    a.q = rows_of(q), a.k = rows_of(k), a.v = rows_of(v);
+    a.t = t, a.q_heads = nq, a.kv_heads = nk, a.dim = D;
+    a.q_norm = options->q_norm ? options->q_norm->data : nullptr;
+    a.k_norm = options->k_norm ? options->k_norm->data : nullptr;
+    a.eps = options->eps;
+    a.turns = options->rope ? options->rope->d_turns : nullptr;
+    a.pairs = options->rope ? options->rope->pairs : 0;
+    a.neighbours = options->neighbours != 0;
+    a.positions = d_positions;
+    a.q_out = d_q_out, a.k_out = d_k_out, a.v_out = d_v_out;
+    if (cache) a.cache = cache_of(*cache);
+    a.slots = d_slots;
+    a.status = d_status;
+    Prof p(ctx);
+    const hipError_t e = launch_qk_rope(ctx->stream, a, x_type);
+    if (e != hipSuccess) return hip_fail(ctx, "rotation kernel launch", e);
+    p.end(TQF_HIP_KERNEL_QK_ROPE,
+          (double)t * D * ((double)(nq + 2 * nk) * xb + 2.0 * nq + (d_k_out ? 2.0 * nk : 0.0) + (d_v_out ? 2.0 * nk : 0.0) +
+                           (cache ? (cache->type == TQF_HIP_TYPE_F8 ? 2.0 : 4.0) * nk : 0.0)), 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale, const tqf_hip_head_rows *q,
+                                              const tqf_hip_head_rows *k, const tqf_hip_head_rows *v, const tqf_hip_head_rows *gate,
+                                              const int32_t *d_cu_q, const int32_t *d_cu_k, uint32_t n_seqs, uint32_t total_q,
+                                              uint32_t total_k, uint16_t *d_y, int32_t *d_status) {
+    TQF_ENTER(ctx);
+    if (int32_t rc = check_heads(ctx, heads)) return rc;
+    if (!d_cu_q || !d_cu_k || !d_y) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    const uint32_t D = heads->head_dim, nq = heads->q_heads, nk = heads->kv_heads;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, TQF_HIP_ERR_INVALID, "scale must be positive and finite");
+    if (total_q == 0 || total_q > TQF_HIP_ATTN_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "total_q must be in 1..2^20");
+    if (total_k >= (1u << 31)) return fail(ctx, TQF_HIP_ERR_INVALID, "total_k must be below 2^31");
+    if (n_seqs == 0 || n_seqs > TQF_HIP_ATTN_MAX_SEQS) return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs must be in 1..16384");
+    if (int32_t rc = check_rows(ctx, q, total_q, nq, D)) return rc;
+    if (total_k) {
+        if (int32_t rc = check_rows(ctx, k, total_k, nk, D)) return rc;
+        if (int32_t rc = check_rows(ctx, v, total_k, nk, D)) return rc;
+    }
+    if (gate)
+        if (int32_t rc = check_rows(ctx, gate, total_q, nq, D)) return rc;
+    if (!aligned_to(d_y, 16) || !aligned_to(d_cu_q, 4) || !aligned_to(d_cu_k, 4) || !aligned_to(d_status, 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "y must be aligned to 16 bytes, integers to 4");
+    const Range y{d_y, (size_t)total_q * nq * D * 2};
+    const Range none{nullptr, 0};
+    if (any_overlap(y, {Range{q->data, span(*q, total_q, nq, D, 2)}, total_k ? Range{k->data, span(*k, total_k, nk, D, 2)} : none,
+                        total_k ? Range{v->data, span(*v, total_k, nk, D, 2)} : none, gate ? Range{gate->data, span(*gate, total_q, nq, D, 2)} : none,
+                        Range{d_cu_q, ((size_t)n_seqs + 1) * 4}, Range{d_cu_k, ((size_t)n_seqs + 1) * 4}}))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "y must not overlap the inputs");
+    PromptArgs a{};
+    a.q = rows_of(q), a.gate = rows_of(gate);
+    if (total_k) a.k = rows_of(k), a.v = rows_of(v);
+    a.cu_q = d_cu_q, a.cu_k = d_cu_k;
+    a.n_seqs = n_seqs, a.total_q = total_q, a.total_k = total_k;
+    a.q_heads = nq, a.kv_heads = nk, a.dim = D;
+    a.scale = scale;
+    a.y = d_y;
+    a.status = d_status;
+    Prof p(ctx);
+    const hipError_t e = launch_attn_prompt(ctx->stream, a);
+    if (e != hipSuccess) return hip_fail(ctx, "prompt attention launch", e);
+    p.end(TQF_HIP_KERNEL_ATTN_PROMPT, 2.0 * D * ((double)total_q * nq * (gate ? 3 : 2) + 2.0 * total_k * nk), 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_attn_paged_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale, const tqf_hip_head_rows *q,
+                                             const tqf_hip_head_rows *gate, uint32_t n_seqs, uint32_t rows, const tqf_hip_kv_cache *cache,
+                                             const int32_t *d_pages, uint32_t max_pages, const int32_t *d_lens, uint16_t *d_y,
+                                             int32_t *d_status) {
+    TQF_ENTER(ctx);
+    if (int32_t rc = check_heads(ctx, heads)) return rc;
+    if (!d_pages || !d_lens || !d_y) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    const uint32_t D = heads->head_dim, nq = heads->q_heads;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, TQF_HIP_ERR_INVALID, "scale must be positive and finite");
+    if (n_seqs == 0 || n_seqs > TQF_HIP_ATTN_MAX_SEQS) return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs must be in 1..16384");
+    if (rows == 0 || rows > TQF_HIP_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "rows must be in 1..8");
+    if (int32_t rc = check_cache(ctx, cache, *heads)) return rc;
+    if (max_pages == 0 || (uint64_t)max_pages * cache->page_size >= (uint64_t(1) << 31))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "max_pages * page_size must be in 1..2^31 - 1");
+    const uint64_t t = (uint64_t)n_seqs * rows;
+    if (int32_t rc = check_rows(ctx, q, t, nq, D)) return rc;
+    if (gate)
+        if (int32_t rc = check_rows(ctx, gate, t, nq, D)) return rc;
+    if (!aligned_to(d_y, 16) || !aligned_to(d_pages, 4) || !aligned_to(d_lens, 4) || !aligned_to(d_status, 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "y must be aligned to 16 bytes, integers to 4");
+    const Range y{d_y, (size_t)t * nq * D * 2}, none{nullptr, 0};
+    if (any_overlap(y, {Range{q->data, span(*q, t, nq, D, 2)}, gate ? Range{gate->data, span(*gate, t, nq, D, 2)} : none,
+                        Range{cache->d_k, cache_bytes(*cache)}, Range{cache->d_v, cache_bytes(*cache)},
+                        Range{cache->type == TQF_HIP_TYPE_F8 ? cache->d_k_scales : nullptr, cache_scale_bytes(*cache)},
+                        Range{cache->type == TQF_HIP_TYPE_F8 ? cache->d_v_scales : nullptr, cache_scale_bytes(*cache)},
+                        Range{d_pages, (size_t)n_seqs * max_pages * 4}, Range{d_lens, (size_t)n_seqs * 4}}))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "y must not overlap the inputs");
+    PagedArgs a{};
+    a.q = rows_of(q), a.gate = rows_of(gate);
+    a.n_seqs = n_seqs, a.rows = rows, a.q_heads = nq;
+    a.scale = scale;
+    a.cache = cache_of(*cache);
+    a.pages = d_pages, a.max_pages = max_pages, a.lens = d_lens;
+    a.y = d_y;
+    a.status = d_status;
+    if (int32_t rc = ensure_f8_scratch(ctx, attn_paged_scratch_bytes(a))) return rc;
+    Prof p(ctx);
+    const hipError_t e = launch_attn_paged(ctx->stream, a, ctx->d_grouped);
+    if (e != hipSuccess) return hip_fail(ctx, "paged attention launch", e);
+    p.end(TQF_HIP_KERNEL_ATTN_PAGED, 0.0, 0, nullptr);
+    return TQF_HIP_OK;
+}
+
+extern "C" int32_t tqf_hip_add_rows_device(tqf_hip_ctx *ctx, const float *d_a, const float *d_b, size_t n, float *d_out) {
+    TQF_ENTER(ctx);
+    if (!d_a || !d_b || !d_out) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
+    if (n == 0 || n > (size_t(1) << 31)) return fail(ctx, TQF_HIP_ERR_INVALID, "n must be in 1..2^31");
+    if (!aligned_to(d_a, 4) || !aligned_to(d_b, 4) || !aligned_to(d_out, 4))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "buffers must be aligned to their elements");
+    if ((d_out != d_a && overlap(d_a, n * 4, d_out, n * 4)) || (d_out != d_b && overlap(d_b, n * 4, d_out, n * 4)))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "out may be one of the operands, but not overlap it in part");
+    const hipError_t e = launch_add_rows(ctx->stream, d_a, d_b, n, d_out);
+    if (e != hipSuccess) return hip_fail(ctx, "add kernel launch", e);
     return TQF_HIP_OK;
 }

@@ -1,0 +1,471 @@
+// tqf_paged.hip -- attention of a few rows of every sequence (a token, or the verify
+// rows of its drafts) over a paged cache in bf16 or e4m3 (gfx950).
+//
+//   y[i][h] = sum_j softmax_j(scale q[i][h] . k[j][h / group]) v[j][h / group]
+//             (* sigmoid(gate[i][h])),  j < len - rows + i + 1.
+//
+// Bound by the cache's bytes, each of which is needed once: the rows of a sequence
+// and the heads of a group stand side by side as the columns of the matrix
+// instructions, so a key is multiplied with all of them when it arrives.  The work
+// of all sequences, in steps of 128 keys of one (sequence, key head), is one line
+// that is cut into equal parts, a part to a workgroup, whatever the lengths; what a
+// workgroup has of a (sequence, key head) that it does not have whole goes to
+// memory (maximum, sum, sum of values) and a second kernel joins it, in the order of
+// the keys.  Wavefronts take 32 keys of a step each, by themselves, and join theirs
+// in LDS at the end.
+//
+// As in tqf_prompt.hip: S^T = K Q^T (here 16 x 16 x 32) leaves a row's weights as an
+// operand of O^T = V^T P^T; V^T comes from LDS by transposing reads; infinities and
+// NaN among values that only some rows see are counted apart.
+#include <hip/hip_runtime.h>
+
+#include "tqf_attn_device.h"
+
+namespace tqf {
+
+namespace {
+
+constexpr int kWaves = 4, kWaveKeys = 32, kStepKeys = kWaves * kWaveKeys;
+
+struct Kernel {
+    PagedArgs a;
+    uint32_t group, row_blocks, parts, page_shift;  // parts: workgroups of a row block
+    float scale_log2;
+    float *partial;  // [2 parts][row_blocks][rows of a block][dim + 2]: values, maximum, sum
+};
+
+// Steps of a sequence's one key head: at least one, which writes the rows of an empty sequence.
+__device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
+    const bool bad = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * a.cache.page;
+    const uint32_t n = bad ? 0 : ((uint32_t)len + kStepKeys - 1) / kStepKeys;
+    return n ? n : 1;
+}
+
+// The line of all steps: sequence by sequence, key head by key head.
+struct Line {
+    uint64_t total;
+    // of the step asked for
+    uint32_t seq, steps;
+    uint64_t first;  // of the sequence
+};
+__device__ __forceinline__ uint64_t line_total(const PagedArgs &a) {
+    const uint32_t l = threadIdx.x & 63;
+    uint64_t sum = 0;
+    for (uint32_t s = l; s < a.n_seqs; s += 64) sum += steps_of(a, a.lens[s]);
+#pragma unroll
+    for (int o = 32; o >= 1; o /= 2) sum += __shfl_xor(sum, o);
+    return sum * a.cache.kv_heads;
+}
+__device__ __forceinline__ void line_find(const PagedArgs &a, uint64_t step, Line &p) {
+    const uint32_t l = threadIdx.x & 63;
+    uint64_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        const uint32_t s = s0 + l, mine = s < a.n_seqs ? steps_of(a, a.lens[s]) : 0;
+        uint64_t upto = (uint64_t)mine * a.cache.kv_heads;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const uint64_t v = __shfl_up(upto, o);
+            if ((int)l >= o) upto += v;
+        }
+        const uint64_t past = __ballot(before + upto > step);
+        if (past) {
+            const int who = __builtin_ctzll(past);
+            p.seq = s0 + who;
+            p.steps = __shfl(mine, who);
+            p.first = before + __shfl(upto, who) - (uint64_t)p.steps * a.cache.kv_heads;
+            return;
+        }
+        before += __shfl(upto, 63);
+    }
+    p.seq = a.n_seqs;  // no such step
+}
+__device__ __forceinline__ uint64_t part_begin(uint64_t total, uint32_t part, uint32_t parts) { return total * part / parts; }
+
+__device__ __forceinline__ float gate_of(uint16_t b) { return sigmoid(__uint_as_float((uint32_t)b << 16)); }
+
+// NR: tiles of 16 rows that a workgroup has.
+template <int D, int NR, bool F8>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
+    constexpr int kRow = 2 * D, kDims = D / 16, kSteps = D / 32, kRows = 16 * NR, kChunks = D / 8;
+    constexpr int kKLoads = F8 ? D / 64 : D / 32;  // 16-byte loads of a lane for 16 keys
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[kWaves][kWaveKeys * kRow];
+    __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
+    const PagedArgs &a = p.a;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 16, g = l / 16;
+    const uint32_t part = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
+    const uint64_t total = line_total(a);
+    uint64_t at = part_begin(total, part, p.parts);
+    const uint64_t begin = at, end = part_begin(total, part + 1, p.parts);
+    const uint32_t all_rows = a.rows * p.group;
+    const size_t page_size = a.cache.page;
+    // V^T: dimension 16 d + l % 16, the keys that the lane's weights have (4 g and 16 + 4 g on)
+    constexpr int kVAt = kDims < 8 ? kDims : 8;
+    uint32_t v_at[kVAt];
+    {
+        const int key = 4 * g + r / 4, turn = D == 64 ? (key >> 1 & 3) << 1 : (key & 7) << 1;
+#pragma unroll
+        for (int d = 0; d < kVAt; ++d) v_at[d] = key * kRow + ((d * 2 + r % 4 / 2) ^ turn) * 16 + r % 2 * 8;
+    }
+
+    while (at < end) {
+        Line line;
+        line_find(a, at, line);
+        if (line.seq >= a.n_seqs) return;
+        const uint32_t seq = __builtin_amdgcn_readfirstlane(line.seq), steps = __builtin_amdgcn_readfirstlane(line.steps);
+        const uint64_t in_seq = at - line.first;
+        const uint32_t kv = __builtin_amdgcn_readfirstlane((uint32_t)(in_seq / steps)), from = __builtin_amdgcn_readfirstlane((uint32_t)(in_seq % steps));
+        const uint32_t upto = __builtin_amdgcn_readfirstlane((uint32_t)(steps - from < end - at ? steps : from + (end - at)));
+        int32_t len = a.lens[seq];
+        bool poison = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * page_size;
+        if (poison) {
+            if (a.status) *a.status = TQF_HIP_ERR_INVALID;
+            len = 0;
+        }
+
+        // the rows: column r of tile n is row block * kRows + 16 n + r, of query row / group and head row % group
+        bf16x8 q[NR][kSteps];
+        int limit[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            uint32_t row = block * kRows + n * 16 + r;
+            if (row >= all_rows) row = all_rows - 1;
+            const uint32_t i = row / p.group, head = kv * p.group + row % p.group;
+            limit[n] = len - (int)a.rows + (int)i;
+            const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + ((size_t)seq * a.rows + i) * a.q.row + (size_t)head * a.q.head;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+                q[n][s] = *reinterpret_cast<const bf16x8 *>(qp + (F8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8));
+        }
+        const int limit_min = len - (int)a.rows;
+        f32x4 o[kDims][NR];
+        float m[NR], sum[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            m[n] = -kInf;
+            sum[n] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) o[d][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        for (uint32_t step = from; step < upto; ++step) {
+            const int k0 = (int)(step * kStepKeys) + wave * kWaveKeys;
+            if (k0 >= len) break;
+            size_t row0[2];  // of the 16 keys in the cache
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int key = k0 + 16 * j < len ? k0 + 16 * j : k0;
+                int32_t page = a.pages[(size_t)seq * a.max_pages + ((uint32_t)key >> p.page_shift)];
+                if (page < 0 || (uint32_t)page >= a.cache.n_pages) {
+                    poison = true;
+                    page = 0;
+                }
+                row0[j] = ((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1));
+            }
+            u32x4 kx[2][kKLoads], vx[2][kKLoads];
+            f32x4 ks[2], vs[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint8_t *kb = static_cast<const uint8_t *>(a.cache.k) + row0[j] * (F8 ? D : kRow);
+                const uint8_t *vb = static_cast<const uint8_t *>(a.cache.v) + row0[j] * (F8 ? D : kRow);
+#pragma unroll
+                for (int i = 0; i < kKLoads; ++i) {
+                    kx[j][i] = *reinterpret_cast<const u32x4 *>(kb + r * (F8 ? D : kRow) + i * 64 + g * 16);
+                    vx[j][i] = *reinterpret_cast<const u32x4 *>(vb + i * 1024 + l * 16);
+                }
+                if constexpr (F8) {
+                    ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + row0[j] + 4 * g);
+                    vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + row0[j] + 4 * g);
+                }
+            }
+            // values to LDS, as bf16, [key][chunk c of 8 at c ^ its place]; those behind the end are zero
+            uint8_t *vl = s_v[wave];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < kKLoads; ++i) {
+                    const int byte = i * 1024 + l * 16, key = 16 * j + byte / (F8 ? D : kRow), c = byte % (F8 ? D : kRow) / 16;
+                    const int turn = D == 64 ? (key >> 1 & 3) << 1 : (key & 7) << 1;
+                    const bool in = k0 + key < len;
+                    if constexpr (F8) {
+                        const u32x4 x = in ? vx[j][i] : u32x4{0, 0, 0, 0};
+                        *reinterpret_cast<bf16x8 *>(vl + key * kRow + ((2 * c) ^ turn) * 16) = f8_widen(x[0], x[1]);
+                        *reinterpret_cast<bf16x8 *>(vl + key * kRow + ((2 * c + 1) ^ turn) * 16) = f8_widen(x[2], x[3]);
+                    } else {
+                        *reinterpret_cast<u32x4 *>(vl + key * kRow + (c ^ turn) * 16) = in ? vx[j][i] : u32x4{0, 0, 0, 0};
+                    }
+                }
+            const bool partly = k0 + kWaveKeys - 1 > limit_min;  // some row does not see all keys
+            bool odd = false;  // infinities or NaN among values that some rows do not see
+            if (partly && a.rows > 1) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < kKLoads; ++i) {
+                        if (k0 + 16 * j + (i * 1024 + l * 16) / (F8 ? D : kRow) >= len) continue;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t x = vx[j][i][e];
+                            // e4m3: all but the sign set; bf16: the exponent's carry
+                            if constexpr (F8) any |= ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                            else any |= ((x & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
+                        }
+                    }
+                odd = __any(any != 0);
+            }
+            bf16x8 w[NR];
+            bool grown = false;
+            float keep[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                f32x4 s[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        bf16x8 kk;
+                        if constexpr (F8) kk = f8_widen(kx[j][i / 2][i % 2 * 2], kx[j][i / 2][i % 2 * 2 + 1]);
+                        else kk = __builtin_bit_cast(bf16x8, kx[j][i]);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[n][i], acc, 0, 0, 0);
+                    }
+                    if constexpr (F8) acc *= ks[j];
+                    s[j] = acc * p.scale_log2;
+                    if (partly) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (k0 + 16 * j + 4 * g + i > limit[n]) s[j][i] = -kInf;
+                    }
+                }
+                float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = fmaxf(m[n], top), m_use = m_new == -kInf ? 0.0f : m_new;
+                grown |= m_new != m[n];
+                keep[n] = __builtin_amdgcn_exp2f(m[n] - m_use);
+                m[n] = m_new;
+                float add = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(s[e / 4][e % 4] - m_use);
+                    add += x;
+                    if constexpr (F8) w[n][e] = (__bf16)(partly && k0 + 16 * (e / 4) + 4 * g + e % 4 > limit[n] ? 0.0f : x * vs[e / 4][e % 4]);
+                    else w[n][e] = (__bf16)x;
+                }
+                sum[n] = sum[n] * keep[n] + add;
+            }
+            if (__any(grown)) {
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d) o[d][n] *= keep[n];
+            }
+            auto values = [&](int d) {
+                const uint8_t *at_v = vl + v_at[d % kVAt] + d / kVAt * 256;
+                const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 16 * kRow);
+                return u32x4{x.x, x.y, y.x, y.y};
+            };
+            if (!odd) {
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) {
+                    const bf16x8 v = __builtin_bit_cast(bf16x8, values(d));
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[n], o[d][n], 0, 0, 0);
+                }
+            } else {
+#pragma unroll 1
+                for (int what = kFinite; what <= kNan; ++what) {
+                    const float add_odd = odd_value(what);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        bf16x8 y = w[n];
+                        if (what != kFinite) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = (__bf16)(k0 + 16 * (e / 4) + 4 * g + e % 4 <= limit[n] ? 1.0f : 0.0f);
+                        }
+#pragma unroll
+                        for (int d = 0; d < kDims; ++d) {
+                            const f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pick(values(d), what), y, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[d][n][i] += what == kFinite ? acc[i] : acc[i] > 0.0f ? add_odd : 0.0f;
+                        }
+                    }
+                }
+            }
+        }
+
+        // join the wavefronts
+        if (__any(poison)) {
+            if (a.status && l == 0) *a.status = TQF_HIP_ERR_INVALID;
+            poison = true;
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            sum[n] += __shfl_xor(sum[n], 16);
+            sum[n] += __shfl_xor(sum[n], 32);
+            if (poison) sum[n] = __builtin_nanf("");
+            if (g == 0) {
+                s_m[wave][n * 16 + r] = m[n];
+                s_l[wave][n * 16 + r] = sum[n];
+            }
+        }
+        __syncthreads();
+        const bool whole = from == 0 && upto == steps;
+        float *to = p.partial + ((size_t)(2 * part + (at == begin ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const int row = n * 16 + r;
+            float top = s_m[0][row], mine = 0.0f;
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][row]);
+            mine = m[n] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+            // [row][chunk of 4 at chunk ^ row] f32
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                const int c = d * 4 + g;
+                *reinterpret_cast<f32x4 *>(s_v[wave] + r * D * 4 + (c ^ r) * 16) = o[d][n] * mine;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = tid; i < 16 * kChunks * 2; i += 64 * kWaves) {
+                const int rr = i / (2 * kChunks), c = i % (2 * kChunks), of_block = n * 16 + rr;
+                f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                float all = s_m[0][of_block], total_l = 0.0f;
+#pragma unroll
+                for (int x = 1; x < kWaves; ++x) all = fmaxf(all, s_m[x][of_block]);
+#pragma unroll
+                for (int x = 0; x < kWaves; ++x) {
+                    v += *reinterpret_cast<const f32x4 *>(s_v[x] + rr * D * 4 + (c ^ rr) * 16);
+                    // a wavefront without keys has sum 0, or NaN where its sequence or a page is bad
+                    total_l += s_m[x][of_block] == -kInf ? s_l[x][of_block] : s_l[x][of_block] * __builtin_amdgcn_exp2f(s_m[x][of_block] - all);
+                }
+                const uint32_t out_row = block * kRows + of_block;
+                if (whole) {
+                    if (out_row < all_rows) {
+                        const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
+                        const size_t token = (size_t)seq * a.rows + out_row / p.group, head = kv * p.group + out_row % p.group;
+                        v *= inv;
+                        if (a.gate.d) {
+                            const uint16_t *gp = static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head + c * 4;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] *= gate_of(gp[e]);
+                        }
+                        store4(a.y + (token * a.q_heads + head) * D + c * 4, 4, v);
+                    }
+                } else {
+                    float *row_to = to + (size_t)of_block * (D + 2);
+                    __builtin_memcpy(row_to + c * 4, &v, 16);
+                    if (c == 0) {
+                        row_to[D] = all;
+                        row_to[D + 1] = total_l;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        at += upto - from;
+    }
+}
+
+// Joins what several workgroups have of one (sequence, key head).  A workgroup takes
+// a row of the unit that the boundary at the beginning of its part cuts first; its
+// wavefronts take the parts in turn.
+constexpr int kJoinWaves = 8;
+template <int D, int NR>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p) {
+    constexpr int kRows = 16 * NR;
+    __shared__ float s_o[kJoinWaves][D], s_m[kJoinWaves], s_l[kJoinWaves];
+    const PagedArgs &a = p.a;
+    const int tid = threadIdx.x, wave = tid / 64, l = tid % 64;
+    const uint32_t all_rows = a.rows * p.group, part = blockIdx.x / all_rows + 1, row = blockIdx.x % all_rows;
+    const uint64_t total = line_total(a), cut = part_begin(total, part, p.parts);
+    if (cut == 0 || cut >= total) return;
+    Line line;
+    line_find(a, cut, line);
+    if (line.seq >= a.n_seqs) return;
+    const uint64_t in_seq = cut - line.first, kv = in_seq / line.steps, begin = line.first + kv * line.steps, end = begin + line.steps;
+    if (cut == begin || part_begin(total, part - 1, p.parts) > begin) return;  // no unit is cut here, or not here first
+    const uint32_t block = row / kRows, of_block = row % kRows;
+    // part - 1 (from `begin` on, or before it) to the last part that begins before `end`
+    float m = -kInf, sum = 0.0f, o[D / 64] = {};
+    for (uint32_t i = part - 1 + wave; i < p.parts; i += kJoinWaves) {
+        const uint64_t b = part_begin(total, i, p.parts);
+        if (b >= end) break;
+        if (part_begin(total, i + 1, p.parts) == b) continue;  // an empty part
+        const float *from = p.partial + ((size_t)(2 * i + (b >= begin ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2) + (size_t)of_block * (D + 2);
+        const float pm = from[D], pl = from[D + 1], top = fmaxf(m, pm);
+        const float keep = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top), take = pm == -kInf ? 0.0f : __builtin_amdgcn_exp2f(pm - top);
+        m = top;
+        sum = sum * (sum != sum ? 1.0f : keep) + (pl != pl ? pl : pl * take);
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) o[d] = o[d] * keep + from[d * 64 + l] * take;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) s_o[wave][d * 64 + l] = o[d];
+    if (l == 0) {
+        s_m[wave] = m;
+        s_l[wave] = sum;
+    }
+    __syncthreads();
+    float top = -kInf, all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoinWaves; ++i) top = fmaxf(top, s_m[i]);
+    for (int d = tid; d < D; d += 64 * kJoinWaves) {
+        float v = 0.0f;
+        all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kJoinWaves; ++i) {
+            const float f = s_m[i] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top);
+            all += s_l[i] != s_l[i] ? s_l[i] : s_l[i] * f;
+            v += s_o[i][d] * f;
+        }
+        v *= all == 0.0f ? 0.0f : 1.0f / all;
+        const size_t token = (size_t)line.seq * a.rows + row / p.group, head = kv * p.group + row % p.group;
+        if (a.gate.d) v *= gate_of(static_cast<const uint16_t *>(a.gate.d)[token * a.gate.row + head * a.gate.head + d]);
+        a.y[(token * a.q_heads + head) * D + d] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    }
+}
+
+uint32_t tiles_of_rows(const PagedArgs &a) { return a.rows * (a.q_heads / a.cache.kv_heads) > 16 ? 2 : 1; }
+uint32_t row_blocks(const PagedArgs &a) {
+    const uint32_t rows = a.rows * (a.q_heads / a.cache.kv_heads), per = 16 * tiles_of_rows(a);
+    return (rows + per - 1) / per;
+}
+// Two workgroups of a compute unit; no more than there can be steps.
+uint32_t parts_of(const PagedArgs &a) {
+    int device = 0, cus = 0;
+    (void)hipGetDevice(&device);
+    (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+    const uint64_t most = (uint64_t)a.n_seqs * a.cache.kv_heads * (((uint64_t)a.max_pages * a.cache.page + kStepKeys - 1) / kStepKeys);
+    const uint64_t want = 2 * (uint64_t)(cus > 0 ? cus : 256) / (row_blocks(a) < 2 ? 1 : 2);
+    return (uint32_t)(most < want ? most : want);
+}
+
+template <int D, int NR>
+hipError_t launch_for(hipStream_t s, const Kernel &p) {
+    const dim3 grid(p.parts * p.row_blocks), block(64 * kWaves);
+    if (p.a.cache.f8) paged_kernel<D, NR, true><<<grid, block, 0, s>>>(p);
+    else paged_kernel<D, NR, false><<<grid, block, 0, s>>>(p);
+    if (p.parts > 1) {
+        if (const hipError_t e = hipGetLastError()) return e;
+        join_kernel<D, NR><<<dim3((p.parts - 1) * p.a.rows * p.group), dim3(64 * kJoinWaves), 0, s>>>(p);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t attn_paged_scratch_bytes(const PagedArgs &a) {
+    return (size_t)2 * parts_of(a) * row_blocks(a) * 16 * tiles_of_rows(a) * (a.cache.dim + 2) * 4;
+}
+
+hipError_t launch_attn_paged(hipStream_t s, const PagedArgs &a, void *scratch) {
+    Kernel p{a, a.q_heads / a.cache.kv_heads, row_blocks(a), parts_of(a), (uint32_t)__builtin_ctz(a.cache.page), a.scale * kLog2e,
+             static_cast<float *>(scratch)};
+    const bool two = tiles_of_rows(a) == 2;
+    if (a.cache.dim == 64) return two ? launch_for<64, 2>(s, p) : launch_for<64, 1>(s, p);
+    if (a.cache.dim == 128) return two ? launch_for<128, 2>(s, p) : launch_for<128, 1>(s, p);
+    return two ? launch_for<256, 2>(s, p) : launch_for<256, 1>(s, p);
+}
+
+}  // namespace tqf

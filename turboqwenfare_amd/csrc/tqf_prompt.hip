@@ -1,0 +1,307 @@
+// tqf_prompt.hip -- causal attention of packed prompts with grouped heads (gfx950).
+//
+//   y[i][h] = sum_j softmax_j(scale q[i][h] . k[j][h / group]) v[j][h / group]
+//             (* sigmoid(gate[i][h])),  j <= i + len_k - len_q of i's sequence.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax: a
+// tile's weights are exp(s - m), and what is summed so far is multiplied by
+// exp(m_old - m) when m grows.
+//
+// A wavefront has 32 rows of one head.  It computes S^T = K Q^T with the
+// 32 x 32 x 16 bf16 instructions: in their result a lane has one row and 16 keys,
+// so a row's maximum and sum stay in two lanes, and the weights, rounded to bf16
+// (2^-9 of each, where bf16 y rounds by as much), are an operand of O^T = V^T P^T
+// as they stand: the order in which an instruction takes its K elements is free so
+// long as both operands have the same.  V^T comes from LDS by transposing reads.
+// A workgroup's wavefronts share tiles of K and V, and so, where heads are
+// grouped, are heads of one group at the same rows.
+//
+// Keys that a row does not see have weight 0, but 0 * inf and 0 * NaN are NaN.
+// Rows behind a sequence's end read as zeros (the copies' bounds).  Tiles that some
+// rows see in part are looked through for infinities and NaN; where there are any,
+// each row's are counted by matrix products of their own.
+#include <hip/hip_runtime.h>
+
+#include "tqf_attn_device.h"
+
+namespace tqf {
+
+namespace {
+
+typedef __amdgpu_buffer_rsrc_t Desc;  // loads past its bytes give zero
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ void copy16(Desc d, uint32_t voff, void *lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, 0, 0, 0);
+}
+constexpr int kWaves = 4;
+
+struct Kernel {
+    PromptArgs a;
+    uint32_t head_waves;  // wavefronts of a workgroup that have heads of their own (of one group)
+    uint32_t head_sets;   // q_heads / head_waves
+    float scale_log2;
+};
+
+// The sequence and the tile in it of a workgroup's tile number; false: none.
+struct Place {
+    int32_t q0, lq, k0, lk;
+    uint32_t tile;
+};
+__device__ __forceinline__ bool find_place(const PromptArgs &a, uint32_t number, uint32_t tokens, Place &p) {
+    const uint32_t l = threadIdx.x & 63;
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        const uint32_t s = s0 + l;
+        int32_t q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+        if (s < a.n_seqs) {
+            q0 = a.cu_q[s], q1 = a.cu_q[s + 1], k0 = a.cu_k[s], k1 = a.cu_k[s + 1];
+            const bool bad = q0 < 0 || q1 < q0 || (uint32_t)q1 > a.total_q || k0 < 0 || k1 < k0 || (uint32_t)k1 > a.total_k;
+            if (bad) {
+                if (a.status) *a.status = TQF_HIP_ERR_INVALID;
+                q0 = q1 = k0 = k1 = 0;
+            }
+        }
+        const uint32_t mine = ((uint32_t)(q1 - q0) + tokens - 1) / tokens;
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const uint32_t v = __shfl_up(upto, o);
+            if ((int)l >= o) upto += v;
+        }
+        const uint64_t past = __ballot(before + upto > number);
+        if (past) {
+            const int who = __builtin_ctzll(past);
+            p.q0 = __shfl(q0, who);
+            p.lq = __shfl(q1 - q0, who);
+            p.k0 = __shfl(k0, who);
+            p.lk = __shfl(k1 - k0, who);
+            const uint32_t n = __shfl(mine, who), first = before + __shfl(upto, who) - n;
+            p.tile = n - 1 - (number - first);  // the longest first
+            return true;
+        }
+        before += __shfl(upto, 63);
+    }
+    return false;
+}
+
+// A tile of K or V in LDS: rows of 2 D bytes, the 16-byte chunk c of row r in slot
+// c ^ swizzle(r).  K: 16 lanes that read a chunk of 16 rows find 16 different
+// places in the banks.  V: the four rows that 16 lanes read transposed.
+template <int D>
+__device__ __forceinline__ uint32_t k_swizzle(uint32_t row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+template <int D>
+__device__ __forceinline__ uint32_t v_swizzle(uint32_t row) { return D == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
+
+// D: head dimension, KT: keys of a tile (a multiple of 32).
+template <int D, int KT>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
+    constexpr int kRow = 2 * D, kTile = KT * kRow, kCopies = kTile / 1024 / kWaves, kSub = KT / 32, kDims = D / 32, kSteps = D / 16;
+    static_assert(kCopies >= 1, "every wavefront copies");
+    __shared__ __attribute__((aligned(1024))) uint8_t s_k[kTile], s_v[kTile];
+    const PromptArgs &a = p.a;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 32, half = l / 32;
+    const uint32_t tokens = 32u * kWaves / p.head_waves;  // of the workgroup
+    Place at;
+    if (!find_place(a, blockIdx.x / p.head_sets, tokens, at)) return;
+    const uint32_t head = blockIdx.x % p.head_sets * p.head_waves + (uint32_t)wave % p.head_waves;
+    const uint32_t kv = head / (a.q_heads / a.kv_heads);
+    const int q0 = __builtin_amdgcn_readfirstlane(at.q0), lq = __builtin_amdgcn_readfirstlane(at.lq);
+    const int k0 = __builtin_amdgcn_readfirstlane(at.k0), lk = __builtin_amdgcn_readfirstlane(at.lk);
+    const int first = (int)(__builtin_amdgcn_readfirstlane(at.tile) * tokens), mine = first + 32 * (wave / (int)p.head_waves);
+    const int shift = lk - lq;
+    const int row = mine + r < lq ? mine + r : lq - 1;  // rows past the end do as the last one and are not stored
+    const int limit = row + shift;                       // the last key that the lane's row sees
+    const int limit_min = (mine < lq ? mine : lq - 1) + shift;
+    const int limit_max = (mine + 31 < lq ? mine + 31 : lq - 1) + shift;
+    const int last = (first + (int)tokens < lq ? first + (int)tokens : lq) - 1 + shift;  // of the workgroup
+    const bool live = mine < lq;
+
+    bf16x8 q[kSteps];
+    const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + (size_t)(q0 + row) * a.q.row + (size_t)head * a.q.head + half * 8;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) q[i] = *reinterpret_cast<const bf16x8 *>(qp + i * 16);
+    f32x16 o[kDims];
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    float m = -kInf, sum = 0.0f;
+
+    const uint8_t *kp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.k.d) + (size_t)k0 * a.k.row + (size_t)kv * a.k.head);
+    const uint8_t *vp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.v.d) + (size_t)k0 * a.v.row + (size_t)kv * a.v.head);
+    const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2;
+
+    // Where the lane's operands are in a tile: chunk 2 i + half of key r (+ 32), and, transposed, dimensions
+    // 32 d + l % 32 of the keys that its half's weights have.  The swizzles depend on the lane alone, so that
+    // few addresses serve all and the rest is constant.
+    constexpr int kKAt = kSteps < 8 ? kSteps : 8, kVAt = kDims < 4 ? kDims : 4;
+    uint32_t k_at[kKAt], v_at[kVAt];
+#pragma unroll
+    for (int i = 0; i < kKAt; ++i) k_at[i] = r * kRow + ((i * 2 + half) ^ k_swizzle<D>(r)) * 16;
+    {
+        const int g = l / 16, i16 = l % 16;
+        const uint32_t r0 = 4 * half + i16 / 4;
+#pragma unroll
+        for (int d = 0; d < kVAt; ++d) v_at[d] = r0 * kRow + ((d * 4 + 2 * (g % 2) + i16 % 4 / 2) ^ v_swizzle<D>(r0)) * 16 + i16 % 2 * 8;
+    }
+
+    for (int kt = last < 0 ? -1 : last / KT; kt >= 0; --kt) {
+        __syncthreads();
+        {
+            const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
+            const Desc dk = make_desc(kp + (size_t)kt * KT * k_row, (rows - 1) * k_row + kRow);
+            const Desc dv = make_desc(vp + (size_t)kt * KT * v_row, (rows - 1) * v_row + kRow);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const uint32_t base = (wave * kCopies + i) * 1024, byte = base + l * 16, rr = byte / kRow, c = byte % kRow / 16;
+                copy16(dk, rr * k_row + (c ^ k_swizzle<D>(rr)) * 16, s_k + base);
+                copy16(dv, rr * v_row + (c ^ v_swizzle<D>(rr)) * 16, s_v + base);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (!live || kt * KT > limit_max) continue;
+        const bool part = kt * KT + KT - 1 > limit_min;  // some row does not see all keys
+
+        f32x16 s[kSub];
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+            f32x16 acc = {};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const bf16x8 k = *reinterpret_cast<const bf16x8 *>(s_k + k_at[i % kKAt] + (i / kKAt * 256 + j * 32 * kRow));
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i], acc, 0, 0, 0);
+            }
+            s[j] = acc;
+        }
+        if (part) {
+#pragma unroll
+            for (int j = 0; j < kSub; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (kt * KT + j * 32 + 8 * (i / 4) + 4 * half + i % 4 > limit) s[j][i] = -kInf;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int j = 0; j < kSub; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale_log2;
+        const float m_new = fmaxf(m, top), m_use = m_new == -kInf ? 0.0f : m_new;
+        const float keep = __builtin_amdgcn_exp2f(m - m_use);
+        m = m_new;
+        bf16x8 w[kSub][2];
+        float add = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kSub; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], p.scale_log2, -m_use));
+                add += e;
+                w[j][i / 8][i % 8] = (__bf16)e;
+            }
+        sum = sum * keep + add;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+
+        auto values = [&](int j, int st, int d) {
+            const uint8_t *at_v = s_v + v_at[d % kVAt] + (d / kVAt * 256 + (j * 32 + st * 16) * kRow);
+            const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 8 * kRow);
+            return u32x4{x.x, x.y, y.x, y.y};
+        };
+        bool odd = false;  // infinities or NaN among values that some rows do not see
+        if (part) {
+            u16x2 most = {0, 0};
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int j = 0; j < kSub; ++j)
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        const u32x4 x = values(j, st, d);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[e] & 0x7FFF7FFFu));
+                    }
+            odd = __any(most[0] >= 0x7F80 || most[1] >= 0x7F80);
+        }
+        if (!odd) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int j = 0; j < kSub; ++j)
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(j, st, d)), w[j][st], o[d], 0, 0, 0);
+        } else {
+#pragma unroll 1
+            for (int what = kFinite; what <= kNan; ++what) {
+                const float add_odd = odd_value(what);
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) {
+                    f32x16 acc = {};
+#pragma unroll
+                    for (int j = 0; j < kSub; ++j)
+#pragma unroll
+                        for (int st = 0; st < 2; ++st) {
+                            bf16x8 y = w[j][st];
+                            if (what != kFinite) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    y[e] = (__bf16)(kt * KT + j * 32 + st * 16 + 8 * (e / 4) + 4 * half + e % 4 <= limit ? 1.0f : 0.0f);
+                            }
+                            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pick(values(j, st, d), what), y, acc, 0, 0, 0);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] += what == kFinite ? acc[i] : acc[i] > 0.0f ? add_odd : 0.0f;
+                }
+            }
+        }
+    }
+
+    if (!live || mine + r >= lq) return;
+    sum += __shfl_xor(sum, 32);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const size_t token = (size_t)(q0 + mine + r);
+    uint16_t *y = a.y + (token * a.q_heads + head) * D;
+    const uint16_t *gate = a.gate.d ? static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + (size_t)head * a.gate.head : nullptr;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int dim = d * 32 + 8 * (i / 4) + 4 * half;
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = o[d][i + e] * inv;
+            if (gate) {
+                const uint2 b = *reinterpret_cast<const uint2 *>(gate + dim);
+                const float gv[4] = {__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xFFFF0000u), __uint_as_float(b.y << 16),
+                                     __uint_as_float(b.y & 0xFFFF0000u)};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gv[e]);
+            }
+            store4(y + dim, 4, v);
+        }
+}
+
+}  // namespace
+
+hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a) {
+    Kernel p{a, 1, 0, a.scale * kLog2e};
+    const uint32_t group = a.q_heads / a.kv_heads;
+    while (p.head_waves < kWaves && group % (p.head_waves * 2) == 0) p.head_waves *= 2;
+    p.head_sets = a.q_heads / p.head_waves;
+    const uint32_t tokens = 32 * kWaves / p.head_waves;
+    const uint64_t tiles = (uint64_t)a.total_q / tokens + a.n_seqs;  // at least as many as there are
+    const dim3 grid((uint32_t)(tiles * p.head_sets)), block(64 * kWaves);
+    if (a.dim == 64) prompt_kernel<64, 64><<<grid, block, 0, s>>>(p);
+    if (a.dim == 128) prompt_kernel<128, 64><<<grid, block, 0, s>>>(p);
+    if (a.dim == 256) prompt_kernel<256, 32><<<grid, block, 0, s>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace tqf

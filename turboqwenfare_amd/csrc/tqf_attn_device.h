@@ -21,26 +21,4 @@ __device__ __forceinline__ uint2 read_transposed(const uint8_t *lds) {
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
 
-// Weights of 0 do not keep infinities and NaN out of a matrix product.  A tile of
-// values with any that not every row sees is multiplied four times: its finite
-// values by the weights, then, as ones, its infinities of either sign and its NaN
-// by whether a row sees their key; a row with any gets their sum.
-enum Odd { kFinite, kPlusInf, kMinusInf, kNan };
-__device__ __forceinline__ float odd_value(int what) { return what == kPlusInf ? kInf : what == kMinusInf ? -kInf : __builtin_nanf(""); }
-__device__ __forceinline__ bf16x8 pick(u32x4 v, int what) {
-    u32x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        uint32_t both = 0;
-#pragma unroll
-        for (int b = 0; b < 32; b += 16) {
-            const uint32_t bits = v[e] >> b & 0xFFFFu, mag = bits & 0x7FFFu;
-            const bool hit = what == kNan ? mag > 0x7F80u : bits == (what == kPlusInf ? 0x7F80u : 0xFF80u);
-            both |= (what == kFinite ? (mag >= 0x7F80u ? 0u : bits) : hit ? 0x3F80u : 0u) << b;
-        }
-        x[e] = both;
-    }
-    return __builtin_bit_cast(bf16x8, x);
-}
-
 }  // namespace tqf

@@ -16,7 +16,7 @@
 //
 // As in tqf_prompt.hip: S^T = K Q^T (here 16 x 16 x 32) leaves a row's weights as an
 // operand of O^T = V^T P^T; V^T comes from LDS by transposing reads; infinities and
-// NaN among values that only some rows see are counted apart.
+// NaN among values that only some rows see are added at the end, key by key.
 #include <hip/hip_runtime.h>
 
 #include "tqf_attn_device.h"
@@ -81,6 +81,11 @@ __device__ __forceinline__ void line_find(const PagedArgs &a, uint64_t step, Lin
 }
 __device__ __forceinline__ uint64_t part_begin(uint64_t total, uint32_t part, uint32_t parts) { return total * part / parts; }
 
+__device__ __forceinline__ void four_bf16(const uint16_t *p, float (&v)[4]) {
+    const uint2 b = *reinterpret_cast<const uint2 *>(p);
+    v[0] = __uint_as_float(b.x << 16), v[1] = __uint_as_float(b.x & 0xFFFF0000u);
+    v[2] = __uint_as_float(b.y << 16), v[3] = __uint_as_float(b.y & 0xFFFF0000u);
+}
 __device__ __forceinline__ float gate_of(uint16_t b) { return sigmoid(__uint_as_float((uint32_t)b << 16)); }
 
 // NR: tiles of 16 rows that a workgroup has.
@@ -137,6 +142,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
                 q[n][s] = *reinterpret_cast<const bf16x8 *>(qp + (F8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8));
         }
         const int limit_min = len - (int)a.rows;
+        int odd_at = -1;  // the wavefront's keys from here on are left to the end: only the sequence's last step can be such
         f32x4 o[kDims][NR];
         float m[NR], sum[NR];
 #pragma unroll
@@ -195,7 +201,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
                     }
                 }
             const bool partly = k0 + kWaveKeys - 1 > limit_min;  // some row does not see all keys
-            bool odd = false;  // infinities or NaN among values that some rows do not see
             if (partly && a.rows > 1) {
                 uint32_t any = 0;
 #pragma unroll
@@ -211,7 +216,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
                             else any |= ((x & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
                         }
                     }
-                odd = __any(any != 0);
+                if (__any(any != 0)) odd_at = k0;
             }
             bf16x8 w[NR];
             bool grown = false;
@@ -265,30 +270,59 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
                 const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 16 * kRow);
                 return u32x4{x.x, x.y, y.x, y.y};
             };
-            if (!odd) {
+            if (odd_at != k0) {
 #pragma unroll
                 for (int d = 0; d < kDims; ++d) {
                     const bf16x8 v = __builtin_bit_cast(bf16x8, values(d));
 #pragma unroll
                     for (int n = 0; n < NR; ++n) o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[n], o[d][n], 0, 0, 0);
                 }
-            } else {
+            }
+        }
+        // Infinities or NaN that only some rows see: key by key.
+        if (odd_at >= 0) {
 #pragma unroll 1
-                for (int what = kFinite; what <= kNan; ++what) {
-                    const float add_odd = odd_value(what);
+            for (int key = odd_at; key < (odd_at + kWaveKeys < len ? odd_at + kWaveKeys : len); ++key) {
+                int32_t page = a.pages[(size_t)seq * a.max_pages + ((uint32_t)key >> p.page_shift)];
+                if (page < 0 || (uint32_t)page >= a.cache.n_pages) page = 0;  // noticed before
+                const size_t at_row = ((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1));
+                float dot[NR] = {};
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) {
-                        bf16x8 y = w[n];
-                        if (what != kFinite) {
+                for (int s = 0; s < kSteps; ++s) {
+                    const uint32_t e0 = F8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8;
+                    bf16x8 x;
+                    if constexpr (F8) {
+                        const uint2 b = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.cache.k) + at_row * D + e0);
+                        x = f8_widen(b.x, b.y);
+                    } else {
+                        x = *reinterpret_cast<const bf16x8 *>(static_cast<const uint16_t *>(a.cache.k) + at_row * D + e0);
+                    }
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = (__bf16)(k0 + 16 * (e / 4) + 4 * g + e % 4 <= limit[n] ? 1.0f : 0.0f);
+                    for (int n = 0; n < NR; ++n)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dot[n] = __builtin_fmaf((float)x[e], (float)q[n][s][e], dot[n]);
+                }
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    dot[n] += __shfl_xor(dot[n], 16);
+                    dot[n] += __shfl_xor(dot[n], 32);
+                    if constexpr (F8) dot[n] *= a.cache.k_scales[at_row];
+                    float e = __builtin_amdgcn_exp2f(dot[n] * p.scale_log2 - (m[n] == -kInf ? 0.0f : m[n]));
+                    if constexpr (F8) e *= a.cache.v_scales[at_row];
+                    const bool sees = key <= limit[n];
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d) {
+                        float v[4];
+                        if constexpr (F8) {
+                            const uint32_t b = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.cache.v) + at_row * D + d * 16 + 4 * g);
+                            const bf16x8 x = f8_widen(b, 0);
+                            for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+                        } else {
+                            four_bf16(static_cast<const uint16_t *>(a.cache.v) + at_row * D + d * 16 + 4 * g, v);
                         }
 #pragma unroll
-                        for (int d = 0; d < kDims; ++d) {
-                            const f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pick(values(d), what), y, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[d][n][i] += what == kFinite ? acc[i] : acc[i] > 0.0f ? add_odd : 0.0f;
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            if (sees) o[d][n][i] = __builtin_fmaf(e, v[i], o[d][n][i]);
                     }
                 }
             }

@@ -19,8 +19,10 @@
 // Keys that a row does not see have weight 0, but 0 * inf and 0 * NaN are NaN.
 // Rows behind a sequence's end read as zeros (the copies' bounds).  Tiles that some
 // rows see in part are looked through for infinities and NaN; where there are any,
-// each row's are counted by matrix products of their own.
+// the tile's values are added at the end, key by key, to the rows that see them.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "tqf_attn_device.h"
 
@@ -37,6 +39,16 @@ __device__ __forceinline__ void copy16(Desc d, uint32_t voff, void *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, 0, 0, 0);
 }
 constexpr int kWaves = 4;
+// A row's reference m follows its maximum only when that is 2^8 above it: the
+// weights are then at most 2^8, their sums in f32 as exact as ever, and the sums
+// of values are hardly ever multiplied again.
+constexpr float kSlack = 8.0f;
+
+// The larger of lanes l and l ^ 32.
+__device__ __forceinline__ float other_half_max(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
 
 struct Kernel {
     PromptArgs a;
@@ -100,7 +112,7 @@ template <int D, int KT>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     constexpr int kRow = 2 * D, kTile = KT * kRow, kCopies = kTile / 1024 / kWaves, kSub = KT / 32, kDims = D / 32, kSteps = D / 16;
     static_assert(kCopies >= 1, "every wavefront copies");
-    __shared__ __attribute__((aligned(1024))) uint8_t s_k[kTile], s_v[kTile];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_k0[kTile], s_v0[kTile], s_k1[kTile], s_v1[kTile];
     const PromptArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 32, half = l / 32;
     const uint32_t tokens = 32u * kWaves / p.head_waves;  // of the workgroup
@@ -129,6 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
     float m = -kInf, sum = 0.0f;
+    uint32_t odd = 0;  // tiles, from the last one on, whose values are left to the end
 
     const uint8_t *kp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.k.d) + (size_t)k0 * a.k.row + (size_t)kv * a.k.head);
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.v.d) + (size_t)k0 * a.v.row + (size_t)kv * a.v.head);
@@ -148,31 +161,33 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         for (int d = 0; d < kVAt; ++d) v_at[d] = r0 * kRow + ((d * 4 + 2 * (g % 2) + i16 % 4 / 2) ^ v_swizzle<D>(r0)) * 16 + i16 % 2 * 8;
     }
 
-    for (int kt = last < 0 ? -1 : last / KT; kt >= 0; --kt) {
-        __syncthreads();
-        {
-            const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
-            const Desc dk = make_desc(kp + (size_t)kt * KT * k_row, (rows - 1) * k_row + kRow);
-            const Desc dv = make_desc(vp + (size_t)kt * KT * v_row, (rows - 1) * v_row + kRow);
+    auto copy = [&](int kt, uint8_t *to_k, uint8_t *to_v) {
+        const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
+        const Desc dk = make_desc(kp + (size_t)kt * KT * k_row, (rows - 1) * k_row + kRow);
+        const Desc dv = make_desc(vp + (size_t)kt * KT * v_row, (rows - 1) * v_row + kRow);
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) {
-                const uint32_t base = (wave * kCopies + i) * 1024, byte = base + l * 16, rr = byte / kRow, c = byte % kRow / 16;
-                copy16(dk, rr * k_row + (c ^ k_swizzle<D>(rr)) * 16, s_k + base);
-                copy16(dv, rr * v_row + (c ^ v_swizzle<D>(rr)) * 16, s_v + base);
-            }
+        for (int i = 0; i < kCopies; ++i) {
+            const uint32_t base = (wave * kCopies + i) * 1024, byte = base + l * 16, rr = byte / kRow, c = byte % kRow / 16;
+            copy16(dk, rr * k_row + (c ^ k_swizzle<D>(rr)) * 16, to_k + base);
+            copy16(dv, rr * v_row + (c ^ v_swizzle<D>(rr)) * 16, to_v + base);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (!live || kt * KT > limit_max) continue;
-        const bool part = kt * KT + KT - 1 > limit_min;  // some row does not see all keys
-
+    };
+    auto values = [&](const uint8_t *sv, int j, int st, int d) {
+        const uint8_t *at_v = sv + v_at[d % kVAt] + (d / kVAt * 256 + (j * 32 + st * 16) * kRow);
+        const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 8 * kRow);
+        return u32x4{x.x, x.y, y.x, y.y};
+    };
+    // One tile.  EDGE: some row of the workgroup does not see all of its keys.
+    auto step = [&](const uint8_t *sk, const uint8_t *sv, int kt, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const bool part = EDGE && kt * KT + KT - 1 > limit_min;  // some row of the wavefront
         f32x16 s[kSub];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
             f32x16 acc = {};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                const bf16x8 k = *reinterpret_cast<const bf16x8 *>(s_k + k_at[i % kKAt] + (i / kKAt * 256 + j * 32 * kRow));
+                const bf16x8 k = *reinterpret_cast<const bf16x8 *>(sk + k_at[i % kKAt] + (i / kKAt * 256 + j * 32 * kRow));
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i], acc, 0, 0, 0);
             }
             s[j] = acc;
@@ -189,77 +204,102 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         for (int j = 0; j < kSub; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale_log2;
-        const float m_new = fmaxf(m, top), m_use = m_new == -kInf ? 0.0f : m_new;
-        const float keep = __builtin_amdgcn_exp2f(m - m_use);
-        m = m_new;
+        top = other_half_max(top) * p.scale_log2;
+        if (__any(top > m + kSlack)) {
+            const float m_new = fmaxf(m, top), keep = m_new == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+        }
+        const float m_use = m == -kInf ? 0.0f : m;
         bf16x8 w[kSub][2];
-        float add = 0.0f;
 #pragma unroll
         for (int j = 0; j < kSub; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], p.scale_log2, -m_use));
-                add += e;
+                sum += e;
                 w[j][i / 8][i % 8] = (__bf16)e;
             }
-        sum = sum * keep + add;
+        if (part) {
+            u16x2 most = {0, 0};  // largest magnitudes among values that some rows do not see
+#pragma unroll
+            for (int i = 0; i < kTile / 1024; ++i) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(sv + i * 1024 + l * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[e] & 0x7FFF7FFFu));
+            }
+            if (__any(most[0] >= 0x7F80 || most[1] >= 0x7F80)) {
+                odd |= 1u << (last / KT - kt);
+                return;
+            }
+        }
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+            for (int j = 0; j < kSub; ++j)
+#pragma unroll
+                for (int st = 0; st < 2; ++st)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(sv, j, st, d)), w[j][st], o[d], 0, 0, 0);
+    };
 
-        auto values = [&](int j, int st, int d) {
-            const uint8_t *at_v = s_v + v_at[d % kVAt] + (d / kVAt * 256 + (j * 32 + st * 16) * kRow);
-            const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 8 * kRow);
-            return u32x4{x.x, x.y, y.x, y.y};
-        };
-        bool odd = false;  // infinities or NaN among values that some rows do not see
-        if (part) {
-            u16x2 most = {0, 0};
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                for (int j = 0; j < kSub; ++j)
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        const u32x4 x = values(j, st, d);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[e] & 0x7FFF7FFFu));
-                    }
-            odd = __any(most[0] >= 0x7F80 || most[1] >= 0x7F80);
+    // Two stages of LDS, each a variable of its own: the next tile's copies are under way while one is computed.
+    // publish(): this wavefront's copies are there and its reads done, then the workgroup's.
+    auto publish = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    if (last >= 0) {
+        const int edge = (first + shift + 1 > 0 ? first + shift + 1 : 0) / KT;  // the tiles from here on are seen in part
+        int kt = last / KT;
+        copy(kt, s_k0, s_v0);
+        bool one = false;
+        for (; kt >= edge; --kt) {
+            publish();
+            if (kt > 0) copy(kt - 1, one ? s_k0 : s_k1, one ? s_v0 : s_v1);
+            if (live && kt * KT <= limit_max) step(one ? s_k1 : s_k0, one ? s_v1 : s_v0, kt, std::true_type());
+            one = !one;
         }
-        if (!odd) {
+        if (one && kt >= 0) {
+            publish();
+            if (kt > 0) copy(kt - 1, s_k0, s_v0);
+            if (live) step(s_k1, s_v1, kt, std::false_type());
+            --kt;
+        }
+        for (; kt >= 0; --kt) {
+            publish();
+            if (kt > 0) copy(kt - 1, s_k1, s_v1);
+            if (live) step(s_k0, s_v0, kt, std::false_type());
+            if (--kt < 0) break;
+            publish();
+            if (kt > 0) copy(kt - 1, s_k0, s_v0);
+            if (live) step(s_k1, s_v1, kt, std::false_type());
+        }
+    }
+
+    // Tiles with infinities or NaN that only some rows see: key by key.
+    while (odd) {
+        const int kt = last / KT - __builtin_ctz(odd);
+        odd &= odd - 1;
+#pragma unroll 1
+        for (int key = kt * KT; key < (kt * KT + KT < lk ? kt * KT + KT : lk); ++key) {
+            const uint16_t *kr = reinterpret_cast<const uint16_t *>(kp + (size_t)key * k_row) + half * 8;
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const bf16x8 x = *reinterpret_cast<const bf16x8 *>(kr + i * 16);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dot = __builtin_fmaf((float)x[e], (float)q[i][e], dot);
+            }
+            dot += __shfl_xor(dot, 32);
+            if (key > limit) continue;
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, p.scale_log2, m == -kInf ? 0.0f : -m));
+            const uint16_t *vr = reinterpret_cast<const uint16_t *>(vp + (size_t)key * v_row) + half * 4;
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
 #pragma unroll
-                for (int j = 0; j < kSub; ++j)
-#pragma unroll
-                    for (int st = 0; st < 2; ++st)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(j, st, d)), w[j][st], o[d], 0, 0, 0);
-        } else {
-#pragma unroll 1
-            for (int what = kFinite; what <= kNan; ++what) {
-                const float add_odd = odd_value(what);
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) {
-                    f32x16 acc = {};
-#pragma unroll
-                    for (int j = 0; j < kSub; ++j)
-#pragma unroll
-                        for (int st = 0; st < 2; ++st) {
-                            bf16x8 y = w[j][st];
-                            if (what != kFinite) {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    y[e] = (__bf16)(kt * KT + j * 32 + st * 16 + 8 * (e / 4) + 4 * half + e % 4 <= limit ? 1.0f : 0.0f);
-                            }
-                            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pick(values(j, st, d), what), y, acc, 0, 0, 0);
-                        }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] += what == kFinite ? acc[i] : acc[i] > 0.0f ? add_odd : 0.0f;
-                }
-            }
+                for (int i = 0; i < 16; ++i)
+                    o[d][i] = __builtin_fmaf(e, __uint_as_float((uint32_t)vr[d * 32 + 8 * (i / 4) + i % 4] << 16), o[d][i]);
         }
     }
 

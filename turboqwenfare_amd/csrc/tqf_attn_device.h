@@ -13,6 +13,26 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
 
+// A row's reference m follows its maximum only when that is 2^8 above it: the
+// weights are then at most 2^8, their sums in f32 as exact as ever, and the sums
+// of values are hardly ever multiplied again.
+constexpr float kSlack = 8.0f;
+
+// Copies to LDS: lane l's 16 bytes go to lds + 16 l.
+typedef __amdgpu_buffer_rsrc_t Desc;  // loads past its bytes give zero
+typedef __attribute__((address_space(3))) void lds_void;
+// p and bytes are the same in every lane: said to the compiler, which would else make
+// a loop over their values of each copy.
+__device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint64_t low = __builtin_amdgcn_readfirstlane((uint32_t)at), high = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(high << 32 | (uint32_t)low), (short)0, __builtin_amdgcn_readfirstlane((int)bytes),
+                                             0x00020000);
+}
+__device__ __forceinline__ void copy16(Desc d, uint32_t voff, void *lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, 0, 0, 0);
+}
+
 // Four rows of 16 elements of 16 bits, transposed: lane i of 16 points at four
 // elements, 4 (i % 4) on, of row i / 4, and gets element i of the four rows.
 __device__ __forceinline__ uint2 read_transposed(const uint8_t *lds) {

@@ -25,6 +25,17 @@ namespace tqf {
 
 namespace {
 
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+
+// This wavefront's loads (those to LDS among them) but the last N are done.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Its LDS reads are.
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 constexpr int kWaves = 4, kWaveKeys = 32, kStepKeys = kWaves * kWaveKeys;
 
 struct Kernel {
@@ -41,45 +52,46 @@ __device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
     return n ? n : 1;
 }
 
-// The line of all steps: sequence by sequence, key head by key head.
+// The line of all steps: sequence by sequence, key head by key head; fewer than 2^31
+// (the caller has checked the most there can be).  All results are the same in
+// every lane, and the compiler is told so: descriptors made of them stay scalar.
 struct Line {
-    uint64_t total;
-    // of the step asked for
-    uint32_t seq, steps;
-    uint64_t first;  // of the sequence
+    uint32_t seq, steps, first;  // a sequence, its steps for a key head, its first step
 };
-__device__ __forceinline__ uint64_t line_total(const PagedArgs &a) {
+__device__ __forceinline__ uint32_t line_total(const PagedArgs &a) {
     const uint32_t l = threadIdx.x & 63;
-    uint64_t sum = 0;
+    uint32_t sum = 0;
     for (uint32_t s = l; s < a.n_seqs; s += 64) sum += steps_of(a, a.lens[s]);
 #pragma unroll
     for (int o = 32; o >= 1; o /= 2) sum += __shfl_xor(sum, o);
-    return sum * a.cache.kv_heads;
+    return __builtin_amdgcn_readfirstlane(sum * a.cache.kv_heads);
 }
-__device__ __forceinline__ void line_find(const PagedArgs &a, uint64_t step, Line &p) {
+__device__ __forceinline__ Line line_find(const PagedArgs &a, uint32_t step) {
     const uint32_t l = threadIdx.x & 63;
-    uint64_t before = 0;
+    uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64) {
         const uint32_t s = s0 + l, mine = s < a.n_seqs ? steps_of(a, a.lens[s]) : 0;
-        uint64_t upto = (uint64_t)mine * a.cache.kv_heads;
+        uint32_t upto = mine * a.cache.kv_heads;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
-            const uint64_t v = __shfl_up(upto, o);
+            const uint32_t v = __shfl_up(upto, o);
             if ((int)l >= o) upto += v;
         }
         const uint64_t past = __ballot(before + upto > step);
         if (past) {
             const int who = __builtin_ctzll(past);
-            p.seq = s0 + who;
-            p.steps = __shfl(mine, who);
-            p.first = before + __shfl(upto, who) - (uint64_t)p.steps * a.cache.kv_heads;
-            return;
+            const uint32_t n = __builtin_amdgcn_readlane(mine, who);
+            return Line{s0 + who, n, before + __builtin_amdgcn_readlane(upto, who) - n * a.cache.kv_heads};
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
-    p.seq = a.n_seqs;  // no such step
+    return Line{a.n_seqs, 1, 0};  // no such step
 }
-__device__ __forceinline__ uint64_t part_begin(uint64_t total, uint32_t part, uint32_t parts) { return total * part / parts; }
+// Equal parts, the first ones a step longer.
+__device__ __forceinline__ uint32_t part_begin(uint32_t total, uint32_t part, uint32_t parts) {
+    const uint32_t each = total / parts, more = total % parts;
+    return part * each + (part < more ? part : more);
+}
 
 __device__ __forceinline__ void four_bf16(const uint16_t *p, float (&v)[4]) {
     const uint2 b = *reinterpret_cast<const uint2 *>(p);
@@ -88,43 +100,115 @@ __device__ __forceinline__ void four_bf16(const uint16_t *p, float (&v)[4]) {
 }
 __device__ __forceinline__ float gate_of(uint16_t b) { return sigmoid(__uint_as_float((uint32_t)b << 16)); }
 
-// NR: tiles of 16 rows that a workgroup has.
+// Rows of the cache in LDS as the copies bring them, 16-byte chunk c of row r in slot
+// c ^ its swizzle: the copies read whole rows, and both the 16 rows of which 16
+// lanes read a chunk of keys and those that 32 lanes read transposed are in
+// different places of the banks.  kPitch: bytes of a row.
+template <int kPitch>
+__device__ __forceinline__ uint32_t k_swizzle(uint32_t row) {
+    return kPitch >= 256 ? row & 15 : kPitch == 128 ? row >> 1 & 7 : row >> 2 & 3;
+}
+template <int kPitch, bool F8>
+__device__ __forceinline__ uint32_t v_swizzle(uint32_t row) {
+    if (F8) {
+        const uint32_t upper = row >> 4 & 1;
+        return kPitch == 256 ? (row & 7) | upper << 3 : kPitch == 128 ? (row >> 1 & 3) | upper << 2 : (row >> 2 & 1) | upper << 1;
+    }
+    return kPitch >= 256 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
+}
+
+// NR: tiles of 16 rows that a workgroup has.  A wavefront's 32 keys and values come
+// by copies to LDS that is its own: the next keys are asked for when these have been
+// multiplied, the next values likewise, so there is always one of the two under way,
+// and no registers wait for them.
 template <int D, int NR, bool F8>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
-    constexpr int kRow = 2 * D, kDims = D / 16, kSteps = D / 32, kRows = 16 * NR, kChunks = D / 8;
-    constexpr int kKLoads = F8 ? D / 64 : D / 32;  // 16-byte loads of a lane for 16 keys
-    __shared__ __attribute__((aligned(16))) uint8_t s_v[kWaves][kWaveKeys * kRow];
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Kernel p) {
+    constexpr int kRow = F8 ? D : 2 * D, kDims = D / 16, kSteps = D / 32, kRows = 16 * NR, kChunks = D / 8;
+    constexpr int kCopies = kRow / 64;  // of 1 KiB for 16 keys
+    constexpr int kOutRound = 16 * D * 4, kTile = kWaveKeys * kRow;
+    // keys, then values; at the end the rows' sums of values
+    __shared__ __attribute__((aligned(1024))) uint8_t s_k[kWaves][kTile], s_v[kWaves][kTile > kOutRound ? kTile : kOutRound];
     __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 16, g = l / 16;
     const uint32_t part = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
-    const uint64_t total = line_total(a);
-    uint64_t at = part_begin(total, part, p.parts);
-    const uint64_t begin = at, end = part_begin(total, part + 1, p.parts);
+    const uint32_t total = line_total(a);
+    uint32_t at = part_begin(total, part, p.parts);
+    const uint32_t begin = at, end = part_begin(total, part + 1, p.parts);
     const uint32_t all_rows = a.rows * p.group;
     const size_t page_size = a.cache.page;
-    // V^T: dimension 16 d + l % 16, the keys that the lane's weights have (4 g and 16 + 4 g on)
-    constexpr int kVAt = kDims < 8 ? kDims : 8;
-    uint32_t v_at[kVAt];
-    {
-        const int key = 4 * g + r / 4, turn = D == 64 ? (key >> 1 & 3) << 1 : (key & 7) << 1;
-#pragma unroll
-        for (int d = 0; d < kVAt; ++d) v_at[d] = key * kRow + ((d * 2 + r % 4 / 2) ^ turn) * 16 + r % 2 * 8;
+    uint8_t *const kl = s_k[wave], *const vl = s_v[wave];
+    // K: chunk of key r (and r + 16) that a lane has of a step of 32 dimensions; V^T: dimension 16 d + l % 16 of the
+    // keys that its weights have (4 g and 16 + 4 g on).  Other steps' and dimensions' are these with bits flipped.
+    const uint32_t k_at = r * kRow + (g ^ k_swizzle<kRow>(r)) * 16;
+    uint32_t v_at, v_at2;
+    if constexpr (F8) {
+        const uint32_t key = r / 2 < 4 ? 4 * g + r / 2 : 16 + 4 * g + r / 2 - 4;  // of the eight rows
+        v_at = key * kRow + v_swizzle<kRow, true>(key) * 16 + r % 2 * 8;
+        v_at2 = 0;
+    } else {
+        const uint32_t key = 4 * g + r / 4;
+        v_at = key * kRow + ((r % 4 / 2) ^ v_swizzle<kRow, false>(key)) * 16 + r % 2 * 8;
+        v_at2 = v_at + 16 * kRow;  // the swizzle of row + 16 is that of the row
     }
 
     while (at < end) {
-        Line line;
-        line_find(a, at, line);
+        const Line line = line_find(a, at);
         if (line.seq >= a.n_seqs) return;
-        const uint32_t seq = __builtin_amdgcn_readfirstlane(line.seq), steps = __builtin_amdgcn_readfirstlane(line.steps);
-        const uint64_t in_seq = at - line.first;
-        const uint32_t kv = __builtin_amdgcn_readfirstlane((uint32_t)(in_seq / steps)), from = __builtin_amdgcn_readfirstlane((uint32_t)(in_seq % steps));
-        const uint32_t upto = __builtin_amdgcn_readfirstlane((uint32_t)(steps - from < end - at ? steps : from + (end - at)));
-        int32_t len = a.lens[seq];
+        const uint32_t seq = line.seq, steps = line.steps, kv = __builtin_amdgcn_readfirstlane((at - line.first) / steps), from = at - line.first - kv * steps;
+        const uint32_t upto = steps - from < end - at ? steps : from + (end - at);
+        int32_t len = __builtin_amdgcn_readfirstlane(a.lens[seq]);
         bool poison = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * page_size;
         if (poison) {
             if (a.status) *a.status = TQF_HIP_ERR_INVALID;
             len = 0;
+        }
+        const int32_t *table = a.pages + (size_t)seq * a.max_pages;
+
+        // the first of 16 keys in the cache; keys behind the end: -1
+        auto find = [&](int key) -> int64_t {
+            if (key >= len) return -1;
+            int32_t page = __builtin_amdgcn_readfirstlane(table[(uint32_t)key >> p.page_shift]);
+            if (page < 0 || (uint32_t)page >= a.cache.n_pages) {
+                poison = true;
+                page = 0;
+            }
+            return (int64_t)(((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1)));
+        };
+        // copies of 32 keys' rows; those behind the end are zero
+        auto copy = [&](const void *from_cache, const int64_t (&row0)[2], int k0, uint8_t *to, bool values) {
+            uint32_t lane = l;
+            asm volatile("" : "+v"(lane));  // offsets are computed where they are used: they would take registers all along
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int left = len - k0 - 16 * j, rows = left < 0 ? 0 : left < 16 ? left : 16;
+                const Desc d = make_desc(static_cast<const uint8_t *>(from_cache) + (row0[j] < 0 ? 0 : (size_t)row0[j]) * kRow, rows * kRow);
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    const uint32_t byte = i * 1024 + lane * 16, rr = byte / kRow, c = byte % kRow / 16;
+                    const uint32_t sw = values ? v_swizzle<kRow, F8>(16 * j + rr) : k_swizzle<kRow>(rr);
+                    copy16(d, rr * kRow + (c ^ sw) * 16, to + j * 16 * kRow + i * 1024);
+                }
+            }
+        };
+        const int first = (int)(from * kStepKeys) + wave * kWaveKeys, behind = (int)(upto * kStepKeys) < len ? (int)(upto * kStepKeys) : len;
+        int64_t row0[2];
+        f32x4 ks[2], vs[2];
+        auto scales = [&] {
+            if constexpr (F8) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int64_t at_row = row0[j] < 0 ? row0[0] : row0[j];
+                    ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + at_row + 4 * g);
+                    vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + at_row + 4 * g);
+                }
+            }
+        };
+        if (first < behind) {
+            row0[0] = find(first), row0[1] = find(first + 16);
+            copy(a.cache.k, row0, first, kl, false);
+            scales();
+            copy(a.cache.v, row0, first, vl, true);
         }
 
         // the rows: column r of tile n is row block * kRows + 16 n + r, of query row / group and head row % group
@@ -153,131 +237,131 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(Kernel p) {
             for (int d = 0; d < kDims; ++d) o[d][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        for (uint32_t step = from; step < upto; ++step) {
-            const int k0 = (int)(step * kStepKeys) + wave * kWaveKeys;
-            if (k0 >= len) break;
-            size_t row0[2];  // of the 16 keys in the cache
+        for (int k0 = first; k0 < behind; k0 += kStepKeys) {
+            const int next = k0 + kStepKeys;
+            const bool more = next < behind;
+            f32x4 s[2][NR];
+            wait_copies<2 * kCopies>();  // the keys are there, the values' copies may be under way
+            {
+                uint32_t at_k = k_at;
+                asm volatile("" : "+v"(at_k));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int key = k0 + 16 * j < len ? k0 + 16 * j : k0;
-                int32_t page = a.pages[(size_t)seq * a.max_pages + ((uint32_t)key >> p.page_shift)];
-                if (page < 0 || (uint32_t)page >= a.cache.n_pages) {
-                    poison = true;
-                    page = 0;
-                }
-                row0[j] = ((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1));
-            }
-            u32x4 kx[2][kKLoads], vx[2][kKLoads];
-            f32x4 ks[2], vs[2];
+                for (int j = 0; j < 2; ++j) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint8_t *kb = static_cast<const uint8_t *>(a.cache.k) + row0[j] * (F8 ? D : kRow);
-                const uint8_t *vb = static_cast<const uint8_t *>(a.cache.v) + row0[j] * (F8 ? D : kRow);
+                    for (int n = 0; n < NR; ++n) s[j][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < kKLoads; ++i) {
-                    kx[j][i] = *reinterpret_cast<const u32x4 *>(kb + r * (F8 ? D : kRow) + i * 64 + g * 16);
-                    vx[j][i] = *reinterpret_cast<const u32x4 *>(vb + i * 1024 + l * 16);
-                }
-                if constexpr (F8) {
-                    ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + row0[j] + 4 * g);
-                    vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + row0[j] + 4 * g);
-                }
-            }
-            // values to LDS, as bf16, [key][chunk c of 8 at c ^ its place]; those behind the end are zero
-            uint8_t *vl = s_v[wave];
+                    for (int i = 0; i < kSteps; i += F8 ? 2 : 1) {
+                        // chunk 4 i + g (of e4m3, two steps' dimensions)
+                        const int c = F8 ? i / 2 * 4 : i * 4;
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(kl + (at_k ^ (c % 16 * 16)) + c / 16 * 256 + j * 16 * kRow);
+                        if constexpr (F8) {
+                            const bf16x8 lo = f8_widen(x[0], x[1]), hi = f8_widen(x[2], x[3]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                            for (int n = 0; n < NR; ++n) {
+                                s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, q[n][i], s[j][n], 0, 0, 0);
+                                s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, q[n][i + 1], s[j][n], 0, 0, 0);
+                            }
+                        } else {
 #pragma unroll
-                for (int i = 0; i < kKLoads; ++i) {
-                    const int byte = i * 1024 + l * 16, key = 16 * j + byte / (F8 ? D : kRow), c = byte % (F8 ? D : kRow) / 16;
-                    const int turn = D == 64 ? (key >> 1 & 3) << 1 : (key & 7) << 1;
-                    const bool in = k0 + key < len;
-                    if constexpr (F8) {
-                        const u32x4 x = in ? vx[j][i] : u32x4{0, 0, 0, 0};
-                        *reinterpret_cast<bf16x8 *>(vl + key * kRow + ((2 * c) ^ turn) * 16) = f8_widen(x[0], x[1]);
-                        *reinterpret_cast<bf16x8 *>(vl + key * kRow + ((2 * c + 1) ^ turn) * 16) = f8_widen(x[2], x[3]);
-                    } else {
-                        *reinterpret_cast<u32x4 *>(vl + key * kRow + (c ^ turn) * 16) = in ? vx[j][i] : u32x4{0, 0, 0, 0};
+                            for (int n = 0; n < NR; ++n)
+                                s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), q[n][i], s[j][n], 0, 0, 0);
+                        }
                     }
                 }
+            }
+            f32x4 vscale[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if constexpr (F8) {
+                    vscale[j] = vs[j];
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) s[j][n] *= ks[j];
+                }
+            }
+            reads_done();
+            if (more) {
+                row0[0] = find(next), row0[1] = find(next + 16);
+                copy(a.cache.k, row0, next, kl, false);
+                scales();
+            }
             const bool partly = k0 + kWaveKeys - 1 > limit_min;  // some row does not see all keys
-            if (partly && a.rows > 1) {
-                uint32_t any = 0;
+            bf16x8 w[NR];
+            bool grown = false;
+            float top[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < kKLoads; ++i) {
-                        if (k0 + 16 * j + (i * 1024 + l * 16) / (F8 ? D : kRow) >= len) continue;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t x = vx[j][i][e];
-                            // e4m3: all but the sign set; bf16: the exponent's carry
-                            if constexpr (F8) any |= ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                            else any |= ((x & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        s[j][n][i] *= p.scale_log2;
+                        if (partly && k0 + 16 * j + 4 * g + i > limit[n]) s[j][n][i] = -kInf;
                     }
-                if (__any(any != 0)) odd_at = k0;
-            }
-            bf16x8 w[NR];
-            bool grown = false;
-            float keep[NR];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                f32x4 s[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        bf16x8 kk;
-                        if constexpr (F8) kk = f8_widen(kx[j][i / 2][i % 2 * 2], kx[j][i / 2][i % 2 * 2 + 1]);
-                        else kk = __builtin_bit_cast(bf16x8, kx[j][i]);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[n][i], acc, 0, 0, 0);
-                    }
-                    if constexpr (F8) acc *= ks[j];
-                    s[j] = acc * p.scale_log2;
-                    if (partly) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (k0 + 16 * j + 4 * g + i > limit[n]) s[j][i] = -kInf;
-                    }
-                }
-                float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m_new = fmaxf(m[n], top), m_use = m_new == -kInf ? 0.0f : m_new;
-                grown |= m_new != m[n];
-                keep[n] = __builtin_amdgcn_exp2f(m[n] - m_use);
-                m[n] = m_new;
-                float add = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(s[e / 4][e % 4] - m_use);
-                    add += x;
-                    if constexpr (F8) w[n][e] = (__bf16)(partly && k0 + 16 * (e / 4) + 4 * g + e % 4 > limit[n] ? 0.0f : x * vs[e / 4][e % 4]);
-                    else w[n][e] = (__bf16)x;
-                }
-                sum[n] = sum[n] * keep[n] + add;
+                top[n] = fmaxf(fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[0][n][2], s[0][n][3])),
+                               fmaxf(fmaxf(s[1][n][0], s[1][n][1]), fmaxf(s[1][n][2], s[1][n][3])));
+                top[n] = fmaxf(top[n], __shfl_xor(top[n], 16));
+                top[n] = fmaxf(top[n], __shfl_xor(top[n], 32));
+                grown |= top[n] > m[n] + kSlack;
             }
             if (__any(grown)) {
 #pragma unroll
-                for (int n = 0; n < NR; ++n)
+                for (int n = 0; n < NR; ++n) {
+                    const float m_new = fmaxf(m[n], top[n]), keep = m_new == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - m_new);
+                    m[n] = m_new;
+                    sum[n] *= keep;
 #pragma unroll
-                    for (int d = 0; d < kDims; ++d) o[d][n] *= keep[n];
+                    for (int d = 0; d < kDims; ++d) o[d][n] *= keep;
+                }
             }
-            auto values = [&](int d) {
-                const uint8_t *at_v = vl + v_at[d % kVAt] + d / kVAt * 256;
-                const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 16 * kRow);
-                return u32x4{x.x, x.y, y.x, y.y};
-            };
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                const float m_use = m[n] == -kInf ? 0.0f : m[n];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(s[e / 4][n][e % 4] - m_use);
+                    sum[n] += x;
+                    if constexpr (F8) w[n][e] = (__bf16)(partly && k0 + 16 * (e / 4) + 4 * g + e % 4 > limit[n] ? 0.0f : x * vscale[e / 4][e % 4]);
+                    else w[n][e] = (__bf16)x;
+                }
+            }
+            // the values are there; the next keys' copies (and scales) may be under way
+            if (more) wait_copies<2 * kCopies>();
+            else wait_copies<0>();
+            if (partly && a.rows > 1) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int i = 0; i < kTile / 1024; ++i) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(vl + i * 1024 + l * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // e4m3: all but the sign set; bf16: the exponent's carry
+                        if constexpr (F8) any |= ((x[e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                        else any |= ((x[e] & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
+                    }
+                }
+                if (__any(any != 0)) odd_at = k0;
+            }
             if (odd_at != k0) {
+                uint32_t at_v = v_at, at_v2 = v_at2;
+                asm volatile("" : "+v"(at_v), "+v"(at_v2));
 #pragma unroll
                 for (int d = 0; d < kDims; ++d) {
-                    const bf16x8 v = __builtin_bit_cast(bf16x8, values(d));
+                    bf16x8 v;
+                    if constexpr (F8) {
+                        const int c = d;
+                        const auto x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(vl + (at_v ^ (c * 16))));
+                        v = f8_widen((uint32_t)x[0], (uint32_t)x[1]);
+                    } else {
+                        const int c = d * 2;
+                        const uint2 x = read_transposed(vl + (at_v ^ (c % 16 * 16)) + c / 16 * 256), y = read_transposed(vl + (at_v2 ^ (c % 16 * 16)) + c / 16 * 256);
+                        v = __builtin_bit_cast(bf16x8, u32x4{x.x, x.y, y.x, y.y});
+                    }
 #pragma unroll
                     for (int n = 0; n < NR; ++n) o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[n], o[d][n], 0, 0, 0);
                 }
             }
+            reads_done();
+            if (more) copy(a.cache.v, row0, next, vl, true);
         }
         // Infinities or NaN that only some rows see: key by key.
         if (odd_at >= 0) {
@@ -412,18 +496,17 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p) {
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, wave = tid / 64, l = tid % 64;
     const uint32_t all_rows = a.rows * p.group, part = blockIdx.x / all_rows + 1, row = blockIdx.x % all_rows;
-    const uint64_t total = line_total(a), cut = part_begin(total, part, p.parts);
+    const uint32_t total = line_total(a), cut = part_begin(total, part, p.parts);
     if (cut == 0 || cut >= total) return;
-    Line line;
-    line_find(a, cut, line);
+    const Line line = line_find(a, cut);
     if (line.seq >= a.n_seqs) return;
-    const uint64_t in_seq = cut - line.first, kv = in_seq / line.steps, begin = line.first + kv * line.steps, end = begin + line.steps;
+    const uint32_t kv = (cut - line.first) / line.steps, begin = line.first + kv * line.steps, end = begin + line.steps;
     if (cut == begin || part_begin(total, part - 1, p.parts) > begin) return;  // no unit is cut here, or not here first
     const uint32_t block = row / kRows, of_block = row % kRows;
     // part - 1 (from `begin` on, or before it) to the last part that begins before `end`
     float m = -kInf, sum = 0.0f, o[D / 64] = {};
     for (uint32_t i = part - 1 + wave; i < p.parts; i += kJoinWaves) {
-        const uint64_t b = part_begin(total, i, p.parts);
+        const uint32_t b = part_begin(total, i, p.parts);
         if (b >= end) break;
         if (part_begin(total, i + 1, p.parts) == b) continue;  // an empty part
         const float *from = p.partial + ((size_t)(2 * i + (b >= begin ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2) + (size_t)of_block * (D + 2);
@@ -454,7 +537,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p) {
             v += s_o[i][d] * f;
         }
         v *= all == 0.0f ? 0.0f : 1.0f / all;
-        const size_t token = (size_t)line.seq * a.rows + row / p.group, head = kv * p.group + row % p.group;
+        const size_t token = (size_t)line.seq * a.rows + row / p.group, head = (size_t)kv * p.group + row % p.group;
         if (a.gate.d) v *= gate_of(static_cast<const uint16_t *>(a.gate.d)[token * a.gate.row + head * a.gate.head + d]);
         a.y[(token * a.q_heads + head) * D + d] = __builtin_bit_cast(uint16_t, (__bf16)v);
     }

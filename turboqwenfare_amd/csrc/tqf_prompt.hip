@@ -30,20 +30,7 @@ namespace tqf {
 
 namespace {
 
-typedef __amdgpu_buffer_rsrc_t Desc;  // loads past its bytes give zero
-typedef __attribute__((address_space(3))) void lds_void;
-__device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
-}
-__device__ __forceinline__ void copy16(Desc d, uint32_t voff, void *lds) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, 0, 0, 0);
-}
 constexpr int kWaves = 4;
-// A row's reference m follows its maximum only when that is 2^8 above it: the
-// weights are then at most 2^8, their sums in f32 as exact as ever, and the sums
-// of values are hardly ever multiplied again.
-constexpr float kSlack = 8.0f;
-
 // The larger of lanes l and l ^ 32.
 __device__ __forceinline__ float other_half_max(float x) {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

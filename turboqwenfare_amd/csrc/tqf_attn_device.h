@@ -39,6 +39,24 @@ __device__ __forceinline__ uint2 read_transposed(const uint8_t *lds) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)lds));
 }
 
+// The larger of lanes l and l ^ 32.
+__device__ __forceinline__ float other_half_max(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+// Of lanes l and l ^ 16.
+__device__ __forceinline__ float other_row_max(float x) {
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
+// x, as a value that is made here: what is computed from it is computed where it is
+// used, and takes no register all along.
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
 
 }  // namespace tqf

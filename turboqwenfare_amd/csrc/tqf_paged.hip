@@ -25,6 +25,8 @@ namespace tqf {
 
 namespace {
 
+// Page numbers are read by scalar loads: a vector load's wait would be one for the copies too.
+typedef __attribute__((address_space(4))) int32_t constant_i32;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
@@ -157,18 +159,18 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
         if (line.seq >= a.n_seqs) return;
         const uint32_t seq = line.seq, steps = line.steps, kv = __builtin_amdgcn_readfirstlane((at - line.first) / steps), from = at - line.first - kv * steps;
         const uint32_t upto = steps - from < end - at ? steps : from + (end - at);
-        int32_t len = __builtin_amdgcn_readfirstlane(a.lens[seq]);
+        int32_t len = ((const constant_i32 *)(uintptr_t)a.lens)[seq];
         bool poison = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * page_size;
         if (poison) {
             if (a.status) *a.status = TQF_HIP_ERR_INVALID;
             len = 0;
         }
-        const int32_t *table = a.pages + (size_t)seq * a.max_pages;
+        const constant_i32 *table = (const constant_i32 *)(uintptr_t)(a.pages + (size_t)seq * a.max_pages);
 
         // the first of 16 keys in the cache; keys behind the end: -1
         auto find = [&](int key) -> int64_t {
             if (key >= len) return -1;
-            int32_t page = __builtin_amdgcn_readfirstlane(table[(uint32_t)key >> p.page_shift]);
+            int32_t page = table[__builtin_amdgcn_readfirstlane((uint32_t)key >> p.page_shift)];
             if (page < 0 || (uint32_t)page >= a.cache.n_pages) {
                 poison = true;
                 page = 0;
@@ -191,26 +193,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
                 }
             }
         };
-        const int first = (int)(from * kStepKeys) + wave * kWaveKeys, behind = (int)(upto * kStepKeys) < len ? (int)(upto * kStepKeys) : len;
-        int64_t row0[2];
-        f32x4 ks[2], vs[2];
-        auto scales = [&] {
-            if constexpr (F8) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int64_t at_row = row0[j] < 0 ? row0[0] : row0[j];
-                    ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + at_row + 4 * g);
-                    vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + at_row + 4 * g);
-                }
-            }
-        };
-        if (first < behind) {
-            row0[0] = find(first), row0[1] = find(first + 16);
-            copy(a.cache.k, row0, first, kl, false);
-            scales();
-            copy(a.cache.v, row0, first, vl, true);
-        }
-
         // the rows: column r of tile n is row block * kRows + 16 n + r, of query row / group and head row % group
         bf16x8 q[NR][kSteps];
         int limit[NR];
@@ -225,6 +207,19 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             for (int s = 0; s < kSteps; ++s)
                 q[n][s] = *reinterpret_cast<const bf16x8 *>(qp + (F8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8));
         }
+        const int first = (int)(from * kStepKeys) + wave * kWaveKeys, behind = (int)(upto * kStepKeys) < len ? (int)(upto * kStepKeys) : len;
+        int64_t row0[2];
+        f32x4 ks[2], vs[2];
+        auto scales = [&] {
+            if constexpr (F8) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int64_t at_row = row0[j] < 0 ? row0[0] : row0[j];
+                    ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + at_row + 4 * g);
+                    vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + at_row + 4 * g);
+                }
+            }
+        };
         const int limit_min = len - (int)a.rows;
         int odd_at = -1;  // the wavefront's keys from here on are left to the end: only the sequence's last step can be such
         f32x4 o[kDims][NR];
@@ -237,131 +232,145 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             for (int d = 0; d < kDims; ++d) o[d][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        for (int k0 = first; k0 < behind; k0 += kStepKeys) {
-            const int next = k0 + kStepKeys;
-            const bool more = next < behind;
-            f32x4 s[2][NR];
-            wait_copies<2 * kCopies>();  // the keys are there, the values' copies may be under way
-            {
-                uint32_t at_k = k_at;
-                asm volatile("" : "+v"(at_k));
+        if (first < behind) {
+            row0[0] = find(first), row0[1] = find(first + 16);
+            copy(a.cache.k, row0, first, kl, false);
+            scales();
+            copy(a.cache.v, row0, first, vl, true);
+            // waited for here, so that no wait inside the loop is for them
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) s[j][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[n][s]));
+            int k0 = first;
+            do {
+                const int next = k0 + kStepKeys;
+                const bool more = next < behind;
+                f32x4 s[2][NR];
+                int64_t row_next[2] = {0, 0};
+                if (more) row_next[0] = find(next), row_next[1] = find(next + 16);
+                wait_copies<2 * kCopies>();  // the keys are there, the values' copies may be under way
+                {
+                    uint32_t at_k = k_at;
+                    asm volatile("" : "+v"(at_k));
 #pragma unroll
-                    for (int i = 0; i < kSteps; i += F8 ? 2 : 1) {
-                        // chunk 4 i + g (of e4m3, two steps' dimensions)
-                        const int c = F8 ? i / 2 * 4 : i * 4;
-                        const u32x4 x = *reinterpret_cast<const u32x4 *>(kl + (at_k ^ (c % 16 * 16)) + c / 16 * 256 + j * 16 * kRow);
-                        if constexpr (F8) {
-                            const bf16x8 lo = f8_widen(x[0], x[1]), hi = f8_widen(x[2], x[3]);
+                    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                            for (int n = 0; n < NR; ++n) {
-                                s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, q[n][i], s[j][n], 0, 0, 0);
-                                s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, q[n][i + 1], s[j][n], 0, 0, 0);
+                        for (int n = 0; n < NR; ++n) s[j][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < kSteps; i += F8 ? 2 : 1) {
+                            // chunk 4 i + g (of e4m3, two steps' dimensions)
+                            const int c = F8 ? i / 2 * 4 : i * 4;
+                            const u32x4 x = *reinterpret_cast<const u32x4 *>(kl + (at_k ^ (c % 16 * 16)) + c / 16 * 256 + j * 16 * kRow);
+                            if constexpr (F8) {
+                                const bf16x8 lo = f8_widen(x[0], x[1]), hi = f8_widen(x[2], x[3]);
+#pragma unroll
+                                for (int n = 0; n < NR; ++n) {
+                                    s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, q[n][i], s[j][n], 0, 0, 0);
+                                    s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, q[n][i + 1], s[j][n], 0, 0, 0);
+                                }
+                            } else {
+#pragma unroll
+                                for (int n = 0; n < NR; ++n)
+                                    s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), q[n][i], s[j][n], 0, 0, 0);
                             }
-                        } else {
-#pragma unroll
-                            for (int n = 0; n < NR; ++n)
-                                s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), q[n][i], s[j][n], 0, 0, 0);
                         }
                     }
                 }
-            }
-            f32x4 vscale[2];
+                f32x4 vscale[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if constexpr (F8) {
-                    vscale[j] = vs[j];
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (F8) {
+                        vscale[j] = vs[j];
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) s[j][n] *= ks[j];
-                }
-            }
-            reads_done();
-            if (more) {
-                row0[0] = find(next), row0[1] = find(next + 16);
-                copy(a.cache.k, row0, next, kl, false);
-                scales();
-            }
-            const bool partly = k0 + kWaveKeys - 1 > limit_min;  // some row does not see all keys
-            bf16x8 w[NR];
-            bool grown = false;
-            float top[NR];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[j][n][i] *= p.scale_log2;
-                        if (partly && k0 + 16 * j + 4 * g + i > limit[n]) s[j][n][i] = -kInf;
+                        for (int n = 0; n < NR; ++n) s[j][n] *= ks[j];
                     }
-                top[n] = fmaxf(fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[0][n][2], s[0][n][3])),
-                               fmaxf(fmaxf(s[1][n][0], s[1][n][1]), fmaxf(s[1][n][2], s[1][n][3])));
-                top[n] = fmaxf(top[n], __shfl_xor(top[n], 16));
-                top[n] = fmaxf(top[n], __shfl_xor(top[n], 32));
-                grown |= top[n] > m[n] + kSlack;
-            }
-            if (__any(grown)) {
+                }
+                reads_done();
+                if (more) {
+                    row0[0] = row_next[0], row0[1] = row_next[1];
+                    copy(a.cache.k, row0, next, kl, false);
+                    scales();
+                }
+                const bool partly = k0 + kWaveKeys - 1 > limit_min;  // some row does not see all keys
+                bf16x8 w[NR];
+                bool grown = false;
+                float top[NR];
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    const float m_new = fmaxf(m[n], top[n]), keep = m_new == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - m_new);
-                    m[n] = m_new;
-                    sum[n] *= keep;
 #pragma unroll
-                    for (int d = 0; d < kDims; ++d) o[d][n] *= keep;
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s[j][n][i] *= p.scale_log2;
+                            if (partly && k0 + 16 * j + 4 * g + i > limit[n]) s[j][n][i] = -kInf;
+                        }
+                    top[n] = fmaxf(fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[0][n][2], s[0][n][3])),
+                                   fmaxf(fmaxf(s[1][n][0], s[1][n][1]), fmaxf(s[1][n][2], s[1][n][3])));
+                    top[n] = other_half_max(other_row_max(top[n]));
+                    grown |= top[n] > m[n] + kSlack;
                 }
-            }
+                if (__any(grown)) {
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                const float m_use = m[n] == -kInf ? 0.0f : m[n];
+                    for (int n = 0; n < NR; ++n) {
+                        const float m_new = fmaxf(m[n], top[n]), keep = m_new == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - m_new);
+                        m[n] = m_new;
+                        sum[n] *= keep;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(s[e / 4][n][e % 4] - m_use);
-                    sum[n] += x;
-                    if constexpr (F8) w[n][e] = (__bf16)(partly && k0 + 16 * (e / 4) + 4 * g + e % 4 > limit[n] ? 0.0f : x * vscale[e / 4][e % 4]);
-                    else w[n][e] = (__bf16)x;
-                }
-            }
-            // the values are there; the next keys' copies (and scales) may be under way
-            if (more) wait_copies<2 * kCopies>();
-            else wait_copies<0>();
-            if (partly && a.rows > 1) {
-                uint32_t any = 0;
-#pragma unroll
-                for (int i = 0; i < kTile / 1024; ++i) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(vl + i * 1024 + l * 16);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        // e4m3: all but the sign set; bf16: the exponent's carry
-                        if constexpr (F8) any |= ((x[e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                        else any |= ((x[e] & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
+                        for (int d = 0; d < kDims; ++d) o[d][n] *= keep;
                     }
                 }
-                if (__any(any != 0)) odd_at = k0;
-            }
-            if (odd_at != k0) {
-                uint32_t at_v = v_at, at_v2 = v_at2;
-                asm volatile("" : "+v"(at_v), "+v"(at_v2));
 #pragma unroll
-                for (int d = 0; d < kDims; ++d) {
-                    bf16x8 v;
-                    if constexpr (F8) {
-                        const int c = d;
-                        const auto x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(vl + (at_v ^ (c * 16))));
-                        v = f8_widen((uint32_t)x[0], (uint32_t)x[1]);
-                    } else {
-                        const int c = d * 2;
-                        const uint2 x = read_transposed(vl + (at_v ^ (c % 16 * 16)) + c / 16 * 256), y = read_transposed(vl + (at_v2 ^ (c % 16 * 16)) + c / 16 * 256);
-                        v = __builtin_bit_cast(bf16x8, u32x4{x.x, x.y, y.x, y.y});
+                for (int n = 0; n < NR; ++n) {
+                    const float m_use = m[n] == -kInf ? 0.0f : m[n];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = __builtin_amdgcn_exp2f(s[e / 4][n][e % 4] - m_use);
+                        sum[n] += x;
+                        if constexpr (F8) w[n][e] = (__bf16)(partly && k0 + 16 * (e / 4) + 4 * g + e % 4 > limit[n] ? 0.0f : x * vscale[e / 4][e % 4]);
+                        else w[n][e] = (__bf16)x;
                     }
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[n], o[d][n], 0, 0, 0);
                 }
-            }
-            reads_done();
-            if (more) copy(a.cache.v, row0, next, vl, true);
+                // the values are there; the next keys' copies (and scales) may be under way
+                if (more) wait_copies<2 * kCopies + (F8 ? 4 : 0)>();
+                else wait_copies<0>();
+                if (partly && a.rows > 1) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < kTile / 1024; ++i) {
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(vl + i * 1024 + l * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            // e4m3: all but the sign set; bf16: the exponent's carry
+                            if constexpr (F8) any |= ((x[e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                            else any |= ((x[e] & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
+                        }
+                    }
+                    if (__any(any != 0)) odd_at = k0;
+                }
+                if (odd_at != k0) {
+                    uint32_t at_v = v_at, at_v2 = v_at2;
+                    asm volatile("" : "+v"(at_v), "+v"(at_v2));
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d) {
+                        bf16x8 v;
+                        if constexpr (F8) {
+                            const int c = d;
+                            const auto x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(vl + (at_v ^ (c * 16))));
+                            v = f8_widen((uint32_t)x[0], (uint32_t)x[1]);
+                        } else {
+                            const int c = d * 2;
+                            const uint2 x = read_transposed(vl + (at_v ^ (c % 16 * 16)) + c / 16 * 256), y = read_transposed(vl + (at_v2 ^ (c % 16 * 16)) + c / 16 * 256);
+                            v = __builtin_bit_cast(bf16x8, u32x4{x.x, x.y, y.x, y.y});
+                        }
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[n], o[d][n], 0, 0, 0);
+                    }
+                }
+                reads_done();
+                if (more) copy(a.cache.v, row0, next, vl, true);
+                k0 = next;
+            } while (k0 < behind);
         }
         // Infinities or NaN that only some rows see: key by key.
         if (odd_at >= 0) {
@@ -413,8 +422,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
         }
 
         // join the wavefronts
+        const int here_l = here(l), here_r = here_l % 16, here_g = here_l / 16;
         if (__any(poison)) {
-            if (a.status && l == 0) *a.status = TQF_HIP_ERR_INVALID;
+            if (a.status && here_l == 0) *a.status = TQF_HIP_ERR_INVALID;
             poison = true;
         }
 #pragma unroll
@@ -422,9 +432,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             sum[n] += __shfl_xor(sum[n], 16);
             sum[n] += __shfl_xor(sum[n], 32);
             if (poison) sum[n] = __builtin_nanf("");
-            if (g == 0) {
-                s_m[wave][n * 16 + r] = m[n];
-                s_l[wave][n * 16 + r] = sum[n];
+            if (here_g == 0) {
+                s_m[wave][n * 16 + here_r] = m[n];
+                s_l[wave][n * 16 + here_r] = sum[n];
             }
         }
         __syncthreads();
@@ -432,7 +442,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
         float *to = p.partial + ((size_t)(2 * part + (at == begin ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            const int row = n * 16 + r;
+            const int row = n * 16 + here_r;
             float top = s_m[0][row], mine = 0.0f;
 #pragma unroll
             for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][row]);
@@ -440,22 +450,22 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             // [row][chunk of 4 at chunk ^ row] f32
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
-                const int c = d * 4 + g;
-                *reinterpret_cast<f32x4 *>(s_v[wave] + r * D * 4 + (c ^ r) * 16) = o[d][n] * mine;
+                const int c = d * 4 + here_g;
+                *reinterpret_cast<f32x4 *>(s_v[wave] + here_r * D * 4 + (c ^ here_r) * 16) = o[d][n] * mine;
             }
             __syncthreads();
 #pragma unroll
-            for (int i = tid; i < 16 * kChunks * 2; i += 64 * kWaves) {
-                const int rr = i / (2 * kChunks), c = i % (2 * kChunks), of_block = n * 16 + rr;
+            for (int x = 0; x < 16 * kChunks * 2; x += 64 * kWaves) {
+                const int i = x + wave * 64 + here_l, rr = i / (2 * kChunks), c = i % (2 * kChunks), of_block = n * 16 + rr;
                 f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
                 float all = s_m[0][of_block], total_l = 0.0f;
 #pragma unroll
-                for (int x = 1; x < kWaves; ++x) all = fmaxf(all, s_m[x][of_block]);
+                for (int u = 1; u < kWaves; ++u) all = fmaxf(all, s_m[u][of_block]);
 #pragma unroll
-                for (int x = 0; x < kWaves; ++x) {
-                    v += *reinterpret_cast<const f32x4 *>(s_v[x] + rr * D * 4 + (c ^ rr) * 16);
+                for (int u = 0; u < kWaves; ++u) {
+                    v += *reinterpret_cast<const f32x4 *>(s_v[u] + rr * D * 4 + (c ^ rr) * 16);
                     // a wavefront without keys has sum 0, or NaN where its sequence or a page is bad
-                    total_l += s_m[x][of_block] == -kInf ? s_l[x][of_block] : s_l[x][of_block] * __builtin_amdgcn_exp2f(s_m[x][of_block] - all);
+                    total_l += s_m[u][of_block] == -kInf ? s_l[u][of_block] : s_l[u][of_block] * __builtin_amdgcn_exp2f(s_m[u][of_block] - all);
                 }
                 const uint32_t out_row = block * kRows + of_block;
                 if (whole) {
@@ -548,13 +558,14 @@ uint32_t row_blocks(const PagedArgs &a) {
     const uint32_t rows = a.rows * (a.q_heads / a.cache.kv_heads), per = 16 * tiles_of_rows(a);
     return (rows + per - 1) / per;
 }
-// Two workgroups of a compute unit; no more than there can be steps.
+// As many workgroups as compute units hold at once (one of heads of 256, by its LDS, else
+// two); no more than there can be steps.
 uint32_t parts_of(const PagedArgs &a) {
     int device = 0, cus = 0;
     (void)hipGetDevice(&device);
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
     const uint64_t most = (uint64_t)a.n_seqs * a.cache.kv_heads * (((uint64_t)a.max_pages * a.cache.page + kStepKeys - 1) / kStepKeys);
-    const uint64_t want = 2 * (uint64_t)(cus > 0 ? cus : 256) / (row_blocks(a) < 2 ? 1 : 2);
+    const uint64_t want = (uint64_t)(a.cache.dim == 256 ? 1 : 2) * (uint64_t)(cus > 0 ? cus : 256);
     return (uint32_t)(most < want ? most : want);
 }
 

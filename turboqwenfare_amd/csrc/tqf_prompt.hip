@@ -31,12 +31,6 @@ namespace tqf {
 namespace {
 
 constexpr int kWaves = 4;
-// The larger of lanes l and l ^ 32.
-__device__ __forceinline__ float other_half_max(float x) {
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-}
-
 struct Kernel {
     PromptArgs a;
     uint32_t head_waves;  // wavefronts of a workgroup that have heads of their own (of one group)
@@ -134,33 +128,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.v.d) + (size_t)k0 * a.v.row + (size_t)kv * a.v.head);
     const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2;
 
-    // Where the lane's operands are in a tile: chunk 2 i + half of key r (+ 32), and, transposed, dimensions
-    // 32 d + l % 32 of the keys that its half's weights have.  The swizzles depend on the lane alone, so that
-    // few addresses serve all and the rest is constant.
-    constexpr int kKAt = kSteps < 8 ? kSteps : 8, kVAt = kDims < 4 ? kDims : 4;
-    uint32_t k_at[kKAt], v_at[kVAt];
-#pragma unroll
-    for (int i = 0; i < kKAt; ++i) k_at[i] = r * kRow + ((i * 2 + half) ^ k_swizzle<D>(r)) * 16;
-    {
-        const int g = l / 16, i16 = l % 16;
-        const uint32_t r0 = 4 * half + i16 / 4;
-#pragma unroll
-        for (int d = 0; d < kVAt; ++d) v_at[d] = r0 * kRow + ((d * 4 + 2 * (g % 2) + i16 % 4 / 2) ^ v_swizzle<D>(r0)) * 16 + i16 % 2 * 8;
-    }
+    // Where the lane's operands are in a tile: chunk half of key r, and, transposed, dimensions l % 32 of the first keys
+    // that its half's weights have.  Other chunks and dimensions are these with bits flipped (the swizzles depend on the
+    // lane alone), other keys a constant further; so few registers hold addresses.
+    const uint32_t k_at = r * kRow + (half ^ k_swizzle<D>(r)) * 16;
+    const uint32_t v_row0 = 4 * half + l % 16 / 4, v_at = v_row0 * kRow + ((2 * (l / 16 % 2) + l % 4 / 2) ^ v_swizzle<D>(v_row0)) * 16 + l % 2 * 8;
 
     auto copy = [&](int kt, uint8_t *to_k, uint8_t *to_v) {
         const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
         const Desc dk = make_desc(kp + (size_t)kt * KT * k_row, (rows - 1) * k_row + kRow);
         const Desc dv = make_desc(vp + (size_t)kt * KT * v_row, (rows - 1) * v_row + kRow);
+        const uint32_t lane = here(l);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const uint32_t base = (wave * kCopies + i) * 1024, byte = base + l * 16, rr = byte / kRow, c = byte % kRow / 16;
+            const uint32_t base = (wave * kCopies + i) * 1024, byte = base + lane * 16, rr = byte / kRow, c = byte % kRow / 16;
             copy16(dk, rr * k_row + (c ^ k_swizzle<D>(rr)) * 16, to_k + base);
             copy16(dv, rr * v_row + (c ^ v_swizzle<D>(rr)) * 16, to_v + base);
         }
     };
-    auto values = [&](const uint8_t *sv, int j, int st, int d) {
-        const uint8_t *at_v = sv + v_at[d % kVAt] + (d / kVAt * 256 + (j * 32 + st * 16) * kRow);
+    auto values = [&](const uint8_t *sv, uint32_t v0, int j, int st, int d) {
+        const uint8_t *at_v = sv + (v0 ^ (d % 4 * 64)) + (d / 4 * 256 + (j * 32 + st * 16) * kRow);
         const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 8 * kRow);
         return u32x4{x.x, x.y, y.x, y.y};
     };
@@ -169,12 +156,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         constexpr bool EDGE = decltype(edge)::value;
         const bool part = EDGE && kt * KT + KT - 1 > limit_min;  // some row of the wavefront
         f32x16 s[kSub];
+        const uint32_t k0_at = here(k_at);
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
             f32x16 acc = {};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                const bf16x8 k = *reinterpret_cast<const bf16x8 *>(sk + k_at[i % kKAt] + (i / kKAt * 256 + j * 32 * kRow));
+                const bf16x8 k = *reinterpret_cast<const bf16x8 *>(sk + (k0_at ^ (i % 8 * 32)) + (i / 8 * 256 + j * 32 * kRow));
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i], acc, 0, 0, 0);
             }
             s[j] = acc;
@@ -224,13 +212,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
                 return;
             }
         }
+        const uint32_t v0_at = here(v_at);
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
             for (int j = 0; j < kSub; ++j)
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(sv, j, st, d)), w[j][st], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(sv, v0_at, j, st, d)), w[j][st], o[d], 0, 0, 0);
     };
 
     // Two stages of LDS, each a variable of its own: the next tile's copies are under way while one is computed.

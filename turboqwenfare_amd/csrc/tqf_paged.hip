@@ -40,10 +40,19 @@ __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0
 
 constexpr int kWaves = 4, kWaveKeys = 32, kStepKeys = kWaves * kWaveKeys;
 
+// What the join needs to know of a (sequence, key head) that several parts have: kept
+// by the part after the first.  The first part has it from its own beginning on or
+// behind others.
+struct Cut {
+    uint32_t seq, kv, first, parts;  // parts 0: none is cut here first; kBehind: the first part begins with others
+};
+constexpr uint32_t kBehind = 1u << 31;
+
 struct Kernel {
     PagedArgs a;
     uint32_t group, row_blocks, parts, page_shift;  // parts: workgroups of a row block
     float scale_log2;
+    Cut *cuts;       // [parts]
     float *partial;  // [2 parts][row_blocks][rows of a block][dim + 2]: values, maximum, sum
 };
 
@@ -58,41 +67,61 @@ __device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
 // (the caller has checked the most there can be).  All results are the same in
 // every lane, and the compiler is told so: descriptors made of them stay scalar.
 struct Line {
+    uint32_t mine, upto;  // of sequence `lane`: steps of a key head; steps of all heads of the sequences up to it
+    uint32_t total;
+};
+__device__ __forceinline__ uint32_t steps_up_to(uint32_t mine) {
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t v = __shfl_up(upto, o);
+        if ((int)(threadIdx.x & 63) >= o) upto += v;
+    }
+    return upto;
+}
+__device__ __forceinline__ Line line_of(const PagedArgs &a) {
+    const uint32_t l = threadIdx.x & 63;
+    Line line;
+    line.mine = l < a.n_seqs ? steps_of(a, a.lens[l]) : 0;
+    uint32_t rest = 0;
+    for (uint32_t s = l + 64; s < a.n_seqs; s += 64) rest += steps_of(a, a.lens[s]);
+    line.upto = steps_up_to(line.mine * a.cache.kv_heads);
+    line.total = __builtin_amdgcn_readlane(line.upto, 63);
+    if (a.n_seqs > 64) {
+#pragma unroll
+        for (int o = 32; o >= 1; o /= 2) rest += __shfl_xor(rest, o);
+        line.total += __builtin_amdgcn_readfirstlane(rest) * a.cache.kv_heads;
+    }
+    return line;
+}
+struct Place {
     uint32_t seq, steps, first;  // a sequence, its steps for a key head, its first step
 };
-__device__ __forceinline__ uint32_t line_total(const PagedArgs &a) {
+__device__ __forceinline__ Place place_of(const PagedArgs &a, const Line &line, uint32_t step) {
     const uint32_t l = threadIdx.x & 63;
-    uint32_t sum = 0;
-    for (uint32_t s = l; s < a.n_seqs; s += 64) sum += steps_of(a, a.lens[s]);
-#pragma unroll
-    for (int o = 32; o >= 1; o /= 2) sum += __shfl_xor(sum, o);
-    return __builtin_amdgcn_readfirstlane(sum * a.cache.kv_heads);
-}
-__device__ __forceinline__ Line line_find(const PagedArgs &a, uint32_t step) {
-    const uint32_t l = threadIdx.x & 63;
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64) {
-        const uint32_t s = s0 + l, mine = s < a.n_seqs ? steps_of(a, a.lens[s]) : 0;
-        uint32_t upto = mine * a.cache.kv_heads;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t v = __shfl_up(upto, o);
-            if ((int)l >= o) upto += v;
-        }
+    uint32_t before = 0, mine = line.mine, upto = line.upto;
+    for (uint32_t s0 = 0;;) {
         const uint64_t past = __ballot(before + upto > step);
         if (past) {
             const int who = __builtin_ctzll(past);
             const uint32_t n = __builtin_amdgcn_readlane(mine, who);
-            return Line{s0 + who, n, before + __builtin_amdgcn_readlane(upto, who) - n * a.cache.kv_heads};
+            return Place{s0 + who, n, before + __builtin_amdgcn_readlane(upto, who) - n * a.cache.kv_heads};
         }
         before += __builtin_amdgcn_readlane(upto, 63);
+        s0 += 64;
+        if (s0 >= a.n_seqs) return Place{a.n_seqs, 1, 0};  // no such step
+        mine = s0 + l < a.n_seqs ? steps_of(a, a.lens[s0 + l]) : 0;
+        upto = steps_up_to(mine * a.cache.kv_heads);
     }
-    return Line{a.n_seqs, 1, 0};  // no such step
 }
 // Equal parts, the first ones a step longer.
 __device__ __forceinline__ uint32_t part_begin(uint32_t total, uint32_t part, uint32_t parts) {
     const uint32_t each = total / parts, more = total % parts;
     return part * each + (part < more ? part : more);
+}
+__device__ __forceinline__ uint32_t part_of(uint32_t total, uint32_t step, uint32_t parts) {
+    const uint32_t each = total / parts, more = total % parts, longer = more * (each + 1);
+    return step < longer ? step / (each + 1) : more + (step - longer) / (each ? each : 1);
 }
 
 __device__ __forceinline__ void four_bf16(const uint16_t *p, float (&v)[4]) {
@@ -134,9 +163,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 16, g = l / 16;
     const uint32_t part = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
-    const uint32_t total = line_total(a);
-    uint32_t at = part_begin(total, part, p.parts);
-    const uint32_t begin = at, end = part_begin(total, part + 1, p.parts);
+    const Line line = line_of(a);
+    const uint32_t total = line.total, begin = part_begin(total, part, p.parts), end = part_begin(total, part + 1, p.parts);
     const uint32_t all_rows = a.rows * p.group;
     const size_t page_size = a.cache.page;
     uint8_t *const kl = s_k[wave], *const vl = s_v[wave];
@@ -154,72 +182,102 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
         v_at2 = v_at + 16 * kRow;  // the swizzle of row + 16 is that of the row
     }
 
-    while (at < end) {
-        const Line line = line_find(a, at);
-        if (line.seq >= a.n_seqs) return;
-        const uint32_t seq = line.seq, steps = line.steps, kv = __builtin_amdgcn_readfirstlane((at - line.first) / steps), from = at - line.first - kv * steps;
-        const uint32_t upto = steps - from < end - at ? steps : from + (end - at);
-        int32_t len = ((const constant_i32 *)(uintptr_t)a.lens)[seq];
-        bool poison = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * page_size;
-        if (poison) {
-            if (a.status) *a.status = TQF_HIP_ERR_INVALID;
-            len = 0;
-        }
-        const constant_i32 *table = (const constant_i32 *)(uintptr_t)(a.pages + (size_t)seq * a.max_pages);
+    Cut *const cut = block == 0 && tid == 0 && part > 0 ? p.cuts + part : nullptr;
+    if (begin >= end) {
+        if (cut) cut->parts = 0;
+        return;
+    }
+    const Place place = place_of(a, line, begin);
+    if (place.seq >= a.n_seqs) {
+        if (cut) cut->parts = 0;
+        return;
+    }
+    uint32_t seq = place.seq, steps = place.steps, kv = __builtin_amdgcn_readfirstlane((begin - place.first) / steps);
+    uint32_t from = begin - place.first - kv * steps, at = begin;
+    if (cut) {
+        const uint32_t unit = begin - from, before = part_begin(total, part - 1, p.parts);
+        const bool here_first = from > 0 && before <= unit;
+        const uint32_t n = here_first ? part_of(total, unit + steps - 1, p.parts) - part + 2 : 0;
+        *cut = Cut{seq, kv, part - 1, n | (before < unit ? kBehind : 0)};
+    }
 
-        // the first of 16 keys in the cache; keys behind the end: -1
-        auto find = [&](int key) -> int64_t {
-            if (key >= len) return -1;
-            int32_t page = table[__builtin_amdgcn_readfirstlane((uint32_t)key >> p.page_shift)];
-            if (page < 0 || (uint32_t)page >= a.cache.n_pages) {
-                poison = true;
-                page = 0;
+    int32_t len = 0;
+    bool poison = false;
+    const constant_i32 *table = nullptr;
+    int first = 0, behind = 0;  // the wavefront's first key, and the end of the workgroup's
+    int64_t row0[2] = {0, 0};
+    f32x4 ks[2], vs[2];
+    bf16x8 q[NR][kSteps];
+    int limit[NR];
+
+    // the first of 16 keys in the cache; keys behind the end: -1
+    auto find = [&](int key) -> int64_t {
+        if (key >= len) return -1;
+        int32_t page = table[__builtin_amdgcn_readfirstlane((uint32_t)key >> p.page_shift)];
+        if (page < 0 || (uint32_t)page >= a.cache.n_pages) {
+            poison = true;
+            page = 0;
+        }
+        return (int64_t)(((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1)));
+    };
+    // copies of 32 keys' rows; those behind the end are zero
+    auto copy = [&](const void *from_cache, const int64_t (&row0)[2], int k0, uint8_t *to, bool values) {
+        uint32_t lane = l;
+        asm volatile("" : "+v"(lane));  // offsets are computed where they are used: they would take registers all along
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int left = len - k0 - 16 * j, rows = left < 0 ? 0 : left < 16 ? left : 16;
+            const Desc d = make_desc(static_cast<const uint8_t *>(from_cache) + (row0[j] < 0 ? 0 : (size_t)row0[j]) * kRow, rows * kRow);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const uint32_t byte = i * 1024 + lane * 16, rr = byte / kRow, c = byte % kRow / 16;
+                const uint32_t sw = values ? v_swizzle<kRow, F8>(16 * j + rr) : k_swizzle<kRow>(rr);
+                copy16(d, rr * kRow + (c ^ sw) * 16, to + j * 16 * kRow + i * 1024);
             }
-            return (int64_t)(((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1)));
-        };
-        // copies of 32 keys' rows; those behind the end are zero
-        auto copy = [&](const void *from_cache, const int64_t (&row0)[2], int k0, uint8_t *to, bool values) {
-            uint32_t lane = l;
-            asm volatile("" : "+v"(lane));  // offsets are computed where they are used: they would take registers all along
+        }
+    };
+    auto scales = [&] {
+        if constexpr (F8) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int left = len - k0 - 16 * j, rows = left < 0 ? 0 : left < 16 ? left : 16;
-                const Desc d = make_desc(static_cast<const uint8_t *>(from_cache) + (row0[j] < 0 ? 0 : (size_t)row0[j]) * kRow, rows * kRow);
-#pragma unroll
-                for (int i = 0; i < kCopies; ++i) {
-                    const uint32_t byte = i * 1024 + lane * 16, rr = byte / kRow, c = byte % kRow / 16;
-                    const uint32_t sw = values ? v_swizzle<kRow, F8>(16 * j + rr) : k_swizzle<kRow>(rr);
-                    copy16(d, rr * kRow + (c ^ sw) * 16, to + j * 16 * kRow + i * 1024);
-                }
+                const int64_t at_row = row0[j] < 0 ? row0[0] : row0[j];
+                ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + at_row + 4 * g);
+                vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + at_row + 4 * g);
             }
-        };
-        // the rows: column r of tile n is row block * kRows + 16 n + r, of query row / group and head row % group
-        bf16x8 q[NR][kSteps];
-        int limit[NR];
+        }
+    };
+    // Asks for the rows and the first keys of steps from..upto of (seq, kv).
+    uint32_t upto = 0;
+    auto ask = [&] {
+        upto = steps - from < end - at ? steps : from + (end - at);
+        len = ((const constant_i32 *)(uintptr_t)a.lens)[seq];
+        poison = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * page_size;
+        if (poison) len = 0;
+        table = (const constant_i32 *)(uintptr_t)(a.pages + (size_t)seq * a.max_pages);
+        first = (int)(from * kStepKeys) + wave * kWaveKeys;
+        behind = (int)(upto * kStepKeys) < len ? (int)(upto * kStepKeys) : len;
+        // column r of tile n is row block * kRows + 16 n + r, of query row / group and head row % group
+        const uint32_t here_r = here(r), here_g = here(g);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            uint32_t row = block * kRows + n * 16 + r;
+            uint32_t row = block * kRows + n * 16 + here_r;
             if (row >= all_rows) row = all_rows - 1;
             const uint32_t i = row / p.group, head = kv * p.group + row % p.group;
             limit[n] = len - (int)a.rows + (int)i;
             const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + ((size_t)seq * a.rows + i) * a.q.row + (size_t)head * a.q.head;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
-                q[n][s] = *reinterpret_cast<const bf16x8 *>(qp + (F8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8));
+                q[n][s] = *reinterpret_cast<const bf16x8 *>(qp + (F8 ? s / 2 * 64 + here_g * 16 + s % 2 * 8 : s * 32 + here_g * 8));
         }
-        const int first = (int)(from * kStepKeys) + wave * kWaveKeys, behind = (int)(upto * kStepKeys) < len ? (int)(upto * kStepKeys) : len;
-        int64_t row0[2];
-        f32x4 ks[2], vs[2];
-        auto scales = [&] {
-            if constexpr (F8) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int64_t at_row = row0[j] < 0 ? row0[0] : row0[j];
-                    ks[j] = *reinterpret_cast<const f32x4 *>(a.cache.k_scales + at_row + 4 * g);
-                    vs[j] = *reinterpret_cast<const f32x4 *>(a.cache.v_scales + at_row + 4 * g);
-                }
-            }
-        };
+        if (first < behind) {
+            row0[0] = find(first), row0[1] = find(first + 16);
+            copy(a.cache.k, row0, first, kl, false);
+            scales();
+        }
+    };
+
+    ask();
+    for (;;) {
         const int limit_min = len - (int)a.rows;
         int odd_at = -1;  // the wavefront's keys from here on are left to the end: only the sequence's last step can be such
         f32x4 o[kDims][NR];
@@ -233,11 +291,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
         }
 
         if (first < behind) {
-            row0[0] = find(first), row0[1] = find(first + 16);
-            copy(a.cache.k, row0, first, kl, false);
-            scales();
             copy(a.cache.v, row0, first, vl, true);
-            // waited for here, so that no wait inside the loop is for them
+            // the rows are waited for here, so that no wait inside the loop is for them
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -421,25 +476,31 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             }
         }
 
-        // join the wavefronts
-        const int here_l = here(l), here_r = here_l % 16, here_g = here_l / 16;
-        if (__any(poison)) {
-            if (a.status && here_l == 0) *a.status = TQF_HIP_ERR_INVALID;
-            poison = true;
+        // the next (sequence, key head) of the part is asked for before the wavefronts' shares of this one are joined
+        const uint32_t of_seq = seq, of_kv = kv;
+        const bool bad = __any(poison), whole = from == 0 && upto == steps, part_first = at == begin;
+        if (bad && a.status && tid % 64 == 0) *a.status = TQF_HIP_ERR_INVALID;
+        at += upto - from;
+        from = 0;
+        if (++kv == a.cache.kv_heads) kv = 0, ++seq;
+        const bool again = at < end && seq < a.n_seqs;
+        if (again) {
+            if (kv == 0) steps = steps_of(a, ((const constant_i32 *)(uintptr_t)a.lens)[seq]);
+            ask();
         }
+        const int here_l = here(l), here_r = here_l % 16, here_g = here_l / 16;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             sum[n] += __shfl_xor(sum[n], 16);
             sum[n] += __shfl_xor(sum[n], 32);
-            if (poison) sum[n] = __builtin_nanf("");
+            if (bad) sum[n] = __builtin_nanf("");
             if (here_g == 0) {
                 s_m[wave][n * 16 + here_r] = m[n];
                 s_l[wave][n * 16 + here_r] = sum[n];
             }
         }
         __syncthreads();
-        const bool whole = from == 0 && upto == steps;
-        float *to = p.partial + ((size_t)(2 * part + (at == begin ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2);
+        float *to = p.partial + ((size_t)(2 * part + (part_first ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const int row = n * 16 + here_r;
@@ -471,7 +532,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
                 if (whole) {
                     if (out_row < all_rows) {
                         const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-                        const size_t token = (size_t)seq * a.rows + out_row / p.group, head = kv * p.group + out_row % p.group;
+                        const size_t token = (size_t)of_seq * a.rows + out_row / p.group, head = (size_t)of_kv * p.group + out_row % p.group;
                         v *= inv;
                         if (a.gate.d) {
                             const uint16_t *gp = static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head + c * 4;
@@ -491,65 +552,98 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             }
             __syncthreads();
         }
-        at += upto - from;
+        if (!again) break;
     }
 }
 
-// Joins what several workgroups have of one (sequence, key head).  A workgroup takes
-// a row of the unit that the boundary at the beginning of its part cuts first; its
-// wavefronts take the parts in turn.
-constexpr int kJoinWaves = 8;
-template <int D, int NR>
-__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p) {
-    constexpr int kRows = 16 * NR;
+// Joins what several parts have of one (sequence, key head): a workgroup for each
+// part's beginning, if one is cut there first, and `each` rows.  Of few parts a
+// wavefront has a row; of many it has some for every row in turn.
+constexpr int kJoinWaves = 8, kJoinAhead = 4;
+template <int D>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_t block_rows, uint32_t each) {
+    constexpr int kPer = D / 64;
     __shared__ float s_o[kJoinWaves][D], s_m[kJoinWaves], s_l[kJoinWaves];
     const PagedArgs &a = p.a;
-    const int tid = threadIdx.x, wave = tid / 64, l = tid % 64;
-    const uint32_t all_rows = a.rows * p.group, part = blockIdx.x / all_rows + 1, row = blockIdx.x % all_rows;
-    const uint32_t total = line_total(a), cut = part_begin(total, part, p.parts);
-    if (cut == 0 || cut >= total) return;
-    const Line line = line_find(a, cut);
-    if (line.seq >= a.n_seqs) return;
-    const uint32_t kv = (cut - line.first) / line.steps, begin = line.first + kv * line.steps, end = begin + line.steps;
-    if (cut == begin || part_begin(total, part - 1, p.parts) > begin) return;  // no unit is cut here, or not here first
-    const uint32_t block = row / kRows, of_block = row % kRows;
-    // part - 1 (from `begin` on, or before it) to the last part that begins before `end`
-    float m = -kInf, sum = 0.0f, o[D / 64] = {};
-    for (uint32_t i = part - 1 + wave; i < p.parts; i += kJoinWaves) {
-        const uint32_t b = part_begin(total, i, p.parts);
-        if (b >= end) break;
-        if (part_begin(total, i + 1, p.parts) == b) continue;  // an empty part
-        const float *from = p.partial + ((size_t)(2 * i + (b >= begin ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2) + (size_t)of_block * (D + 2);
-        const float pm = from[D], pl = from[D + 1], top = fmaxf(m, pm);
-        const float keep = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top), take = pm == -kInf ? 0.0f : __builtin_amdgcn_exp2f(pm - top);
-        m = top;
-        sum = sum * (sum != sum ? 1.0f : keep) + (pl != pl ? pl : pl * take);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
+    const uint32_t all_rows = a.rows * p.group, sets = (all_rows + each - 1) / each;
+    const Cut cut = p.cuts[blockIdx.x / sets + 1];
+    const uint32_t parts = cut.parts & ~kBehind, row0 = blockIdx.x % sets * each;
+    if (parts == 0) return;
+    const size_t stride = (size_t)2 * p.row_blocks * block_rows * (D + 2);  // of a part
+    float m, sum, o[kPer];
+    // parts `begin`, begin + step, ... of a row
+    auto gather = [&](uint32_t row, uint32_t begin, uint32_t step) {
+        m = -kInf, sum = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 64; ++d) o[d] = o[d] * keep + from[d * 64 + l] * take;
-    }
+        for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
+        for (uint32_t i = begin; i < parts; i += kJoinAhead * step) {
+            float pm[kJoinAhead], pl[kJoinAhead], po[kJoinAhead][kPer];
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) s_o[wave][d * 64 + l] = o[d];
-    if (l == 0) {
-        s_m[wave] = m;
-        s_l[wave] = sum;
-    }
-    __syncthreads();
-    float top = -kInf, all = 0.0f;
+            for (int x = 0; x < kJoinAhead; ++x) {
+                const uint32_t at = i + x * step < parts ? i + x * step : parts - 1;
+                const size_t slot = at == 0 && (cut.parts & kBehind) ? 1 : 0;
+                const float *from = p.partial + (cut.first + at) * stride + ((slot * p.row_blocks + row / block_rows) * block_rows + row % block_rows) * (D + 2);
+                pm[x] = from[D], pl[x] = from[D + 1];
+                if constexpr (kPer == 1) po[x][0] = from[l];
+                else __builtin_memcpy(po[x], from + l * kPer, 4 * kPer);
+            }
 #pragma unroll
-    for (int i = 0; i < kJoinWaves; ++i) top = fmaxf(top, s_m[i]);
-    for (int d = tid; d < D; d += 64 * kJoinWaves) {
-        float v = 0.0f;
-        all = 0.0f;
+            for (int x = 0; x < kJoinAhead; ++x) {
+                if (i + x * step >= parts) break;
+                const float top = fmaxf(m, pm[x]), keep = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+                const float take = pm[x] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(pm[x] - top);
+                m = top;
+                // a part without keys has sum 0, or NaN where its sequence or a page is bad: NaN stays
+                sum = sum * (m == -kInf ? 1.0f : keep) + (pm[x] == -kInf ? pl[x] : pl[x] * take);
 #pragma unroll
-        for (int i = 0; i < kJoinWaves; ++i) {
-            const float f = s_m[i] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top);
-            all += s_l[i] != s_l[i] ? s_l[i] : s_l[i] * f;
-            v += s_o[i][d] * f;
+                for (int d = 0; d < kPer; ++d) o[d] = o[d] * keep + po[x][d] * take;
+            }
         }
-        v *= all == 0.0f ? 0.0f : 1.0f / all;
-        const size_t token = (size_t)line.seq * a.rows + row / p.group, head = (size_t)kv * p.group + row % p.group;
-        if (a.gate.d) v *= gate_of(static_cast<const uint16_t *>(a.gate.d)[token * a.gate.row + head * a.gate.head + d]);
-        a.y[(token * a.q_heads + head) * D + d] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    };
+    auto store = [&](uint32_t row) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const size_t token = (size_t)cut.seq * a.rows + row / p.group, head = (size_t)cut.kv * p.group + row % p.group;
+        const uint16_t *gate = a.gate.d ? static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head : nullptr;
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) {
+            const float v = o[d] * inv * (gate ? gate_of(gate[l * kPer + d]) : 1.0f);
+            a.y[(token * a.q_heads + head) * D + l * kPer + d] = __builtin_bit_cast(uint16_t, (__bf16)v);
+        }
+    };
+    if (parts <= kJoinWaves) {
+        for (uint32_t row = row0 + wave; row < row0 + each && row < all_rows; row += kJoinWaves) {
+            gather(row, 0, 1);
+            store(row);
+        }
+        return;
+    }
+    for (uint32_t row = row0; row < row0 + each && row < all_rows; ++row) {
+        gather(row, wave, kJoinWaves);
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) s_o[wave][l * kPer + d] = o[d];
+        if (l == 0) {
+            s_m[wave] = m;
+            s_l[wave] = sum;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            float top = -kInf;
+#pragma unroll
+            for (int i = 0; i < kJoinWaves; ++i) top = fmaxf(top, s_m[i]);
+            sum = 0.0f;
+#pragma unroll
+            for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kJoinWaves; ++i) {
+                const float f = s_m[i] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top);
+                sum += s_m[i] == -kInf ? s_l[i] : s_l[i] * f;
+#pragma unroll
+                for (int d = 0; d < kPer; ++d) o[d] += s_o[i][l * kPer + d] * f;
+            }
+            store(row);
+        }
+        __syncthreads();
     }
 }
 
@@ -569,6 +663,8 @@ uint32_t parts_of(const PagedArgs &a) {
     return (uint32_t)(most < want ? most : want);
 }
 
+size_t cuts_bytes(uint32_t parts) { return ((size_t)parts * sizeof(Cut) + 255) / 256 * 256; }
+
 template <int D, int NR>
 hipError_t launch_for(hipStream_t s, const Kernel &p) {
     const dim3 grid(p.parts * p.row_blocks), block(64 * kWaves);
@@ -576,7 +672,10 @@ hipError_t launch_for(hipStream_t s, const Kernel &p) {
     else paged_kernel<D, NR, false><<<grid, block, 0, s>>>(p);
     if (p.parts > 1) {
         if (const hipError_t e = hipGetLastError()) return e;
-        join_kernel<D, NR><<<dim3((p.parts - 1) * p.a.rows * p.group), dim3(64 * kJoinWaves), 0, s>>>(p);
+        // about two thousand workgroups at most: more would wait for one another's places
+        const uint32_t rows = p.a.rows * p.group, all = (p.parts - 1) * rows;
+        const uint32_t each = all <= 2048 ? 1 : all <= 4096 ? 2 : all <= 8192 ? 4 : 8;
+        join_kernel<D><<<dim3((p.parts - 1) * ((rows + each - 1) / each)), dim3(64 * kJoinWaves), 0, s>>>(p, 16 * NR, each);
     }
     return hipGetLastError();
 }
@@ -584,12 +683,13 @@ hipError_t launch_for(hipStream_t s, const Kernel &p) {
 }  // namespace
 
 size_t attn_paged_scratch_bytes(const PagedArgs &a) {
-    return (size_t)2 * parts_of(a) * row_blocks(a) * 16 * tiles_of_rows(a) * (a.cache.dim + 2) * 4;
+    return cuts_bytes(parts_of(a)) + (size_t)2 * parts_of(a) * row_blocks(a) * 16 * tiles_of_rows(a) * (a.cache.dim + 2) * 4;
 }
 
 hipError_t launch_attn_paged(hipStream_t s, const PagedArgs &a, void *scratch) {
     Kernel p{a, a.q_heads / a.cache.kv_heads, row_blocks(a), parts_of(a), (uint32_t)__builtin_ctz(a.cache.page), a.scale * kLog2e,
-             static_cast<float *>(scratch)};
+             static_cast<Cut *>(scratch), nullptr};
+    p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + cuts_bytes(p.parts));
     const bool two = tiles_of_rows(a) == 2;
     if (a.cache.dim == 64) return two ? launch_for<64, 2>(s, p) : launch_for<64, 1>(s, p);
     if (a.cache.dim == 128) return two ? launch_for<128, 2>(s, p) : launch_for<128, 1>(s, p);

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -121,7 +122,7 @@ class Rope:
     pairs: int
 
 
-@dataclass
+@dataclass(frozen=True)
 class KvCache:
     """A layer's paged cache: keys and values [n_pages, kv_heads, page_size, head_dim], "bf16" or "f8" (e4m3, with
     scales [n_pages, kv_heads, page_size])."""
@@ -135,10 +136,12 @@ class KvCache:
     d_k_scales: DeviceBuffer | None = None
     d_v_scales: DeviceBuffer | None = None
 
-    def as_struct(self) -> _lib.KvCache:
-        p = lambda b: b.ptr if b else None  # noqa: E731
-        return _lib.KvCache(p(self.d_k), p(self.d_v), p(self.d_k_scales), p(self.d_v_scales), _CACHE_TYPES[self.type],
-                            self.n_pages, self.page_size, self.kv_heads, self.head_dim)
+    @functools.cached_property
+    def ref(self):
+        """The ``tqf_hip_kv_cache`` that calls take."""
+        return C.byref(_lib.KvCache(self.d_k.ptr, self.d_v.ptr, self.d_k_scales.ptr if self.d_k_scales else None,
+                                    self.d_v_scales.ptr if self.d_v_scales else None, _CACHE_TYPES[self.type], self.n_pages,
+                                    self.page_size, self.kv_heads, self.head_dim))
 
 
 class MoeLayer:
@@ -719,14 +722,27 @@ class HipBackend:
             if b:
                 self.free(b)
 
-    @staticmethod
-    def _head_rows(what: str, buf: DeviceBuffer, t: int, heads: int, dim: int, strides, nbytes: int) -> _lib.HeadRows:
+    @functools.cached_property
+    def _places(self):
+        """The structs that a call's arguments are put in: a context has one call at a time."""
+        rows = [_lib.HeadRows() for _ in range(4)]
+        heads, options = _lib.Heads(), _lib.QkOptions()
+        return [(r, C.byref(r)) for r in rows], (heads, C.byref(heads)), (options, C.byref(options))
+
+    def _heads(self, heads):
+        s, ref = self._places[1]
+        s.q_heads, s.kv_heads, s.head_dim = heads
+        return ref
+
+    def _rows(self, place: int, what: str, buf: DeviceBuffer, t: int, heads: int, dim: int, strides, nbytes: int):
         row, head = strides if strides is not None else (heads * dim, dim)
         if row < 0 or head < 0:
             raise ValueError(f"{what}: strides must not be negative")
-        if t > 0:
-            _hold(what, (buf, ((t - 1) * row + (heads - 1) * head + dim) * nbytes))
-        return _lib.HeadRows(buf.ptr, row, head)
+        if t > 0 and ((t - 1) * row + (heads - 1) * head + dim) * nbytes > buf.nbytes:
+            raise ValueError(f"{what}: rows behind the end of a buffer of {buf.nbytes} bytes")
+        s, ref = self._places[0][place]
+        s.data, s.row_stride, s.head_stride = buf.ptr, row, head
+        return ref
 
     def qk_rope_device(self, d_q: DeviceBuffer, d_k: DeviceBuffer, d_v: DeviceBuffer, t: int, heads, d_positions: DeviceBuffer | None,
                        d_q_out: DeviceBuffer, d_k_out: DeviceBuffer | None = None, d_v_out: DeviceBuffer | None = None,
@@ -737,17 +753,21 @@ class HipBackend:
         """Norms and rotation of q and k heads; bf16 rows out, k and v into the cache (tqf_hip_qk_rope_device)."""
         if pairs not in _PAIRS:
             raise ValueError('pairs are "half" or "neighbours"')
-        xt, (nq, nk, dim) = _row_type(x_type), heads
-        size, what = _TYPE_BYTES[xt], "qk_rope_device"
-        rows = [self._head_rows(what, b, t, n, dim, s, size) for b, n, s in zip((d_q, d_k, d_v), (nq, nk, nk), strides)]
-        _hold(what, (d_q_out, 2 * t * nq * dim), *[(b, 2 * t * nk * dim) for b in (d_k_out, d_v_out) if b],
-              *[(b, 4 * t) for b in (d_positions, d_slots) if b])
-        p = lambda b: b.ptr if b else None  # noqa: E731
-        o = _lib.QkOptions(q_norm.handle if q_norm else None, k_norm.handle if k_norm else None, float(eps),
-                           rope.handle if rope else None, _PAIRS[pairs])
+        xt, what = _row_type(x_type), "qk_rope_device"
+        nq, nk, dim = heads
+        size, n = _TYPE_BYTES[xt], 2 * t * nk * dim
+        q, k, v = (self._rows(0, what, d_q, t, nq, dim, strides[0], size), self._rows(1, what, d_k, t, nk, dim, strides[1], size),
+                   self._rows(2, what, d_v, t, nk, dim, strides[2], size))
+        if (d_q_out.nbytes < 2 * t * nq * dim or (d_k_out and d_k_out.nbytes < n) or (d_v_out and d_v_out.nbytes < n)
+                or (d_positions and d_positions.nbytes < 4 * t) or (d_slots and d_slots.nbytes < 4 * t)):
+            raise ValueError(f"{what}: a buffer is too small for {t} rows")
+        o, options = self._places[2]
+        o.q_norm, o.k_norm, o.eps = q_norm.handle if q_norm else None, k_norm.handle if k_norm else None, eps
+        o.rope, o.neighbours = rope.handle if rope else None, _PAIRS[pairs]
         self._check(self.lib.tqf_hip_qk_rope_device(
-            self.ctx, C.byref(_lib.Heads(*heads)), C.byref(o), *[C.byref(r) for r in rows], xt, t, p(d_positions), d_q_out.ptr,
-            p(d_k_out), p(d_v_out), C.byref(cache.as_struct()) if cache else None, p(d_slots), p(d_status)))
+            self.ctx, self._heads(heads), options, q, k, v, xt, t, d_positions.ptr if d_positions else None, d_q_out.ptr,
+            d_k_out.ptr if d_k_out else None, d_v_out.ptr if d_v_out else None, cache.ref if cache else None,
+            d_slots.ptr if d_slots else None, d_status.ptr if d_status else None))
 
     def attn_prompt_device(self, d_q: DeviceBuffer, d_k: DeviceBuffer, d_v: DeviceBuffer, heads, d_cu_q: DeviceBuffer,
                            d_cu_k: DeviceBuffer, n_seqs: int, total_q: int, total_k: int, d_y: DeviceBuffer,
@@ -756,14 +776,14 @@ class HipBackend:
         """Causal attention of packed sequences, bf16 (tqf_hip_attn_prompt_device); scale: head_dim^-1/2 unless given."""
         nq, nk, dim = heads
         what = "attn_prompt_device"
-        q, k, v = [self._head_rows(what, b, n, h, dim, s, 2)
-                   for b, n, h, s in zip((d_q, d_k, d_v), (total_q, total_k, total_k), (nq, nk, nk), strides)]
-        gate = self._head_rows(what, d_gate, total_q, nq, dim, gate_strides, 2) if d_gate else None
-        _hold(what, (d_y, 2 * total_q * nq * dim), (d_cu_q, 4 * (n_seqs + 1)), (d_cu_k, 4 * (n_seqs + 1)))
+        q, k, v = (self._rows(0, what, d_q, total_q, nq, dim, strides[0], 2), self._rows(1, what, d_k, total_k, nk, dim, strides[1], 2),
+                   self._rows(2, what, d_v, total_k, nk, dim, strides[2], 2))
+        gate = self._rows(3, what, d_gate, total_q, nq, dim, gate_strides, 2) if d_gate else None
+        if d_y.nbytes < 2 * total_q * nq * dim or d_cu_q.nbytes < 4 * (n_seqs + 1) or d_cu_k.nbytes < 4 * (n_seqs + 1):
+            raise ValueError(f"{what}: a buffer is too small for {total_q} rows of {n_seqs} sequences")
         self._check(self.lib.tqf_hip_attn_prompt_device(
-            self.ctx, C.byref(_lib.Heads(*heads)), dim ** -0.5 if scale is None else float(scale), C.byref(q), C.byref(k),
-            C.byref(v), C.byref(gate) if gate else None, d_cu_q.ptr, d_cu_k.ptr, n_seqs, total_q, total_k, d_y.ptr,
-            d_status.ptr if d_status else None))
+            self.ctx, self._heads(heads), dim ** -0.5 if scale is None else scale, q, k, v, gate, d_cu_q.ptr, d_cu_k.ptr, n_seqs,
+            total_q, total_k, d_y.ptr, d_status.ptr if d_status else None))
 
     def attn_paged_device(self, d_q: DeviceBuffer, heads, n_seqs: int, rows: int, cache: KvCache, d_pages: DeviceBuffer,
                           max_pages: int, d_lens: DeviceBuffer, d_y: DeviceBuffer, scale: float | None = None, q_strides=None,
@@ -772,13 +792,13 @@ class HipBackend:
         """Attention of the last `rows` tokens of every sequence over its cache (tqf_hip_attn_paged_device)."""
         nq, _, dim = heads
         t, what = n_seqs * rows, "attn_paged_device"
-        q = self._head_rows(what, d_q, t, nq, dim, q_strides, 2)
-        gate = self._head_rows(what, d_gate, t, nq, dim, gate_strides, 2) if d_gate else None
-        _hold(what, (d_y, 2 * t * nq * dim), (d_pages, 4 * n_seqs * max_pages), (d_lens, 4 * n_seqs))
+        q = self._rows(0, what, d_q, t, nq, dim, q_strides, 2)
+        gate = self._rows(3, what, d_gate, t, nq, dim, gate_strides, 2) if d_gate else None
+        if d_y.nbytes < 2 * t * nq * dim or d_pages.nbytes < 4 * n_seqs * max_pages or d_lens.nbytes < 4 * n_seqs:
+            raise ValueError(f"{what}: a buffer is too small for {rows} rows of {n_seqs} sequences")
         self._check(self.lib.tqf_hip_attn_paged_device(
-            self.ctx, C.byref(_lib.Heads(*heads)), dim ** -0.5 if scale is None else float(scale), C.byref(q),
-            C.byref(gate) if gate else None, n_seqs, rows, C.byref(cache.as_struct()), d_pages.ptr, max_pages, d_lens.ptr, d_y.ptr,
-            d_status.ptr if d_status else None))
+            self.ctx, self._heads(heads), dim ** -0.5 if scale is None else scale, q, gate, n_seqs, rows, cache.ref, d_pages.ptr,
+            max_pages, d_lens.ptr, d_y.ptr, d_status.ptr if d_status else None))
 
     def add_rows_device(self, d_a: DeviceBuffer, d_b: DeviceBuffer, n: int, d_out: DeviceBuffer) -> None:
         """d_out[i] = d_a[i] + d_b[i], n f32 values; d_out may be one of them."""

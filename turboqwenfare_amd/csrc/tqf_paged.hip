@@ -41,18 +41,18 @@ __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0
 constexpr int kWaves = 4, kWaveKeys = 32, kStepKeys = kWaves * kWaveKeys;
 
 // What the join needs to know of a (sequence, key head) that several parts have: kept
-// by the part after the first.  The first part has it from its own beginning on or
-// behind others.
+// by the part that begins it.
 struct Cut {
-    uint32_t seq, kv, first, parts;  // parts 0: none is cut here first; kBehind: the first part begins with others
+    uint32_t seq, kv, first, parts;  // parts 0: none is cut here
 };
-constexpr uint32_t kBehind = 1u << 31;
 
 struct Kernel {
     PagedArgs a;
     uint32_t group, row_blocks, parts, page_shift;  // parts: workgroups of a row block
     float scale_log2;
-    Cut *cuts;       // [parts]
+    uint32_t extra;  // what a (sequence, key head) costs beside its steps, in steps
+    bool by_unit;    // cuts [n_seqs x kv_heads], where those are fewer, else [parts]
+    Cut *cuts;
     float *partial;  // [2 parts][row_blocks][rows of a block][dim + 2]: values, maximum, sum
 };
 
@@ -64,10 +64,13 @@ __device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
 }
 
 // The line of all steps: sequence by sequence, key head by key head; fewer than 2^31
-// (the caller has checked the most there can be).  All results are the same in
+// (the caller has checked the most there can be).  Before the steps of each stand
+// `extra` places for what beginning and ending it costs: without them a part of
+// many short sequences takes longer than one of a long one (64 sequences of 50 to
+// 8192 tokens, 4 rows of heads of 256: 92 us, with one place 77).  All results are the same in
 // every lane, and the compiler is told so: descriptors made of them stay scalar.
 struct Line {
-    uint32_t mine, upto;  // of sequence `lane`: steps of a key head; steps of all heads of the sequences up to it
+    uint32_t mine, upto;  // of sequence `lane`: places of a key head; places of all heads of the sequences up to it
     uint32_t total;
 };
 __device__ __forceinline__ uint32_t steps_up_to(uint32_t mine) {
@@ -79,12 +82,12 @@ __device__ __forceinline__ uint32_t steps_up_to(uint32_t mine) {
     }
     return upto;
 }
-__device__ __forceinline__ Line line_of(const PagedArgs &a) {
+__device__ __forceinline__ Line line_of(const PagedArgs &a, uint32_t extra) {
     const uint32_t l = threadIdx.x & 63;
     Line line;
-    line.mine = l < a.n_seqs ? steps_of(a, a.lens[l]) : 0;
+    line.mine = l < a.n_seqs ? steps_of(a, a.lens[l]) + extra : 0;
     uint32_t rest = 0;
-    for (uint32_t s = l + 64; s < a.n_seqs; s += 64) rest += steps_of(a, a.lens[s]);
+    for (uint32_t s = l + 64; s < a.n_seqs; s += 64) rest += steps_of(a, a.lens[s]) + extra;
     line.upto = steps_up_to(line.mine * a.cache.kv_heads);
     line.total = __builtin_amdgcn_readlane(line.upto, 63);
     if (a.n_seqs > 64) {
@@ -95,13 +98,13 @@ __device__ __forceinline__ Line line_of(const PagedArgs &a) {
     return line;
 }
 struct Place {
-    uint32_t seq, steps, first;  // a sequence, its steps for a key head, its first step
+    uint32_t seq, places, first;  // a sequence, its places for a key head, its first place
 };
-__device__ __forceinline__ Place place_of(const PagedArgs &a, const Line &line, uint32_t step) {
+__device__ __forceinline__ Place place_of(const PagedArgs &a, const Line &line, uint32_t extra, uint32_t place) {
     const uint32_t l = threadIdx.x & 63;
     uint32_t before = 0, mine = line.mine, upto = line.upto;
     for (uint32_t s0 = 0;;) {
-        const uint64_t past = __ballot(before + upto > step);
+        const uint64_t past = __ballot(before + upto > place);
         if (past) {
             const int who = __builtin_ctzll(past);
             const uint32_t n = __builtin_amdgcn_readlane(mine, who);
@@ -109,19 +112,19 @@ __device__ __forceinline__ Place place_of(const PagedArgs &a, const Line &line, 
         }
         before += __builtin_amdgcn_readlane(upto, 63);
         s0 += 64;
-        if (s0 >= a.n_seqs) return Place{a.n_seqs, 1, 0};  // no such step
-        mine = s0 + l < a.n_seqs ? steps_of(a, a.lens[s0 + l]) : 0;
+        if (s0 >= a.n_seqs) return Place{a.n_seqs, 1, 0};  // no such place
+        mine = s0 + l < a.n_seqs ? steps_of(a, a.lens[s0 + l]) + extra : 0;
         upto = steps_up_to(mine * a.cache.kv_heads);
     }
 }
-// Equal parts, the first ones a step longer.
+// Equal parts, the first ones a place longer.
 __device__ __forceinline__ uint32_t part_begin(uint32_t total, uint32_t part, uint32_t parts) {
     const uint32_t each = total / parts, more = total % parts;
     return part * each + (part < more ? part : more);
 }
-__device__ __forceinline__ uint32_t part_of(uint32_t total, uint32_t step, uint32_t parts) {
+__device__ __forceinline__ uint32_t part_of(uint32_t total, uint32_t place, uint32_t parts) {
     const uint32_t each = total / parts, more = total % parts, longer = more * (each + 1);
-    return step < longer ? step / (each + 1) : more + (step - longer) / (each ? each : 1);
+    return place < longer ? place / (each + 1) : more + (place - longer) / (each ? each : 1);
 }
 
 __device__ __forceinline__ void four_bf16(const uint16_t *p, float (&v)[4]) {
@@ -148,22 +151,30 @@ __device__ __forceinline__ uint32_t v_swizzle(uint32_t row) {
     return kPitch >= 256 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
 }
 
+// Workgroups that a compute unit holds, by their LDS (160 KiB; for 32 keys and values
+// of four wavefronts) and registers (the sums of values, the rows).
+constexpr int residents(int dim, int row_tiles, bool f8) {
+    const int by_lds = 160 / (dim * (f8 ? 1 : 2) / 4 + 2), by_registers = dim * row_tiles >= 512 ? 1 : dim * row_tiles >= 256 ? 2 : dim * row_tiles >= 128 ? 3 : 4;
+    return by_lds < by_registers ? by_lds : by_registers;
+}
+
 // NR: tiles of 16 rows that a workgroup has.  A wavefront's 32 keys and values come
 // by copies to LDS that is its own: the next keys are asked for when these have been
 // multiplied, the next values likewise, so there is always one of the two under way,
 // and no registers wait for them.
 template <int D, int NR, bool F8>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Kernel p) {
+__global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kernel(Kernel p) {
     constexpr int kRow = F8 ? D : 2 * D, kDims = D / 16, kSteps = D / 32, kRows = 16 * NR, kChunks = D / 8;
     constexpr int kCopies = kRow / 64;  // of 1 KiB for 16 keys
-    constexpr int kOutRound = 16 * D * 4, kTile = kWaveKeys * kRow;
+    constexpr int kTile = kWaveKeys * kRow, kOutRows = F8 ? 8 : 16;  // rows joined at a time: as many as fit the values' place
+    static_assert(kOutRows * D * 4 == kTile, "shares in the place of values");
     // keys, then values; at the end the rows' sums of values
-    __shared__ __attribute__((aligned(1024))) uint8_t s_k[kWaves][kTile], s_v[kWaves][kTile > kOutRound ? kTile : kOutRound];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_k[kWaves][kTile], s_v[kWaves][kTile];
     __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 16, g = l / 16;
     const uint32_t part = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
-    const Line line = line_of(a);
+    const Line line = line_of(a, p.extra);
     const uint32_t total = line.total, begin = part_begin(total, part, p.parts), end = part_begin(total, part + 1, p.parts);
     const uint32_t all_rows = a.rows * p.group;
     const size_t page_size = a.cache.page;
@@ -182,23 +193,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
         v_at2 = v_at + 16 * kRow;  // the swizzle of row + 16 is that of the row
     }
 
-    Cut *const cut = block == 0 && tid == 0 && part > 0 ? p.cuts + part : nullptr;
-    if (begin >= end) {
-        if (cut) cut->parts = 0;
+    const bool keeps_cuts = block == 0 && tid == 0;
+    const Place place = begin < end ? place_of(a, line, p.extra, begin) : Place{a.n_seqs, 1, 0};
+    uint32_t seq = place.seq, steps = place.places - p.extra, kv = __builtin_amdgcn_readfirstlane((begin - place.first) / place.places);
+    uint32_t unit = place.first + kv * place.places;  // its first place
+    uint32_t from = begin - unit > p.extra ? begin - unit - p.extra : 0;
+    if (seq >= a.n_seqs || unit + p.extra >= end) {  // no step
+        if (keeps_cuts && !p.by_unit) p.cuts[part].parts = 0;
         return;
-    }
-    const Place place = place_of(a, line, begin);
-    if (place.seq >= a.n_seqs) {
-        if (cut) cut->parts = 0;
-        return;
-    }
-    uint32_t seq = place.seq, steps = place.steps, kv = __builtin_amdgcn_readfirstlane((begin - place.first) / steps);
-    uint32_t from = begin - place.first - kv * steps, at = begin;
-    if (cut) {
-        const uint32_t unit = begin - from, before = part_begin(total, part - 1, p.parts);
-        const bool here_first = from > 0 && before <= unit;
-        const uint32_t n = here_first ? part_of(total, unit + steps - 1, p.parts) - part + 2 : 0;
-        *cut = Cut{seq, kv, part - 1, n | (before < unit ? kBehind : 0)};
     }
 
     int32_t len = 0;
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
     // Asks for the rows and the first keys of steps from..upto of (seq, kv).
     uint32_t upto = 0;
     auto ask = [&] {
-        upto = steps - from < end - at ? steps : from + (end - at);
+        upto = steps < end - unit - p.extra ? steps : end - unit - p.extra;
         len = ((const constant_i32 *)(uintptr_t)a.lens)[seq];
         poison = len < 0 || (uint64_t)len > (uint64_t)a.max_pages * page_size;
         if (poison) len = 0;
@@ -478,14 +480,25 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
 
         // the next (sequence, key head) of the part is asked for before the wavefronts' shares of this one are joined
         const uint32_t of_seq = seq, of_kv = kv;
-        const bool bad = __any(poison), whole = from == 0 && upto == steps, part_first = at == begin;
+        const bool bad = __any(poison), begins = from == 0, whole = begins && upto == steps;
         if (bad && a.status && tid % 64 == 0) *a.status = TQF_HIP_ERR_INVALID;
-        at += upto - from;
+        if (keeps_cuts && begins && p.by_unit) {
+            const uint32_t n = whole ? 0 : part_of(total, unit + p.extra + steps - 1, p.parts) - part + 1;
+            p.cuts[seq * a.cache.kv_heads + kv] = Cut{seq, kv, part, n};
+        }
         from = 0;
-        if (++kv == a.cache.kv_heads) kv = 0, ++seq;
-        const bool again = at < end && seq < a.n_seqs;
+        unit += steps + p.extra;
+        const bool again = unit + p.extra < end && (kv + 1 < a.cache.kv_heads || seq + 1 < a.n_seqs);
+        if (keeps_cuts && !again && !p.by_unit) {
+            const uint32_t n = whole || !begins ? 0 : part_of(total, unit - 1, p.parts) - part + 1;
+            p.cuts[part] = Cut{seq, kv, part, n};
+        }
         if (again) {
-            if (kv == 0) steps = steps_of(a, ((const constant_i32 *)(uintptr_t)a.lens)[seq]);
+            if (++kv == a.cache.kv_heads) {
+                kv = 0;
+                ++seq;
+                steps = steps_of(a, ((const constant_i32 *)(uintptr_t)a.lens)[seq]);
+            }
             ask();
         }
         const int here_l = here(l), here_r = here_l % 16, here_g = here_l / 16;
@@ -500,7 +513,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
             }
         }
         __syncthreads();
-        float *to = p.partial + ((size_t)(2 * part + (part_first ? 0 : 1)) * p.row_blocks + block) * kRows * (D + 2);
+        float *to = p.partial + ((size_t)(2 * part + (begins ? 1 : 0)) * p.row_blocks + block) * kRows * (D + 2);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const int row = n * 16 + here_r;
@@ -508,56 +521,61 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_kernel(Ke
 #pragma unroll
             for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][row]);
             mine = m[n] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
-            // [row][chunk of 4 at chunk ^ row] f32
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-                const int c = d * 4 + here_g;
-                *reinterpret_cast<f32x4 *>(s_v[wave] + here_r * D * 4 + (c ^ here_r) * 16) = o[d][n] * mine;
-            }
-            __syncthreads();
+            for (int half = 0; half < 16 / kOutRows; ++half) {
+                // [row][chunk of 4 at chunk ^ row] f32
+                if (here_r / kOutRows == half) {
 #pragma unroll
-            for (int x = 0; x < 16 * kChunks * 2; x += 64 * kWaves) {
-                const int i = x + wave * 64 + here_l, rr = i / (2 * kChunks), c = i % (2 * kChunks), of_block = n * 16 + rr;
-                f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                float all = s_m[0][of_block], total_l = 0.0f;
-#pragma unroll
-                for (int u = 1; u < kWaves; ++u) all = fmaxf(all, s_m[u][of_block]);
-#pragma unroll
-                for (int u = 0; u < kWaves; ++u) {
-                    v += *reinterpret_cast<const f32x4 *>(s_v[u] + rr * D * 4 + (c ^ rr) * 16);
-                    // a wavefront without keys has sum 0, or NaN where its sequence or a page is bad
-                    total_l += s_m[u][of_block] == -kInf ? s_l[u][of_block] : s_l[u][of_block] * __builtin_amdgcn_exp2f(s_m[u][of_block] - all);
+                    for (int d = 0; d < kDims; ++d) {
+                        const int c = d * 4 + here_g, rr = here_r % kOutRows;
+                        *reinterpret_cast<f32x4 *>(s_v[wave] + rr * D * 4 + (c ^ rr) * 16) = o[d][n] * mine;
+                    }
                 }
-                const uint32_t out_row = block * kRows + of_block;
-                if (whole) {
-                    if (out_row < all_rows) {
+                __syncthreads();
+#pragma unroll
+                for (int x = 0; x < kOutRows * kChunks * 2; x += 64 * kWaves) {
+                    const int i = x + wave * 64 + here_l, rr = i / (2 * kChunks), c = i % (2 * kChunks), of_block = n * 16 + half * kOutRows + rr;
+                    if (kOutRows * kChunks * 2 < 64 * kWaves && rr >= kOutRows) break;
+                    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float all = s_m[0][of_block], total_l = 0.0f;
+#pragma unroll
+                    for (int u = 1; u < kWaves; ++u) all = fmaxf(all, s_m[u][of_block]);
+#pragma unroll
+                    for (int u = 0; u < kWaves; ++u) {
+                        v += *reinterpret_cast<const f32x4 *>(s_v[u] + rr * D * 4 + (c ^ rr) * 16);
+                        // a wavefront without keys has sum 0, or NaN where its sequence or a page is bad
+                        total_l += s_m[u][of_block] == -kInf ? s_l[u][of_block] : s_l[u][of_block] * __builtin_amdgcn_exp2f(s_m[u][of_block] - all);
+                    }
+                    const uint32_t out_row = block * kRows + of_block;
+                    if (!whole) {
+                        float *row_to = to + (size_t)of_block * (D + 2);
+                        __builtin_memcpy(row_to + c * 4, &v, 16);
+                        if (c == 0) {
+                            row_to[D] = all;
+                            row_to[D + 1] = total_l;
+                        }
+                    } else if (out_row < all_rows) {
                         const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
                         const size_t token = (size_t)of_seq * a.rows + out_row / p.group, head = (size_t)of_kv * p.group + out_row % p.group;
                         v *= inv;
                         if (a.gate.d) {
-                            const uint16_t *gp = static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head + c * 4;
+                            float gate[4];
+                            four_bf16(static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head + c * 4, gate);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] *= gate_of(gp[e]);
+                            for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gate[e]);
                         }
                         store4(a.y + (token * a.q_heads + head) * D + c * 4, 4, v);
                     }
-                } else {
-                    float *row_to = to + (size_t)of_block * (D + 2);
-                    __builtin_memcpy(row_to + c * 4, &v, 16);
-                    if (c == 0) {
-                        row_to[D] = all;
-                        row_to[D + 1] = total_l;
-                    }
                 }
+                __syncthreads();
             }
-            __syncthreads();
         }
         if (!again) break;
     }
 }
 
 // Joins what several parts have of one (sequence, key head): a workgroup for each
-// part's beginning, if one is cut there first, and `each` rows.  Of few parts a
+// cut and `each` rows.  Of few parts a
 // wavefront has a row; of many it has some for every row in turn.
 constexpr int kJoinWaves = 8, kJoinAhead = 4;
 template <int D>
@@ -567,8 +585,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64;
     const uint32_t all_rows = a.rows * p.group, sets = (all_rows + each - 1) / each;
-    const Cut cut = p.cuts[blockIdx.x / sets + 1];
-    const uint32_t parts = cut.parts & ~kBehind, row0 = blockIdx.x % sets * each;
+    const Cut cut = p.cuts[blockIdx.x / sets];
+    const uint32_t parts = cut.parts, row0 = blockIdx.x % sets * each;
     if (parts == 0) return;
     const size_t stride = (size_t)2 * p.row_blocks * block_rows * (D + 2);  // of a part
     float m, sum, o[kPer];
@@ -582,7 +600,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_
 #pragma unroll
             for (int x = 0; x < kJoinAhead; ++x) {
                 const uint32_t at = i + x * step < parts ? i + x * step : parts - 1;
-                const size_t slot = at == 0 && (cut.parts & kBehind) ? 1 : 0;
+                const size_t slot = at == 0 ? 1 : 0;  // a part keeps what begins in it apart from what goes on
                 const float *from = p.partial + (cut.first + at) * stride + ((slot * p.row_blocks + row / block_rows) * block_rows + row % block_rows) * (D + 2);
                 pm[x] = from[D], pl[x] = from[D + 1];
                 if constexpr (kPer == 1) po[x][0] = from[l];
@@ -652,18 +670,19 @@ uint32_t row_blocks(const PagedArgs &a) {
     const uint32_t rows = a.rows * (a.q_heads / a.cache.kv_heads), per = 16 * tiles_of_rows(a);
     return (rows + per - 1) / per;
 }
-// As many workgroups as compute units hold at once (one of heads of 256, by its LDS, else
-// two); no more than there can be steps.
+uint64_t units_of(const PagedArgs &a) { return (uint64_t)a.n_seqs * a.cache.kv_heads; }
+uint64_t most_steps(const PagedArgs &a) { return units_of(a) * (((uint64_t)a.max_pages * a.cache.page + kStepKeys - 1) / kStepKeys); }
+// As many workgroups as the compute units hold at once; no more than there can be steps.
 uint32_t parts_of(const PagedArgs &a) {
     int device = 0, cus = 0;
     (void)hipGetDevice(&device);
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
-    const uint64_t most = (uint64_t)a.n_seqs * a.cache.kv_heads * (((uint64_t)a.max_pages * a.cache.page + kStepKeys - 1) / kStepKeys);
-    const uint64_t want = (uint64_t)(a.cache.dim == 256 ? 1 : 2) * (uint64_t)(cus > 0 ? cus : 256);
-    return (uint32_t)(most < want ? most : want);
+    const uint64_t want = (uint64_t)residents(a.cache.dim, tiles_of_rows(a), a.cache.f8) * (uint64_t)(cus > 0 ? cus : 256);
+    return (uint32_t)(most_steps(a) < want ? most_steps(a) : want);
 }
 
-size_t cuts_bytes(uint32_t parts) { return ((size_t)parts * sizeof(Cut) + 255) / 256 * 256; }
+uint32_t cuts_of(const PagedArgs &a) { return (uint32_t)(units_of(a) < parts_of(a) ? units_of(a) : parts_of(a)); }
+size_t cuts_bytes(const PagedArgs &a) { return ((size_t)cuts_of(a) * sizeof(Cut) + 255) / 256 * 256; }
 
 template <int D, int NR>
 hipError_t launch_for(hipStream_t s, const Kernel &p) {
@@ -673,9 +692,9 @@ hipError_t launch_for(hipStream_t s, const Kernel &p) {
     if (p.parts > 1) {
         if (const hipError_t e = hipGetLastError()) return e;
         // about two thousand workgroups at most: more would wait for one another's places
-        const uint32_t rows = p.a.rows * p.group, all = (p.parts - 1) * rows;
-        const uint32_t each = all <= 2048 ? 1 : all <= 4096 ? 2 : all <= 8192 ? 4 : 8;
-        join_kernel<D><<<dim3((p.parts - 1) * ((rows + each - 1) / each)), dim3(64 * kJoinWaves), 0, s>>>(p, 16 * NR, each);
+        const uint32_t rows = p.a.rows * p.group, cuts = cuts_of(p.a);
+        const uint32_t each = cuts * rows <= 2048 ? 1 : cuts * rows <= 4096 ? 2 : cuts * rows <= 8192 ? 4 : 8;
+        join_kernel<D><<<dim3(cuts * ((rows + each - 1) / each)), dim3(64 * kJoinWaves), 0, s>>>(p, 16 * NR, each);
     }
     return hipGetLastError();
 }
@@ -683,13 +702,21 @@ hipError_t launch_for(hipStream_t s, const Kernel &p) {
 }  // namespace
 
 size_t attn_paged_scratch_bytes(const PagedArgs &a) {
-    return cuts_bytes(parts_of(a)) + (size_t)2 * parts_of(a) * row_blocks(a) * 16 * tiles_of_rows(a) * (a.cache.dim + 2) * 4;
+    return cuts_bytes(a) + (size_t)2 * parts_of(a) * row_blocks(a) * 16 * tiles_of_rows(a) * (a.cache.dim + 2) * 4;
 }
 
 hipError_t launch_attn_paged(hipStream_t s, const PagedArgs &a, void *scratch) {
-    Kernel p{a, a.q_heads / a.cache.kv_heads, row_blocks(a), parts_of(a), (uint32_t)__builtin_ctz(a.cache.page), a.scale * kLog2e,
-             static_cast<Cut *>(scratch), nullptr};
-    p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + cuts_bytes(p.parts));
+    Kernel p{};
+    p.a = a;
+    p.group = a.q_heads / a.cache.kv_heads;
+    p.row_blocks = row_blocks(a);
+    p.parts = parts_of(a);
+    p.page_shift = (uint32_t)__builtin_ctz(a.cache.page);
+    p.scale_log2 = a.scale * kLog2e;
+    p.extra = most_steps(a) > p.parts ? 1 : 0;  // with a workgroup for every step there is nothing to balance
+    p.by_unit = units_of(a) <= p.parts;
+    p.cuts = static_cast<Cut *>(scratch);
+    p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + cuts_bytes(a));
     const bool two = tiles_of_rows(a) == 2;
     if (a.cache.dim == 64) return two ? launch_for<64, 2>(s, p) : launch_for<64, 1>(s, p);
     if (a.cache.dim == 128) return two ? launch_for<128, 2>(s, p) : launch_for<128, 1>(s, p);

@@ -1,6 +1,8 @@
 // tqf_attn_device.h -- what the attention kernels share.
 #pragma once
 
+#include <atomic>
+
 #include "tqf_attn.h"
 #include "tqf_f8.h"
 
@@ -17,6 +19,17 @@ constexpr float kInf = __builtin_inff();
 // weights are then at most 2^8, their sums in f32 as exact as ever, and the sums
 // of values are hardly ever multiplied again.
 constexpr float kSlack = 8.0f;
+
+// Compute units of the current device.
+inline int cu_count() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
 
 // Copies to LDS: lane l's 16 bytes go to lds + 16 l.
 typedef __amdgpu_buffer_rsrc_t Desc;  // loads past its bytes give zero

@@ -31,10 +31,12 @@ namespace tqf {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kMfma = 0x8, kDsRead = 0x100, kAhead = 4;  // for the scheduler: kinds of instructions; how far reads are ahead
 struct Kernel {
     PromptArgs a;
     uint32_t head_waves;  // wavefronts of a workgroup that have heads of their own (of one group)
     uint32_t head_sets;   // q_heads / head_waves
+    uint32_t turn;        // workgroups from here on are taken from the end
     float scale_log2;
 };
 
@@ -98,8 +100,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 32, half = l / 32;
     const uint32_t tokens = 32u * kWaves / p.head_waves;  // of the workgroup
     Place at;
-    if (!find_place(a, blockIdx.x / p.head_sets, tokens, at)) return;
-    const uint32_t head = blockIdx.x % p.head_sets * p.head_waves + (uint32_t)wave % p.head_waves;
+    const uint32_t number = blockIdx.x < p.turn ? blockIdx.x : gridDim.x - 1 - (blockIdx.x - p.turn);
+    if (!find_place(a, number / p.head_sets, tokens, at)) return;
+    const uint32_t head = number % p.head_sets * p.head_waves + (uint32_t)wave % p.head_waves;
     const uint32_t kv = head / (a.q_heads / a.kv_heads);
     const int q0 = __builtin_amdgcn_readfirstlane(at.q0), lq = __builtin_amdgcn_readfirstlane(at.lq);
     const int k0 = __builtin_amdgcn_readfirstlane(at.k0), lk = __builtin_amdgcn_readfirstlane(at.lk);
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
         const Desc dk = make_desc(kp + (size_t)kt * KT * k_row, (rows - 1) * k_row + kRow);
         const Desc dv = make_desc(vp + (size_t)kt * KT * v_row, (rows - 1) * v_row + kRow);
-        const uint32_t lane = here(l);
+        const uint32_t lane = D == 256 ? here(l) : (uint32_t)l;  // smaller heads leave registers for the offsets
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const uint32_t base = (wave * kCopies + i) * 1024, byte = base + lane * 16, rr = byte / kRow, c = byte % kRow / 16;
@@ -167,6 +170,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             }
             s[j] = acc;
         }
+        // reads go ahead of the products that need them, which the compiler would not do where registers are scarce
+        __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < kSub * kSteps - kAhead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
         if (part) {
 #pragma unroll
             for (int j = 0; j < kSub; ++j)
@@ -220,6 +231,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(sv, v0_at, j, st, d)), w[j][st], o[d], 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kAhead, 1);
+#pragma unroll
+        for (int i = 0; i < kDims * kSub * 2 - kAhead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 1);
     };
 
     // Two stages of LDS, each a variable of its own: the next tile's copies are under way while one is computed.
@@ -279,41 +297,77 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         }
     }
 
-    if (!live || mine + r >= lq) return;
+    // Rows leave through LDS (the tiles' place, a stage for each wavefront), so that neighbouring lanes have
+    // neighbouring bytes of a row: [row][chunk of 4 at chunk ^ row], kOut dimensions at a time.
+    constexpr int kOut = kTile / 128, kLanes = kOut / 8;  // lanes of a row
+    __syncthreads();
+    if (!live) return;
+    uint8_t *const out = wave == 0 ? s_k0 : wave == 1 ? s_v0 : wave == 2 ? s_k1 : s_v1;
     sum += __shfl_xor(sum, 32);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const size_t token = (size_t)(q0 + mine + r);
-    uint16_t *y = a.y + (token * a.q_heads + head) * D;
-    const uint16_t *gate = a.gate.d ? static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + (size_t)head * a.gate.head : nullptr;
+    const size_t first_row = (size_t)(q0 + mine);
+    const int rows = lq - mine < 32 ? lq - mine : 32, lane = here(l), row_of = lane / kLanes, at_dim = lane % kLanes * 8;
+    uint16_t *const y = a.y + (first_row * a.q_heads + head) * D + at_dim;
+    const uint16_t *const gate = static_cast<const uint16_t *>(a.gate.d) + first_row * a.gate.row + (size_t)head * a.gate.head + at_dim;
 #pragma unroll
-    for (int d = 0; d < kDims; ++d)
+    for (int part = 0; part < D / kOut; ++part) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int dim = d * 32 + 8 * (i / 4) + 4 * half;
-            f32x4 v;
+        for (int d = 0; d < kOut / 32; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = o[d][i + e] * inv;
-            if (gate) {
-                const uint2 b = *reinterpret_cast<const uint2 *>(gate + dim);
-                const float gv[4] = {__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xFFFF0000u), __uint_as_float(b.y << 16),
-                                     __uint_as_float(b.y & 0xFFFF0000u)};
+            for (int i = 0; i < 16; i += 4) {
+                f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gv[e]);
+                for (int e = 0; e < 4; ++e) v[e] = o[part * (kOut / 32) + d][i + e] * inv;
+                const int c = d * 8 + 2 * (i / 4) + half;
+                *reinterpret_cast<f32x4 *>(out + r * (kOut * 4) + (c ^ (r & (kOut / 4 - 1))) * 16) = v;
             }
-            store4(y + dim, 4, v);
+        u32x4 g[32 * kLanes / 64];
+        if (a.gate.d) {
+#pragma unroll
+            for (int i = 0; i < 32 * kLanes / 64; ++i) {
+                const int rr = i * (64 / kLanes) + row_of;
+                g[i] = *reinterpret_cast<const u32x4 *>(gate + (size_t)(rr < rows ? rr : 0) * a.gate.row + part * kOut);
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 32 * kLanes / 64; ++i) {
+            const int rr = i * (64 / kLanes) + row_of, c = at_dim / 4;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(out + rr * (kOut * 4) + ((c + e) ^ (rr & (kOut / 4 - 1))) * 16);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[4 * e + u] = x[u];
+            }
+            if (a.gate.d) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[2 * e] *= sigmoid(__uint_as_float(g[i][e] << 16));
+                    v[2 * e + 1] *= sigmoid(__uint_as_float(g[i][e] & 0xFFFF0000u));
+                }
+            }
+            if (rr < rows) {
+                const u32x4 bits = {bf16_bits2(v[0], v[1]), bf16_bits2(v[2], v[3]), bf16_bits2(v[4], v[5]), bf16_bits2(v[6], v[7])};
+                *reinterpret_cast<u32x4 *>(y + (size_t)rr * a.q_heads * D + part * kOut) = bits;
+            }
+        }
+    }
 }
 
 }  // namespace
 
 hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a) {
-    Kernel p{a, 1, 0, a.scale * kLog2e};
+    Kernel p{a, 1, 0, 0, a.scale * kLog2e};
     const uint32_t group = a.q_heads / a.kv_heads;
     while (p.head_waves < kWaves && group % (p.head_waves * 2) == 0) p.head_waves *= 2;
     p.head_sets = a.q_heads / p.head_waves;
     const uint32_t tokens = 32 * kWaves / p.head_waves;
     const uint64_t tiles = (uint64_t)a.total_q / tokens + a.n_seqs;  // at least as many as there are
     const dim3 grid((uint32_t)(tiles * p.head_sets)), block(64 * kWaves);
+    // Tiles of a prompt begin with the longest, and what is free first takes the next.  Where all run at once, two to
+    // a compute unit, the second of each comes from the end, so that their sums are alike.
+    const uint32_t cus = (uint32_t)cu_count();
+    p.turn = a.n_seqs == 1 && grid.x > cus && grid.x <= 2 * cus + p.head_sets ? cus : grid.x;
     if (a.dim == 64) prompt_kernel<64, 64><<<grid, block, 0, s>>>(p);
     if (a.dim == 128) prompt_kernel<128, 64><<<grid, block, 0, s>>>(p);
     if (a.dim == 256) prompt_kernel<256, 32><<<grid, block, 0, s>>>(p);

@@ -45,6 +45,10 @@ __device__ __forceinline__ Desc make_desc(const void *p, uint32_t bytes) {
 __device__ __forceinline__ void copy16(Desc d, uint32_t voff, void *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, 0, 0, 0);
 }
+// soff: the same in every lane, and not held against the descriptor's end.
+__device__ __forceinline__ void copy16(Desc d, uint32_t voff, uint32_t soff, void *lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, soff, 0, 0);
+}
 
 // Four rows of 16 elements of 16 bits, transposed: lane i of 16 points at four
 // elements, 4 (i % 4) on, of row i / 4, and gets element i of the four rows.

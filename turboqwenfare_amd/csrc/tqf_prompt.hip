@@ -10,7 +10,7 @@
 // A wavefront has 32 rows of one head.  It computes S^T = K Q^T with the
 // 32 x 32 x 16 bf16 instructions: in their result a lane has one row and 16 keys,
 // so a row's maximum and sum stay in two lanes, and the weights, rounded to bf16
-// (2^-9 of each, where bf16 y rounds by as much), are an operand of O^T = V^T P^T
+// (at most 2^-8 of each, as y is), are an operand of O^T = V^T P^T
 // as they stand: the order in which an instruction takes its K elements is free so
 // long as both operands have the same.  V^T comes from LDS by transposing reads.
 // A workgroup's wavefronts share tiles of K and V, and so, where heads are
@@ -22,8 +22,6 @@
 // the tile's values are added at the end, key by key, to the rows that see them.
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "tqf_attn_device.h"
 
 namespace tqf {
@@ -31,7 +29,7 @@ namespace tqf {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kMfma = 0x8, kDsRead = 0x100, kAhead = 4;  // for the scheduler: kinds of instructions; how far reads are ahead
+constexpr int kAhead = 4;  // products that LDS reads go ahead of theirs
 struct Kernel {
     PromptArgs a;
     uint32_t head_waves;  // wavefronts of a workgroup that have heads of their own (of one group)
@@ -94,8 +92,12 @@ __device__ __forceinline__ uint32_t v_swizzle(uint32_t row) { return D == 64 ? (
 template <int D, int KT>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     constexpr int kRow = 2 * D, kTile = KT * kRow, kCopies = kTile / 1024 / kWaves, kSub = KT / 32, kDims = D / 32, kSteps = D / 16;
-    static_assert(kCopies >= 1, "every wavefront copies");
+    static_assert(kCopies >= 1 && 2 * kCopies <= kSub * kSteps, "every wavefront copies, one after a product");
     __shared__ __attribute__((aligned(1024))) uint8_t s_k0[kTile], s_v0[kTile], s_k1[kTile], s_v1[kTile];
+    // Heads of 256: every fourth 16 dimensions of the rows wait in LDS (two workgroups then take all of a compute
+    // unit's): with all of them in registers there are too few for anything else.
+    constexpr int kWaiting = D == 256 ? 4 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t s_q[kWaiting ? kWaves * kWaiting * 1024 : 16];
     const PromptArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 32, half = l / 32;
     const uint32_t tokens = 32u * kWaves / p.head_waves;  // of the workgroup
@@ -103,7 +105,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const uint32_t number = blockIdx.x < p.turn ? blockIdx.x : gridDim.x - 1 - (blockIdx.x - p.turn);
     if (!find_place(a, number / p.head_sets, tokens, at)) return;
     const uint32_t head = number % p.head_sets * p.head_waves + (uint32_t)wave % p.head_waves;
-    const uint32_t kv = head / (a.q_heads / a.kv_heads);
+    const uint32_t kv = __builtin_amdgcn_readfirstlane(head / (a.q_heads / a.kv_heads));
     const int q0 = __builtin_amdgcn_readfirstlane(at.q0), lq = __builtin_amdgcn_readfirstlane(at.lq);
     const int k0 = __builtin_amdgcn_readfirstlane(at.k0), lk = __builtin_amdgcn_readfirstlane(at.lk);
     const int first = (int)(__builtin_amdgcn_readfirstlane(at.tile) * tokens), mine = first + 32 * (wave / (int)p.head_waves);
@@ -115,10 +117,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const int last = (first + (int)tokens < lq ? first + (int)tokens : lq) - 1 + shift;  // of the workgroup
     const bool live = mine < lq;
 
-    bf16x8 q[kSteps];
+    bf16x8 q[kSteps];  // those that wait are not kept here
+    auto waits = [](int i) { return kWaiting && i % 4 == 3; };
+    uint8_t *const waiting = s_q + wave * kWaiting * 1024;
     const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + (size_t)(q0 + row) * a.q.row + (size_t)head * a.q.head + half * 8;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) q[i] = *reinterpret_cast<const bf16x8 *>(qp + i * 16);
+    for (int i = 0; i < kSteps; ++i) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8 *>(qp + i * 16);
+        if (waits(i)) *reinterpret_cast<bf16x8 *>(waiting + i / 4 * 1024 + l * 16) = x;
+        else q[i] = x;
+    }
     f32x16 o[kDims];
 #pragma unroll
     for (int i = 0; i < kDims; ++i)
@@ -127,57 +135,79 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     float m = -kInf, sum = 0.0f;
     uint32_t odd = 0;  // tiles, from the last one on, whose values are left to the end
 
-    const uint8_t *kp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.k.d) + (size_t)k0 * a.k.row + (size_t)kv * a.k.head);
-    const uint8_t *vp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.v.d) + (size_t)k0 * a.v.row + (size_t)kv * a.v.head);
+    const uint8_t *const kp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.k.d) + (size_t)k0 * a.k.row + (size_t)kv * a.k.head);
+    const uint8_t *const vp = reinterpret_cast<const uint8_t *>(static_cast<const uint16_t *>(a.v.d) + (size_t)k0 * a.v.row + (size_t)kv * a.v.head);
     const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2;
 
     // Where the lane's operands are in a tile: chunk half of key r, and, transposed, dimensions l % 32 of the first keys
     // that its half's weights have.  Other chunks and dimensions are these with bits flipped (the swizzles depend on the
-    // lane alone), other keys a constant further; so few registers hold addresses.
-    const uint32_t k_at = r * kRow + (half ^ k_swizzle<D>(r)) * 16;
-    const uint32_t v_row0 = 4 * half + l % 16 / 4, v_at = v_row0 * kRow + ((2 * (l / 16 % 2) + l % 4 / 2) ^ v_swizzle<D>(v_row0)) * 16 + l % 2 * 8;
+    // lane alone), other keys a constant further.  Made anew for each tile: no registers hold addresses.
+    auto k_at = [&] {
+        const uint32_t lane = here(l), row = lane % 32;
+        return row * kRow + (lane / 32 ^ k_swizzle<D>(row)) * 16;
+    };
+    auto v_at = [&] {
+        const uint32_t lane = here(l), row = 4 * (lane / 32) + lane % 16 / 4;
+        return row * kRow + ((2 * (lane / 16 % 2) + lane % 4 / 2) ^ v_swizzle<D>(row)) * 16 + lane % 2 * 8;
+    };
 
-    auto copy = [&](int kt, uint8_t *to_k, uint8_t *to_v) {
+    // Copies of a tile: a wavefront's `i` takes 1 KiB, which is kCopyRows rows.  Its rows' swizzle is that of the first
+    // copy's with constant bits flipped, and the rows' distance a scalar, so an offset is one instruction.  Scalar offsets
+    // are not held against the descriptor's end: the sequence's last tile, whose rows may end, has whole ones (copy_last).
+    constexpr int kCopyRows = 1024 / kRow, kRowLanes = kRow / 16;
+    const uint32_t copy_row = l / kRowLanes, copy_tile_row = wave * kCopies * kCopyRows + copy_row;
+    const uint32_t k_chunk = (l % kRowLanes ^ k_swizzle<D>(copy_tile_row)) * 16, v_chunk = (l % kRowLanes ^ v_swizzle<D>(copy_tile_row)) * 16;
+    const uint32_t k_first = copy_row * k_row, v_first = copy_row * v_row;
+    auto copy_last = [&](const uint8_t *from, uint32_t row_bytes, bool of_k, int kt, uint8_t *to) {
         const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
-        const Desc dk = make_desc(kp + (size_t)kt * KT * k_row, (rows - 1) * k_row + kRow);
-        const Desc dv = make_desc(vp + (size_t)kt * KT * v_row, (rows - 1) * v_row + kRow);
-        const uint32_t lane = D == 256 ? here(l) : (uint32_t)l;  // smaller heads leave registers for the offsets
+        const Desc d = make_desc(from + (size_t)kt * KT * row_bytes, (rows - 1) * row_bytes + kRow);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const uint32_t base = (wave * kCopies + i) * 1024, byte = base + lane * 16, rr = byte / kRow, c = byte % kRow / 16;
-            copy16(dk, rr * k_row + (c ^ k_swizzle<D>(rr)) * 16, to_k + base);
-            copy16(dv, rr * v_row + (c ^ v_swizzle<D>(rr)) * 16, to_v + base);
+            const uint32_t rr = copy_tile_row + i * kCopyRows;
+            copy16(d, rr * row_bytes + (l % kRowLanes ^ (of_k ? k_swizzle<D>(rr) : v_swizzle<D>(rr))) * 16, to + (wave * kCopies + i) * 1024);
         }
+    };
+    // A tile all of whose rows are there.  Before the first one there are none: nothing is in such a descriptor's bounds,
+    // and zeros go to LDS.  No branch, so that the copies can stand among the products, one after each.
+    struct Tile {
+        Desc d;
+        uint32_t step;  // from copy to copy
+    };
+    auto tile_at = [&](const uint8_t *from, uint32_t row_bytes, int kt) {
+        return Tile{make_desc(from + (size_t)(kt < 0 ? 0 : kt) * KT * row_bytes, kt < 0 ? 0 : 0xFFFFFFFFu), kt < 0 ? 0 : kCopyRows * row_bytes};
+    };
+    auto copy_k = [&](const Tile &t, int i, uint8_t *to) {
+        const uint32_t n = wave * kCopies + i;
+        copy16(t.d, (here(k_chunk) ^ k_swizzle<D>(i * kCopyRows) * 16) + k_first, n * t.step, to + n * 1024);
+    };
+    auto copy_v = [&](const Tile &t, int i, uint8_t *to) {
+        const uint32_t n = wave * kCopies + i;
+        copy16(t.d, (here(v_chunk) ^ v_swizzle<D>(i * kCopyRows) * 16) + v_first, n * t.step, to + n * 1024);
     };
     auto values = [&](const uint8_t *sv, uint32_t v0, int j, int st, int d) {
         const uint8_t *at_v = sv + (v0 ^ (d % 4 * 64)) + (d / 4 * 256 + (j * 32 + st * 16) * kRow);
         const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 8 * kRow);
         return u32x4{x.x, x.y, y.x, y.y};
     };
-    // One tile.  EDGE: some row of the workgroup does not see all of its keys.
-    auto step = [&](const uint8_t *sk, const uint8_t *sv, int kt, auto edge) {
-        constexpr bool EDGE = decltype(edge)::value;
-        const bool part = EDGE && kt * KT + KT - 1 > limit_min;  // some row of the wavefront
-        f32x16 s[kSub];
-        const uint32_t k0_at = here(k_at);
+    // Two stages of LDS, each a variable of its own: while a tile is worked on, the one before it comes.  publish(): this
+    // wavefront's copies are there and its reads done, then the workgroup's.
+    auto publish = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // A tile at the end of what the workgroup's rows see: some of them may not see all of its keys.
+    auto edge_scores = [&](const uint8_t *sk, f32x16 (&s)[kSub]) {
+        const uint32_t k0_at = k_at();
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
             f32x16 acc = {};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const bf16x8 k = *reinterpret_cast<const bf16x8 *>(sk + (k0_at ^ (i % 8 * 32)) + (i / 8 * 256 + j * 32 * kRow));
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, waits(i) ? *reinterpret_cast<const bf16x8 *>(waiting + i / 4 * 1024 + l * 16) : q[i], acc, 0, 0, 0);
             }
             s[j] = acc;
         }
-        // reads go ahead of the products that need them, which the compiler would not do where registers are scarce
-        __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
-#pragma unroll
-        for (int i = 0; i < kSub * kSteps - kAhead; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+    };
+    auto edge_step = [&](f32x16 (&s)[kSub], const uint8_t *sv, int kt) {
+        const bool part = kt * KT + KT - 1 > limit_min;  // some row of the wavefront
         if (part) {
 #pragma unroll
             for (int j = 0; j < kSub; ++j)
@@ -212,7 +242,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             }
         if (part) {
             u16x2 most = {0, 0};  // largest magnitudes among values that some rows do not see
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < kTile / 1024; ++i) {
                 const u32x4 x = *reinterpret_cast<const u32x4 *>(sv + i * 1024 + l * 16);
 #pragma unroll
@@ -223,7 +253,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
                 return;
             }
         }
-        const uint32_t v0_at = here(v_at);
+        const uint32_t v0_at = v_at();
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -231,44 +261,111 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(sv, v0_at, j, st, d)), w[j][st], o[d], 0, 0, 0);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kAhead, 1);
-#pragma unroll
-        for (int i = 0; i < kDims * kSub * 2 - kAhead; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
-        }
-        __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 1);
     };
 
-    // Two stages of LDS, each a variable of its own: the next tile's copies are under way while one is computed.
-    // publish(): this wavefront's copies are there and its reads done, then the workgroup's.
-    auto publish = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // A tile all of whose keys all rows see, and the copies of the one before it.
+    auto step = [&](const uint8_t *sk, const uint8_t *sv, uint8_t *other_k, uint8_t *other_v, int kt) {
+        // The order of the instructions is set by hand here and below: reads go kAhead products ahead, and the copies'
+        // and the exponentials' instructions stand between the products, in their shadow.
+        f32x16 s[kSub];
+        const uint32_t k0_at = k_at();
+        const Tile next_k = tile_at(kp, k_row, kt - 1), next_v = tile_at(vp, v_row, kt - 1);
+        auto keys = [&](int n) {
+            const int j = n / kSteps, i = n % kSteps;
+            return *reinterpret_cast<const bf16x8 *>(sk + (k0_at ^ (i % 8 * 32)) + (i / 8 * 256 + j * 32 * kRow));
+        };
+        bf16x8 ahead_k[kAhead], waited = {};
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) ahead_k[n] = keys(n);
+#pragma unroll
+        for (int n = 0; n < kSub * kSteps; ++n) {
+            __builtin_amdgcn_sched_barrier(0);
+            const f32x16 zero = {};
+            s[n / kSteps] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ahead_k[n % kAhead], waits(n % kSteps) ? waited : q[n % kSteps],
+                                                                    n % kSteps ? s[n / kSteps] : zero, 0, 0, 0);
+            if (kWaiting && n % 4 == 0) waited = *reinterpret_cast<const bf16x8 *>(waiting + n % kSteps / 4 * 1024 + here(l) * 16);
+            if (n + kAhead < kSub * kSteps) ahead_k[n % kAhead] = keys(n + kAhead);
+            if (n < kCopies) copy_k(next_k, n, other_k);
+            else if (n < 2 * kCopies) copy_v(next_v, n - kCopies, other_v);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float top = s[0][0];
+#pragma unroll
+        for (int j = 0; j < kSub; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
+        top = other_half_max(top) * p.scale_log2;
+        if (__any(top > m + kSlack)) {
+            const float m_new = fmaxf(m, top), keep = m_new == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+        }
+        const float m_use = m == -kInf ? 0.0f : m;
+        auto weight = [&](int g, int i) {  // of the group's 8 keys
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], p.scale_log2, -m_use));
+            sum += e;
+            return (__bf16)e;
+        };
+        // 16 keys at a time; the next ones' exponentials are between these ones' products
+        constexpr int kGroups = kSub * 2, kEach = 8 / kDims;
+        const uint32_t v0_at = v_at();
+        u32x4 ahead_v[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) ahead_v[n] = values(sv, v0_at, n / kDims / 2, n / kDims % 2, n % kDims);
+        bf16x8 w[2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[0][i] = weight(0, i);
+#pragma unroll
+        for (int n = 0; n < kGroups * kDims; ++n) {
+            const int g = n / kDims, d = n % kDims, then = n + kAhead;
+            __builtin_amdgcn_sched_barrier(0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ahead_v[n % kAhead]), w[g % 2], o[d], 0, 0, 0);
+            if (then < kGroups * kDims) ahead_v[n % kAhead] = values(sv, v0_at, then / kDims / 2, then / kDims % 2, then % kDims);
+            if (g + 1 < kGroups) {
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) w[(g + 1) % 2][d * kEach + i] = weight(g + 1, d * kEach + i);
+            }
+        }
+    };
+
     if (last >= 0) {
-        const int edge = (first + shift + 1 > 0 ? first + shift + 1 : 0) / KT;  // the tiles from here on are seen in part
         int kt = last / KT;
-        copy(kt, s_k0, s_v0);
-        bool one = false;
+        copy_last(kp, k_row, true, kt, s_k0);
+        copy_last(vp, v_row, false, kt, s_v0);
+        auto copy_before = [&](uint8_t *other_k, uint8_t *other_v) {
+            const Tile k = tile_at(kp, k_row, kt - 1), v = tile_at(vp, v_row, kt - 1);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) copy_k(k, i, other_k), copy_v(v, i, other_v);
+        };
+        const int edge = (first + shift + 1 > 0 ? first + shift + 1 : 0) / KT;  // all rows see all of the tiles before this
+        bool second = false;
         for (; kt >= edge; --kt) {
             publish();
-            if (kt > 0) copy(kt - 1, one ? s_k0 : s_k1, one ? s_v0 : s_v1);
-            if (live && kt * KT <= limit_max) step(one ? s_k1 : s_k0, one ? s_v1 : s_v0, kt, std::true_type());
-            one = !one;
+            copy_before(second ? s_k0 : s_k1, second ? s_v0 : s_v1);
+            if (live && kt * KT <= limit_max) {
+                f32x16 s[kSub];
+                edge_scores(second ? s_k1 : s_k0, s);
+                edge_step(s, second ? s_v1 : s_v0, kt);
+            }
+            second = !second;
         }
-        if (one && kt >= 0) {
+        auto whole = [&](const uint8_t *sk, const uint8_t *sv, uint8_t *other_k, uint8_t *other_v) {
             publish();
-            if (kt > 0) copy(kt - 1, s_k0, s_v0);
-            if (live) step(s_k1, s_v1, kt, std::false_type());
+            if (live) step(sk, sv, other_k, other_v, kt);
+            else copy_before(other_k, other_v);
             --kt;
+        };
+        if (second && kt >= 0) whole(s_k1, s_v1, s_k0, s_v0);
+        while (kt >= 0) {
+            whole(s_k0, s_v0, s_k1, s_v1);
+            if (kt < 0) break;
+            whole(s_k1, s_v1, s_k0, s_v0);
         }
-        for (; kt >= 0; --kt) {
-            publish();
-            if (kt > 0) copy(kt - 1, s_k1, s_v1);
-            if (live) step(s_k0, s_v0, kt, std::false_type());
-            if (--kt < 0) break;
-            publish();
-            if (kt > 0) copy(kt - 1, s_k0, s_v0);
-            if (live) step(s_k1, s_v1, kt, std::false_type());
-        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
     // Tiles with infinities or NaN that only some rows see: key by key.
@@ -282,8 +379,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const bf16x8 x = *reinterpret_cast<const bf16x8 *>(kr + i * 16);
+                const bf16x8 z = waits(i) ? *reinterpret_cast<const bf16x8 *>(waiting + i / 4 * 1024 + l * 16) : q[i];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dot = __builtin_fmaf((float)x[e], (float)q[i][e], dot);
+                for (int e = 0; e < 8; ++e) dot = __builtin_fmaf((float)x[e], (float)z[e], dot);
             }
             dot += __shfl_xor(dot, 32);
             if (key > limit) continue;

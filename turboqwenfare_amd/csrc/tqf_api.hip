@@ -2662,8 +2662,10 @@ extern "C" int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_he
     a.scale = scale;
     a.y = d_y;
     a.status = d_status;
+    if (const size_t bytes = attn_prompt_scratch_bytes(a))
+        if (int32_t rc = ensure_f8_scratch(ctx, bytes)) return rc;
     Prof p(ctx);
-    const hipError_t e = launch_attn_prompt(ctx->stream, a);
+    const hipError_t e = launch_attn_prompt(ctx->stream, a, ctx->d_grouped);
     if (e != hipSuccess) return hip_fail(ctx, "prompt attention launch", e);
     p.end(TQF_HIP_KERNEL_ATTN_PROMPT, 2.0 * D * ((double)total_q * nq * (gate ? 3 : 2) + 2.0 * total_k * nk), 0, nullptr);
     return TQF_HIP_OK;

@@ -52,7 +52,8 @@ struct PromptArgs {
     uint16_t *y;
     int32_t *status;
 };
-hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a);
+size_t attn_prompt_scratch_bytes(const PromptArgs &a);
+hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a, void *scratch);
 
 struct PagedArgs {
     HeadRows q, gate;

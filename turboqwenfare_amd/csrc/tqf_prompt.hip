@@ -14,7 +14,8 @@
 // as they stand: the order in which an instruction takes its K elements is free so
 // long as both operands have the same.  V^T comes from LDS by transposing reads.
 // A workgroup's wavefronts share tiles of K and V, and so, where heads are
-// grouped, are heads of one group at the same rows.
+// grouped, are heads of one group at the same rows.  Where there are few rows the
+// keys are dealt out to several workgroups, and a second kernel joins their sums.
 //
 // Keys that a row does not see have weight 0, but 0 * inf and 0 * NaN are NaN.
 // Rows behind a sequence's end read as zeros (the copies' bounds).  Tiles that some
@@ -30,13 +31,31 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kAhead = 4;  // products that LDS reads go ahead of theirs
+constexpr uint32_t kMaxParts = 32;
+
 struct Kernel {
     PromptArgs a;
     uint32_t head_waves;  // wavefronts of a workgroup that have heads of their own (of one group)
     uint32_t head_sets;   // q_heads / head_waves
     uint32_t turn;        // workgroups from here on are taken from the end
     float scale_log2;
+    float *o, *top_sum;  // of each part: [total_q][q_heads][dim], and [total_q][q_heads][2]
 };
+
+// The workgroup's place in the order of work, blockIdx.x of gridDim.x.
+__device__ __forceinline__ uint32_t number_of(const Kernel &p) { return blockIdx.x < p.turn ? blockIdx.x : gridDim.x - 1 - (blockIdx.x - p.turn); }
+
+// 8 elements of a row, with its gate (16 bytes) if it has one.
+__device__ __forceinline__ void store_row(float (&v)[8], bool gated, u32x4 gate, uint16_t *y) {
+    if (gated) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] *= sigmoid(__uint_as_float(gate[e] << 16));
+            v[2 * e + 1] *= sigmoid(__uint_as_float(gate[e] & 0xFFFF0000u));
+        }
+    }
+    *reinterpret_cast<u32x4 *>(y) = u32x4{bf16_bits2(v[0], v[1]), bf16_bits2(v[2], v[3]), bf16_bits2(v[4], v[5]), bf16_bits2(v[6], v[7])};
+}
 
 // The sequence and the tile in it of a workgroup's tile number; false: none.
 struct Place {
@@ -102,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 32, half = l / 32;
     const uint32_t tokens = 32u * kWaves / p.head_waves;  // of the workgroup
     Place at;
-    const uint32_t number = blockIdx.x < p.turn ? blockIdx.x : gridDim.x - 1 - (blockIdx.x - p.turn);
+    const uint32_t number = number_of(p);
     if (!find_place(a, number / p.head_sets, tokens, at)) return;
     const uint32_t head = number % p.head_sets * p.head_waves + (uint32_t)wave % p.head_waves;
     const uint32_t kv = __builtin_amdgcn_readfirstlane(head / (a.q_heads / a.kv_heads));
@@ -111,11 +130,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const int first = (int)(__builtin_amdgcn_readfirstlane(at.tile) * tokens), mine = first + 32 * (wave / (int)p.head_waves);
     const int shift = lk - lq;
     const int row = mine + r < lq ? mine + r : lq - 1;  // rows past the end do as the last one and are not stored
-    const int limit = row + shift;                       // the last key that the lane's row sees
+    auto last_key = [&] {  // that the lane's row sees (with heads of 256 what a lane can make anew has no register)
+        const int at = mine + here(l) % 32;
+        return (at < lq ? at : lq - 1) + shift;
+    };
     const int limit_min = (mine < lq ? mine : lq - 1) + shift;
     const int limit_max = (mine + 31 < lq ? mine + 31 : lq - 1) + shift;
     const int last = (first + (int)tokens < lq ? first + (int)tokens : lq) - 1 + shift;  // of the workgroup
     const bool live = mine < lq;
+    // tiles of the part: [begin, end) of those that the workgroup's rows see
+    const uint32_t tiles = last >= 0 ? (uint32_t)last / KT + 1 : 0, part = blockIdx.y, parts = gridDim.y;  // at most 2^26, 2^5
+    const int begin = __builtin_amdgcn_readfirstlane(tiles * part / parts), end = __builtin_amdgcn_readfirstlane(tiles * (part + 1) / parts);
 
     bf16x8 q[kSteps];  // those that wait are not kept here
     auto waits = [](int i) { return kWaiting && i % 4 == 3; };
@@ -155,34 +180,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     // copy's with constant bits flipped, and the rows' distance a scalar, so an offset is one instruction.  Scalar offsets
     // are not held against the descriptor's end: the sequence's last tile, whose rows may end, has whole ones (copy_last).
     constexpr int kCopyRows = 1024 / kRow, kRowLanes = kRow / 16;
-    const uint32_t copy_row = l / kRowLanes, copy_tile_row = wave * kCopies * kCopyRows + copy_row;
-    const uint32_t k_chunk = (l % kRowLanes ^ k_swizzle<D>(copy_tile_row)) * 16, v_chunk = (l % kRowLanes ^ v_swizzle<D>(copy_tile_row)) * 16;
-    const uint32_t k_first = copy_row * k_row, v_first = copy_row * v_row;
+    const int copy_rows = wave * kCopies * kCopyRows;  // those of the wavefronts before
     auto copy_last = [&](const uint8_t *from, uint32_t row_bytes, bool of_k, int kt, uint8_t *to) {
         const uint32_t rows = lk - kt * KT < KT ? lk - kt * KT : KT;
         const Desc d = make_desc(from + (size_t)kt * KT * row_bytes, (rows - 1) * row_bytes + kRow);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const uint32_t rr = copy_tile_row + i * kCopyRows;
+            const uint32_t rr = copy_rows + i * kCopyRows + l / kRowLanes;
             copy16(d, rr * row_bytes + (l % kRowLanes ^ (of_k ? k_swizzle<D>(rr) : v_swizzle<D>(rr))) * 16, to + (wave * kCopies + i) * 1024);
         }
     };
-    // A tile all of whose rows are there.  Before the first one there are none: nothing is in such a descriptor's bounds,
-    // and zeros go to LDS.  No branch, so that the copies can stand among the products, one after each.
+    // A tile all of whose rows are there.  Before the part's first one there are none: nothing is in such a descriptor's
+    // bounds, and zeros go to LDS.  No branch, so that the copies can stand among the products, one after each.
     struct Tile {
         Desc d;
-        uint32_t step;  // from copy to copy
+        uint32_t step;          // from copy to copy
+        uint32_t chunk, first;  // the lane's: 16 bytes of a row, and the row of the first copy
     };
-    auto tile_at = [&](const uint8_t *from, uint32_t row_bytes, int kt) {
-        return Tile{make_desc(from + (size_t)(kt < 0 ? 0 : kt) * KT * row_bytes, kt < 0 ? 0 : 0xFFFFFFFFu), kt < 0 ? 0 : kCopyRows * row_bytes};
+    auto tile_at = [&](const uint8_t *from, uint32_t row_bytes, bool of_k, int kt) {
+        const bool any = kt >= begin;
+        const uint32_t lane = D == 256 ? here(l) : l, row = copy_rows + lane / kRowLanes;
+        return Tile{make_desc(from + (size_t)(any ? kt : 0) * KT * row_bytes, any ? 0xFFFFFFFFu : 0), any ? kCopyRows * row_bytes : 0,
+                    (lane % kRowLanes ^ (of_k ? k_swizzle<D>(row) : v_swizzle<D>(row))) * 16, lane / kRowLanes * row_bytes};
     };
-    auto copy_k = [&](const Tile &t, int i, uint8_t *to) {
+    auto k_tile = [&](int kt) { return tile_at(kp, k_row, true, kt); };
+    auto v_tile = [&](int kt) { return tile_at(vp, v_row, false, kt); };
+    auto copy = [&](const Tile &t, bool of_k, int i, uint8_t *to) {
         const uint32_t n = wave * kCopies + i;
-        copy16(t.d, (here(k_chunk) ^ k_swizzle<D>(i * kCopyRows) * 16) + k_first, n * t.step, to + n * 1024);
-    };
-    auto copy_v = [&](const Tile &t, int i, uint8_t *to) {
-        const uint32_t n = wave * kCopies + i;
-        copy16(t.d, (here(v_chunk) ^ v_swizzle<D>(i * kCopyRows) * 16) + v_first, n * t.step, to + n * 1024);
+        copy16(t.d, (t.chunk ^ (of_k ? k_swizzle<D>(i * kCopyRows) : v_swizzle<D>(i * kCopyRows)) * 16) + t.first, n * t.step, to + n * 1024);
     };
     auto values = [&](const uint8_t *sv, uint32_t v0, int j, int st, int d) {
         const uint8_t *at_v = sv + (v0 ^ (d % 4 * 64)) + (d / 4 * 256 + (j * 32 + st * 16) * kRow);
@@ -209,6 +234,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     auto edge_step = [&](f32x16 (&s)[kSub], const uint8_t *sv, int kt) {
         const bool part = kt * KT + KT - 1 > limit_min;  // some row of the wavefront
         if (part) {
+            const int limit = last_key();
 #pragma unroll
             for (int j = 0; j < kSub; ++j)
 #pragma unroll
@@ -269,7 +295,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         // and the exponentials' instructions stand between the products, in their shadow.
         f32x16 s[kSub];
         const uint32_t k0_at = k_at();
-        const Tile next_k = tile_at(kp, k_row, kt - 1), next_v = tile_at(vp, v_row, kt - 1);
+        Tile next = k_tile(kt - 1);
         auto keys = [&](int n) {
             const int j = n / kSteps, i = n % kSteps;
             return *reinterpret_cast<const bf16x8 *>(sk + (k0_at ^ (i % 8 * 32)) + (i / 8 * 256 + j * 32 * kRow));
@@ -285,8 +311,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
                                                                     n % kSteps ? s[n / kSteps] : zero, 0, 0, 0);
             if (kWaiting && n % 4 == 0) waited = *reinterpret_cast<const bf16x8 *>(waiting + n % kSteps / 4 * 1024 + here(l) * 16);
             if (n + kAhead < kSub * kSteps) ahead_k[n % kAhead] = keys(n + kAhead);
-            if (n < kCopies) copy_k(next_k, n, other_k);
-            else if (n < 2 * kCopies) copy_v(next_v, n - kCopies, other_v);
+            if (n == kCopies) next = v_tile(kt - 1);
+            if (n < kCopies) copy(next, true, n, other_k);
+            else if (n < 2 * kCopies) copy(next, false, n - kCopies, other_v);
         }
         __builtin_amdgcn_sched_barrier(0);
         float top = s[0][0];
@@ -332,18 +359,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         }
     };
 
-    if (last >= 0) {
-        int kt = last / KT;
+    if (begin < end) {
+        int kt = end - 1;
         copy_last(kp, k_row, true, kt, s_k0);
         copy_last(vp, v_row, false, kt, s_v0);
         auto copy_before = [&](uint8_t *other_k, uint8_t *other_v) {
-            const Tile k = tile_at(kp, k_row, kt - 1), v = tile_at(vp, v_row, kt - 1);
+            const Tile k = k_tile(kt - 1), v = v_tile(kt - 1);
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) copy_k(k, i, other_k), copy_v(v, i, other_v);
+            for (int i = 0; i < kCopies; ++i) copy(k, true, i, other_k), copy(v, false, i, other_v);
         };
         const int edge = (first + shift + 1 > 0 ? first + shift + 1 : 0) / KT;  // all rows see all of the tiles before this
         bool second = false;
-        for (; kt >= edge; --kt) {
+        for (; kt >= edge && kt >= begin; --kt) {
             publish();
             copy_before(second ? s_k0 : s_k1, second ? s_v0 : s_v1);
             if (live && kt * KT <= limit_max) {
@@ -359,10 +386,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             else copy_before(other_k, other_v);
             --kt;
         };
-        if (second && kt >= 0) whole(s_k1, s_v1, s_k0, s_v0);
-        while (kt >= 0) {
+        if (second && kt >= begin) whole(s_k1, s_v1, s_k0, s_v0);
+        while (kt >= begin) {
             whole(s_k0, s_v0, s_k1, s_v1);
-            if (kt < 0) break;
+            if (kt < begin) break;
             whole(s_k1, s_v1, s_k0, s_v0);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -384,7 +411,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
                 for (int e = 0; e < 8; ++e) dot = __builtin_fmaf((float)x[e], (float)z[e], dot);
             }
             dot += __shfl_xor(dot, 32);
-            if (key > limit) continue;
+            if (key > last_key()) continue;
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, p.scale_log2, m == -kInf ? 0.0f : -m));
             const uint16_t *vr = reinterpret_cast<const uint16_t *>(vp + (size_t)key * v_row) + half * 4;
 #pragma unroll
@@ -402,29 +429,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     if (!live) return;
     uint8_t *const out = wave == 0 ? s_k0 : wave == 1 ? s_v0 : wave == 2 ? s_k1 : s_v1;
     sum += __shfl_xor(sum, 32);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     const size_t first_row = (size_t)(q0 + mine);
     const int rows = lq - mine < 32 ? lq - mine : 32, lane = here(l), row_of = lane / kLanes, at_dim = lane % kLanes * 8;
+    if (parts > 1 && half == 0 && r < rows) {
+        float *const to = p.top_sum + (((size_t)part * a.total_q + first_row + r) * a.q_heads + head) * 2;
+        to[0] = m, to[1] = sum;
+    }
+    float *const part_o = p.o + (((size_t)part * a.total_q + first_row) * a.q_heads + head) * D + at_dim;
     uint16_t *const y = a.y + (first_row * a.q_heads + head) * D + at_dim;
     const uint16_t *const gate = static_cast<const uint16_t *>(a.gate.d) + first_row * a.gate.row + (size_t)head * a.gate.head + at_dim;
 #pragma unroll
-    for (int part = 0; part < D / kOut; ++part) {
+    for (int piece = 0; piece < D / kOut; ++piece) {
 #pragma unroll
         for (int d = 0; d < kOut / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = o[part * (kOut / 32) + d][i + e] * inv;
+                for (int e = 0; e < 4; ++e) v[e] = o[piece * (kOut / 32) + d][i + e] * inv;
                 const int c = d * 8 + 2 * (i / 4) + half;
                 *reinterpret_cast<f32x4 *>(out + r * (kOut * 4) + (c ^ (r & (kOut / 4 - 1))) * 16) = v;
             }
         u32x4 g[32 * kLanes / 64];
-        if (a.gate.d) {
+        if (a.gate.d && parts == 1) {
 #pragma unroll
             for (int i = 0; i < 32 * kLanes / 64; ++i) {
                 const int rr = i * (64 / kLanes) + row_of;
-                g[i] = *reinterpret_cast<const u32x4 *>(gate + (size_t)(rr < rows ? rr : 0) * a.gate.row + part * kOut);
+                g[i] = *reinterpret_cast<const u32x4 *>(gate + (size_t)(rr < rows ? rr : 0) * a.gate.row + piece * kOut);
             }
         }
 #pragma unroll
@@ -437,39 +469,127 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) v[4 * e + u] = x[u];
             }
-            if (a.gate.d) {
+            if (rr >= rows) continue;
+            if (parts == 1) {
+                store_row(v, a.gate.d, g[i], y + (size_t)rr * a.q_heads * D + piece * kOut);
+            } else {
+                float *const to = part_o + (size_t)rr * a.q_heads * D + piece * kOut;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[2 * e] *= sigmoid(__uint_as_float(g[i][e] << 16));
-                    v[2 * e + 1] *= sigmoid(__uint_as_float(g[i][e] & 0xFFFF0000u));
-                }
-            }
-            if (rr < rows) {
-                const u32x4 bits = {bf16_bits2(v[0], v[1]), bf16_bits2(v[2], v[3]), bf16_bits2(v[4], v[5]), bf16_bits2(v[6], v[7])};
-                *reinterpret_cast<u32x4 *>(y + (size_t)rr * a.q_heads * D + part * kOut) = bits;
+                for (int e = 0; e < 2; ++e) *reinterpret_cast<f32x4 *>(to + 4 * e) = f32x4{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
             }
         }
     }
 }
 
+// Joins the parts: what each summed counts exp2(its maximum - the largest).  A wavefront has as many of the rows of one
+// of the parts' as it can read at once, 8 dimensions to a lane.
+template <int D>
+__global__ __launch_bounds__(64 * kWaves) void prompt_join_kernel(Kernel p, int parts) {
+    constexpr int kLanes = D / 8, kRows = 64 / kLanes, kAtOnce = 8;
+    const PromptArgs &a = p.a;
+    const int wave = threadIdx.x / 64, l = threadIdx.x % 64;
+    const uint32_t tokens = 32u * kWaves / p.head_waves, number = number_of(p);
+    Place at;
+    if (!find_place(a, number / p.head_sets, tokens, at)) return;
+    const uint32_t head = number % p.head_sets * p.head_waves + (uint32_t)wave % p.head_waves;
+    const int mine = (int)(at.tile * tokens) + 32 * (wave / (int)p.head_waves);
+    const int i = blockIdx.y * kRows + l / kLanes;
+    if (mine + i < at.lq) {
+        const size_t row = ((size_t)(at.q0 + mine + i)) * a.q_heads + head, step = (size_t)a.total_q * a.q_heads;
+        const int at_dim = l % kLanes * 8;
+        float top = -kInf, sum = 0.0f, v[8] = {};
+        for (int n0 = 0; n0 < parts; n0 += kAtOnce) {
+            float2 ms[kAtOnce];
+            f32x4 x[kAtOnce][2];
+            float most = top;
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const size_t n = n0 + u < parts ? n0 + u : parts - 1;
+                ms[u] = *reinterpret_cast<const float2 *>(p.top_sum + (n * step + row) * 2);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[u][e] = *reinterpret_cast<const f32x4 *>(p.o + (n * step + row) * D + at_dim + 4 * e);
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) most = fmaxf(most, ms[u].x);
+            // without a maximum there are zeros, or NaN, which stay
+            const float keep = top == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - most);
+            top = most;
+            sum *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= keep;
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (n0 + u >= parts) break;
+                const float take = ms[u].x == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ms[u].x - top);
+                sum = __builtin_fmaf(ms[u].y, take, sum);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(x[u][e / 4][e % 4], take, v[e]);
+            }
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        u32x4 gate = {};
+        if (a.gate.d)
+            gate = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.gate.d) + (size_t)(at.q0 + mine + i) * a.gate.row + (size_t)head * a.gate.head + at_dim);
+        store_row(v, a.gate.d, gate, a.y + row * D + at_dim);
+    }
+}
+
+// How the work is cut: workgroups, and parts that each one's keys are dealt into.
+struct Cutting {
+    uint32_t head_waves, head_sets, groups, parts;
+};
+Cutting cutting_of(const PromptArgs &a) {
+    Cutting c{1, 0, 0, 1};
+    const uint32_t group = a.q_heads / a.kv_heads;
+    while (c.head_waves < kWaves && group % (c.head_waves * 2) == 0) c.head_waves *= 2;
+    c.head_sets = a.q_heads / c.head_waves;
+    const uint32_t tokens = 32 * kWaves / c.head_waves;
+    c.groups = (a.total_q / tokens + a.n_seqs) * c.head_sets;  // at least as many as there are
+    // Few rows before many keys: a workgroup needs about 1 us for a tile, whatever else runs, and the join 5, so
+    // sequences (the usual one here: their lengths are the device's) of 16 tiles are cut while workgroups find a place.
+    // 4096 keys: 32 rows of 16 heads of 256 134 us whole, 33 in parts, 1024 rows 136 and 95; 32 of 32 of 128 70 and 18.
+    const uint32_t places = (a.dim == 64 ? 4 : 2) * (uint32_t)cu_count(), tiles = a.total_k / a.n_seqs / (a.dim == 256 ? 32 : 64);
+    if (tiles >= 16) {
+        c.parts = places / c.groups < tiles / 4 ? places / c.groups : tiles / 4;
+        c.parts = c.parts < 1 ? 1 : c.parts < kMaxParts ? c.parts : kMaxParts;
+    }
+    return c;
+}
+
+template <int D, int KT>
+hipError_t launch_for(hipStream_t s, const Kernel &p, const Cutting &cut) {
+    prompt_kernel<D, KT><<<dim3(cut.groups, cut.parts), dim3(64 * kWaves), 0, s>>>(p);
+    if (cut.parts > 1) {
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        prompt_join_kernel<D><<<dim3(cut.groups, 32 * D / 512), dim3(64 * kWaves), 0, s>>>(p, (int)cut.parts);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
-hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a) {
-    Kernel p{a, 1, 0, 0, a.scale * kLog2e};
-    const uint32_t group = a.q_heads / a.kv_heads;
-    while (p.head_waves < kWaves && group % (p.head_waves * 2) == 0) p.head_waves *= 2;
-    p.head_sets = a.q_heads / p.head_waves;
-    const uint32_t tokens = 32 * kWaves / p.head_waves;
-    const uint64_t tiles = (uint64_t)a.total_q / tokens + a.n_seqs;  // at least as many as there are
-    const dim3 grid((uint32_t)(tiles * p.head_sets)), block(64 * kWaves);
+size_t attn_prompt_scratch_bytes(const PromptArgs &a) {
+    const Cutting cut = cutting_of(a);
+    return cut.parts == 1 ? 0 : (size_t)cut.parts * a.total_q * a.q_heads * (a.dim + 2) * 4;
+}
+
+hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a, void *scratch) {
+    const Cutting cut = cutting_of(a);
+    Kernel p{a, cut.head_waves, cut.head_sets, 0, a.scale * kLog2e, nullptr, nullptr};
+    if (cut.parts > 1) {
+        p.o = static_cast<float *>(scratch);
+        p.top_sum = p.o + (size_t)cut.parts * a.total_q * a.q_heads * a.dim;
+    }
     // Tiles of a prompt begin with the longest, and what is free first takes the next.  Where all run at once, two to
     // a compute unit, the second of each comes from the end, so that their sums are alike.
     const uint32_t cus = (uint32_t)cu_count();
-    p.turn = a.n_seqs == 1 && grid.x > cus && grid.x <= 2 * cus + p.head_sets ? cus : grid.x;
-    if (a.dim == 64) prompt_kernel<64, 64><<<grid, block, 0, s>>>(p);
-    if (a.dim == 128) prompt_kernel<128, 64><<<grid, block, 0, s>>>(p);
-    if (a.dim == 256) prompt_kernel<256, 32><<<grid, block, 0, s>>>(p);
-    return hipGetLastError();
+    p.turn = a.n_seqs == 1 && cut.groups > cus && cut.groups <= 2 * cus + p.head_sets ? cus : cut.groups;
+    if (a.dim == 64) return launch_for<64, 64>(s, p, cut);
+    if (a.dim == 128) return launch_for<128, 64>(s, p, cut);
+    return launch_for<256, 32>(s, p, cut);
 }
 
 }  // namespace tqf

@@ -19,10 +19,14 @@ between stages:
   ``tqf_hip_lm_head_logits_device``);
 - draft head: ``x = h_prev + embed(d_prev)``, then ``x += MoE_mtp(rmsnorm(x))``
   (one Q4_0 MoE layer, the sidecar's FFN), then its final norm and the shared
-  LM head. This build has no attention at all, so each verify row is computed
-  from its own token, and the draft head's attention and its
-  embedding/hidden projection are out of scope. The sum stands in for that
-  projection;
+  LM head. The draft head's attention and its embedding/hidden projection are
+  out of scope. The sum stands in for that projection;
+- attention: none unless the model is made with ``attention``, and each verify
+  row is then computed from its own token. With it, attention layers stand in
+  front of the MoE layers (attention.py): the generation starts from a whole
+  prompt, whose keys and values fill a cache, a verify row attends to what is
+  in front of it, and the drafts that were not accepted are forgotten with
+  the cache's length;
 - selection: greedy takes the LM head's fused top-1
   (``top_logit_candidates``). Stochastic, with ``sampler="fast"`` (the
   default), makes one draw from E_x / S of the row: the acceptance kernel at
@@ -63,6 +67,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from . import mtp, synth
+from .attention import AttentionLayers
 from .backend import DeviceBuffer
 from .sampling import Sampler
 from .workloads import H, SyntheticStack
@@ -84,7 +89,9 @@ def q6k_synthetic(rows: int, cols: int, seed: int) -> np.ndarray:
 
 class MtpModel:
     """The resident pieces of the loop:
-    - the target stack (``n_layers`` seeded Q4_0 MoE layers);
+    - the target stack (``n_layers`` seeded Q4_0 MoE layers). With
+      ``attention``, a dict of keywords of ``AttentionLayers``, it is a stack
+      for each MoE layer (``parts``) with an attention layer in front;
     - the draft head's MoE layer;
     - a Q4_0 embedding [vocab x H];
     - the target and draft final-norm weights;
@@ -93,9 +100,14 @@ class MtpModel:
     The host copies the oracle needs are kept as well."""
 
     def __init__(self, be, n_layers: int, vocab: int, seed: int = 0, recipe: str = "zero_mean",
-                 log=None):
-        self.be, self.vocab, self.seed = be, vocab, seed
-        self.target = SyntheticStack(be, n_layers, seed=seed, recipe=recipe, log=log)
+                 log=None, attention: dict | None = None):
+        self.be, self.vocab, self.seed, self.n_layers = be, vocab, seed, n_layers
+        self.target, self.parts, self.attention = None, [], None
+        if attention is None:
+            self.target = SyntheticStack(be, n_layers, seed=seed, recipe=recipe, log=log)
+        else:
+            self.attention = AttentionLayers(be, n_layers, **{"seed": seed, **attention})
+            self.parts = [SyntheticStack(be, 1, seed=seed, recipe=recipe, log=log, first_layer=l) for l in range(n_layers)]
         self.draft = SyntheticStack(be, 1, seed=seed, recipe=recipe, first_layer=DRAFT_FIRST_LAYER)
         self.embed = be.synth_q4_0(vocab, H, EMBED_TENSOR, seed, recipe)
         self.norm_host = (1.0 + 0.05 * synth.normal((H,), seed=seed + 11)).astype(np.float32)
@@ -111,7 +123,10 @@ class MtpModel:
 
     def free(self) -> None:
         be = self.be
-        self.target.free()
+        if self.attention is not None:
+            self.attention.free()
+        for stack in self.parts if self.target is None else [self.target]:
+            stack.free()
         self.draft.free()
         be.free_weights(self.embed)
         be.free_tensor(self.norm)
@@ -134,7 +149,8 @@ class StepRecord:
 class MtpLoop:
     """The loop's policy and accounting over an engine that runs the passes
     (``DeviceEngine`` on the HIP backend):
-    - ``engine.start(token)`` -> (first token, trace);
+    - ``engine.start(token)`` -> (first token, trace); the token may be a
+      whole prompt where the engine's model has attention;
     - ``engine.plain(step, boundary)`` -> (token, trace);
     - ``engine.speculative(step, boundary)`` -> (emitted tokens, accepted, trace).
     See the module docstring for the policy."""
@@ -153,7 +169,7 @@ class MtpLoop:
         c = self.controller
         return c.enabled or len(c.window) < c.window_capacity
 
-    def start(self, token: int) -> StepRecord:
+    def start(self, token) -> StepRecord:
         t, trace = self.engine.start(token)
         self.boundary = t
         return StepRecord([t], -1, False, self.controller.enabled, trace)
@@ -173,7 +189,7 @@ class MtpLoop:
         enabled = self.controller.record_and_decide(a + 1)
         return StepRecord(emitted, a, True, enabled, trace)
 
-    def run(self, token: int, steps: int) -> list:
+    def run(self, token, steps: int) -> list:
         """start(token), then `steps` steps; the records of all of them."""
         out = [self.start(token)]
         for _ in range(steps):
@@ -201,7 +217,9 @@ class DeviceEngine:
         # the plain-decode picks' Sampler (reference mode): Sampler::new's
         # generator, seeded once per generation
         self.ref_sampler = Sampler(be, temperature, seed) if sampler == "reference" and not greedy else None
-        V, m, L = model.vocab, k + 1, max(model.target.n_layers, 1)
+        V, m, L = model.vocab, k + 1, max(model.n_layers, 1)
+        self.length = 0  # tokens in the attention layers' caches
+        self.attended = None  # host copies of the attention layers' stages since the pass began (tracing)
         self.d_tok = be.alloc(4 * m)
         self.d_hin, self.d_h, self.d_hn = (be.alloc(4 * m * H) for _ in range(3))
         self.d_target = be.alloc(4 * m * V)
@@ -210,6 +228,9 @@ class DeviceEngine:
         self.d_t4, self.d_l4 = be.alloc(16 * m), be.alloc(16 * m)
         self.d_ids, self.d_w = be.alloc(2 * 8 * m * L), be.alloc(4 * 8 * m * L)
         self.d_status = be.alloc(4)
+        if model.attention is not None:  # a prompt's rows
+            n = model.attention.max_tokens
+            self.d_prompt, self.d_rows = be.alloc(4 * n), be.alloc(4 * n * H)
         self.d_sel_u, self.d_sel_acc, self.d_sel_tok = be.alloc(4), be.alloc(4), be.alloc(4 * m)
         # a speculative step's host traffic, one write and one read: the verify
         # rows' tokens (boundary, then the drafts as the device picks them),
@@ -227,13 +248,37 @@ class DeviceEngine:
 
     def _target_pass(self, tokens: list) -> None:
         """d_h <- stack(embed(tokens)); d_hn <- rmsnorm; d_target <- LM head."""
+        self.be.write(self.d_tok, np.asarray(tokens, np.int32))
+        self._target_pass_device(self.d_tok, len(tokens))
+
+    def _room(self, n: int) -> None:
+        a = self.model.attention
+        if a is not None and self.length + n > a.max_tokens:
+            raise ValueError(f"{self.length} + {n} tokens in a cache of {a.max_tokens}")
+
+    def _layers(self, d_h: DeviceBuffer, n: int, at: int) -> None:
+        """d_h <- the target's layers, rows at positions at..at + n of the sequence."""
+        be, md = self.be, self.model
+        if md.attention is None:
+            be.stack_forward_device(md.target.stack, d_h, n, self.d_ids, self.d_w, self.d_status)
+            return
+        for l, part in enumerate(md.parts):
+            md.attention.forward(l, d_h, n, at, self.d_status, self.attended)
+            for first in range(0, n, self.k + 1):
+                rows = min(n - first, self.k + 1)
+                be.stack_forward_device(part.stack, be.view(d_h, 4 * first * H, 4 * rows * H), rows, self.d_ids, self.d_w, self.d_status)
+
+    def _prompt_pass(self, tokens: list) -> None:
+        """Fills the caches with a prompt; row 0 of d_hin, d_h, d_hn and d_target are its last token's."""
         be, md, n = self.be, self.model, len(tokens)
-        be.write(self.d_tok, np.asarray(tokens, np.int32))
-        be.embed_rows_device(md.embed, self.d_tok, n, self.d_hin, d_status=self.d_status)
-        be.copy_device(self.d_h, self.d_hin, 4 * n * H)
-        be.stack_forward_device(md.target.stack, self.d_h, n, self.d_ids, self.d_w, self.d_status)
-        be.rmsnorm_rows_device(self.d_h, n, H, md.norm, self.d_hn)
-        be.lm_head_logits_device(md.lm_head, self.d_hn, n, self.d_target, self.d_t4, self.d_l4)
+        be.write(self.d_prompt, np.asarray(tokens, np.int32))
+        be.embed_rows_device(md.embed, self.d_prompt, n, self.d_rows, d_status=self.d_status)
+        last = be.view(self.d_rows, 4 * (n - 1) * H, 4 * H)
+        be.copy_device(self.d_hin, last, 4 * H)
+        self._layers(self.d_rows, n, 0)
+        be.copy_device(self.d_h, last, 4 * H)
+        be.rmsnorm_rows_device(self.d_h, 1, H, md.norm, self.d_hn)
+        be.lm_head_logits_device(md.lm_head, self.d_hn, 1, self.d_target, self.d_t4, self.d_l4)
 
     def _pick(self, d_logits: DeviceBuffer, row: int, uniform: float) -> int:
         """One token from logits row `row` of the last LM head call: its
@@ -266,25 +311,48 @@ class DeviceEngine:
         if not self.trace_on:
             return {}
         n, V = len(tokens), self.model.vocab
-        return dict(tokens=list(tokens), hin=self._snap(self.d_hin, (n, H)),
+        attended, self.attended = self.attended, None
+        return dict(tokens=list(tokens), **({"attention": attended} if attended is not None else {}), hin=self._snap(self.d_hin, (n, H)),
                     h=self._snap(self.d_h, (n, H)), hn=self._snap(self.d_hn, (n, H)),
                     target=self._snap(self.d_target, (n, V)), u_select=u)
 
     # ---- the passes ----------------------------------------------------------------------
-    def start(self, token: int):
-        """A plain decode of the prompt's last token."""
-        if not 0 <= token < self.model.vocab:
-            raise ValueError("token out of vocabulary")
+    def start(self, token):
+        """A plain decode of the prompt's last token; with attention, of a whole prompt (one token or several), which
+        begins a sequence."""
+        md = self.model
+        prompt = [int(t) for t in np.atleast_1d(np.asarray(token))]
+        if not prompt or not all(0 <= t < md.vocab for t in prompt):
+            raise ValueError("token out of vocabulary" if prompt else "an empty prompt")
+        if md.attention is None:
+            if len(prompt) != 1:
+                raise ValueError("a prompt of several tokens needs a model with attention")
+            return self.plain(None, prompt[0], self._plain_uniform(4, None))
+        self.length = 0
+        self._room(len(prompt))
         u = self._plain_uniform(4, None)
-        return self.plain(None, token, u)
+        self._begin_trace()
+        self._prompt_pass(prompt)
+        t = self._pick(self.d_target, 0, u)
+        self._check_status()
+        self.length = len(prompt)
+        self.be.copy_device(self.d_hprev, self.d_h, 4 * H)
+        return t, self._plain_trace(prompt[-1:], u)
+
+    def _begin_trace(self) -> None:
+        if self.trace_on and self.model.attention is not None:
+            self.attended = []
 
     def plain(self, step, boundary: int, u: float | None = None):
         """One token without drafts; its hidden row becomes h_prev."""
+        self._room(1)
         if u is None:
             u = self._plain_uniform(3, step)
+        self._begin_trace()
         self._target_pass([boundary])
         t = self._pick(self.d_target, 0, u)
         self._check_status()
+        self.length += 1
         self.be.copy_device(self.d_hprev, self.d_h, 4 * H)
         return t, self._plain_trace([boundary], u)
 
@@ -298,6 +366,7 @@ class DeviceEngine:
         uniforms) before it and one read (drafts, acceptance) after it, unless
         tracing."""
         be, md, k, V = self.be, self.model, self.k, self.model.vocab
+        self._room(k + 1)
         u = synth.philox_uniforms(self.seed + step, 0, k)
         ur = synth.philox_uniforms(self.seed + step, 1, k + 1)
         ud = synth.philox_uniforms(self.seed + step, 2, k)
@@ -311,14 +380,17 @@ class DeviceEngine:
         be.write(self.d_io, io)
         trace = dict(draft_x=[], draft_y=[], draft_yn=[]) if self.trace_on else {}
         # draft: x = h_prev + embed(d_prev); x += MoE_mtp(rmsnorm(x)); logits
-        stack, norm = (md.target, md.norm) if self.self_draft else (md.draft, md.draft_norm)
+        norm = md.norm if self.self_draft else md.draft_norm
         be.copy_device(self.d_x, self.d_hprev, 4 * H)
         for i in range(k):
             be.embed_rows_device(md.embed, self._io(w_tok + i), 1, self.d_x,
                                  d_add=None if self.self_draft else self.d_x, d_status=self.d_status)
             if self.trace_on:
                 trace["draft_x"].append(self._snap(self.d_x, (H,)))
-            be.stack_forward_device(stack.stack, self.d_x, 1, self.d_ids, self.d_w, self.d_status)
+            if self.self_draft:
+                self._layers(self.d_x, 1, self.length + i)
+            else:
+                be.stack_forward_device(md.draft.stack, self.d_x, 1, self.d_ids, self.d_w, self.d_status)
             be.rmsnorm_rows_device(self.d_x, 1, H, norm, self.d_xn)
             d_row = be.view(self.d_draft, 4 * i * V, 4 * V)
             be.lm_head_logits_device(md.lm_head, self.d_xn, 1, d_row, self.d_t4, self.d_l4)
@@ -337,6 +409,7 @@ class DeviceEngine:
                                  self.d_sel_acc, self.d_sel_tok)
                 be.copy_device(self._io(w_tok + 1 + i), be.view(self.d_sel_tok, 0, 4), 4)
         # verify and accept
+        self._begin_trace()
         self._target_pass_device(self._io(w_tok, k + 1), k + 1)
         be.accept_device(self.d_target, None if self.greedy else self.d_draft, self._io(w_tok + 1, k),
                          k, V, self.T, self.greedy, None if self.greedy else self._io(w_u, k),
@@ -349,6 +422,7 @@ class DeviceEngine:
         if a < 0:
             raise RuntimeError("the acceptance kernel reported a timed-out exchange")
         emitted = [int(v) for v in out[w_toks:w_toks + a + 1]]
+        self.length += a + 1  # the boundary and what was accepted; the last emitted token is the next pass's first
         if self.trace_on:
             trace.update(self._plain_trace([boundary] + drafts, None))
             trace.update(drafts=drafts, u=u, ur=ur, ud=ud, draft=self._snap(self.d_draft, (k, V)))
@@ -357,11 +431,11 @@ class DeviceEngine:
         return emitted, a, trace
 
     def _target_pass_device(self, d_tokens: DeviceBuffer, n: int) -> None:
-        """_target_pass over tokens already on the device."""
+        """_target_pass over tokens already on the device, behind those in the caches."""
         be, md = self.be, self.model
         be.embed_rows_device(md.embed, d_tokens, n, self.d_hin, d_status=self.d_status)
         be.copy_device(self.d_h, self.d_hin, 4 * n * H)
-        be.stack_forward_device(md.target.stack, self.d_h, n, self.d_ids, self.d_w, self.d_status)
+        self._layers(self.d_h, n, self.length)
         be.rmsnorm_rows_device(self.d_h, n, H, md.norm, self.d_hn)
         be.lm_head_logits_device(md.lm_head, self.d_hn, n, self.d_target, self.d_t4, self.d_l4)
 

@@ -546,7 +546,7 @@ Cutting cutting_of(const PromptArgs &a) {
     while (c.head_waves < kWaves && group % (c.head_waves * 2) == 0) c.head_waves *= 2;
     c.head_sets = a.q_heads / c.head_waves;
     const uint32_t tokens = 32 * kWaves / c.head_waves;
-    c.groups = (a.total_q / tokens + a.n_seqs) * c.head_sets;  // at least as many as there are
+    c.groups = (uint32_t)(((uint64_t)a.total_q + (uint64_t)a.n_seqs * (tokens - 1)) / tokens) * c.head_sets;  // at least as many as there are
     // Few rows before many keys: a workgroup needs about 1 us for a tile, whatever else runs, and the join 5, so
     // sequences (the usual one here: their lengths are the device's) of 16 tiles are cut while workgroups find a place.
     // 4096 keys: 32 rows of 16 heads of 256 134 us whole, 33 in parts, 1024 rows 136 and 95; 32 of 32 of 128 70 and 18.
@@ -586,7 +586,7 @@ hipError_t launch_attn_prompt(hipStream_t s, const PromptArgs &a, void *scratch)
     // Tiles of a prompt begin with the longest, and what is free first takes the next.  Where all run at once, two to
     // a compute unit, the second of each comes from the end, so that their sums are alike.
     const uint32_t cus = (uint32_t)cu_count();
-    p.turn = a.n_seqs == 1 && cut.groups > cus && cut.groups <= 2 * cus + p.head_sets ? cus : cut.groups;
+    p.turn = a.n_seqs == 1 && cut.groups > cus && cut.groups <= 2 * cus ? cus : cut.groups;
     if (a.dim == 64) return launch_for<64, 64>(s, p, cut);
     if (a.dim == 128) return launch_for<128, 64>(s, p, cut);
     return launch_for<256, 32>(s, p, cut);

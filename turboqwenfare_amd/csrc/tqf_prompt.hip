@@ -142,16 +142,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const uint32_t tiles = last >= 0 ? (uint32_t)last / KT + 1 : 0, part = blockIdx.y, parts = gridDim.y;  // at most 2^26, 2^5
     const int begin = __builtin_amdgcn_readfirstlane(tiles * part / parts), end = __builtin_amdgcn_readfirstlane(tiles * (part + 1) / parts);
 
-    bf16x8 q[kSteps];  // those that wait are not kept here
-    auto waits = [](int i) { return kWaiting && i % 4 == 3; };
-    uint8_t *const waiting = s_q + wave * kWaiting * 1024;
-    const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + (size_t)(q0 + row) * a.q.row + (size_t)head * a.q.head + half * 8;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8 *>(qp + i * 16);
-        if (waits(i)) *reinterpret_cast<bf16x8 *>(waiting + i / 4 * 1024 + l * 16) = x;
-        else q[i] = x;
-    }
     f32x16 o[kDims];
 #pragma unroll
     for (int i = 0; i < kDims; ++i)
@@ -209,6 +199,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         const uint32_t n = wave * kCopies + i;
         copy16(t.d, (t.chunk ^ (of_k ? k_swizzle<D>(i * kCopyRows) : v_swizzle<D>(i * kCopyRows)) * 16) + t.first, n * t.step, to + n * 1024);
     };
+    // The first tile is asked for before the rows.
+    if (begin < end) {
+        copy_last(kp, k_row, true, end - 1, s_k0);
+        copy_last(vp, v_row, false, end - 1, s_v0);
+    }
+    bf16x8 q[kSteps];  // those that wait are not kept here
+    auto waits = [](int i) { return kWaiting && i % 4 == 3; };
+    uint8_t *const waiting = s_q + wave * kWaiting * 1024;
+    const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + (size_t)(q0 + row) * a.q.row + (size_t)head * a.q.head + half * 8;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8 *>(qp + i * 16);
+        if (waits(i)) *reinterpret_cast<bf16x8 *>(waiting + i / 4 * 1024 + l * 16) = x;
+        else q[i] = x;
+    }
     auto values = [&](const uint8_t *sv, uint32_t v0, int j, int st, int d) {
         const uint8_t *at_v = sv + (v0 ^ (d % 4 * 64)) + (d / 4 * 256 + (j * 32 + st * 16) * kRow);
         const uint2 x = read_transposed(at_v), y = read_transposed(at_v + 8 * kRow);
@@ -361,8 +366,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
 
     if (begin < end) {
         int kt = end - 1;
-        copy_last(kp, k_row, true, kt, s_k0);
-        copy_last(vp, v_row, false, kt, s_v0);
         auto copy_before = [&](uint8_t *other_k, uint8_t *other_v) {
             const Tile k = k_tile(kt - 1), v = v_tile(kt - 1);
 #pragma unroll

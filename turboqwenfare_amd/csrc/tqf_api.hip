@@ -2471,14 +2471,13 @@ int32_t check_heads(tqf_hip_ctx *ctx, const tqf_hip_heads *h) {
     return TQF_HIP_OK;
 }
 
-int32_t check_rows(tqf_hip_ctx *ctx, const tqf_hip_head_rows *r, uint64_t t, uint32_t heads, uint32_t dim) {
+int32_t check_rows(tqf_hip_ctx *ctx, const tqf_hip_head_rows *r, uint64_t t, uint32_t dim) {
     if (!r || !r->data) return fail(ctx, TQF_HIP_ERR_INVALID, "null pointer");
     if (!aligned_to(r->data, 16) || r->row_stride % 8 || r->head_stride % 8)
         return fail(ctx, TQF_HIP_ERR_INVALID, "rows of heads must be aligned to 16 bytes and their strides be multiples of 8");
     if (r->row_stride >= kMaxStride || r->head_stride >= kMaxStride)
         return fail(ctx, TQF_HIP_ERR_INVALID, "strides must be below 2^24");
     if (t > 1 && r->row_stride < dim) return fail(ctx, TQF_HIP_ERR_INVALID, "row_stride must be at least head_dim");
-    (void)heads;
     return TQF_HIP_OK;
 }
 // Bytes from the first element of the rows to behind the last.
@@ -2573,9 +2572,9 @@ extern "C" int32_t tqf_hip_qk_rope_device(tqf_hip_ctx *ctx, const tqf_hip_heads 
     const uint32_t D = heads->head_dim, nq = heads->q_heads, nk = heads->kv_heads;
     if (!valid_type(x_type)) return fail(ctx, TQF_HIP_ERR_INVALID, "unknown element type");
     if (t == 0 || t > TQF_HIP_F8_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "t must be in 1..65536");
-    if (int32_t rc = check_rows(ctx, q, t, nq, D)) return rc;
-    if (int32_t rc = check_rows(ctx, k, t, nk, D)) return rc;
-    if (int32_t rc = check_rows(ctx, v, t, nk, D)) return rc;
+    if (int32_t rc = check_rows(ctx, q, t, D)) return rc;
+    if (int32_t rc = check_rows(ctx, k, t, D)) return rc;
+    if (int32_t rc = check_rows(ctx, v, t, D)) return rc;
     if ((options->q_norm && (!options->q_norm->data || options->q_norm->count != D)) ||
         (options->k_norm && (!options->k_norm->data || options->k_norm->count != D)))
         return fail(ctx, TQF_HIP_ERR_INVALID, "a norm's weights must be f32 [head_dim]");
@@ -2638,13 +2637,13 @@ extern "C" int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_he
     if (total_q == 0 || total_q > TQF_HIP_ATTN_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "total_q must be in 1..2^20");
     if (total_k >= (1u << 31)) return fail(ctx, TQF_HIP_ERR_INVALID, "total_k must be below 2^31");
     if (n_seqs == 0 || n_seqs > TQF_HIP_ATTN_MAX_SEQS) return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs must be in 1..16384");
-    if (int32_t rc = check_rows(ctx, q, total_q, nq, D)) return rc;
+    if (int32_t rc = check_rows(ctx, q, total_q, D)) return rc;
     if (total_k) {
-        if (int32_t rc = check_rows(ctx, k, total_k, nk, D)) return rc;
-        if (int32_t rc = check_rows(ctx, v, total_k, nk, D)) return rc;
+        if (int32_t rc = check_rows(ctx, k, total_k, D)) return rc;
+        if (int32_t rc = check_rows(ctx, v, total_k, D)) return rc;
     }
     if (gate)
-        if (int32_t rc = check_rows(ctx, gate, total_q, nq, D)) return rc;
+        if (int32_t rc = check_rows(ctx, gate, total_q, D)) return rc;
     if (!aligned_to(d_y, 16) || !aligned_to(d_cu_q, 4) || !aligned_to(d_cu_k, 4) || !aligned_to(d_status, 4))
         return fail(ctx, TQF_HIP_ERR_INVALID, "y must be aligned to 16 bytes, integers to 4");
     const Range y{d_y, (size_t)total_q * nq * D * 2};
@@ -2688,9 +2687,9 @@ extern "C" int32_t tqf_hip_attn_paged_device(tqf_hip_ctx *ctx, const tqf_hip_hea
     if ((uint64_t)n_seqs * heads->kv_heads * (((uint64_t)max_pages * cache->page_size + 127) / 128 + 1) >= (uint64_t(1) << 31))
         return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs * kv_heads * (max_pages * page_size / 128 + 1) must be below 2^31");
     const uint64_t t = (uint64_t)n_seqs * rows;
-    if (int32_t rc = check_rows(ctx, q, t, nq, D)) return rc;
+    if (int32_t rc = check_rows(ctx, q, t, D)) return rc;
     if (gate)
-        if (int32_t rc = check_rows(ctx, gate, t, nq, D)) return rc;
+        if (int32_t rc = check_rows(ctx, gate, t, D)) return rc;
     if (!aligned_to(d_y, 16) || !aligned_to(d_pages, 4) || !aligned_to(d_lens, 4) || !aligned_to(d_status, 4))
         return fail(ctx, TQF_HIP_ERR_INVALID, "y must be aligned to 16 bytes, integers to 4");
     const Range y{d_y, (size_t)t * nq * D * 2}, none{nullptr, 0};

@@ -117,6 +117,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     // unit's): with all of them in registers there are too few for anything else.
     constexpr int kWaiting = D == 256 ? 4 : 0;
     __shared__ __attribute__((aligned(16))) uint8_t s_q[kWaiting ? kWaves * kWaiting * 1024 : 16];
+    // Two wavefronts of different workgroups share a SIMD, and the older one goes first where both could: priorities in
+    // the keys' products, the softmax and the values' products keep them at different ones.  8192 rows and keys, without:
+    // 16 heads of 256 526 us, now 484; 32 of 128 509 and 503 (4096: 146 and 137; with those of 256 140); of 64 298, with
+    // either of the two 300 and 304.
+    constexpr int kPriority[3] = {D == 256 ? 2 : 0, D == 256 ? 1 : 0, D == 128 ? 1 : 0};
     const PromptArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 32, half = l / 32;
     const uint32_t tokens = 32u * kWaves / p.head_waves;  // of the workgroup
@@ -306,6 +311,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             return *reinterpret_cast<const bf16x8 *>(sk + (k0_at ^ (i % 8 * 32)) + (i / 8 * 256 + j * 32 * kRow));
         };
         bf16x8 ahead_k[kAhead], waited = {};
+        __builtin_amdgcn_s_setprio(kPriority[0]);
 #pragma unroll
         for (int n = 0; n < kAhead; ++n) ahead_k[n] = keys(n);
 #pragma unroll
@@ -321,6 +327,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             else if (n < 2 * kCopies) copy(next, false, n - kCopies, other_v);
         }
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(kPriority[1]);
         float top = s[0][0];
 #pragma unroll
         for (int j = 0; j < kSub; ++j)
@@ -351,6 +358,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
         bf16x8 w[2];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[0][i] = weight(0, i);
+        __builtin_amdgcn_s_setprio(kPriority[2]);
 #pragma unroll
         for (int n = 0; n < kGroups * kDims; ++n) {
             const int g = n / kDims, d = n % kDims, then = n + kAhead;
@@ -384,6 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             second = !second;
         }
         auto whole = [&](const uint8_t *sk, const uint8_t *sv, uint8_t *other_k, uint8_t *other_v) {
+            __builtin_amdgcn_s_setprio(0);
             publish();
             if (live) step(sk, sv, other_k, other_v, kt);
             else copy_before(other_k, other_v);

@@ -630,7 +630,8 @@ int32_t tqf_hip_qk_rope_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, con
  * (gate NULL: no factor), y [total_q x q_heads x head_dim].  Rows that see no key
  * are 0; keys that a row does not see do not change it, NaN or not; rows of y
  * outside every sequence stay as they are.  Scores, maxima and sums are f32,
- * weights are rounded to bf16 for their product with v.  A sequence whose bounds
+ * weights are rounded to bf16 for their product with v; the order of the sums depends
+ * on the number of sequences and the totals.  A sequence whose bounds
  * are out of order or range is left out and sets *d_status (may be NULL, zeroed by the
  * caller) to TQF_HIP_ERR_INVALID; y is then undefined.  scale > 0.  1 <= total_q <=
  * TQF_HIP_ATTN_MAX_TOKENS, total_k < 2^31 (0: k and v are not read), 1 <= n_seqs <=

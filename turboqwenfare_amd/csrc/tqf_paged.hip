@@ -14,6 +14,11 @@
 // the keys.  Wavefronts take 32 keys of a step each, by themselves, and join theirs
 // in LDS at the end.
 //
+// One sequence of 131072 tokens (2 key heads of 256, bf16) takes 60 us, of which the
+// join 8: 4.5 TB/s; 256 of 4000 (8 heads of 128) 713 us, 5.9 TB/s, as fast as reads
+// go on this card.  Between them stand the join and, with sequences of many lengths,
+// what each costs beside its bytes (64 of 50..8192 tokens, 4 rows: 64 us, 3.0 TB/s).
+//
 // As in tqf_prompt.hip: S^T = K Q^T (here 16 x 16 x 32) leaves a row's weights as an
 // operand of O^T = V^T P^T; V^T comes from LDS by transposing reads; infinities and
 // NaN among values that only some rows see are added at the end, key by key.
@@ -67,8 +72,10 @@ __device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
 // (the caller has checked the most there can be).  Before the steps of each stand
 // `extra` places for what beginning and ending it costs: without them a part of
 // many short sequences takes longer than one of a long one (64 sequences of 50 to
-// 8192 tokens, 4 rows of heads of 256: 92 us, with one place 77).  All results are the same in
-// every lane, and the compiler is told so: descriptors made of them stay scalar.
+// 8192 tokens, 4 rows of 16 heads of 256: 86 us without, 64 with one place; 96 in
+// e4m3, 32 heads of 128: 89 and 76; one long sequence: 60 either way).  All results
+// are the same in every lane, and the compiler is told so: descriptors made of them
+// stay scalar.
 struct Line {
     uint32_t mine, upto;  // of sequence `lane`: places of a key head; places of all heads of the sequences up to it
     uint32_t total;
@@ -577,7 +584,9 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
 // Joins what several parts have of one (sequence, key head): a workgroup for each
 // cut and `each` rows.  With one row its wavefronts have some of the parts each, with
 // several, if the parts are few, a row each.  Sixteen wavefronts for the one (cut into
-// 128 parts: 7.4 us, with eight 9.1), eight for the other.
+// 128 parts: 7.4 us, with eight 9.1), eight for the other.  Cuts are kept by unit
+// where those are fewer than the parts, so that only as many workgroups look for
+// one: one sequence of 131072 tokens 60 us, a cut for each part 111.
 constexpr int kJoinWaves = 16, kJoinAhead = 4;
 template <int D>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_t block_rows, uint32_t each) {
@@ -688,7 +697,8 @@ hipError_t launch_for(hipStream_t s, const Kernel &p) {
     else paged_kernel<D, NR, false><<<grid, block, 0, s>>>(p);
     if (p.parts > 1) {
         if (const hipError_t e = hipGetLastError()) return e;
-        // a workgroup a row while there are few, else eight rows: more workgroups would wait for one another's places
+        // A workgroup a row while there are few, else eight rows: more workgroups would wait for one another's places.
+        // 64 sequences of 4 rows of 16 heads: 64 us with eight, 90 with one; one sequence of 131072 tokens: 110 and 60.
         const uint32_t rows = p.a.rows * p.group, cuts = cuts_of(p.a), each = cuts * rows <= 1024 ? 1 : 8;
         join_kernel<D><<<dim3(cuts * ((rows + each - 1) / each)), dim3(each == 1 ? 1024 : 512), 0, s>>>(p, 16 * NR, each);
     }

@@ -17,6 +17,14 @@
 // grouped, are heads of one group at the same rows.  Where there are few rows the
 // keys are dealt out to several workgroups, and a second kernel joins their sums.
 //
+// Bound by how a wavefront's products, softmax and LDS reads take turns: the matrix
+// cores are busy for 56% of 8192 rows' time (32 heads of 128: 500 us, 1.1 PFLOP/s;
+// large library products reach 1.26 on this card).  4096 rows of 16 heads of 256 take
+// 160 us, 0.86 PFLOP/s: the last row's workgroup has all 128 tiles, 1.1 us each when
+// it is alone on its compute unit, where two together need 0.8 for one.  Dealing out
+// such rows' keys too costs more in the join than it saves (167 us), and so do eight
+// wavefronts that have every other tile each and wait for one another (178).
+//
 // Keys that a row does not see have weight 0, but 0 * inf and 0 * NaN are NaN.
 // Rows behind a sequence's end read as zeros (the copies' bounds).  Tiles that some
 // rows see in part are looked through for infinities and NaN; where there are any,
@@ -561,7 +569,7 @@ Cutting cutting_of(const PromptArgs &a) {
     c.groups = (uint32_t)(((uint64_t)a.total_q + (uint64_t)a.n_seqs * (tokens - 1)) / tokens) * c.head_sets;  // at least as many as there are
     // Few rows before many keys: a workgroup needs about 1 us for a tile, whatever else runs, and the join 5, so
     // sequences (the usual one here: their lengths are the device's) of 16 tiles are cut while workgroups find a place.
-    // 4096 keys: 32 rows of 16 heads of 256 134 us whole, 33 in parts, 1024 rows 136 and 95; 32 of 32 of 128 70 and 18.
+    // 4096 keys: 32 rows of 16 heads of 256 134 us whole, 31 in parts, 1024 rows 136 and 86; 32 of 32 of 128 70 and 18.
     const uint32_t places = (a.dim == 64 ? 4 : 2) * (uint32_t)cu_count(), tiles = a.total_k / a.n_seqs / (a.dim == 256 ? 32 : 64);
     if (tiles >= 16) {
         c.parts = places / c.groups < tiles / 4 ? places / c.groups : tiles / 4;

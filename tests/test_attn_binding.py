@@ -64,13 +64,37 @@ def test_options_of_one_call_do_not_stay_for_the_next(be):
     assert (o.q_norm, o.k_norm, o.rope, o.neighbours) == (None, None, None, 0)
 
 
+def test_packing_has_the_structs_layout():
+    p = backend._AttnStructs
+    at = lambda *path: sum(getattr(k, n).offset for k, n in path)  # noqa: E731
+    o = _lib.QkOptions
+    assert C.sizeof(_lib.HeadRows) == 24 and p.rows.offset == 0 and p.options.offset == 96 and p.heads.offset == 136
+    assert [getattr(o, n).offset for n in ("q_norm", "k_norm", "eps", "rope", "neighbours")] == [0, 8, 16, 24, 32]
+    assert [getattr(_lib.HeadRows, n).offset for n in ("data", "row_stride", "head_stride")] == [0, 8, 16]
+    assert [at((p, "heads"), (_lib.Heads, n)) for n in ("q_heads", "kv_heads", "head_dim")] == [136, 140, 144]
+    assert backend._ROPE_STRUCTS.size == backend._ATTN_STRUCTS.size == 148
+
+
+def test_numbers_that_no_field_holds(be):
+    args = buf(16), buf(32), buf(48), 5
+    for heads in ((1 << 32, 2, 64), (-1, 1, 64)):
+        with pytest.raises(ValueError):
+            be.qk_rope_device(*args, heads, None, buf(80, 1 << 60))
+    with pytest.raises(ValueError):
+        be.qk_rope_device(*args, (4, 2, 64), None, buf(80), eps=1e39)
+    assert be.lib.calls == []
+
+
 def test_attention_calls(be):
     be.attn_prompt_device(buf(16), buf(32), buf(48), (4, 2, 64), buf(64), buf(80), 3, 10, 12, buf(96), d_gate=buf(128), gate_strides=(512, 128))
-    be.attn_paged_device(buf(16), (4, 2, 64), 3, 2, CACHE, buf(64), 4, buf(80), buf(96), scale=0.5)
-    (n1, a), (n2, b) = be.lib.calls
+    (n1, a), = be.lib.calls
     assert n1 == "tqf_hip_attn_prompt_device" and a[2] == 0.125 and a[7:] == (64, 80, 3, 10, 12, 96, None)
     g = struct(a[6], _lib.HeadRows)
     assert (g.data, g.row_stride, g.head_stride) == (128, 512, 128)
+    be.attn_paged_device(buf(16), (4, 2, 64), 3, 2, CACHE, buf(64), 4, buf(80), buf(96), scale=0.5)
+    _, (n2, b) = be.lib.calls
+    q, h = struct(b[3], _lib.HeadRows), struct(b[1], _lib.Heads)
+    assert (q.data, q.row_stride, q.head_stride, h.q_heads, h.kv_heads, h.head_dim) == (16, 256, 64, 4, 2, 64)
     assert n2 == "tqf_hip_attn_paged_device" and b[2] == 0.5 and b[4] is None and b[5:7] == (3, 2) and b[8:] == (64, 4, 80, 96, None)
 
 

@@ -21,6 +21,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import struct
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -51,6 +52,35 @@ def _hold(what: str, *needs) -> None:
     for buf, nbytes in needs:
         if buf.nbytes < nbytes:
             raise ValueError(f"{what}: a buffer of {buf.nbytes} bytes, {nbytes} needed")
+
+
+class _AttnStructs(C.Structure):
+    """The structs of an attention call beside one another, filled by one packing: setting the fields one by one takes
+    three times as long, and more than the smallest call."""
+
+    _fields_ = [("rows", _lib.HeadRows * 4), ("options", _lib.QkOptions), ("heads", _lib.Heads)]
+
+
+_ROPE_STRUCTS = struct.Struct("=9Q24xQQf4xQi4x3I")  # rows of q, k, v; options; heads
+_ATTN_STRUCTS = struct.Struct("=12Q40x3I")  # rows of q, k, v, gate; heads
+_NO_ROWS = (0, 0, 0)
+
+
+def _put(layout: struct.Struct, place: _AttnStructs, *values) -> None:
+    try:
+        layout.pack_into(place, 0, *values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"heads, strides and eps: {e}") from None
+
+
+def _head_rows(what: str, buf: DeviceBuffer, t: int, heads: int, dim: int, strides, nbytes: int):
+    """(address, row stride, head stride) of a ``tqf_hip_head_rows``."""
+    row, head = strides if strides is not None else (heads * dim, dim)
+    if row < 0 or head < 0:
+        raise ValueError(f"{what}: strides must not be negative")
+    if t > 0 and ((t - 1) * row + (heads - 1) * head + dim) * nbytes > buf.nbytes:
+        raise ValueError(f"{what}: rows behind the end of a buffer of {buf.nbytes} bytes")
+    return buf.ptr, row, head
 
 
 def _integers(what: str, a, dtype, low: int, high: int) -> np.ndarray:
@@ -723,26 +753,10 @@ class HipBackend:
                 self.free(b)
 
     @functools.cached_property
-    def _places(self):
-        """The structs that a call's arguments are put in: a context has one call at a time."""
-        rows = [_lib.HeadRows() for _ in range(4)]
-        heads, options = _lib.Heads(), _lib.QkOptions()
-        return [(r, C.byref(r)) for r in rows], (heads, C.byref(heads)), (options, C.byref(options))
-
-    def _heads(self, heads):
-        s, ref = self._places[1]
-        s.q_heads, s.kv_heads, s.head_dim = heads
-        return ref
-
-    def _rows(self, place: int, what: str, buf: DeviceBuffer, t: int, heads: int, dim: int, strides, nbytes: int):
-        row, head = strides if strides is not None else (heads * dim, dim)
-        if row < 0 or head < 0:
-            raise ValueError(f"{what}: strides must not be negative")
-        if t > 0 and ((t - 1) * row + (heads - 1) * head + dim) * nbytes > buf.nbytes:
-            raise ValueError(f"{what}: rows behind the end of a buffer of {buf.nbytes} bytes")
-        s, ref = self._places[0][place]
-        s.data, s.row_stride, s.head_stride = buf.ptr, row, head
-        return ref
+    def _place(self):
+        """What an attention call's structs are put in, and references to them: a context has one call at a time."""
+        p = _AttnStructs()
+        return p, [C.byref(r) for r in p.rows], C.byref(p.options), C.byref(p.heads)
 
     def qk_rope_device(self, d_q: DeviceBuffer, d_k: DeviceBuffer, d_v: DeviceBuffer, t: int, heads, d_positions: DeviceBuffer | None,
                        d_q_out: DeviceBuffer, d_k_out: DeviceBuffer | None = None, d_v_out: DeviceBuffer | None = None,
@@ -756,16 +770,16 @@ class HipBackend:
         xt, what = _row_type(x_type), "qk_rope_device"
         nq, nk, dim = heads
         size, n = _TYPE_BYTES[xt], 2 * t * nk * dim
-        q, k, v = (self._rows(0, what, d_q, t, nq, dim, strides[0], size), self._rows(1, what, d_k, t, nk, dim, strides[1], size),
-                   self._rows(2, what, d_v, t, nk, dim, strides[2], size))
+        q, k, v = (_head_rows(what, d_q, t, nq, dim, strides[0], size), _head_rows(what, d_k, t, nk, dim, strides[1], size),
+                   _head_rows(what, d_v, t, nk, dim, strides[2], size))
         if (d_q_out.nbytes < 2 * t * nq * dim or (d_k_out and d_k_out.nbytes < n) or (d_v_out and d_v_out.nbytes < n)
                 or (d_positions and d_positions.nbytes < 4 * t) or (d_slots and d_slots.nbytes < 4 * t)):
             raise ValueError(f"{what}: a buffer is too small for {t} rows")
-        o, options = self._places[2]
-        o.q_norm, o.k_norm, o.eps = q_norm.handle if q_norm else None, k_norm.handle if k_norm else None, eps
-        o.rope, o.neighbours = rope.handle if rope else None, _PAIRS[pairs]
+        place, rows, options, h = self._place
+        _put(_ROPE_STRUCTS, place, *q, *k, *v, q_norm.handle if q_norm else 0, k_norm.handle if k_norm else 0, eps, rope.handle if rope else 0,
+             _PAIRS[pairs], nq, nk, dim)
         self._check(self.lib.tqf_hip_qk_rope_device(
-            self.ctx, self._heads(heads), options, q, k, v, xt, t, d_positions.ptr if d_positions else None, d_q_out.ptr,
+            self.ctx, h, options, rows[0], rows[1], rows[2], xt, t, d_positions.ptr if d_positions else None, d_q_out.ptr,
             d_k_out.ptr if d_k_out else None, d_v_out.ptr if d_v_out else None, cache.ref if cache else None,
             d_slots.ptr if d_slots else None, d_status.ptr if d_status else None))
 
@@ -776,28 +790,32 @@ class HipBackend:
         """Causal attention of packed sequences, bf16 (tqf_hip_attn_prompt_device); scale: head_dim^-1/2 unless given."""
         nq, nk, dim = heads
         what = "attn_prompt_device"
-        q, k, v = (self._rows(0, what, d_q, total_q, nq, dim, strides[0], 2), self._rows(1, what, d_k, total_k, nk, dim, strides[1], 2),
-                   self._rows(2, what, d_v, total_k, nk, dim, strides[2], 2))
-        gate = self._rows(3, what, d_gate, total_q, nq, dim, gate_strides, 2) if d_gate else None
+        q, k, v = (_head_rows(what, d_q, total_q, nq, dim, strides[0], 2), _head_rows(what, d_k, total_k, nk, dim, strides[1], 2),
+                   _head_rows(what, d_v, total_k, nk, dim, strides[2], 2))
+        gate = _head_rows(what, d_gate, total_q, nq, dim, gate_strides, 2) if d_gate else _NO_ROWS
         if d_y.nbytes < 2 * total_q * nq * dim or d_cu_q.nbytes < 4 * (n_seqs + 1) or d_cu_k.nbytes < 4 * (n_seqs + 1):
             raise ValueError(f"{what}: a buffer is too small for {total_q} rows of {n_seqs} sequences")
+        place, rows, _, h = self._place
+        _put(_ATTN_STRUCTS, place, *q, *k, *v, *gate, nq, nk, dim)
         self._check(self.lib.tqf_hip_attn_prompt_device(
-            self.ctx, self._heads(heads), dim ** -0.5 if scale is None else scale, q, k, v, gate, d_cu_q.ptr, d_cu_k.ptr, n_seqs,
-            total_q, total_k, d_y.ptr, d_status.ptr if d_status else None))
+            self.ctx, h, dim ** -0.5 if scale is None else scale, rows[0], rows[1], rows[2], rows[3] if d_gate else None, d_cu_q.ptr,
+            d_cu_k.ptr, n_seqs, total_q, total_k, d_y.ptr, d_status.ptr if d_status else None))
 
     def attn_paged_device(self, d_q: DeviceBuffer, heads, n_seqs: int, rows: int, cache: KvCache, d_pages: DeviceBuffer,
                           max_pages: int, d_lens: DeviceBuffer, d_y: DeviceBuffer, scale: float | None = None, q_strides=None,
                           d_gate: DeviceBuffer | None = None, gate_strides=None,
                           d_status: DeviceBuffer | None = None) -> None:
         """Attention of the last `rows` tokens of every sequence over its cache (tqf_hip_attn_paged_device)."""
-        nq, _, dim = heads
+        nq, nk, dim = heads
         t, what = n_seqs * rows, "attn_paged_device"
-        q = self._rows(0, what, d_q, t, nq, dim, q_strides, 2)
-        gate = self._rows(3, what, d_gate, t, nq, dim, gate_strides, 2) if d_gate else None
+        q = _head_rows(what, d_q, t, nq, dim, q_strides, 2)
+        gate = _head_rows(what, d_gate, t, nq, dim, gate_strides, 2) if d_gate else _NO_ROWS
         if d_y.nbytes < 2 * t * nq * dim or d_pages.nbytes < 4 * n_seqs * max_pages or d_lens.nbytes < 4 * n_seqs:
             raise ValueError(f"{what}: a buffer is too small for {rows} rows of {n_seqs} sequences")
+        place, refs, _, h = self._place
+        _put(_ATTN_STRUCTS, place, *q, *_NO_ROWS, *_NO_ROWS, *gate, nq, nk, dim)
         self._check(self.lib.tqf_hip_attn_paged_device(
-            self.ctx, self._heads(heads), dim ** -0.5 if scale is None else scale, q, gate, n_seqs, rows, cache.ref, d_pages.ptr,
+            self.ctx, h, dim ** -0.5 if scale is None else scale, refs[0], refs[3] if d_gate else None, n_seqs, rows, cache.ref, d_pages.ptr,
             max_pages, d_lens.ptr, d_y.ptr, d_status.ptr if d_status else None))
 
     def add_rows_device(self, d_a: DeviceBuffer, d_b: DeviceBuffer, n: int, d_out: DeviceBuffer) -> None:

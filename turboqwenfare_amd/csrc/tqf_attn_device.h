@@ -50,6 +50,10 @@ __device__ __forceinline__ void copy16(Desc d, uint32_t voff, uint32_t soff, voi
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void *)lds, 16, voff, soff, 0, 0);
 }
 
+// 16 bytes at an offset; past the descriptor's end nothing is read (zeros) or written.
+__device__ __forceinline__ u32x4 read16(Desc d, uint32_t voff) { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, voff, 0, 0)); }
+__device__ __forceinline__ void write16(Desc d, uint32_t voff, u32x4 x) { __builtin_amdgcn_raw_buffer_store_b128(x, d, voff, 0, 0); }
+
 // Four rows of 16 elements of 16 bits, transposed: lane i of 16 points at four
 // elements, 4 (i % 4) on, of row i / 4, and gets element i of the four rows.
 __device__ __forceinline__ uint2 read_transposed(const uint8_t *lds) {

@@ -18,9 +18,9 @@
 // keys are dealt out to several workgroups, and a second kernel joins their sums.
 //
 // Bound by how a wavefront's products, softmax and LDS reads take turns: the matrix
-// cores are busy for 56% of 8192 rows' time (32 heads of 128: 500 us, 1.1 PFLOP/s;
+// cores are busy for 56% of 8192 rows' time (32 heads of 128: 490 us, 1.1 PFLOP/s;
 // large library products reach 1.26 on this card).  4096 rows of 16 heads of 256 take
-// 160 us, 0.86 PFLOP/s: the last row's workgroup has all 128 tiles, 1.1 us each when
+// 158 us, 0.87 PFLOP/s: the last row's workgroup has all 128 tiles, 1.1 us each when
 // it is alone on its compute unit, where two together need 0.8 for one.  Dealing out
 // such rows' keys too costs more in the join than it saves (167 us), and so do eight
 // wavefronts that have every other tile each and wait for one another (178).
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const int k0 = __builtin_amdgcn_readfirstlane(at.k0), lk = __builtin_amdgcn_readfirstlane(at.lk);
     const int first = (int)(__builtin_amdgcn_readfirstlane(at.tile) * tokens), mine = first + 32 * (wave / (int)p.head_waves);
     const int shift = lk - lq;
-    const int row = mine + r < lq ? mine + r : lq - 1;  // rows past the end do as the last one and are not stored
+    // rows past the end are zeros, see what the last one does and are not stored
     auto last_key = [&] {  // that the lane's row sees (with heads of 256 what a lane can make anew has no register)
         const int at = mine + here(l) % 32;
         return (at < lq ? at : lq - 1) + shift;
@@ -222,12 +222,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     bf16x8 q[kSteps];  // those that wait are not kept here
     auto waits = [](int i) { return kWaiting && i % 4 == 3; };
     uint8_t *const waiting = s_q + wave * kWaiting * 1024;
-    const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + (size_t)(q0 + row) * a.q.row + (size_t)head * a.q.head + half * 8;
+    {
+        const uint32_t q_row = (uint32_t)a.q.row * 2, rows = live ? (lq - mine < 32 ? lq - mine : 32) : 0, q_at = r * q_row + half * 16;
+        const Desc from = make_desc(static_cast<const uint16_t *>(a.q.d) + (size_t)(q0 + mine) * a.q.row + (size_t)head * a.q.head,
+                                    rows ? (rows - 1) * q_row + D * 2 : 0);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8 *>(qp + i * 16);
-        if (waits(i)) *reinterpret_cast<bf16x8 *>(waiting + i / 4 * 1024 + l * 16) = x;
-        else q[i] = x;
+        for (int i = 0; i < kSteps; ++i) {
+            if (waits(i)) copy16(from, q_at + i * 32, waiting + i / 4 * 1024);
+            else q[i] = __builtin_bit_cast(bf16x8, read16(from, q_at + i * 32));
+        }
     }
     auto values = [&](const uint8_t *sv, uint32_t v0, int j, int st, int d) {
         const uint8_t *at_v = sv + (v0 ^ (d % 4 * 64)) + (d / 4 * 256 + (j * 32 + st * 16) * kRow);
@@ -414,8 +417,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
             if (kt < begin) break;
             whole(s_k1, s_v1, s_k0, s_v0);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies to LDS, also where no tile waited for them
 
     // Tiles with infinities or NaN that only some rows see: key by key.
     while (odd) {

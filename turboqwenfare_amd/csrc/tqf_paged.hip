@@ -530,6 +530,19 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
             mine = m[n] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
             for (int half = 0; half < 16 / kOutRows; ++half) {
+                // gates are asked for before the shares meet: one by one each would be a trip to memory
+                constexpr int kOuts = (kOutRows * kChunks * 2 + 64 * kWaves - 1) / (64 * kWaves);
+                uint2 gates[kOuts] = {};
+                if (whole && a.gate.d) {
+#pragma unroll
+                    for (int x = 0; x < kOuts; ++x) {
+                        const int i = x * 64 * kWaves + wave * 64 + here_l;
+                        uint32_t row_of = block * kRows + n * 16 + half * kOutRows + i / (2 * kChunks);
+                        if (row_of >= all_rows) row_of = all_rows - 1;
+                        gates[x] = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.gate.d) + ((size_t)of_seq * a.rows + row_of / p.group) * a.gate.row +
+                                                                    ((size_t)of_kv * p.group + row_of % p.group) * a.gate.head + i % (2 * kChunks) * 4);
+                    }
+                }
                 // [row][chunk of 4 at chunk ^ row] f32
                 if (here_r / kOutRows == half) {
 #pragma unroll
@@ -566,10 +579,9 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
                         const size_t token = (size_t)of_seq * a.rows + out_row / p.group, head = (size_t)of_kv * p.group + out_row % p.group;
                         v *= inv;
                         if (a.gate.d) {
-                            float gate[4];
-                            four_bf16(static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head + c * 4, gate);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gate[e]);
+                            const uint2 g2 = gates[x / (64 * kWaves)];
+                            v[0] *= sigmoid(__uint_as_float(g2.x << 16)), v[1] *= sigmoid(__uint_as_float(g2.x & 0xFFFF0000u));
+                            v[2] *= sigmoid(__uint_as_float(g2.y << 16)), v[3] *= sigmoid(__uint_as_float(g2.y & 0xFFFF0000u));
                         }
                         store4(a.y + (token * a.q_heads + head) * D + c * 4, 4, v);
                     }

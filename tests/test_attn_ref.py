@@ -111,3 +111,12 @@ def test_rotation_keeps_lengths_and_turns_by_the_distance(pairs):
         assert np.isclose((x * x).sum(), (a * a).sum())
         dots.append((x * y).sum())
     assert np.allclose(dots, dots[0])
+
+
+def test_rows_are_divided_by_a_product():
+    """The paged kernel's row / group for all of its rows (8 queries of groups of up to 256): row * (2^20 / group + 1) >> 20,
+    in 32 bits."""
+    for group in range(1, 257):
+        row = np.arange(8 * group, dtype=np.uint64)
+        product = row * (2 ** 20 // group + 1)
+        assert product.max() < 2 ** 32 and np.array_equal(product >> np.uint64(20), row // group)

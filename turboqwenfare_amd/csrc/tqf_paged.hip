@@ -54,12 +54,16 @@ struct Cut {
 struct Kernel {
     PagedArgs a;
     uint32_t group, row_blocks, parts, page_shift;  // parts: workgroups of a row block
+    uint32_t of_group;                              // 2^20 / group, and one
     float scale_log2;
     uint32_t extra;  // what a (sequence, key head) costs beside its steps, in steps
     bool by_unit;    // cuts [n_seqs x kv_heads], where those are fewer, else [parts]
     Cut *cuts;
     float *partial;  // [2 parts][row_blocks][rows of a block][dim + 2]: values, maximum, sum
 };
+
+// row / group.  Rows are fewer than 2^11 and a group is at most 2^8, so what is too much in row * of_group is below 2^20.
+__device__ __forceinline__ uint32_t query_of(const Kernel &p, uint32_t row) { return row * p.of_group >> 20; }
 
 // Steps of a sequence's one key head: at least one, which writes the rows of an empty sequence.
 __device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
@@ -177,7 +181,7 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
     static_assert(kOutRows * D * 4 == kTile, "shares in the place of values");
     // keys, then values; at the end the rows' sums of values
     __shared__ __attribute__((aligned(1024))) uint8_t s_k[kWaves][kTile], s_v[kWaves][kTile];
-    __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
+    __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows], s_top[kRows], s_sum[kRows];
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid % 64, r = l % 16, g = l / 16;
     const uint32_t part = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
@@ -271,7 +275,7 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
         for (int n = 0; n < NR; ++n) {
             uint32_t row = block * kRows + n * 16 + here_r;
             if (row >= all_rows) row = all_rows - 1;
-            const uint32_t i = row / p.group, head = kv * p.group + row % p.group;
+            const uint32_t i = query_of(p, row), head = kv * p.group + (row - query_of(p, row) * p.group);
             limit[n] = len - (int)a.rows + (int)i;
             const uint16_t *qp = static_cast<const uint16_t *>(a.q.d) + ((size_t)seq * a.rows + i) * a.q.row + (size_t)head * a.q.head;
 #pragma unroll
@@ -524,10 +528,14 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const int row = n * 16 + here_r;
-            float top = s_m[0][row], mine = 0.0f;
+            float top = s_m[0][row], all = 0.0f;
 #pragma unroll
-            for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][row]);
-            mine = m[n] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+            for (int u = 1; u < kWaves; ++u) top = fmaxf(top, s_m[u][row]);
+            const float mine = m[n] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+#pragma unroll
+            for (int u = 0; u < kWaves; ++u)  // a wavefront without keys has sum 0, or NaN where its sequence or a page is bad
+                all += s_m[u][row] == -kInf ? s_l[u][row] : s_l[u][row] * __builtin_amdgcn_exp2f(s_m[u][row] - top);
+            if (wave == 0 && here_g == 0) s_top[row] = top, s_sum[row] = all;
 #pragma unroll
             for (int half = 0; half < 16 / kOutRows; ++half) {
                 // gates are asked for before the shares meet: one by one each would be a trip to memory
@@ -539,8 +547,8 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
                         const int i = x * 64 * kWaves + wave * 64 + here_l;
                         uint32_t row_of = block * kRows + n * 16 + half * kOutRows + i / (2 * kChunks);
                         if (row_of >= all_rows) row_of = all_rows - 1;
-                        gates[x] = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.gate.d) + ((size_t)of_seq * a.rows + row_of / p.group) * a.gate.row +
-                                                                    ((size_t)of_kv * p.group + row_of % p.group) * a.gate.head + i % (2 * kChunks) * 4);
+                        gates[x] = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.gate.d) + ((size_t)of_seq * a.rows + query_of(p, row_of)) * a.gate.row +
+                                                                    ((size_t)of_kv * p.group + (row_of - query_of(p, row_of) * p.group)) * a.gate.head + i % (2 * kChunks) * 4);
                     }
                 }
                 // [row][chunk of 4 at chunk ^ row] f32
@@ -557,26 +565,20 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
                     const int i = x + wave * 64 + here_l, rr = i / (2 * kChunks), c = i % (2 * kChunks), of_block = n * 16 + half * kOutRows + rr;
                     if (kOutRows * kChunks * 2 < 64 * kWaves && rr >= kOutRows) break;
                     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                    float all = s_m[0][of_block], total_l = 0.0f;
+                    const float total_l = s_sum[of_block];
 #pragma unroll
-                    for (int u = 1; u < kWaves; ++u) all = fmaxf(all, s_m[u][of_block]);
-#pragma unroll
-                    for (int u = 0; u < kWaves; ++u) {
-                        v += *reinterpret_cast<const f32x4 *>(s_v[u] + rr * D * 4 + (c ^ rr) * 16);
-                        // a wavefront without keys has sum 0, or NaN where its sequence or a page is bad
-                        total_l += s_m[u][of_block] == -kInf ? s_l[u][of_block] : s_l[u][of_block] * __builtin_amdgcn_exp2f(s_m[u][of_block] - all);
-                    }
+                    for (int u = 0; u < kWaves; ++u) v += *reinterpret_cast<const f32x4 *>(s_v[u] + rr * D * 4 + (c ^ rr) * 16);
                     const uint32_t out_row = block * kRows + of_block;
                     if (!whole) {
                         float *row_to = to + (size_t)of_block * (D + 2);
                         __builtin_memcpy(row_to + c * 4, &v, 16);
                         if (c == 0) {
-                            row_to[D] = all;
+                            row_to[D] = s_top[of_block];
                             row_to[D + 1] = total_l;
                         }
                     } else if (out_row < all_rows) {
                         const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-                        const size_t token = (size_t)of_seq * a.rows + out_row / p.group, head = (size_t)of_kv * p.group + out_row % p.group;
+                        const size_t token = (size_t)of_seq * a.rows + query_of(p, out_row), head = (size_t)of_kv * p.group + (out_row - query_of(p, out_row) * p.group);
                         v *= inv;
                         if (a.gate.d) {
                             const uint2 g2 = gates[x / (64 * kWaves)];
@@ -643,7 +645,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_
     };
     auto store = [&](uint32_t row) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const size_t token = (size_t)cut.seq * a.rows + row / p.group, head = (size_t)cut.kv * p.group + row % p.group;
+        const size_t token = (size_t)cut.seq * a.rows + query_of(p, row), head = (size_t)cut.kv * p.group + (row - query_of(p, row) * p.group);
         const uint16_t *gate = a.gate.d ? static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head : nullptr;
 #pragma unroll
         for (int d = 0; d < kPer; ++d) {
@@ -727,6 +729,7 @@ hipError_t launch_attn_paged(hipStream_t s, const PagedArgs &a, void *scratch) {
     Kernel p{};
     p.a = a;
     p.group = a.q_heads / a.cache.kv_heads;
+    p.of_group = (1u << 20) / p.group + 1;
     p.row_blocks = row_blocks(a);
     p.parts = parts_of(a);
     p.page_shift = (uint32_t)__builtin_ctz(a.cache.page);

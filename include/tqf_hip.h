@@ -653,7 +653,7 @@ int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads,
  * below 0 or above max_pages * page_size, gives NaN rows and sets *d_status (may be
  * NULL, zeroed by the caller) to TQF_HIP_ERR_INVALID.  1 <= n_seqs <=
  * TQF_HIP_ATTN_MAX_SEQS, 1 <= max_pages, max_pages * page_size < 2^31, and n_seqs *
- * kv_heads * (that / 128, rounded up, + 1) too.  y must not overlap the inputs. */
+ * kv_heads * (that / 128, rounded up, + 2) too.  y must not overlap the inputs. */
 int32_t tqf_hip_attn_paged_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale,
                                   const tqf_hip_head_rows *q, const tqf_hip_head_rows *gate, uint32_t n_seqs,
                                   uint32_t rows, const tqf_hip_kv_cache *cache, const int32_t *d_pages,

@@ -2684,8 +2684,8 @@ extern "C" int32_t tqf_hip_attn_paged_device(tqf_hip_ctx *ctx, const tqf_hip_hea
     if (int32_t rc = check_cache(ctx, cache, *heads)) return rc;
     if (max_pages == 0 || (uint64_t)max_pages * cache->page_size >= (uint64_t(1) << 31))
         return fail(ctx, TQF_HIP_ERR_INVALID, "max_pages * page_size must be in 1..2^31 - 1");
-    if ((uint64_t)n_seqs * heads->kv_heads * (((uint64_t)max_pages * cache->page_size + 127) / 128 + 1) >= (uint64_t(1) << 31))
-        return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs * kv_heads * (max_pages * page_size / 128 + 1) must be below 2^31");
+    if ((uint64_t)n_seqs * heads->kv_heads * (((uint64_t)max_pages * cache->page_size + 127) / 128 + 2) >= (uint64_t(1) << 31))
+        return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs * kv_heads * (max_pages * page_size / 128 + 2) must be below 2^31");
     const uint64_t t = (uint64_t)n_seqs * rows;
     if (int32_t rc = check_rows(ctx, q, t, D)) return rc;
     if (gate)

@@ -17,7 +17,7 @@
 // One sequence of 131072 tokens (2 key heads of 256, bf16) takes 60 us, of which the
 // join 8: 4.5 TB/s; 256 of 4000 (8 heads of 128) 713 us, 5.9 TB/s, as fast as reads
 // go on this card.  Between them stand the join and, with sequences of many lengths,
-// what each costs beside its bytes (64 of 50..8192 tokens, 4 rows: 64 us, 3.0 TB/s).
+// what each costs beside its bytes (64 of 50..8192 tokens, 4 rows: 54 us, 3.5 TB/s).
 //
 // As in tqf_prompt.hip: S^T = K Q^T (here 16 x 16 x 32) leaves a row's weights as an
 // operand of O^T = V^T P^T; V^T comes from LDS by transposing reads; infinities and
@@ -72,12 +72,15 @@ __device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, int32_t len) {
     return n ? n : 1;
 }
 
+constexpr uint32_t kMostExtra = 2;
 // The line of all steps: sequence by sequence, key head by key head; fewer than 2^31
 // (the caller has checked the most there can be).  Before the steps of each stand
 // `extra` places for what beginning and ending it costs: without them a part of
 // many short sequences takes longer than one of a long one (64 sequences of 50 to
-// 8192 tokens, 4 rows of 16 heads of 256: 86 us without, 64 with one place; 96 in
-// e4m3, 32 heads of 128: 89 and 76; one long sequence: 60 either way).  All results
+// 8192 tokens, 4 rows of 16 heads of 256: 69 us without, 58 with one place, 54 with
+// two, 55 with three; 96 in e4m3, 32 heads of 128: 89, 75 and 76; 64 rows of 16 heads
+// of 256: one 55, two 53, but 200 of 20 to 2000 tokens 50 and 52; one long sequence:
+// 60 in any case).  All results
 // are the same in every lane, and the compiler is told so: descriptors made of them
 // stay scalar.
 struct Line {
@@ -712,7 +715,7 @@ hipError_t launch_for(hipStream_t s, const Kernel &p) {
     if (p.parts > 1) {
         if (const hipError_t e = hipGetLastError()) return e;
         // A workgroup a row while there are few, else eight rows: more workgroups would wait for one another's places.
-        // 64 sequences of 4 rows of 16 heads: 64 us with eight, 90 with one; one sequence of 131072 tokens: 110 and 60.
+        // 64 sequences of 4 rows of 16 heads: 58 us with eight, 84 with one; one sequence of 131072 tokens: 110 and 60.
         const uint32_t rows = p.a.rows * p.group, cuts = cuts_of(p.a), each = cuts * rows <= 1024 ? 1 : 8;
         join_kernel<D><<<dim3(cuts * ((rows + each - 1) / each)), dim3(each == 1 ? 1024 : 512), 0, s>>>(p, 16 * NR, each);
     }
@@ -734,7 +737,8 @@ hipError_t launch_attn_paged(hipStream_t s, const PagedArgs &a, void *scratch) {
     p.parts = parts_of(a);
     p.page_shift = (uint32_t)__builtin_ctz(a.cache.page);
     p.scale_log2 = a.scale * kLog2e;
-    p.extra = most_steps(a) > p.parts ? 1 : 0;  // with a workgroup for every step there is nothing to balance
+    // with a workgroup for every step there is nothing to balance; two tiles of rows of 256 take longest to leave
+    p.extra = most_steps(a) <= p.parts ? 0 : a.cache.dim * tiles_of_rows(a) >= 512 ? kMostExtra : 1;
     p.by_unit = units_of(a) <= p.parts;
     p.cuts = static_cast<Cut *>(scratch);
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + cuts_bytes(a));

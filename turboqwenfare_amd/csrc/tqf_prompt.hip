@@ -18,7 +18,7 @@
 // keys are dealt out to several workgroups, and a second kernel joins their sums.
 //
 // Bound by how a wavefront's products, softmax and LDS reads take turns: the matrix
-// cores are busy for 56% of 8192 rows' time (32 heads of 128: 490 us, 1.1 PFLOP/s;
+// cores are busy for 59% of 8192 rows' time (32 heads of 128: 490 us, 1.1 PFLOP/s;
 // large library products reach 1.26 on this card).  4096 rows of 16 heads of 256 take
 // 158 us, 0.87 PFLOP/s: the last row's workgroup has all 128 tiles, 1.1 us each when
 // it is alone on its compute unit, where two together need 0.8 for one.  Dealing out

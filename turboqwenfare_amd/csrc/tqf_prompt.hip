@@ -41,7 +41,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kAhead = 4;  // products that LDS reads go ahead of theirs
-constexpr uint32_t kMaxParts = 32;
+constexpr uint32_t kMaxParts = 16;
 
 struct Kernel {
     PromptArgs a;
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     const int last = (first + (int)tokens < lq ? first + (int)tokens : lq) - 1 + shift;  // of the workgroup
     const bool live = mine < lq;
     // tiles of the part: [begin, end) of those that the workgroup's rows see
-    const uint32_t tiles = last >= 0 ? (uint32_t)last / KT + 1 : 0, part = blockIdx.y, parts = gridDim.y;  // at most 2^26, 2^5
+    const uint32_t tiles = last >= 0 ? (uint32_t)last / KT + 1 : 0, part = blockIdx.y, parts = gridDim.y;  // at most 2^26, 2^4
     const int begin = __builtin_amdgcn_readfirstlane(tiles * part / parts), end = __builtin_amdgcn_readfirstlane(tiles * (part + 1) / parts);
 
     f32x16 o[kDims];
@@ -577,13 +577,17 @@ Cutting cutting_of(const PromptArgs &a) {
     c.head_sets = a.q_heads / c.head_waves;
     const uint32_t tokens = 32 * kWaves / c.head_waves;
     c.groups = (uint32_t)(((uint64_t)a.total_q + (uint64_t)a.n_seqs * (tokens - 1)) / tokens) * c.head_sets;  // at least as many as there are
-    // Few rows before many keys: a workgroup needs about 1 us for a tile, whatever else runs, and the join 5, so
-    // sequences (the usual one here: their lengths are the device's) of 16 tiles are cut while workgroups find a place.
-    // 4096 keys: 32 rows of 16 heads of 256 134 us whole, 31 in parts, 1024 rows 136 and 86; 32 of 32 of 128 70 and 18.
-    const uint32_t places = (a.dim == 64 ? 4 : 2) * (uint32_t)cu_count(), tiles = a.total_k / a.n_seqs / (a.dim == 256 ? 32 : 64);
-    if (tiles >= 16) {
-        c.parts = places / c.groups < tiles / 4 ? places / c.groups : tiles / 4;
-        c.parts = c.parts < 1 ? 1 : c.parts < kMaxParts ? c.parts : kMaxParts;
+    // Few rows before many keys: a workgroup needs about 1 us for a tile, whatever else runs, the join 5 and what its
+    // rows' bytes take.  Sequences (the usual one here: their lengths are the device's) of 12 tiles on average are cut as
+    // long as every workgroup has a compute unit to itself, into parts of four tiles at least.  4096 keys, whole and in
+    // parts: 32 rows of 16 heads of 256 124 us and 26 (sixteen; thirty-two 31), 512 rows 124 and 56 (four; eight 60), 2048
+    // rows 137 (two 138); 32 rows of 32 of 128 67 and 18, 512 rows 69 and 51, 1024 rows 77 (two 81).  As many rows as
+    // keys: 1024 of 256 39 and 38, 2048 of 256 71 (two 78), of 128 48 (two 68).
+    const uint32_t keys = a.dim == 256 ? 32 : 64, tiles = a.total_k / a.n_seqs / keys, last = a.total_q / a.n_seqs / keys;
+    const uint32_t usual = tiles - (last < tiles ? last : tiles) / 2, units = (uint32_t)cu_count() / c.groups;
+    if (usual >= 12 && units > 1) {
+        c.parts = units < usual / 4 ? units : usual / 4;
+        if (c.parts > kMaxParts) c.parts = kMaxParts;
     }
     return c;
 }

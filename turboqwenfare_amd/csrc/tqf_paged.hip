@@ -14,10 +14,10 @@
 // the keys.  Wavefronts take 32 keys of a step each, by themselves, and join theirs
 // in LDS at the end.
 //
-// One sequence of 131072 tokens (2 key heads of 256, bf16) takes 60 us, of which the
-// join 8: 4.5 TB/s; 256 of 4000 (8 heads of 128) 713 us, 5.9 TB/s, as fast as reads
+// One sequence of 131072 tokens (2 key heads of 256, bf16) takes 59 us, of which the
+// join 7: 4.5 TB/s; 256 of 4000 (8 heads of 128) 713 us, 5.9 TB/s, as fast as reads
 // go on this card.  Between them stand the join and, with sequences of many lengths,
-// what each costs beside its bytes (64 of 50..8192 tokens, 4 rows: 54 us, 3.5 TB/s).
+// what each costs beside its bytes (64 of 50..8192 tokens, 4 rows: 53 us, 3.6 TB/s).
 //
 // As in tqf_prompt.hip: S^T = K Q^T (here 16 x 16 x 32) leaves a row's weights as an
 // operand of O^T = V^T P^T; V^T comes from LDS by transposing reads; infinities and
@@ -646,24 +646,32 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_
             }
         }
     };
+    // a row's gates, asked for before its parts: behind them they would be a trip to memory more
+    uint16_t gate[kPer];
+    auto ask_gate = [&](uint32_t row) {
+        if (!a.gate.d) return;
+        const size_t token = (size_t)cut.seq * a.rows + query_of(p, row), head = (size_t)cut.kv * p.group + (row - query_of(p, row) * p.group);
+        const void *from = static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head + l * kPer;
+        __builtin_memcpy(gate, __builtin_assume_aligned(from, 2 * kPer), 2 * kPer);
+    };
     auto store = [&](uint32_t row) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const size_t token = (size_t)cut.seq * a.rows + query_of(p, row), head = (size_t)cut.kv * p.group + (row - query_of(p, row) * p.group);
-        const uint16_t *gate = a.gate.d ? static_cast<const uint16_t *>(a.gate.d) + token * a.gate.row + head * a.gate.head : nullptr;
+        uint16_t y[kPer];
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) {
-            const float v = o[d] * inv * (gate ? gate_of(gate[l * kPer + d]) : 1.0f);
-            a.y[(token * a.q_heads + head) * D + l * kPer + d] = __builtin_bit_cast(uint16_t, (__bf16)v);
-        }
+        for (int d = 0; d < kPer; ++d) y[d] = __builtin_bit_cast(uint16_t, (__bf16)(o[d] * inv * (a.gate.d ? gate_of(gate[d]) : 1.0f)));
+        __builtin_memcpy(__builtin_assume_aligned(a.y + (token * a.q_heads + head) * D + l * kPer, 2 * kPer), y, 2 * kPer);
     };
     if (each > 1 && parts <= kJoinWaves) {
         for (uint32_t row = row0 + wave; row < row0 + each && row < all_rows; row += waves) {
+            ask_gate(row);
             gather(row, 0, 1);
             store(row);
         }
         return;
     }
     for (uint32_t row = row0; row < row0 + each && row < all_rows; ++row) {
+        if (wave == 0) ask_gate(row);
         gather(row, wave, waves);
 #pragma unroll
         for (int d = 0; d < kPer; ++d) s_o[wave][l * kPer + d] = o[d];

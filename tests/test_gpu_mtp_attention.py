@@ -166,3 +166,21 @@ def test_refusals(backend, model):
             model.attention.forward(0, eng.d_h, 9, 1)
     finally:
         eng.free()
+
+
+def test_one_sequence_at_a_time(backend, model):
+    """Two engines on a model's caches: the one whose sequence was overwritten does not go on with the other's."""
+    a, b = (DeviceEngine(backend, model, k=K, greedy=True) for _ in range(2))
+    try:
+        with pytest.raises(RuntimeError):
+            a.plain(0, 5)
+        t, _ = a.start(prompt_of(9))
+        t, _ = a.plain(0, t)
+        u, _ = b.start(prompt_of(10))
+        for call in (a.plain, a.speculative):
+            with pytest.raises(RuntimeError):
+                call(1, t)
+        b.speculative(0, u)
+        a.start(prompt_of(9))
+    finally:
+        a.free(), b.free()

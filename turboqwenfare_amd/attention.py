@@ -46,7 +46,8 @@ def f8_synthetic(rows: int, cols: int, seed: int) -> tuple[np.ndarray, np.ndarra
 class AttentionLayers:
     """`n_layers` seeded attention layers of (query heads, key and value heads, head dimension), with a cache of
     `max_tokens` positions each (`cache`: "bf16" or "f8") in pages of `page`.  `rotary` elements of a head turn, by
-    theta^(-2 i / rotary) a position.  One sequence: `forward` is told how many tokens the cache holds."""
+    theta^(-2 i / rotary) a position.  One sequence: `forward` is told how many tokens the cache holds; `sequence` is
+    whoever began the one that is there."""
 
     def __init__(self, be, n_layers: int, heads=(16, 2, 256), rotary: int = 64, theta: float = 1e7, gated: bool = True,
                  max_tokens: int = 4096, page: int = 64, cache: str = "bf16", seed: int = 0):
@@ -60,7 +61,7 @@ class AttentionLayers:
         self.q_width = d * (2 if gated else 1)  # a query head with its gate
         self.width = nq * self.q_width + 2 * nk * d
         self.host, self.norms, self.q_norms, self.k_norms, self.qkv, self.out, self.caches = [], [], [], [], [], [], []
-        self.rope, self._bufs = None, []
+        self.rope, self._bufs, self.sequence = None, [], None
         try:
             self.rope = be.prepare_rope(self.frequencies) if rotary else None
             pages = -(-max_tokens // page)

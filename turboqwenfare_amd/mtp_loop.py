@@ -253,6 +253,8 @@ class DeviceEngine:
 
     def _room(self, n: int) -> None:
         a = self.model.attention
+        if a is not None and a.sequence is not self:
+            raise RuntimeError("the caches hold no sequence of this engine (one at a time: start(prompt) begins it)")
         if a is not None and self.length + n > a.max_tokens:
             raise ValueError(f"{self.length} + {n} tokens in a cache of {a.max_tokens}")
 
@@ -328,7 +330,7 @@ class DeviceEngine:
             if len(prompt) != 1:
                 raise ValueError("a prompt of several tokens needs a model with attention")
             return self.plain(None, prompt[0], self._plain_uniform(4, None))
-        self.length = 0
+        self.length, md.attention.sequence = 0, self
         self._room(len(prompt))
         u = self._plain_uniform(4, None)
         self._begin_trace()

@@ -73,6 +73,9 @@ from .sampling import Sampler
 from .workloads import H, SyntheticStack
 
 EMBED_TENSOR = 2_000_000_000
+# rows of a one-layer stack's call: up to four are plain launches, more a graph of the call, and there are more layers
+# than a context keeps graphs (2048 rows through 40 layers: 481 ms, eight rows at once 1222)
+ROWS_AT_ONCE = 4
 DRAFT_FIRST_LAYER = 999  # the draft head's MoE layer ids: base 1,000,000,000
 
 
@@ -226,7 +229,8 @@ class DeviceEngine:
         self.d_draft = be.alloc(4 * k * V)
         self.d_x, self.d_xn, self.d_hprev = be.alloc(4 * H), be.alloc(4 * H), be.alloc(4 * H)
         self.d_t4, self.d_l4 = be.alloc(16 * m), be.alloc(16 * m)
-        self.d_ids, self.d_w = be.alloc(2 * 8 * m * L), be.alloc(4 * 8 * m * L)
+        routed = m * L if model.attention is None else ROWS_AT_ONCE
+        self.d_ids, self.d_w = be.alloc(2 * 8 * routed), be.alloc(4 * 8 * routed)
         self.d_status = be.alloc(4)
         if model.attention is not None:  # a prompt's rows
             n = model.attention.max_tokens
@@ -266,8 +270,8 @@ class DeviceEngine:
             return
         for l, part in enumerate(md.parts):
             md.attention.forward(l, d_h, n, at, self.d_status, self.attended)
-            for first in range(0, n, self.k + 1):
-                rows = min(n - first, self.k + 1)
+            for first in range(0, n, ROWS_AT_ONCE):
+                rows = min(n - first, ROWS_AT_ONCE)
                 be.stack_forward_device(part.stack, be.view(d_h, 4 * first * H, 4 * rows * H), rows, self.d_ids, self.d_w, self.d_status)
 
     def _prompt_pass(self, tokens: list) -> None:

@@ -47,7 +47,7 @@ class AttentionLayers:
     """`n_layers` seeded attention layers of (query heads, key and value heads, head dimension), with a cache of
     `max_tokens` positions each (`cache`: "bf16" or "f8") in pages of `page`.  `rotary` elements of a head turn, by
     theta^(-2 i / rotary) a position.  One sequence: `forward` is told how many tokens the cache holds; `sequence` is
-    whoever began the one that is there."""
+    whoever began the one that is there (None: none is whole)."""
 
     def __init__(self, be, n_layers: int, heads=(16, 2, 256), rotary: int = 64, theta: float = 1e7, gated: bool = True,
                  max_tokens: int = 4096, page: int = 64, cache: str = "bf16", seed: int = 0):

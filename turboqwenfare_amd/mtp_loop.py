@@ -334,14 +334,15 @@ class DeviceEngine:
             if len(prompt) != 1:
                 raise ValueError("a prompt of several tokens needs a model with attention")
             return self.plain(None, prompt[0], self._plain_uniform(4, None))
-        self.length, md.attention.sequence = 0, self
-        self._room(len(prompt))
+        if len(prompt) > md.attention.max_tokens:
+            raise ValueError(f"{len(prompt)} tokens in a cache of {md.attention.max_tokens}")
         u = self._plain_uniform(4, None)
         self._begin_trace()
+        md.attention.sequence = None  # nobody's, until the prompt is whole in the caches
         self._prompt_pass(prompt)
         t = self._pick(self.d_target, 0, u)
         self._check_status()
-        self.length = len(prompt)
+        self.length, md.attention.sequence = len(prompt), self
         self.be.copy_device(self.d_hprev, self.d_h, 4 * H)
         return t, self._plain_trace(prompt[-1:], u)
 

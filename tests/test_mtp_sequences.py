@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 from test_attention_layers import SMALL, Recorder
+from turboqwenfare_amd import attention
 from turboqwenfare_amd.attention import AttentionLayers
 from turboqwenfare_amd.mtp_loop import DeviceEngine
 
@@ -62,6 +63,19 @@ def test_a_refused_prompt_changes_nothing(bad):
         with pytest.raises(RuntimeError):
             call(0, 1)
     assert positions(be) == []
+
+
+def test_prompts_longer_than_the_projections_take(monkeypatch):
+    monkeypatch.setattr(attention, "F8_MAX_TOKENS", 20)
+    be, layers, (a, b) = engines(2)
+    a.start([1] * 20)
+    be.calls.clear()
+    with pytest.raises(ValueError):
+        b.start([1] * 21)
+    with pytest.raises(ValueError):
+        layers.forward(0, b.d_h, 21, 0)
+    assert be.calls == [] and layers.sequence is a
+    a.plain(0, 1)
 
 
 @pytest.mark.parametrize("what", ["status", "f8_matmul_device", "lm_head_logits_device"])

@@ -24,7 +24,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import synth
-from ._lib import MAX_TOKENS
+from ._lib import F8_MAX_TOKENS, MAX_TOKENS
 from .workloads import H
 
 F8_BLOCK = 128
@@ -57,6 +57,7 @@ class AttentionLayers:
         if rotary < 0 or rotary % 2 or rotary > d:
             raise ValueError("AttentionLayers: rotary is an even number of a head's elements")
         self.be, self.n_layers, self.heads, self.gated, self.max_tokens, self.page = be, n_layers, (nq, nk, d), gated, max_tokens, page
+        self.max_prompt = min(max_tokens, F8_MAX_TOKENS)  # the projections' rows
         self.frequencies = [theta ** (-2.0 * i / rotary) for i in range(rotary // 2)]
         self.q_width = d * (2 if gated else 1)  # a query head with its gate
         self.width = nq * self.q_width + 2 * nk * d
@@ -81,7 +82,7 @@ class AttentionLayers:
             at = np.arange(max_tokens + 1, dtype=np.int32)
             self.d_pages, self.d_count = self._buf(self.table), self._buf(at)
             self.d_slots = self._buf(self.table[at[:-1] // page] * page + at[:-1] % page)
-            rows = max(max_tokens, MAX_TOKENS)
+            rows = max(self.max_prompt, MAX_TOKENS)
             self.d_cu = self._buf(np.zeros(2, np.int32))
             self.d_xn, self.d_o = self._buf(4 * rows * H), self._buf(4 * rows * H)
             self.d_qkv, self.d_q, self.d_y = self._buf(2 * rows * self.width), self._buf(2 * rows * nq * d), self._buf(2 * rows * nq * d)
@@ -95,11 +96,13 @@ class AttentionLayers:
         return self._bufs[-1]
 
     def forward(self, layer: int, d_x, t: int, at: int, d_status=None, trace: list | None = None) -> None:
-        """d_x [t, H] += attention of the rows at positions at..at + t: all of a prompt (at = 0), or up to 8 rows behind
-        the `at` tokens in the cache.  `trace`: host copies of the stages are added to it."""
+        """d_x [t, H] += attention of the rows at positions at..at + t: all of a prompt (at = 0, up to `max_prompt`), or
+        up to 8 rows behind the `at` tokens in the cache.  `trace`: host copies of the stages are added to it."""
         be, (nq, nk, d) = self.be, self.heads
         if t < 1 or at < 0 or at + t > self.max_tokens:
             raise ValueError(f"positions {at}..{at + t} of a cache of {self.max_tokens} tokens")
+        if t > self.max_prompt:
+            raise ValueError(f"at most {self.max_prompt} rows of a prompt")
         if at and t > MAX_TOKENS:
             raise ValueError(f"at most {MAX_TOKENS} rows behind the first of a sequence")
         x = be.read(d_x, np.float32, (t, H)).copy() if trace is not None else None

@@ -233,7 +233,7 @@ class DeviceEngine:
         self.d_ids, self.d_w = be.alloc(2 * 8 * routed), be.alloc(4 * 8 * routed)
         self.d_status = be.alloc(4)
         if model.attention is not None:  # a prompt's rows
-            n = model.attention.max_tokens
+            n = model.attention.max_prompt
             self.d_prompt, self.d_rows = be.alloc(4 * n), be.alloc(4 * n * H)
         self.d_sel_u, self.d_sel_acc, self.d_sel_tok = be.alloc(4), be.alloc(4), be.alloc(4 * m)
         # a speculative step's host traffic, one write and one read: the verify
@@ -334,8 +334,8 @@ class DeviceEngine:
             if len(prompt) != 1:
                 raise ValueError("a prompt of several tokens needs a model with attention")
             return self.plain(None, prompt[0], self._plain_uniform(4, None))
-        if len(prompt) > md.attention.max_tokens:
-            raise ValueError(f"{len(prompt)} tokens in a cache of {md.attention.max_tokens}")
+        if len(prompt) > md.attention.max_prompt:
+            raise ValueError(f"a prompt of {len(prompt)} tokens, at most {md.attention.max_prompt} go into the caches")
         u = self._plain_uniform(4, None)
         self._begin_trace()
         md.attention.sequence = None  # nobody's, until the prompt is whole in the caches

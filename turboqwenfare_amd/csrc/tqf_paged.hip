@@ -271,7 +271,7 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
         if (poison) len = 0;
         table = (const constant_i32 *)(uintptr_t)(a.pages + (size_t)seq * a.max_pages);
         first = (int)(from * kStepKeys) + wave * kWaveKeys;
-        behind = (int)(upto * kStepKeys) < len ? (int)(upto * kStepKeys) : len;
+        behind = upto * kStepKeys < (uint32_t)len ? (int)(upto * kStepKeys) : len;  // the last step may end at 2^31
         // column r of tile n is row block * kRows + 16 n + r, of query row / group and head row % group
         const uint32_t here_r = here(r), here_g = here(g);
 #pragma unroll
@@ -313,10 +313,9 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
             for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[n][s]));
-            int k0 = first;
-            do {
-                const int next = k0 + kStepKeys;
-                const bool more = next < behind;
+            for (int k0 = first;;) {
+                const bool more = behind - k0 > kStepKeys;
+                const int next = more ? k0 + kStepKeys : behind;
                 f32x4 s[2][NR];
                 int64_t row_next[2] = {0, 0};
                 if (more) row_next[0] = find(next), row_next[1] = find(next + 16);
@@ -439,14 +438,15 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
                     }
                 }
                 reads_done();
-                if (more) copy(a.cache.v, row0, next, vl, true);
+                if (!more) break;
+                copy(a.cache.v, row0, next, vl, true);
                 k0 = next;
-            } while (k0 < behind);
+            }
         }
         // Infinities or NaN that only some rows see: key by key.
         if (odd_at >= 0) {
 #pragma unroll 1
-            for (int key = odd_at; key < (odd_at + kWaveKeys < len ? odd_at + kWaveKeys : len); ++key) {
+            for (int key = odd_at; key < len && key - odd_at < kWaveKeys; ++key) {
                 int32_t page = a.pages[(size_t)seq * a.max_pages + ((uint32_t)key >> p.page_shift)];
                 if (page < 0 || (uint32_t)page >= a.cache.n_pages) page = 0;  // noticed before
                 const size_t at_row = ((size_t)page * a.cache.kv_heads + kv) * page_size + ((uint32_t)key & (uint32_t)(page_size - 1));

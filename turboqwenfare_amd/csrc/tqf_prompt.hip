@@ -589,6 +589,9 @@ Cutting cutting_of(const PromptArgs &a) {
         c.parts = units < usual / 4 ? units : usual / 4;
         if (c.parts > kMaxParts) c.parts = kMaxParts;
     }
+    // A workgroup stops looking at the 64 sequences that have its tile.  The totals may allow for no more tiles than there
+    // are, so one more goes through all of the sequences, whose bounds may be wrong behind the last tile too.
+    if (a.n_seqs > 64) c.groups += c.head_sets;
     return c;
 }
 

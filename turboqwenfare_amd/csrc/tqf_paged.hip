@@ -583,7 +583,7 @@ __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kerne
                         const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
                         const size_t token = (size_t)of_seq * a.rows + query_of(p, out_row), head = (size_t)of_kv * p.group + (out_row - query_of(p, out_row) * p.group);
                         v *= inv;
-                        if (a.gate.d) {
+                        if (a.gate.d && total_l != 0.0f) {  // without a key: 0, also where the gate is NaN
                             const uint2 g2 = gates[x / (64 * kWaves)];
                             v[0] *= sigmoid(__uint_as_float(g2.x << 16)), v[1] *= sigmoid(__uint_as_float(g2.x & 0xFFFF0000u));
                             v[2] *= sigmoid(__uint_as_float(g2.y << 16)), v[3] *= sigmoid(__uint_as_float(g2.y & 0xFFFF0000u));
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Kernel p, uint32_
         const size_t token = (size_t)cut.seq * a.rows + query_of(p, row), head = (size_t)cut.kv * p.group + (row - query_of(p, row) * p.group);
         uint16_t y[kPer];
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) y[d] = __builtin_bit_cast(uint16_t, (__bf16)(o[d] * inv * (a.gate.d ? gate_of(gate[d]) : 1.0f)));
+        for (int d = 0; d < kPer; ++d) y[d] = __builtin_bit_cast(uint16_t, (__bf16)(o[d] * inv * (a.gate.d && sum != 0.0f ? gate_of(gate[d]) : 1.0f)));
         __builtin_memcpy(__builtin_assume_aligned(a.y + (token * a.q_heads + head) * D + l * kPer, 2 * kPer), y, 2 * kPer);
     };
     if (each > 1 && parts <= kJoinWaves) {

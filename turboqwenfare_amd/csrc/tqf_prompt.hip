@@ -455,6 +455,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
     uint8_t *const out = wave == 0 ? s_k0 : wave == 1 ? s_v0 : wave == 2 ? s_k1 : s_v1;
     sum += __shfl_xor(sum, 32);
     const float inv = parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint32_t no_keys = (uint32_t)__ballot(sum == 0.0f);  // of 32 rows
     const size_t first_row = (size_t)(q0 + mine);
     const int rows = lq - mine < 32 ? lq - mine : 32, lane = here(l), row_of = lane / kLanes, at_dim = lane % kLanes * 8;
     if (parts > 1 && half == 0 && r < rows) {
@@ -497,7 +498,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_kernel(Kernel p) {
                 const uint32_t at = y_at + i * kSetRows * y_row + piece * (kOut * (whole ? 2 : 4));
                 if constexpr (whole) {
                     float v[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
-                    if (gated) apply_gate(v, g[i]);
+                    if (gated) apply_gate(v, g[i] & ((no_keys >> rr & 1) - 1));  // a row without keys is 0, also where its gate is NaN
                     write16(to, at, bf16_row(v));
                 } else {
                     write16(to, at, __builtin_bit_cast(u32x4, x[0]));
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(64 * kWaves) void prompt_join_kernel(Kernel p, int 
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
-        if (a.gate.d)
+        if (a.gate.d && sum != 0.0f)
             apply_gate(v, *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.gate.d) + (size_t)(at.q0 + mine + i) * a.gate.row +
                                                             (size_t)head * a.gate.head + at_dim));
         *reinterpret_cast<u32x4 *>(a.y + row * D + at_dim) = bf16_row(v);

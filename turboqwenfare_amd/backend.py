@@ -734,6 +734,8 @@ class HipBackend:
 
     def alloc_kv_cache(self, n_pages: int, kv_heads: int, page_size: int, head_dim: int, type: str = "bf16") -> KvCache:
         """A cache in buffers of its own (free_kv_cache gives them back)."""
+        if type not in _CACHE_TYPES:
+            raise ValueError('cache types are "bf16" and "f8"')
         n = n_pages * kv_heads * page_size
         size = 1 if type == "f8" else 2
         sizes = [n * head_dim * size] * 2 + ([4 * n] * 2 if type == "f8" else [])

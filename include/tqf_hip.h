@@ -634,7 +634,7 @@ int32_t tqf_hip_qk_rope_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, con
  * on the number of sequences and the totals.  A sequence whose bounds
  * are out of order or range is left out and sets *d_status (may be NULL, zeroed by the
  * caller) to TQF_HIP_ERR_INVALID; y is then undefined.  scale > 0.  1 <= total_q <=
- * TQF_HIP_ATTN_MAX_TOKENS, total_k < 2^31 (0: k and v are not read), 1 <= n_seqs <=
+ * TQF_HIP_ATTN_MAX_TOKENS, total_k <= 2^31 - 64 (0: k and v are not read), 1 <= n_seqs <=
  * TQF_HIP_ATTN_MAX_SEQS.  y must not overlap the inputs. */
 int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale,
                                    const tqf_hip_head_rows *q, const tqf_hip_head_rows *k, const tqf_hip_head_rows *v,

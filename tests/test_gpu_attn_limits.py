@@ -10,6 +10,8 @@ import pytest
 import attn_ref as ref
 import f8_ref
 from test_gpu_attn_paged import be, bf16  # noqa: F401
+from turboqwenfare_amd._lib import ERR_INVALID, HipError
+from turboqwenfare_amd.backend import DeviceBuffer
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +67,23 @@ def test_lengths_up_to_2_31(be, kind, odd, page):  # noqa: F811
             assert np.isnan(got[1]).all()
         else:
             assert (np.abs(got[row] - want) <= tol).all(), (row, got[row][:4], want[:4], tol[:4])
+
+
+def test_most_keys_of_a_prompt(be):  # noqa: F811
+    """Totals within a tile's 64 keys of 2^31 are refused: such a tile's end has no signed 32-bit number.  (The sequence itself
+    has 5 keys; y lies in front of the keys, which only the total makes long.)"""
+    whole = be.alloc(1 << 16)
+    d_y, d_q, d_cu, d_k = (DeviceBuffer(whole.ptr + at, nbytes) for at, nbytes in ((0, 1 << 12), (1 << 12, 1 << 12), (1 << 13, 64), (1 << 14, 1 << 40)))
+    be.write(whole, np.zeros(1 << 15, np.uint16))
+    be.write(d_cu, np.array([0, 5], np.int32))
+    be.write(d_k, np.full(5 * D, 0x3F80, np.uint16))
+    try:
+        for total in (2 ** 31 - 63, 2 ** 31 - 1):
+            with pytest.raises(HipError) as e:
+                be.attn_prompt_device(d_q, d_k, d_k, (1, 1, D), d_cu, d_cu, 1, 5, total, d_y)
+            assert e.value.status == ERR_INVALID
+        assert not be.read(d_y, np.uint16, (5 * D,)).any()
+        be.attn_prompt_device(d_q, d_k, d_k, (1, 1, D), d_cu, d_cu, 1, 5, 2 ** 31 - 64, d_y)
+        assert (be.read(d_y, np.uint16, (5 * D,)) == 0x3F80).all()
+    finally:
+        be.free(whole)

@@ -2635,7 +2635,8 @@ extern "C" int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_he
     const uint32_t D = heads->head_dim, nq = heads->q_heads, nk = heads->kv_heads;
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, TQF_HIP_ERR_INVALID, "scale must be positive and finite");
     if (total_q == 0 || total_q > TQF_HIP_ATTN_MAX_TOKENS) return fail(ctx, TQF_HIP_ERR_INVALID, "total_q must be in 1..2^20");
-    if (total_k >= (1u << 31)) return fail(ctx, TQF_HIP_ERR_INVALID, "total_k must be below 2^31");
+    // the kernel counts a tile's keys, up to 64, from their first in signed 32 bits
+    if (total_k > (1u << 31) - 64) return fail(ctx, TQF_HIP_ERR_INVALID, "total_k must be at most 2^31 - 64");
     if (n_seqs == 0 || n_seqs > TQF_HIP_ATTN_MAX_SEQS) return fail(ctx, TQF_HIP_ERR_INVALID, "n_seqs must be in 1..16384");
     if (int32_t rc = check_rows(ctx, q, total_q, D)) return rc;
     if (total_k) {

@@ -628,10 +628,11 @@ int32_t tqf_hip_qk_rope_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, con
  * both, a chunk of one more keys.
  *   y[i][h] = sum_j softmax_j(scale q[i][h] . k[j]) v[j] * sigmoid(gate[i][h])
  * (gate NULL: no factor), y [total_q x q_heads x head_dim].  Rows that see no key
- * are 0; keys that a row does not see do not change it, NaN or not; rows of y
- * outside every sequence stay as they are.  Scores, maxima and sums are f32,
- * weights are rounded to bf16 for their product with v; the order of the sums depends
- * on the number of sequences and the totals.  A sequence whose bounds
+ * are 0, whatever their gates; keys that a row does not see do not change it, NaN or
+ * not; rows of y outside every sequence stay as they are.  Scores, maxima and sums are
+ * f32, weights (up to 2^8 before they are divided by their sum: the values' sums of
+ * them must be f32 numbers) are rounded to bf16 for their product with v; the order of
+ * the sums depends on the number of sequences and the totals.  A sequence whose bounds
  * are out of order or range is left out and sets *d_status (may be NULL, zeroed by the
  * caller) to TQF_HIP_ERR_INVALID; y is then undefined.  scale > 0.  1 <= total_q <=
  * TQF_HIP_ATTN_MAX_TOKENS, total_k <= 2^31 - 64 (0: k and v are not read), 1 <= n_seqs <=
@@ -653,7 +654,10 @@ int32_t tqf_hip_attn_prompt_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads,
  * below 0 or above max_pages * page_size, gives NaN rows and sets *d_status (may be
  * NULL, zeroed by the caller) to TQF_HIP_ERR_INVALID.  1 <= n_seqs <=
  * TQF_HIP_ATTN_MAX_SEQS, 1 <= max_pages, max_pages * page_size < 2^31, and n_seqs *
- * kv_heads * (that / 128, rounded up, + 2) too.  y must not overlap the inputs. */
+ * kv_heads * (that / 128, rounded up, + 2) too.  y must not overlap the inputs.
+ * With more than 32 columns (rows * q_heads / kv_heads) the cache is read once for
+ * every 32 of them.  For what is cut the context keeps up to 0.53 MB a column (1.1 GB
+ * for 8 rows of 256 heads on one key head). */
 int32_t tqf_hip_attn_paged_device(tqf_hip_ctx *ctx, const tqf_hip_heads *heads, float scale,
                                   const tqf_hip_head_rows *q, const tqf_hip_head_rows *gate, uint32_t n_seqs,
                                   uint32_t rows, const tqf_hip_kv_cache *cache, const int32_t *d_pages,

@@ -4,9 +4,11 @@
 //   y[i][h] = sum_j softmax_j(scale q[i][h] . k[j][h / group]) v[j][h / group]
 //             (* sigmoid(gate[i][h])),  j < len - rows + i + 1.
 //
-// Bound by the cache's bytes, each of which is needed once: the rows of a sequence
-// and the heads of a group stand side by side as the columns of the matrix
-// instructions, so a key is multiplied with all of them when it arrives.  The work
+// Bound by the cache's bytes: the rows of a sequence and the heads of a group stand
+// side by side as the columns of the matrix instructions, up to 32 to a workgroup, so
+// a key is multiplied with all of them when it arrives.  With more columns every 32
+// have workgroups of their own, which read the cache again (64 sequences of 50..8192
+// tokens, heads of 256, 4 rows of a group of 8: 53 us, 8 rows 75).  The work
 // of all sequences, in steps of 128 keys of one (sequence, key head), is one line
 // that is cut into equal parts, a part to a workgroup, whatever the lengths; what a
 // workgroup has of a (sequence, key head) that it does not have whole goes to
@@ -174,8 +176,10 @@ constexpr int residents(int dim, int row_tiles, bool f8) {
 
 // NR: tiles of 16 rows that a workgroup has.  A wavefront's 32 keys and values come
 // by copies to LDS that is its own: the next keys are asked for when these have been
-// multiplied, the next values likewise, so there is always one of the two under way,
-// and no registers wait for them.
+// multiplied, the next values likewise, and no registers wait for them.  The source
+// waits for the values alone, but the compiler puts a wait for all copies before their
+// first transposing read (whether the next keys were asked for depends on a branch):
+// the next keys come during the softmax, not beyond it.
 template <int D, int NR, bool F8>
 __global__ __launch_bounds__(64 * kWaves, residents(D, NR, F8)) void paged_kernel(Kernel p) {
     constexpr int kRow = F8 ? D : 2 * D, kDims = D / 16, kSteps = D / 32, kRows = 16 * NR, kChunks = D / 8;
@@ -706,7 +710,8 @@ uint32_t row_blocks(const PagedArgs &a) {
 }
 uint64_t units_of(const PagedArgs &a) { return (uint64_t)a.n_seqs * a.cache.kv_heads; }
 uint64_t most_steps(const PagedArgs &a) { return units_of(a) * (((uint64_t)a.max_pages * a.cache.page + kStepKeys - 1) / kStepKeys); }
-// As many workgroups as the compute units hold at once; no more than there can be steps.
+// As many workgroups as the compute units hold at once, for each block of rows (several of them, of more than 32
+// columns, take turns); no more than there can be steps.
 uint32_t parts_of(const PagedArgs &a) {
     const uint64_t want = (uint64_t)residents(a.cache.dim, tiles_of_rows(a), a.cache.f8) * (uint64_t)cu_count();
     return (uint32_t)(most_steps(a) < want ? most_steps(a) : want);
